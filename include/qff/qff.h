@@ -325,6 +325,86 @@ int qff_gqa_prefill(qff_ctx* ctx, qff_stream_t stream, const qff_gqa_params* p,
                     int start_pos, void* out, qff_dtype out_dtype, int T,
                     int max_ctx);
 
+/* ------------------------------------------------------------ paged KV cache */
+
+/* A full-attention layer's KV cache in pages of a pool: position p of a
+ * sequence is row p % page_size of page table[row][p / page_size]. No
+ * counterpart in the reference (one flat cache per layer and sequence,
+ * QwenQ4ActiveExpertStreamingRunner.swift:726-742); pages let many sequences
+ * of any length use one pool, and let sequences hold the same pages where they
+ * share a prefix.
+ *   k, v   [num_pages, page_size, 2, 256], 16-byte aligned, bf16 (fp16 with
+ *          qff_gqa_params.kv_f16)
+ *   table  int32 device array, one row of table_cols entries per sequence;
+ *          entries past a sequence's last position are not read
+ * page_size is a power of two, 16 .. 4096; table_cols * page_size at most the
+ * context's max_ctx, rounded up to a whole page. An entry in use that lies
+ * outside 0 .. num_pages - 1 makes the outputs that see its positions NaN
+ * (nothing outside the pool is read or written). A page that a call appends
+ * to must belong to one sequence only. Cache rows in use are finite. */
+typedef struct qff_kv_pages {
+    void* k;
+    void* v;
+    const int32_t* table;
+    int num_pages;
+    int page_size;
+    int table_cols;
+} qff_kv_pages;
+
+/* qff_gqa_decode on a paged cache: one token for each of `batch` sequences,
+ * k and v appended to the page of position positions[b] in row b of the
+ * table, which already names it. A position outside 0 .. table_cols *
+ * page_size - 1 (a padded slot) gives a NaN row and touches no page. q_gate and
+ * the norm weights are 16-byte aligned. fp32 outputs are within about 1e-6 of
+ * the exact result (bf16 outputs: their own rounding). */
+int qff_gqa_decode_paged(qff_ctx* ctx, qff_stream_t stream, const qff_gqa_params* p,
+                         const void* q_gate, const void* k_new, const void* v_new,
+                         qff_dtype in_dtype, const qff_kv_pages* kv, const int32_t* positions,
+                         void* out, qff_dtype out_dtype, int batch);
+
+/* qff_gqa_decode_paged where groups of sequences share a prefix (samples of
+ * one prompt, requests under one system prompt): the pages they share are read
+ * once for up to 16 sequences instead of once for each.
+ *   group       [batch] int32 device array: consecutive sequences with the same
+ *               value >= 0 are a group; sequences of a negative value stand
+ *               alone
+ *   shared_len  [batch] int32 device array: how many of its first positions a
+ *               sequence has in common with its group. The positions before the
+ *               least shared_len of a group's sequences are read through the
+ *               table row of the first of them (of each 16), so all of them
+ *               must hold the same K and V there (they may, and usually do, name
+ *               the same pages).
+ * A group's members may be at any positions; any values of the two arrays are
+ * valid as far as the rows they name are the same. Results are those of
+ * qff_gqa_decode_paged up to the order of fp32 sums. */
+int qff_gqa_decode_shared(qff_ctx* ctx, qff_stream_t stream, const qff_gqa_params* p,
+                          const void* q_gate, const void* k_new, const void* v_new,
+                          qff_dtype in_dtype, const qff_kv_pages* kv, const int32_t* positions,
+                          const int32_t* group, const int32_t* shared_len, void* out,
+                          qff_dtype out_dtype, int batch);
+
+/* qff_gqa_prefill on a paged cache: T consecutive tokens of one sequence at
+ * positions start_pos .. start_pos + T - 1, whose pages the one row of
+ * kv->table names. Arguments, precision and limits otherwise as
+ * qff_gqa_prefill (QFF_ERR_INVALID_ARG when start_pos + T exceeds table_cols *
+ * page_size); q_gate and out are 16-byte aligned. */
+int qff_gqa_prefill_paged(qff_ctx* ctx, qff_stream_t stream, const qff_gqa_params* p,
+                          const void* q_gate, const void* k, const void* v, qff_dtype in_dtype,
+                          const qff_kv_pages* kv, int start_pos, void* out, qff_dtype out_dtype,
+                          int T);
+
+/* pool[dst[i]] = pool[src[i]] for i < n in each of npools pools of num_pages
+ * pages of page_bytes bytes (a multiple of 16, at most 2^31; 16-byte aligned):
+ * the copies of a fork (the page its children go on writing, or whole
+ * recurrent states: a DeltaNet layer's ssm_state is a pool of 2 MiB pages) and
+ * the moves of a compaction. pools, src and dst are host arrays, read before
+ * the call returns: the pairs travel with the launch, and a captured call
+ * replays them. One source may go to several destinations; a destination that
+ * occurs twice or is also a source is refused (QFF_ERR_INVALID_ARG), as is an
+ * index outside 0 .. num_pages - 1. */
+int qff_pages_copy(qff_ctx* ctx, qff_stream_t stream, void* const* pools, int npools,
+                   size_t page_bytes, int num_pages, const int32_t* src, const int32_t* dst, int n);
+
 /* Raw KV append, token-major: cache[(pos*2 + kv_head)*256 + d] = k[kv_head*256
  * + d] rounded to cache_dtype (QFF_BF16 or QFF_F16), same for v. No-op when
  * pos >= max_seq. Replaces qwen_update_kv_cache_f16 (deltanet.metal:670-689)

@@ -406,8 +406,129 @@ int qff_gqa_prefill(qff_ctx* ctx, qff_stream_t stream, const qff_gqa_params* p, 
     // the cache copies the attention reads (fp16 K of a bf16 cache, V
     // transposed) hold the context's max_ctx rows
     if (static_cast<long long>(start_pos) + T > ctx->cfg.max_ctx) return QFF_ERR_WORKSPACE;
-    QFF_CHECK_HIP(launch_gqa_prefill(ctx, stream, p, q_gate, k, v, in_dtype, k_cache, v_cache, start_pos,
-                                     out, out_dtype, T, max_ctx));
+    QFF_CHECK_HIP(launch_gqa_prefill(ctx, stream, p, q_gate, k, v, in_dtype, k_cache, v_cache, nullptr, start_pos,
+                                     out, out_dtype, T));
+    return QFF_OK;
+}
+
+// The context's device current while a call launches, the caller's again after.
+namespace {
+struct OnDevice {
+    int prev = -1;
+    bool ok;
+    explicit OnDevice(int device) {
+        ok = hipGetDevice(&prev) == hipSuccess;
+        if (ok && prev == device) prev = -1;
+        else if (ok) ok = hipSetDevice(device) == hipSuccess;
+    }
+    ~OnDevice() {
+        if (prev >= 0) (void)hipSetDevice(prev);
+    }
+};
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+}  // namespace
+
+static int kv_pages_status(const qff_ctx* ctx, const qff_kv_pages* kv) {
+    if (!kv || !kv->k || !kv->v || !kv->table) return QFF_ERR_INVALID_ARG;
+    if (!aligned16(kv->k) || !aligned16(kv->v)) return QFF_ERR_INVALID_ARG;
+    if (kv->num_pages <= 0 || kv->page_size <= 0 || kv->table_cols <= 0) return QFF_ERR_INVALID_ARG;
+    if ((kv->page_size & (kv->page_size - 1)) != 0 || kv->page_size < 16 || kv->page_size > 4096)
+        return QFF_ERR_UNSUPPORTED;
+    const long long page = kv->page_size, room = (ctx->cfg.max_ctx + page - 1) / page * page;
+    if (kv->table_cols * page > room) return QFF_ERR_WORKSPACE;
+    return QFF_OK;
+}
+
+static int decode_paged(qff_ctx* ctx, qff_stream_t stream, const qff_gqa_params* p, const void* q_gate,
+                        const void* k_new, const void* v_new, qff_dtype in_dtype, const qff_kv_pages* kv,
+                        const int32_t* positions, const int32_t* group, const int32_t* shared_len, void* out,
+                        qff_dtype out_dtype, int batch) {
+    if (!ctx || !q_gate || !k_new || !v_new || !positions || !out) return QFF_ERR_INVALID_ARG;
+    if (const int st = gqa_params_status(p)) return st;
+    if (!dtype_ok(in_dtype) || !dtype_ok(out_dtype)) return QFF_ERR_INVALID_ARG;
+    if (!aligned16(q_gate) || !aligned16(p->q_norm_w) || batch <= 0) return QFF_ERR_INVALID_ARG;
+    if (const int st = kv_pages_status(ctx, kv)) return st;
+    if (batch > ctx->cfg.max_batch) return QFF_ERR_WORKSPACE;
+    const OnDevice on(ctx->device);
+    if (!on.ok) return QFF_ERR_HIP;
+    QFF_CHECK_HIP(launch_gqa_decode_paged(ctx, stream, p, q_gate, k_new, v_new, in_dtype, kv, positions, group,
+                                          shared_len, out, out_dtype, batch));
+    return QFF_OK;
+}
+
+int qff_gqa_decode_paged(qff_ctx* ctx, qff_stream_t stream, const qff_gqa_params* p, const void* q_gate,
+                         const void* k_new, const void* v_new, qff_dtype in_dtype, const qff_kv_pages* kv,
+                         const int32_t* positions, void* out, qff_dtype out_dtype, int batch) {
+    return decode_paged(ctx, stream, p, q_gate, k_new, v_new, in_dtype, kv, positions, nullptr, nullptr, out,
+                        out_dtype, batch);
+}
+
+int qff_gqa_decode_shared(qff_ctx* ctx, qff_stream_t stream, const qff_gqa_params* p, const void* q_gate,
+                          const void* k_new, const void* v_new, qff_dtype in_dtype, const qff_kv_pages* kv,
+                          const int32_t* positions, const int32_t* group, const int32_t* shared_len, void* out,
+                          qff_dtype out_dtype, int batch) {
+    if (!group || !shared_len) return QFF_ERR_INVALID_ARG;
+    return decode_paged(ctx, stream, p, q_gate, k_new, v_new, in_dtype, kv, positions, group, shared_len, out,
+                        out_dtype, batch);
+}
+
+int qff_gqa_prefill_paged(qff_ctx* ctx, qff_stream_t stream, const qff_gqa_params* p, const void* q_gate,
+                          const void* k, const void* v, qff_dtype in_dtype, const qff_kv_pages* kv, int start_pos,
+                          void* out, qff_dtype out_dtype, int T) {
+    if (!ctx || !q_gate || !k || !v || !out) return QFF_ERR_INVALID_ARG;
+    if (const int st = gqa_params_status(p)) return st;
+    if (!dtype_ok(in_dtype) || !dtype_ok(out_dtype)) return QFF_ERR_INVALID_ARG;
+    if (!aligned16(q_gate) || !aligned16(out) || T <= 0 || start_pos < 0) return QFF_ERR_INVALID_ARG;
+    if (const int st = kv_pages_status(ctx, kv)) return st;
+    const long long end = static_cast<long long>(start_pos) + T;
+    if (end > static_cast<long long>(kv->table_cols) * kv->page_size) return QFF_ERR_INVALID_ARG;
+    if (T > ctx->cfg.max_prefill_tokens || end > ctx->cfg.max_ctx) return QFF_ERR_WORKSPACE;
+    const OnDevice on(ctx->device);
+    if (!on.ok) return QFF_ERR_HIP;
+    QFF_CHECK_HIP(launch_gqa_prefill(ctx, stream, p, q_gate, k, v, in_dtype, kv->k, kv->v, kv, start_pos, out,
+                                     out_dtype, T));
+    return QFF_OK;
+}
+
+// Every index inside the pools, no page written twice, none both read and
+// written: the pairs may then be copied in any order.
+static int page_pairs_status(qff_ctx* ctx, int num_pages, const int32_t* src, const int32_t* dst, int n) {
+    for (int i = 0; i < n; ++i)
+        if (src[i] < 0 || src[i] >= num_pages || dst[i] < 0 || dst[i] >= num_pages) return QFF_ERR_INVALID_ARG;
+    const size_t words = (static_cast<size_t>(num_pages) + 63) / 64;
+    if (ctx->page_bits.size() < words) {
+        try {
+            ctx->page_bits.resize(words, 0);
+        } catch (...) {
+            return QFF_ERR_OUT_OF_MEMORY;
+        }
+    }
+    uint64_t* bits = ctx->page_bits.data();
+    bool ok = true;
+    for (int i = 0; i < n; ++i) {
+        uint64_t& w = bits[dst[i] >> 6];
+        const uint64_t bit = 1ull << (dst[i] & 63);
+        if (w & bit) ok = false;
+        w |= bit;
+    }
+    for (int i = 0; i < n; ++i)
+        if (bits[src[i] >> 6] >> (src[i] & 63) & 1) ok = false;
+    for (int i = 0; i < n; ++i) bits[dst[i] >> 6] = 0;
+    return ok ? QFF_OK : QFF_ERR_INVALID_ARG;
+}
+
+int qff_pages_copy(qff_ctx* ctx, qff_stream_t stream, void* const* pools, int npools, size_t page_bytes,
+                   int num_pages, const int32_t* src, const int32_t* dst, int n) {
+    if (!ctx || !pools || npools <= 0 || num_pages <= 0 || page_bytes == 0 || n < 0) return QFF_ERR_INVALID_ARG;
+    if (n > 0 && (!src || !dst)) return QFF_ERR_INVALID_ARG;
+    for (int i = 0; i < npools; ++i)
+        if (!pools[i] || !aligned16(pools[i])) return QFF_ERR_INVALID_ARG;
+    if (page_bytes % 16 != 0 || page_bytes > (size_t{1} << 31)) return QFF_ERR_UNSUPPORTED;
+    if (n == 0) return QFF_OK;
+    if (const int st = page_pairs_status(ctx, num_pages, src, dst, n)) return st;
+    const OnDevice on(ctx->device);
+    if (!on.ok) return QFF_ERR_HIP;
+    QFF_CHECK_HIP(launch_pages_copy(ctx, stream, pools, npools, page_bytes, src, dst, n));
     return QFF_OK;
 }
 

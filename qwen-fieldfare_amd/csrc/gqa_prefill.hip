@@ -14,7 +14,10 @@
 //          The same launch's other workgroups write the transposed fp16
 //          copy of V (per kv head and 64-position tile, dims x positions,
 //          so that the attention's V operand is one 16-byte LDS read per
-//          lane) and a bf16 cache's older k rows into the fp16 copy.
+//          lane) and a bf16 cache's older k rows into the fp16 copy. Where the
+//          cache lies in pages (PAGED), every row is found through the page
+//          table here and the fp16 copy of K is made for either cache type, so
+//          the attention reads the same copies.
 //   attn   flash attention. A workgroup owns 16 query tokens x the 8 q heads
 //          of one kv head (128 rows; four wave pairs of 32 rows = 4 tokens
 //          x 8 heads, each wave running its own flash attention over half of
@@ -58,12 +61,25 @@ constexpr int kPfKT = 64;       // K/V positions per tile
 // type first, exactly as the prep workgroups store them, so the copy holds
 // the cache's values), later ones are zero. A workgroup of 512 threads
 // stages one tile through LDS.
+// Where position p's row lies: row p of a flat cache, or row p % page of pool
+// page table[p / page]. An entry outside the pool has no row (-1).
+template <bool PAGED>
+struct KvPlace {
+    const int32_t* table;
+    int num_pages, lg;
+    __device__ __forceinline__ long long row(int p) const {
+        if constexpr (!PAGED) return p;
+        const int page = table[p >> lg];
+        return page < 0 || page >= num_pages ? -1 : (static_cast<long long>(page) << lg) + (p & ((1 << lg) - 1));
+    }
+};
+
 __device__ __forceinline__ int vt_slot_row(int s) { return (s & ~12) | ((s & 4) << 1) | ((s & 8) >> 1); }
 
-template <int IN_DT, int KV_F16>
+template <int IN_DT, int KV_F16, bool PAGED>
 __device__ __forceinline__ void vt_tile_copy(const void* __restrict__ v, const uint16_t* __restrict__ vc,
-                                             uint16_t* __restrict__ vt, int tl, int kvh, int start, int n,
-                                             int ntile_stride) {
+                                             KvPlace<PAGED> at, uint16_t* __restrict__ vt, int tl, int kvh, int start,
+                                             int n, int ntile_stride) {
     __shared__ __attribute__((aligned(16))) uint16_t tile[64][264];   // positions x dims (+8 pad)
     const int t = threadIdx.x;
     const int p0 = tl * 64;
@@ -72,8 +88,11 @@ __device__ __forceinline__ void vt_tile_copy(const void* __restrict__ v, const u
         const int q = t + 512 * i, row = q >> 5, pc = q & 31, p = p0 + row;
         u32x4_t w = u32x4_t{0u, 0u, 0u, 0u};
         if (p < start) {
-            w = *reinterpret_cast<const u32x4_t*>(vc + (static_cast<size_t>(p) * 2 + kvh) * 256 + 8 * pc);
-            if (!KV_F16) w = bf16x8_to_f16x8(w);
+            const long long r = at.row(p);   // (without a row: zeros, its K is NaN)
+            if (!PAGED || r >= 0) {
+                w = *reinterpret_cast<const u32x4_t*>(vc + (static_cast<size_t>(r) * 2 + kvh) * 256 + 8 * pc);
+                if (!KV_F16) w = bf16x8_to_f16x8(w);
+            }
         } else if (p < n) {
             const size_t src = (static_cast<size_t>(p - start) * 2 + kvh) * 256 + 8 * pc;
             float f[8];
@@ -105,8 +124,8 @@ __device__ __forceinline__ void vt_tile_copy(const void* __restrict__ v, const u
 
 // Launch layout of the prep kernel: vt_blocks workgroups of transposed-V
 // tiles (two per 64-position tile, one per kv head), then k16_blocks
-// workgroups copying a bf16 cache's K rows before start into the fp16 copy
-// (512 16-byte pieces each), then one workgroup per 8 tokens of the prep
+// workgroups copying a bf16 or paged cache's K rows before start into the fp16
+// copy (512 16-byte pieces each), then one workgroup per 8 tokens of the prep
 // proper. None depends on another: the copies read only rows the prep does
 // not write, or the step's inputs.
 struct PrepGrid {
@@ -123,23 +142,34 @@ struct PrepGrid {
 constexpr int kPrepWaves = 8;
 constexpr int kPrepRound = 6;
 
-template <int IN_DT, int KV_F16, int ROUNDS>
+template <int IN_DT, int KV_F16, int ROUNDS, bool PAGED>
 __global__ __launch_bounds__(64 * kPrepWaves) void gqa_prefill_prep_kernel(
     const void* __restrict__ q_gate, const void* __restrict__ k, const void* __restrict__ v,
     const float* __restrict__ q_norm_w, const float* __restrict__ k_norm_w, RopeFreqs rf, float scale,
     float eps, int start, int T, uint16_t* __restrict__ qb, uint16_t* __restrict__ k_cache,
-    uint16_t* __restrict__ v_cache, uint16_t* __restrict__ k16, uint16_t* __restrict__ vt, PrepGrid pg) {
+    uint16_t* __restrict__ v_cache, uint16_t* __restrict__ k16, uint16_t* __restrict__ vt, PrepGrid pg,
+    KvPlace<PAGED> at) {
     int blk = static_cast<int>(blockIdx.x);
     if (blk < pg.vt_blocks) {
-        vt_tile_copy<IN_DT, KV_F16>(v, v_cache, vt, blk >> 1, blk & 1, start, start + T, pg.vt_stride);
+        vt_tile_copy<IN_DT, KV_F16, PAGED>(v, v_cache, at, vt, blk >> 1, blk & 1, start, start + T, pg.vt_stride);
         return;
     }
     blk -= pg.vt_blocks;
     if (blk < pg.k16_blocks) {
-        // the fp16 copy of bf16 K cache rows 0 .. start - 1 (both kv heads)
+        // the fp16 copy of K cache rows 0 .. start - 1 (both kv heads); NaN where a page has no row
         const int i = blk * 512 + static_cast<int>(threadIdx.x);
         if (i < start * 64) {
             const size_t o = static_cast<size_t>(i) * 8;
+            if constexpr (PAGED) {
+                const long long r = at.row(i >> 6);
+                u32x4_t w = u32x4_t{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
+                if (r >= 0) {
+                    w = *reinterpret_cast<const u32x4_t*>(k_cache + r * 512 + 8 * (i & 63));
+                    if (!KV_F16) w = bf16x8_to_f16x8(w);
+                }
+                *reinterpret_cast<u32x4_t*>(k16 + o) = w;
+                return;
+            }
             *reinterpret_cast<u32x4_t*>(k16 + o) = bf16x8_to_f16x8(*reinterpret_cast<const u32x4_t*>(k_cache + o));
         }
         return;
@@ -214,7 +244,24 @@ __global__ __launch_bounds__(64 * kPrepWaves) void gqa_prefill_prep_kernel(
             } else {
                 const int kvh = hs - 16;
                 const size_t off = (static_cast<size_t>(pos) * 2 + kvh) * 256 + 4 * lane;
-                if (KV_F16) {
+                if constexpr (PAGED) {
+                    // the rounded entries into the page (dropped where it lies
+                    // outside the pool: the copy's NaN makes the rows that see
+                    // the position NaN), k's fp16 copy
+                    const long long r = at.row(pos);
+                    const u32x2_t kw2 = KV_F16 ? u32x2_t{pack_f16x2(y[0], y[1]), pack_f16x2(y[2], y[3])}
+                                               : u32x2_t{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+                    const float* vr = vv[kvh];
+                    if (r >= 0) {
+                        const size_t o = (static_cast<size_t>(r) * 2 + kvh) * 256 + 4 * lane;
+                        *reinterpret_cast<u32x2_t*>(k_cache + o) = kw2;
+                        *reinterpret_cast<u32x2_t*>(v_cache + o) =
+                            KV_F16 ? u32x2_t{pack_f16x2(vr[0], vr[1]), pack_f16x2(vr[2], vr[3])}
+                                   : u32x2_t{pack_bf16x2(vr[0], vr[1]), pack_bf16x2(vr[2], vr[3])};
+                    }
+                    const u32x2_t copy = KV_F16 ? kw2 : u32x2_t{bf16x2_to_f16x2(kw2[0]), bf16x2_to_f16x2(kw2[1])};
+                    *reinterpret_cast<u32x2_t*>(k16 + off) = r >= 0 ? copy : u32x2_t{0x7e007e00u, 0x7e007e00u};
+                } else if (KV_F16) {
                     *reinterpret_cast<u32x2_t*>(k_cache + off) =
                         u32x2_t{pack_f16x2(y[0], y[1]), pack_f16x2(y[2], y[3])};
                     *reinterpret_cast<u32x2_t*>(v_cache + off) =
@@ -685,8 +732,8 @@ __global__ __launch_bounds__(256) void gqa_prefill_combine_kernel(const float2* 
 
 hipError_t launch_gqa_prefill(qff_ctx* ctx, hipStream_t stream, const qff_gqa_params* p,
                               const void* q_gate, const void* k, const void* v, qff_dtype in_dtype,
-                              void* k_cache, void* v_cache, int start_pos, void* out,
-                              qff_dtype out_dtype, int T, int) {
+                              void* k_cache, void* v_cache, const qff_kv_pages* pages, int start_pos, void* out,
+                              qff_dtype out_dtype, int T) {
     // the fp16 q rows [T][16][256] (workspace)
     uint16_t* qb = ctx->gqa_qb;
     uint16_t* kc = static_cast<uint16_t*>(k_cache);
@@ -696,30 +743,36 @@ hipError_t launch_gqa_prefill(qff_ctx* ctx, hipStream_t stream, const qff_gqa_pa
     // copy in workspace, [max_ctx][2][256]) and the transposed fp16 copy of V
     // ([2][max_ctx / 64][256][64] in workspace), both written by the prep
     // launch
-    uint16_t* k16 = p->kv_f16 ? kc : ctx->gqa_kv16;
+    const bool copy_k = pages || !p->kv_f16;
+    uint16_t* k16 = copy_k ? ctx->gqa_kv16 : kc;
     {
         // one launch: the transposed V copy (cache rows before start_pos and
-        // the step's v), the fp16 copy of a bf16 cache's K rows before
+        // the step's v), the fp16 copy of a bf16 or paged cache's K rows before
         // start_pos, and the per-token prep (q to workspace, k / v appended,
-        // a bf16 cache's new k rows also to the fp16 copy)
-        ProfScope prof(ctx, stream, "gqa_prefill_prep");
+        // the copied cache's new k rows also to the fp16 copy)
+        ProfScope prof(ctx, stream, pages ? "gqa_paged_prefill_prep" : "gqa_prefill_prep");
         PrepGrid pg;
         pg.vt_stride = (ctx->cfg.max_ctx + kPfKT - 1) / kPfKT;   // tiles per kv head
         pg.vt_blocks = 2 * ((start_pos + T + kPfKT - 1) / kPfKT);
-        pg.k16_blocks = p->kv_f16 ? 0 : (start_pos * 64 + 511) / 512;
+        pg.k16_blocks = copy_k ? (start_pos * 64 + 511) / 512 : 0;
         // a wave per round where the tokens do not fill the chip: its time is
         // then one round's chain of load, reduction and store instead of three
         // (us per call at 16, 500, 1000, 8192 tokens from position 0: 22.5,
         // 34.8, 49.5, 586 against 26.2, 38.6, 50.0, 583)
         const bool one = T <= 1024;
         const int grid = pg.vt_blocks + pg.k16_blocks + ((one ? 3 * T : T) + kPrepWaves - 1) / kPrepWaves;
-#define QFF_PREP1(I, F, R)                                                                                     \
-    gqa_prefill_prep_kernel<I, F, R><<<grid, 64 * kPrepWaves, 0, stream>>>(q_gate, k, v, p->q_norm_w,          \
-                                                                          p->k_norm_w, rf, p->scale, p->eps, \
-                                                                          start_pos, T, qb, kc, vc, k16,     \
-                                                                          ctx->gqa_vt, pg)
-#define QFF_PREP(I, F) \
-    if (one) QFF_PREP1(I, F, 1); else QFF_PREP1(I, F, 3)
+#define QFF_PREP1(I, F, R, P, AT)                                                                                 \
+    gqa_prefill_prep_kernel<I, F, R, P><<<grid, 64 * kPrepWaves, 0, stream>>>(q_gate, k, v, p->q_norm_w,          \
+                                                                             p->k_norm_w, rf, p->scale, p->eps, \
+                                                                             start_pos, T, qb, kc, vc, k16,     \
+                                                                             ctx->gqa_vt, pg, AT)
+#define QFF_PREP(I, F)                                                                                    \
+    if (pages) { if (one) QFF_PREP1(I, F, 1, true, paged); else QFF_PREP1(I, F, 3, true, paged); }        \
+    else { if (one) QFF_PREP1(I, F, 1, false, flat); else QFF_PREP1(I, F, 3, false, flat); }
+        const KvPlace<false> flat{};
+        const KvPlace<true> paged = pages ? KvPlace<true>{pages->table, pages->num_pages,
+                                                          __builtin_ctz(static_cast<unsigned>(pages->page_size))}
+                                          : KvPlace<true>{};
         if (p->kv_f16) {
             if (in_dtype == QFF_BF16) { QFF_PREP(1, 1); } else { QFF_PREP(0, 1); }
         } else {

@@ -65,6 +65,8 @@ struct qff_ctx {
     // (each launch's last workgroup resets its pair); kSchedSlots pairs.
     unsigned* sched = nullptr;
     int num_cu = 0;
+    // qff_pages_copy: one bit a page, all clear between calls.
+    std::vector<uint64_t> page_bits;
     // Kernel timing (qff_profile_enable): a pool of event pairs.
     bool prof = false;
     std::vector<qff_prof_record> prof_pool;
@@ -183,8 +185,17 @@ hipError_t launch_gqa_decode_into(qff_ctx* ctx, const GqaPartials& ws, hipStream
                                   int max_ctx);
 hipError_t launch_gqa_prefill(qff_ctx* ctx, hipStream_t stream, const qff_gqa_params* p,
                               const void* q_gate, const void* k, const void* v, qff_dtype in_dtype,
-                              void* k_cache, void* v_cache, int start_pos, void* out,
-                              qff_dtype out_dtype, int T, int max_ctx);
+                              void* k_cache, void* v_cache, const qff_kv_pages* pages, int start_pos, void* out,
+                              qff_dtype out_dtype, int T);   // pages: not null where the caches are pools of pages
+// Chunks per (sequence, kv head) that the context's partial slots allow a decode call of `batch`.
+int gqa_chunk_cap(const qff_ctx_cfg& cfg, int batch);
+// Decode over pages; group / shared_len null where no prefix is shared.
+hipError_t launch_gqa_decode_paged(qff_ctx* ctx, hipStream_t stream, const qff_gqa_params* p, const void* q_gate,
+                                   const void* k_new, const void* v_new, qff_dtype in_dtype, const qff_kv_pages* kv,
+                                   const int32_t* positions, const int32_t* group, const int32_t* shared_len,
+                                   void* out, qff_dtype out_dtype, int batch);
+hipError_t launch_pages_copy(qff_ctx* ctx, hipStream_t stream, void* const* pools, int npools, size_t page_bytes,
+                             const int32_t* src, const int32_t* dst, int n);
 hipError_t launch_q4_dequant(hipStream_t stream, const uint32_t* w, const void* scales,
                              const void* biases, qff_dtype sb_dtype, float* out, int rows, int cols);
 hipError_t launch_q4_matmul(qff_ctx* ctx, hipStream_t stream, const uint32_t* w, const void* scales,

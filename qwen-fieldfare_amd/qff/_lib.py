@@ -39,6 +39,10 @@ class Q4Part(ctypes.Structure):
                 ("residual", _vp)]
 
 
+class KvPages(ctypes.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("table", _vp), ("num_pages", _i), ("page_size", _i), ("table_cols", _i)]
+
+
 Q4_MAX_PARTS = 8
 
 
@@ -69,6 +73,13 @@ SIGNATURES = {
                               _i],
     "qff_gqa_prefill": [_vp, _vp, ctypes.POINTER(GqaParams), _vp, _vp, _vp, _i, _vp, _vp, _i, _vp,
                         _i, _i, _i],
+    "qff_gqa_decode_paged": [_vp, _vp, ctypes.POINTER(GqaParams), _vp, _vp, _vp, _i, ctypes.POINTER(KvPages), _vp,
+                             _vp, _i, _i],
+    "qff_gqa_decode_shared": [_vp, _vp, ctypes.POINTER(GqaParams), _vp, _vp, _vp, _i, ctypes.POINTER(KvPages), _vp,
+                              _vp, _vp, _vp, _i, _i],
+    "qff_gqa_prefill_paged": [_vp, _vp, ctypes.POINTER(GqaParams), _vp, _vp, _vp, _i, ctypes.POINTER(KvPages), _i,
+                              _vp, _i, _i],
+    "qff_pages_copy": [_vp, _vp, ctypes.POINTER(_vp), _i, ctypes.c_size_t, _i, _vp, _vp, _i],
     "qff_kv_append": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i],
     "qff_attention_gate": [_vp, _vp, _vp, _vp, _vp, _i],
     "qff_profile_enable": [_vp, _i],

@@ -13,7 +13,8 @@ import struct
 
 import torch
 
-from ._lib import BF16, F16, F32, Q4_MAX_PARTS, CtxCfg, DeltaNetParams, GqaParams, Q4Part, QffError, check, lib
+from ._lib import (BF16, F16, F32, Q4_MAX_PARTS, CtxCfg, DeltaNetParams, GqaParams, KvPages, Q4Part, QffError,
+                   check, lib)
 
 _DT = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 _TORCH = {F32: torch.float32, BF16: torch.bfloat16, F16: torch.float16}
@@ -27,9 +28,10 @@ _f32, _bf16, _f16, _i32 = torch.float32, torch.bfloat16, torch.float16, torch.in
 # untyped pointers.
 _P_DN = struct.Struct("PPPPf4x")
 _P_GQA = struct.Struct("PPfiffi4x")
+_P_KV = struct.Struct("PPPiii4x")
 _P_Q4 = [struct.Struct("PPPi4xPi4xP" * n) for n in range(Q4_MAX_PARTS + 1)]
 assert _P_DN.size == ctypes.sizeof(DeltaNetParams) and _P_GQA.size == ctypes.sizeof(GqaParams)
-assert _P_Q4[1].size == ctypes.sizeof(Q4Part)
+assert _P_Q4[1].size == ctypes.sizeof(Q4Part) and _P_KV.size == ctypes.sizeof(KvPages)
 
 
 def _pack(layout: struct.Struct, pointers, *fields) -> bytes:
@@ -41,7 +43,7 @@ def _pack(layout: struct.Struct, pointers, *fields) -> bytes:
         return layout.pack(*pointers, *(f if isinstance(f, int) else ctypes.c_float(f).value for f in fields))
 
 
-_BLOCKS = (ctypes.POINTER(DeltaNetParams), ctypes.POINTER(GqaParams), ctypes.POINTER(Q4Part))
+_BLOCKS = (ctypes.POINTER(DeltaNetParams), ctypes.POINTER(GqaParams), ctypes.POINTER(Q4Part), ctypes.POINTER(KvPages))
 
 
 class _Calls:
@@ -49,7 +51,8 @@ class _Calls:
 
     def __init__(self, L):
         for name in ("qff_q4_matmul", "qff_q4_matmul_parts", "qff_q4_norm_matmul_parts", "qff_router_top8",
-                     "qff_deltanet_decode", "qff_deltanet_prefill", "qff_gqa_decode", "qff_gqa_prefill"):
+                     "qff_deltanet_decode", "qff_deltanet_prefill", "qff_gqa_decode", "qff_gqa_prefill",
+                     "qff_gqa_decode_paged", "qff_gqa_decode_shared", "qff_gqa_prefill_paged"):
             fn = L[name]   # a new function object: the typed one of lib() stays as it is
             fn.argtypes = [ctypes.c_void_p if t in _BLOCKS else t for t in getattr(L, name).argtypes]
             fn.restype = ctypes.c_int
@@ -87,6 +90,8 @@ if hasattr(torch._C, "_cuda_getCurrentRawStream"):
     def _stream() -> int:
         return _raw_stream(_device())
 else:
+    _raw_stream = None
+
     def _stream() -> int:
         return torch.cuda.current_stream().cuda_stream
 
@@ -350,5 +355,133 @@ def gqa_prefill(ctx: Context, params: dict, q_gate, k, v, k_cache, v_cache, star
     return out
 
 
+def _ptr_on(ctx: Context, name: str, t: torch.Tensor, dtype=None) -> int:
+    """The address of a contiguous tensor on the context's device."""
+    if t.get_device() != ctx.device:
+        raise ValueError(f"{name} must live on the context's device, cuda:{ctx.device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}")
+    return t.data_ptr()
+
+
+def _stream_of(ctx: Context) -> int:
+    return torch.cuda.current_stream(ctx.device).cuda_stream if _raw_stream is None else _raw_stream(ctx.device)
+
+
+def _paged_args(ctx: Context, params: dict, q_gate, k, v, k_pages, v_pages, table, rows, n, theta, scale, eps):
+    """The checks and parameter blocks that the calls on a paged cache share:
+    n tokens, `rows` rows of the table."""
+    _check_gqa_inputs(q_gate, k, v, k_pages, v_pages, n)
+    if k_pages.dim() != 4 or k_pages.shape[2:] != (2, 256) or v_pages.shape != k_pages.shape:
+        raise ValueError("k_pages and v_pages must be [num_pages, page_size, 2, 256]")
+    if table.dim() != 2 or table.shape[0] != rows:
+        raise ValueError(f"the page table must be [{rows}, entries]")
+    qw, kw = params["q_norm_w"], params["k_norm_w"]
+    if qw.numel() != 256 or kw.numel() != 256:
+        raise ValueError("q_norm_w and k_norm_w must have 256 entries")
+    prm = _pack(_P_GQA, (_ptr_on(ctx, "q_norm_w", qw, _f32), _ptr_on(ctx, "k_norm_w", kw, _f32)), theta, 64, scale, eps,
+                int(k_pages.dtype == _f16))
+    kv = _P_KV.pack(_ptr_on(ctx, "k_pages", k_pages), _ptr_on(ctx, "v_pages", v_pages),
+                    _ptr_on(ctx, "the page table", table, _i32), k_pages.shape[0], k_pages.shape[1], table.shape[1])
+    return prm, _ptr_on(ctx, "q_gate", q_gate), _ptr_on(ctx, "k", k), _ptr_on(ctx, "v", v), _code(q_gate), kv
+
+
+def _paged_out(ctx: Context, q_gate, out, out_dtype, n):
+    if out is None:
+        out = torch.empty(n, 16, 256, dtype=out_dtype, device=q_gate.device)
+    elif out.numel() != n * 4096:
+        raise ValueError(f"out must be [{n}, 16, 256]")
+    return out, _ptr_on(ctx, "out", out)
+
+
+def gqa_decode_paged(ctx: Context, params: dict, q_gate, k_new, v_new, k_pages, v_pages, table, positions,
+                     out=None, out_dtype=torch.bfloat16, theta=1e7, scale=1.0 / 16, eps=1e-6):
+    """gqa_decode on a paged cache: k_pages / v_pages [num_pages, page_size, 2,
+    256] bf16 or fp16, position p of sequence b at row p % page_size of page
+    table[b, p // page_size] (table int32 [B, entries], on the device).
+    q_gate [B,16,512], k_new / v_new [B,2,256], positions int32 [B] (device)
+    -> out [B,16,256]; a position outside the table gives a NaN row."""
+    B = q_gate.shape[0]
+    prm, qp, kp, vp, code, kv = _paged_args(ctx, params, q_gate, k_new, v_new, k_pages, v_pages, table, B, B, theta,
+                                            scale, eps)
+    if positions.numel() != B:
+        raise ValueError(f"positions must be [{B}]")
+    out, op = _paged_out(ctx, q_gate, out, out_dtype, B)
+    st = _hot().qff_gqa_decode_paged(ctx.handle, _stream_of(ctx), prm, qp, kp, vp, code, kv,
+                                     _ptr_on(ctx, "positions", positions, _i32), op, _code(out), B)
+    if st:
+        raise QffError("qff_gqa_decode_paged", st)
+    return out
+
+
+def gqa_decode_shared(ctx: Context, params: dict, q_gate, k_new, v_new, k_pages, v_pages, table, positions, group,
+                      shared_len, out=None, out_dtype=torch.bfloat16, theta=1e7, scale=1.0 / 16, eps=1e-6):
+    """gqa_decode_paged where consecutive sequences with the same group >= 0
+    hold the same K and V at their first positions (as many as the least of
+    their shared_len), which are read once for up to 16 of them. group and
+    shared_len: int32 [B] on the device; sequences of a negative group stand
+    alone."""
+    B = q_gate.shape[0]
+    prm, qp, kp, vp, code, kv = _paged_args(ctx, params, q_gate, k_new, v_new, k_pages, v_pages, table, B, B, theta,
+                                            scale, eps)
+    if positions.numel() != B or group.numel() != B or shared_len.numel() != B:
+        raise ValueError(f"positions, group and shared_len must be [{B}]")
+    out, op = _paged_out(ctx, q_gate, out, out_dtype, B)
+    st = _hot().qff_gqa_decode_shared(ctx.handle, _stream_of(ctx), prm, qp, kp, vp, code, kv,
+                                      _ptr_on(ctx, "positions", positions, _i32), _ptr_on(ctx, "group", group, _i32),
+                                      _ptr_on(ctx, "shared_len", shared_len, _i32), op, _code(out), B)
+    if st:
+        raise QffError("qff_gqa_decode_shared", st)
+    return out
+
+
+def gqa_prefill_paged(ctx: Context, params: dict, q_gate, k, v, k_pages, v_pages, table, start_pos=0, out=None,
+                      out_dtype=torch.bfloat16, theta=1e7, scale=1.0 / 16, eps=1e-6):
+    """gqa_prefill on a paged cache: T tokens of one sequence at positions
+    start_pos .. start_pos + T - 1, appended to the pages its row of the table
+    (int32 [entries]) names -> out [T,16,256]."""
+    T = q_gate.shape[0]
+    prm, qp, kp, vp, code, kv = _paged_args(ctx, params, q_gate, k, v, k_pages, v_pages,
+                                            table[None] if table.dim() == 1 else table, 1, T, theta, scale, eps)
+    out, op = _paged_out(ctx, q_gate, out, out_dtype, T)
+    st = _hot().qff_gqa_prefill_paged(ctx.handle, _stream_of(ctx), prm, qp, kp, vp, code, kv, start_pos, op, _code(out),
+                                      T)
+    if st:
+        raise QffError("qff_gqa_prefill_paged", st)
+    return out
+
+
+def _host_i32(name, x) -> torch.Tensor:
+    t = x if isinstance(x, torch.Tensor) else torch.tensor(x, dtype=_i32)
+    if t.is_cuda or t.dtype != _i32 or t.dim() != 1 or not t.is_contiguous():
+        raise TypeError(f"{name} must be a list of ints or an int32 [n] tensor on the host")
+    return t
+
+
+def pages_copy(ctx: Context, pools, src, dst) -> None:
+    """pool[dst[i]] = pool[src[i]] for every pool and i, in place. pools:
+    tensors [num_pages, ...] of one number of pages and bytes per page (a
+    multiple of 16): K and V pools, or DeltaNet states with one page per
+    sequence. src, dst: page numbers, as lists or int32 host tensors; a
+    destination may be neither repeated nor a source."""
+    pools = list(pools)
+    if not pools:
+        raise ValueError("at least one pool")
+    s, d = _host_i32("src", src), _host_i32("dst", dst)
+    if s.numel() != d.numel():
+        raise ValueError("src and dst must have the same length")
+    pages = pools[0].shape[0]
+    size = pools[0].numel() * pools[0].element_size() // max(pages, 1)
+    for p in pools:
+        if p.shape[0] != pages or p.numel() * p.element_size() != pages * size:
+            raise ValueError("pools must have the same number of pages and bytes per page")
+    arr = (ctypes.c_void_p * len(pools))(*(_ptr_on(ctx, "a pool", p) for p in pools))
+    check("qff_pages_copy", lib().qff_pages_copy(ctx.handle, _stream_of(ctx), arr, len(pools), size, pages,
+                                                 s.data_ptr(), d.data_ptr(), s.numel()))
+
+
 __all__ = ["Context", "QffError", "q4_dequant", "q4_matmul", "deltanet_decode", "deltanet_prefill",
-           "gqa_decode", "gqa_prefill", "BF16", "F16", "F32"]
+           "gqa_decode", "gqa_prefill", "gqa_decode_paged", "gqa_decode_shared", "gqa_prefill_paged", "pages_copy",
+           "BF16", "F16", "F32"]
