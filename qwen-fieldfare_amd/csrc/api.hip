@@ -47,6 +47,7 @@ WorkspaceLayout workspace_layout(const qff_ctx_cfg& cfg) {
     L.gqa_m = take(S * 8 * sizeof(float));
     L.gqa_d = take(S * 8 * sizeof(float));
     L.gqa_o = take(S * 8 * 256 * sizeof(float));
+    L.gqa_nc = take(B * sizeof(int32_t));
     L.gqa_qb = take(T * 16 * 256 * sizeof(uint16_t));
     L.gqa_kv16 = take(static_cast<size_t>(cfg.max_ctx) * 512 * sizeof(uint16_t));
     L.gqa_vt = take(static_cast<size_t>((cfg.max_ctx + 63) / 64) * 64 * 512 * sizeof(uint16_t));
@@ -174,6 +175,7 @@ int qff_ctx_create(qff_ctx** out, int device, const qff_ctx_cfg* cfg) {
     c->gqa_m = reinterpret_cast<float*>(base + L.gqa_m);
     c->gqa_d = reinterpret_cast<float*>(base + L.gqa_d);
     c->gqa_o = reinterpret_cast<float*>(base + L.gqa_o);
+    c->gqa_nc = reinterpret_cast<int32_t*>(base + L.gqa_nc);
     auto u16 = [&](size_t off) { return reinterpret_cast<uint16_t*>(base + off); };
     c->gqa_qb = u16(L.gqa_qb);
     c->gqa_kv16 = u16(L.gqa_kv16);

@@ -27,6 +27,8 @@
 // three of bf16 or two of fp16 (error 2e-7 to 7e-7 of the exact output, where
 // two bf16 terms leave 6e-6). fp16 weights are scaled by 2^7 (kShift), so that
 // weights down to 2^-21 of the row's largest keep all bits of their first term.
+#include <type_traits>
+
 #include "common.hpp"
 #include "internal.hpp"
 #include "mfma.hpp"
@@ -45,8 +47,8 @@ namespace qff {
 // all of it. Any values of the arrays give a valid split.
 //
 // A CU holds one workgroup (its LDS), which leaves the CU idle while it starts,
-// so the chunk length is the least that needs no second round of workgroups
-// where such a length exists.
+// so the chunk length is about the least that needs no second round of
+// workgroups where such a length exists.
 
 constexpr int kBlkSeqs = 16;    // sequences of a block
 constexpr int kTile = 64;       // positions of a tile
@@ -122,8 +124,9 @@ __device__ __forceinline__ int chunk_length(const PagedSeqs& a, const LanePlan& 
         streams += wave_sum_int(items_of(p, 1 << 30, lane));
         longest = max(longest, wave_max_int(p.len));
     }
-    // (sum of ceil(n / ch) <= (tiles / ch) + streams)
-    int ch = static_cast<int>((tiles + a.slots - 1) / a.slots);
+    // sum of ceil(n / ch) is about tiles / ch + streams / 2, and at most tiles / ch + streams
+    const int free = max(a.slots - streams / 2, (a.slots + 1) / 2);
+    int ch = static_cast<int>((tiles + free - 1) / free);
     const int sure = streams < a.slots ? static_cast<int>((tiles + a.slots - streams - 1) / (a.slots - streams)) : ch;
     if (a.batch <= 64) {
         while (ch < sure && wave_sum_int(items_of(p0, ch * kTile, lane)) > a.slots) ch += (ch + 15) / 16;
@@ -176,9 +179,11 @@ struct PageWindow {
     int page, base;
     unsigned long long bad;
 
-    __device__ __forceinline__ void load(const int32_t* row, int first, int last, int num_pages, int lane) {
+    static __device__ __forceinline__ int entry(const int32_t* row, int first, int last, int lane) {
+        return row[min(first + lane, last)];
+    }
+    __device__ __forceinline__ void set(int first, int p, int num_pages) {
         base = first;
-        const int p = row[min(first + lane, last)];
         const bool out = p < 0 || p >= num_pages;
         bad = __ballot(out);
         page = out ? 0 : p;
@@ -206,6 +211,37 @@ __device__ __forceinline__ void load8(const void* p, size_t i, float (&x)[8]) {
             x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
         }
     }
+}
+
+// Four consecutive elements as fp32.
+template <int DT>
+__device__ __forceinline__ void load4(const void* p, size_t i, float* x) {
+    if constexpr (DT == 0) {
+        const f32x4_t a = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p) + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = a[e];
+    } else {
+        const u32x2_t w = *reinterpret_cast<const u32x2_t*>(static_cast<const uint16_t*>(p) + i);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            x[2 * e] = __uint_as_float(w[e] << 16);
+            x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+        }
+    }
+}
+
+// Sum over the four lanes l % 16 + 16 j of an MFMA column, in all of them.
+__device__ __forceinline__ float quad_sum(float v) {
+    v += swizzle_xor16(v);
+    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(h[0]) + __uint_as_float(h[1]);
+}
+
+// 1 / sqrt(ss / 256 + eps) on the hardware's reciprocal square root (1 ulp: a
+// head's scores scaled by as much; a division and a square root take 30
+// instructions more for each row, 0.5 us of a block's start).
+__device__ __forceinline__ float inv_rms(float ss, float eps) {
+    return __builtin_amdgcn_rsqf(fmaf(ss, 1.0f / 256.0f, eps));
 }
 
 // Two floats as NT packed terms of the cache's type, each the rounding of what
@@ -239,73 +275,40 @@ __device__ __forceinline__ f32x4_t mfma32(u32x4_t a, u32x4_t b, f32x4_t c) {
 constexpr float kLazyMax = 8.0f;   // a row's running maximum is raised only past 2^8
 template <int KV_F16> constexpr float kShift = KV_F16 ? 7.0f : 0.0f;   // (p <= 2^(8 + 7) < 65504)
 
-// Head q row of lane l's MFMA column n = l % 16, in the operand order of a
-// 16x16x32 product: lane group kb = l / 16 holds dims 32 jj + 8 kb + e. The
-// RMS sums over the four groups; the rotation's partner of dim d < 32 is jj = 1
-// of the same lane. cs / sn: cos and sin of angle 8 kb + e.
-template <int KV_F16, int NT>
-__device__ __forceinline__ void q_operand(float (&x)[8][8], const float* __restrict__ w, int kb, float eps,
-                                          const float (&cs)[8], const float (&sn)[8], u32x4_t (&q)[NT][8]) {
-    float ss = 0.0f;
-#pragma unroll
-    for (int jj = 0; jj < 8; ++jj)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss += x[jj][e] * x[jj][e];
-    ss += __shfl_xor(ss, 16, 64);
-    ss += __shfl_xor(ss, 32, 64);
-    const float inv = 1.0f / sqrtf(ss / 256.0f + eps);
-#pragma unroll
-    for (int jj = 0; jj < 8; ++jj) {
-        float wv[8];
-        load8<0>(w, 32 * jj + 8 * kb, wv);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[jj][e] = x[jj][e] * inv * wv[e];
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float a = x[0][e], b = x[1][e];
-        x[0][e] = a * cs[e] - b * sn[e];
-        x[1][e] = b * cs[e] + a * sn[e];
-    }
-#pragma unroll
-    for (int jj = 0; jj < 8; ++jj)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t t[NT];
-            split_terms<KV_F16, NT>(x[jj][2 * i], x[jj][2 * i + 1], t);
-#pragma unroll
-            for (int k = 0; k < NT; ++k) q[k][jj][i] = t[k];
-        }
-}
-
 struct PagedPartials {
     float* m;   // [slots][8]
     float* d;   // [slots][8]
     float* o;   // [slots][8][256]
-    int cstride;   // slots per (sequence, kv head): the shared chunks first, then its own
+    int32_t* count;   // [batch] partials of a sequence, per kv head (not written where the length is 0)
+    int cstride;      // slots per (sequence, kv head): the shared chunks first, then its own
 };
 
 // ---- partial ------------------------------------------------------------------------
 //
-// grid 2 x items, 512 threads: kv head u & 1 of item u >> 1. A block of up to
-// 2 R sequences (R a power of two <= 8) has R row blocks of 16 q rows (two
-// sequences x 8 heads); a single sequence fills half of one. Tiles of 64
+// grid 2 x items, 512 threads: kv head u & 1 of item u >> 1. Tiles of 64
 // positions of K and V are copied straight into LDS (two stages of 64 KB,
-// XOR-swizzled rows), the next one while a tile computes. Wave w takes row
-// block w % R: all 64 positions where R = 8, and otherwise half w / R of them
-// (waves past 2 R only copy); the halves are merged at the end through LDS. Per
-// 32 positions a wave reads 16 KB of K and 16 KB of V operands for 32 NT MFMAs:
+// XOR-swizzled rows), the next one while a tile computes.
+//   A block of up to 2 R sequences (R a power of two <= 8) has R row blocks of
+//   16 q rows (two sequences x 8 heads): wave w takes row block w % R, and all
+//   64 positions where R = 8, otherwise half w / R of them. Per 32 positions a
+//   wave reads 16 KB of K and 16 KB of V operands for 32 NT MFMAs.
+//   A single sequence's 8 rows: waves 0-3 take 16 positions each, the products
+//   of two terms in one MFMA (see single_step).
+// Waves beyond these only copy. In both
 //   S^T = K Q^T   A = K rows (b128 reads), B = q in registers; a lane's scores
 //                 belong to its one q row, positions 16 b + 4 kb + i
-//   O^T = V^T P^T A = V^T through two transposed reads (positions 4 kb + i and
-//                 16 + 4 kb + i: the order the lane's weights are in), B = P.
-// The chunk that ends with the new token norms and rotates k (wave 2) and takes
-// v (wave 3), writes both to their page and, once the tile that holds the
+//   O^T = V^T P^T A = V^T through transposed reads (positions 4 kb + i of each
+//                 16: the order the lane's weights are in), B = P.
+// The waves' parts of a row are joined at the end.
+// The chunk that ends with the new token norms and rotates k (wave 4), takes v
+// (wave 5), writes both to their page and, once the tile that holds the
 // position is in LDS, into its rows there; the rows behind them are zeroed
 // (what the page holds there may be any bit pattern).
 struct PartLds {
     uint16_t tile[2][2][kTile * 256];   // stage, K / V
-    float md[8][16][2];                 // the second halves' (m, d)
+    float md[8][16][2];                 // per wave and row (m, d)
+    __attribute__((aligned(16))) float sq[4][16][8];   // sums of squares: row block, row, slice of 32 dims
+    __attribute__((aligned(16))) float2 turn[4][64];   // row block, angle of the two sequences: cos, sin
 };
 
 __device__ __forceinline__ int tile_swz(int r) { return ((r & 7) << 1) | ((r >> 3) & 1); }
@@ -338,7 +341,6 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
     const int32_t* row = kv.table + static_cast<size_t>(lead) * kv.cols;
     const int last_entry = (p_end - 1) >> kv.lg;
     PageWindow win;
-    win.load(row, p_begin >> kv.lg, last_entry, kv.num_pages, lane);
 
     // tile t into stage t & 1: wave wv copies rows 2 wv + 16 i, + 1 of K and V,
     // i < 4; 16 positions past the chunk's end repeat its last ones (masked;
@@ -347,7 +349,7 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
     auto issue = [&](int t) -> unsigned {
         const int t0 = p_begin + t * kTile;
         if ((min(t0 + kTile, p_end) - 1) >> kv.lg > win.base + 63)
-            win.load(row, t0 >> kv.lg, last_entry, kv.num_pages, lane);
+            win.set(t0 >> kv.lg, PageWindow::entry(row, t0 >> kv.lg, last_entry, lane), kv.num_pages);
         unsigned bad = 0;
         const int h = lane >> 5;
         const uint32_t lt = 1024u * h + 16u * ((lane & 31) ^ (2 * h) ^ tile_swz(2 * wv & 15));
@@ -362,78 +364,228 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
         }
         return bad;
     };
-    unsigned bad_next = issue(0);
-
-    // ---- this wave's q rows ---------------------------------------------------
     const int n = lane & 15, kb = lane >> 4;
     const int nrb = (count + 1) / 2;
     const int R = nrb <= 1 ? 1 : nrb <= 2 ? 2 : nrb <= 4 ? 4 : 8;
-    const int halves = R == 8 ? 1 : 2;
-    const int rb = wv & (R - 1), half = wv / R;
-    const bool active = half < halves && rb < nrb;
-    const int seq = lead + min(2 * rb + (n >> 3), count - 1);
-    u32x4_t q[NT][8];
-    u32x2_t fresh = u32x2_t{0u, 0u};   // dims 4 lane .. + 3 of the new k (wave 2) or v (wave 3)
-    if (active) {
+    const bool single = count == 1;
+    const int parts = single ? 4 : R == 8 ? 1 : 2;   // of a tile's positions, one a wave
+    const int rb = wv & (R - 1), part = wv / R;
+    const bool active = part < parts && rb < nrb;
+    const int seq = lead + min(2 * rb + (n >> 3), count - 1);   // of the lane's q row
+
+    // ---- q rows: RMS norm, rotation, terms, by all waves together and handed to
+    // the waves that use them through the second stage's LDS, in the operand
+    // order of a 16x16x32 product. Lane (n, kb) of wave w takes two pieces of
+    // four dims of row n of each row block: for kb = 0 the pairs 4 w + i and
+    // 32 + 4 w + i of the rotation, for the others dims 64 + 24 w + 8 (kb - 1) +
+    // i and 4 + i (turned by an angle of 0). Everything the start needs from
+    // memory is requested together and waited for once, ahead of the first
+    // tile's copies, which land while q is prepared.
+    u32x4_t q[NT][8];             // a block's: term, step of 32 dims
+    u32x4_t qs[(NT + 1) / 2][8];   // a single sequence's: term 2 k in columns l % 16 < 8, term 2 k + 1 in the others
+    u32x2_t fresh = u32x2_t{0u, 0u};   // dims 4 lane .. + 3 of the new k (wave 4) or v (wave 5)
+    unsigned bad_next = 0;
+    auto prepare = [&](auto rr, auto one) {
+        constexpr int RR = decltype(rr)::value;
+        constexpr bool ONE = decltype(one)::value;   // a single sequence
+        int entry0 = PageWindow::entry(row, p_begin >> kv.lg, last_entry, lane);
+        const int dim0 = kb == 0 ? 4 * wv : 56 + 24 * wv + 8 * kb, dim1 = kb == 0 ? 32 + 4 * wv : dim0 + 4;
+        float x[RR][8], w[8], kx[4];
+#pragma unroll
+        for (int r = 0; r < RR; ++r) {
+            const int s = lead + min(2 * r + (n >> 3), count - 1);
+            const size_t at = (static_cast<size_t>(s) * 16 + kvh * 8 + (n & 7)) * 512;
+            load4<IN_DT>(q_gate, at + dim0, &x[r][0]);
+            load4<IN_DT>(q_gate, at + dim1, &x[r][4]);
+        }
+        load4<0>(q_norm_w, dim0, &w[0]);
+        load4<0>(q_norm_w, dim1, &w[4]);
+        if constexpr (ONE) {   // (waves other than 4 and 5 do not use them)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                kx[i] = elem<IN_DT>::load(wv == 5 ? v_new : k_new, (static_cast<size_t>(lead) * 2 + kvh) * 256 + 4 * lane + i);
+        }
+        int pos_a = a.positions[lead + min(2 * min(wv, RR - 1) + (lane >> 5), count - 1)];
+        float freq = rf.f[lane & 31];   // (a load: the arguments lie in memory)
+        // (consumed here, so that no load is moved behind the copies, whose
+        // requests a later wait for it would wait for too)
+        asm volatile("" : "+v"(entry0), "+v"(pos_a), "+v"(freq));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            asm volatile("" : "+v"(w[e]));
+#pragma unroll
+            for (int r = 0; r < RR; ++r) asm volatile("" : "+v"(x[r][e]));
+        }
+        if constexpr (ONE) asm volatile("" : "+v"(kx[0]), "+v"(kx[1]), "+v"(kx[2]), "+v"(kx[3]));
+        win.set(p_begin >> kv.lg, entry0, kv.num_pages);
+        bad_next = issue(0);
+        // cos, sin of angle l % 32 of row block wv's sequence l / 32
+        if (wv < RR) {
+            float s, c2;
+            sincosf(static_cast<float>(pos_a) * freq, &s, &c2);
+            L.turn[wv][lane] = make_float2(c2, s);
+        }
+#pragma unroll
+        for (int r = 0; r < RR; ++r) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss += x[r][e] * x[r][e];
+            ss = quad_sum(ss);
+            if (kb == 0) L.sq[r][n][wv] = ss;
+        }
+        __syncthreads();
+        constexpr int kAtOnce = RR < 8 / NT ? RR : 8 / NT;   // row blocks that 64 KB hold
+        u32x4_t* const hand = reinterpret_cast<u32x4_t*>(L.tile[1]);
+        // piece of four dims d ..: step d / 32, lane 16 (d % 32 / 8) + n, half d % 8 / 4
+        auto piece = [&](int d) { return 2 * (64 * (d >> 5) + 16 * ((d >> 3) & 3) + n) + ((d >> 2) & 1); };
+        u32x2_t* const half0 = reinterpret_cast<u32x2_t*>(hand) + piece(dim0);
+        u32x2_t* const half1 = reinterpret_cast<u32x2_t*>(hand) + piece(dim1);
+#pragma unroll
+        for (int r0 = 0; r0 < RR; r0 += kAtOnce) {
+#pragma unroll
+            for (int r = r0; r < r0 + kAtOnce; ++r) {
+                const f32x4_t a0 = *reinterpret_cast<const f32x4_t*>(&L.sq[r][n][0]);
+                const f32x4_t a1 = *reinterpret_cast<const f32x4_t*>(&L.sq[r][n][4]);
+                const float ss = ((a0[0] + a0[1]) + (a0[2] + a0[3])) + ((a1[0] + a1[1]) + (a1[2] + a1[3]));
+                const float inv = inv_rms(ss, eps);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[r][e] = x[r][e] * inv * w[e];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float2 cs = L.turn[r][32 * (n >> 3) + 4 * wv + i];
+                    if (kb != 0) cs = make_float2(1.0f, 0.0f);
+                    const float lo = x[r][i], hi = x[r][4 + i];
+                    x[r][i] = lo * cs.x - hi * cs.y;
+                    x[r][4 + i] = hi * cs.x + lo * cs.y;
+                }
+                uint32_t t[4][NT];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) split_terms<KV_F16, NT>(x[r][2 * i], x[r][2 * i + 1], t[i]);
+#pragma unroll
+                for (int k = 0; k < NT; ++k) {
+                    half0[((r - r0) * NT + k) * 1024] = u32x2_t{t[0][k], t[1][k]};
+                    half1[((r - r0) * NT + k) * 1024] = u32x2_t{t[2][k], t[3][k]};
+                }
+            }
+            __syncthreads();
+            if constexpr (ONE) {
+                const int from = 16 * kb + (n & 7);
+#pragma unroll
+                for (int k = 0; k < (NT + 1) / 2; ++k)
+#pragma unroll
+                    for (int jj = 0; jj < 8; ++jj) {
+                        const u32x4_t v = hand[(min(2 * k + (n >> 3), NT - 1) * 8 + jj) * 64 + from];
+                        qs[k][jj] = 2 * k + (n >> 3) < NT ? v : u32x4_t{0u, 0u, 0u, 0u};
+                    }
+            } else if (active && rb >= r0 && rb < r0 + kAtOnce) {
+#pragma unroll
+                for (int k = 0; k < NT; ++k)
+#pragma unroll
+                    for (int jj = 0; jj < 8; ++jj) q[k][jj] = hand[(((rb - r0) * NT + k) * 8 + jj) * 64 + lane];
+            }
+            if (r0 + kAtOnce < RR) __syncthreads();
+        }
+        if constexpr (ONE) {
+            if (has_new && (wv == 4 || wv == 5)) {
+                // dims 4 lane .. + 3; the rotation's partner of dim d < 32 is d + 32, 8 lanes on
+                if (wv == 4) {
+                    float ss = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) ss += kx[i] * kx[i];
+                    const float inv = 1.0f / sqrtf(group_sum<64>(ss) / 256.0f + eps);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) kx[i] = kx[i] * inv * k_norm_w[4 * lane + i];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float up = __shfl_down(kx[i], 8, 64), dn = __shfl_up(kx[i], 8, 64);
+                        const int d = 4 * lane + i;
+                        const float2 cs = L.turn[0][d & 31];
+                        if (d < 64) kx[i] = d < 32 ? kx[i] * cs.x - up * cs.y : kx[i] * cs.x + dn * cs.y;
+                    }
+                }
+                uint32_t w0[1], w1[1];
+                split_terms<KV_F16, 1>(kx[0], kx[1], w0);
+                split_terms<KV_F16, 1>(kx[2], kx[3], w1);
+                fresh = u32x2_t{w0[0], w1[0]};
+                const int page = row[last_entry];   // (the chunk ends with the new token)
+                if (page >= 0 && page < kv.num_pages) {   // (dropped where the page lies outside the pool)
+                    const size_t off = ((static_cast<size_t>(page) << kv.lg) + ((plan.len - 1) & mask)) * 512 + kvh * 256 + 4 * lane;
+                    *reinterpret_cast<u32x2_t*>((wv == 4 ? kv.k : kv.v) + off) = fresh;
+                }
+            }
+        }
+    };
+    // Eight row blocks: each wave its own, without the hand-over.
+    auto prepare_own = [&]() {
+        int entry0 = PageWindow::entry(row, p_begin >> kv.lg, last_entry, lane);
         float x[8][8];
         const size_t qbase = (static_cast<size_t>(seq) * 16 + kvh * 8 + (n & 7)) * 512 + 8 * kb;
 #pragma unroll
         for (int jj = 0; jj < 8; ++jj) load8<IN_DT>(q_gate, qbase + 32 * jj, x[jj]);
-        // lane l: angle l % 32 of the row block's sequence l / 32
-        const int s2 = lead + min(2 * rb + (lane >> 5), count - 1);
-        const float ang = static_cast<float>(a.positions[s2]) * rf.f[lane & 31];
-        const float cl = cosf(ang), sl = sinf(ang);
-        float cs[8], sn[8];
+        int pos_a = a.positions[lead + min(2 * rb + (lane >> 5), count - 1)];
+        float freq = rf.f[lane & 31], w[8][8];
+#pragma unroll
+        for (int jj = 0; jj < 8; ++jj) load8<0>(q_norm_w, 32 * jj + 8 * kb, w[jj]);
+        asm volatile("" : "+v"(entry0), "+v"(pos_a), "+v"(freq));
+#pragma unroll
+        for (int jj = 0; jj < 8; ++jj)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(x[jj][e]), "+v"(w[jj][e]));
+        win.set(p_begin >> kv.lg, entry0, kv.num_pages);
+        bad_next = issue(0);
+        float cl, sl, cs[8], sn[8], ss = 0.0f;   // lane l: angle l % 32 of the row block's sequence l / 32
+        sincosf(static_cast<float>(pos_a) * freq, &sl, &cl);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int from = 32 * (n >> 3) + 8 * kb + e;
             cs[e] = __shfl(cl, from, 64);
             sn[e] = __shfl(sl, from, 64);
         }
-        q_operand<KV_F16, NT>(x, q_norm_w, kb, eps, cs, sn, q);
-    } else if (has_new && (wv == 2 || wv == 3)) {
-        // dims 4 lane .. + 3; the rotation's partner of dim d < 32 is d + 32, 8 lanes on
-        const size_t at = (static_cast<size_t>(lead) * 2 + kvh) * 256 + 4 * lane;
-        float x[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = elem<IN_DT>::load(wv == 2 ? k_new : v_new, at + i);
-        if (wv == 2) {
-            const float ang = static_cast<float>(plan.len - 1) * rf.f[lane & 31];
-            const float cl = cosf(ang), sl = sinf(ang);
-            float ss = 0.0f;
+        for (int jj = 0; jj < 8; ++jj)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ss += x[i] * x[i];
-            const float inv = 1.0f / sqrtf(group_sum<64>(ss) / 256.0f + eps);
+            for (int e = 0; e < 8; ++e) {
+                ss += x[jj][e] * x[jj][e];
+                x[jj][e] *= w[jj][e];   // (here, so that w's registers are free before q's are filled)
+                asm volatile("" : "+v"(x[jj][e]));
+            }
+        const float inv = inv_rms(quad_sum(ss), eps);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = x[i] * inv * k_norm_w[4 * lane + i];
+        for (int e = 0; e < 8; ++e) {
+            const float lo = x[0][e] * inv, hi = x[1][e] * inv;
+            x[0][e] = lo * cs[e] - hi * sn[e];
+            x[1][e] = hi * cs[e] + lo * sn[e];
+        }
+#pragma unroll
+        for (int jj = 0; jj < 8; ++jj)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float up = __shfl_down(x[i], 8, 64), dn = __shfl_up(x[i], 8, 64);
-                const float ci = __shfl(cl, (4 * lane + i) & 31, 64), si = __shfl(sl, (4 * lane + i) & 31, 64);
-                const int d = 4 * lane + i;
-                if (d < 64) x[i] = d < 32 ? x[i] * ci - up * si : x[i] * ci + dn * si;
+                uint32_t t[NT];
+                const float f = jj < 2 ? 1.0f : inv;
+                split_terms<KV_F16, NT>(x[jj][2 * i] * f, x[jj][2 * i + 1] * f, t);
+#pragma unroll
+                for (int k = 0; k < NT; ++k) q[k][jj][i] = t[k];
             }
-        }
-        uint32_t w0[1], w1[1];
-        split_terms<KV_F16, 1>(x[0], x[1], w0);
-        split_terms<KV_F16, 1>(x[2], x[3], w1);
-        fresh = u32x2_t{w0[0], w1[0]};
-        const int page = row[(plan.len - 1) >> kv.lg];
-        if (page >= 0 && page < kv.num_pages) {   // (dropped where the page lies outside the pool)
-            const size_t off = ((static_cast<size_t>(page) << kv.lg) + ((plan.len - 1) & mask)) * 512 + kvh * 256 + 4 * lane;
-            *reinterpret_cast<u32x2_t*>((wv == 2 ? kv.k : kv.v) + off) = fresh;
-        }
-    }
+    };
+    if (has_new && kvh == 0 && threadIdx.x == 0) pp.count[lead] = slot_c + 1;   // the sequence's last partial
 
     float m_run = -INFINITY, d_run = 0.0f;
     f32x4_t oacc[16];   // O^T: dims 16 dt + 4 kb + i of the lane's row
+    auto clear = [&] {
 #pragma unroll
-    for (int dt = 0; dt < 16; ++dt) oacc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int dt = 0; dt < 16; ++dt) oacc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    };
     const float sc = scale * 1.44269504088896341f;
     const uint32_t kaddr = 512u * n + 16u * (kb ^ tile_swz(n));
     const int vr = 4 * kb + (n >> 2);
     const uint32_t vaddr = 512u * vr + 16u * (((n >> 1) & 1) ^ tile_swz(vr)) + 8u * (n & 1);
 
+    // a ^ x next to its use: hoisted out of the loop, the operands' 24 addresses would not fit the registers
+    auto at_xor = [](uint32_t a, uint32_t x) {
+        uint32_t r;
+        asm volatile("v_xor_b32 %0, %1, %2" : "=v"(r) : "s"(x), "v"(a));
+        return r;
+    };
     auto lds128 = [](uint32_t at) {
         return *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(static_cast<uintptr_t>(at));
     };
@@ -442,142 +594,246 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
         return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                                (s16x4_l __attribute__((address_space(3)))*)(static_cast<uintptr_t>(at))));
     };
+    // the running maximum of the lane's row against this tile's, in all four lanes of the row
+    auto raise = [&](float tm) {
+        tm = fmaxf(tm, swizzle_xor16(tm));
+        const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(tm), __float_as_uint(tm), false, false);
+        tm = fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
+        if (__any(tm > m_run + kLazyMax)) {
+            const float m_new = tm > m_run + kLazyMax ? tm : m_run;
+            const float alpha = m_new == m_run ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+            m_run = m_new;
+            d_run *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < 16; ++dt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) oacc[dt][i] *= alpha;
+        }
+    };
+    // 32 positions (s0 ..) of a block's row block; sub: which half of the tile
+    auto block_step = [&](uint32_t kt, uint32_t vt, int s0, int sub, unsigned bad) {
+        const uint32_t ka = kt + 16384u * sub + kaddr, va0 = vt + 16384u * sub + vaddr;   // (tiles lie at multiples of 32 KB)
+        f32x4_t s[2][NT];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int k = 0; k < NT; ++k) s[b][k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        // operands two steps ahead of their products (further, and their registers spill)
+        u32x4_t kf[3][2];
+        auto k_read = [&](int jj) {
+            const uint32_t at = at_xor(ka, 64u * jj);
+            kf[jj % 3][0] = lds128(at);
+            kf[jj % 3][1] = lds128(at + 8192u);
+        };
+        k_read(0);
+        k_read(1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int jj = 0; jj < 8; ++jj) {
+            if (jj + 2 < 8) k_read(jj + 2);
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int k = 0; k < NT; ++k) s[b][k] = mfma32<KV_F16>(kf[jj % 3][b], q[k][jj], s[b][k]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        u32x2_t vf[4][2];
+        auto v_read = [&](int dt) {
+            const uint32_t at = at_xor(va0, 32u * dt);
+            vf[dt % 4][0] = lds_tr(at);
+            vf[dt % 4][1] = lds_tr(at + 8192u);
+        };
+#pragma unroll
+        for (int dt = 0; dt < 3; ++dt) v_read(dt);
+        float x[2][4];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float v = s[b][0][i];
+#pragma unroll
+                for (int k = 1; k < NT; ++k) v += s[b][k][i];
+                x[b][i] = v * sc;
+            }
+        if (s0 + 32 > p_end || (bad >> (2 * sub) & 3)) {   // (uniform)
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    x[b][i] = s0 + 16 * b + 4 * kb + i >= p_end ? -INFINITY
+                              : (bad >> (2 * sub + b)) & 1     ? __builtin_nanf("")
+                                                               : x[b][i];
+        }
+        raise(fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
+                    fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3]))));
+        const float mb = m_run - kShift<KV_F16>;
+        u32x4_t pw[NT];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                const float e0 = __builtin_amdgcn_exp2f(x[b][i] - mb), e1 = __builtin_amdgcn_exp2f(x[b][i + 1] - mb);
+                d_run += e0 + e1;
+                uint32_t w[NT];
+                split_terms<KV_F16, NT>(e0, e1, w);
+#pragma unroll
+                for (int k = 0; k < NT; ++k) pw[k][2 * b + i / 2] = w[k];
+            }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int dt = 0; dt < 16; ++dt) {
+            if (dt + 3 < 16) v_read(dt + 3);
+            const u32x2_t v0 = vf[dt % 4][0], v1 = vf[dt % 4][1];
+#pragma unroll
+            for (int k = 0; k < NT; ++k) oacc[dt] = mfma32<KV_F16>(u32x4_t{v0[0], v0[1], v1[0], v1[1]}, pw[k], oacc[dt]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // 16 positions (s0 ..) of a single sequence, whose 8 heads leave 8 columns
+    // free: q's second term scores in those, lanes n and n ^ 8 add up. The
+    // weights' first two terms share one product along its 32 positions (V's 16
+    // rows twice), a third takes the free columns.
+    auto single_step = [&](uint32_t kt, uint32_t vt, int s0, bool bad) {
+        const uint32_t ka = kt + 8192u * part + kaddr, va0 = vt + 8192u * part + vaddr;
+        f32x4_t s[(NT + 1) / 2];
+#pragma unroll
+        for (int k = 0; k < (NT + 1) / 2; ++k) s[k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int jj = 0; jj < 8; ++jj) {
+            const u32x4_t kf = lds128(at_xor(ka, 64u * jj));
+#pragma unroll
+            for (int k = 0; k < (NT + 1) / 2; ++k) s[k] = mfma32<KV_F16>(kf, qs[k][jj], s[k]);
+        }
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float v = s[0][i];
+            if constexpr (NT == 3) v += s[1][i];
+            x[i] = (v + dpp_mov<0x128>(v)) * sc;   // row_ror:8
+        }
+        if (s0 + 16 > p_end || bad) {   // (uniform)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                x[i] = s0 + 4 * kb + i >= p_end ? -INFINITY : bad ? __builtin_nanf("") : x[i];
+        }
+        raise(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+        const float mb = m_run - kShift<KV_F16>;
+        uint32_t w0[NT], w1[NT];
+        const float e0 = __builtin_amdgcn_exp2f(x[0] - mb), e1 = __builtin_amdgcn_exp2f(x[1] - mb);
+        const float e2 = __builtin_amdgcn_exp2f(x[2] - mb), e3 = __builtin_amdgcn_exp2f(x[3] - mb);
+        d_run += (e0 + e1) + (e2 + e3);
+        split_terms<KV_F16, NT>(e0, e1, w0);
+        split_terms<KV_F16, NT>(e2, e3, w1);
+        u32x4_t pw = u32x4_t{w0[0], w1[0], NT > 1 ? w0[NT > 1] : 0u, NT > 1 ? w1[NT > 1] : 0u};
+        if (n >= 8) pw = NT == 3 ? u32x4_t{w0[NT - 1], w1[NT - 1], 0u, 0u} : u32x4_t{0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int dt = 0; dt < 16; ++dt) {
+            const u32x2_t v = lds_tr(at_xor(va0, 32u * dt));
+            oacc[dt] = mfma32<KV_F16>(u32x4_t{v[0], v[1], v[0], v[1]}, pw, oacc[dt]);
+        }
+    };
 
-    for (int t = 0; t < ntiles; ++t) {
+    auto arrive = [&](int t) {   // tile t is in LDS, and the other stage's readers are done
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();   // the tile is in LDS, and the other stage's readers are done
-        const unsigned bad = bad_next;
-        const int t0 = p_begin + t * kTile;
-        if (t + 1 < ntiles) {
-            bad_next = issue(t + 1);
-        } else if (has_new) {
-            // the new token's row, and zeros behind it in the 32 positions it is among
-            const int r = plan.len - 1 - t0, end = (r | 31) + 1;
-            auto at = [&](int which, int rr) {
-                return reinterpret_cast<u32x2_t*>(&L.tile[t & 1][which][rr * 256 + 8 * ((lane >> 1) ^ tile_swz(rr)) + 4 * (lane & 1)]);
-            };
-            if (wv == 2 || wv == 3) *at(wv - 2, r) = fresh;
-            for (int z = r + 1 + wv; z < end; z += 8) *at(1, z) = u32x2_t{0u, 0u};
-            __syncthreads();
+        __syncthreads();
+    };
+    if (single) {
+        prepare(std::integral_constant<int, 1>{}, std::true_type{});
+        clear();
+        for (int t = 0; t < ntiles; ++t) {
+            arrive(t);
+            const unsigned bad = bad_next;
+            const int t0 = p_begin + t * kTile;
+            if (t + 1 < ntiles) {
+                bad_next = issue(t + 1);
+            } else if (has_new) {
+                // the new token's row, and zeros behind it in the 16 positions it is among
+                const int r = plan.len - 1 - t0, end = (r | 15) + 1;
+                auto at = [&](int which, int rr) {
+                    return reinterpret_cast<u32x2_t*>(
+                        &L.tile[t & 1][which][rr * 256 + 8 * ((lane >> 1) ^ tile_swz(rr)) + 4 * (lane & 1)]);
+                };
+                if (wv == 4 || wv == 5) *at(wv - 4, r) = fresh;
+                for (int z = r + 1 + wv; z < end; z += 8) *at(1, z) = u32x2_t{0u, 0u};
+                __syncthreads();
+            }
+            if (active && t0 + 16 * part < p_end)
+                single_step(lds_addr(L.tile[t & 1][0]), lds_addr(L.tile[t & 1][1]), t0 + 16 * part, (bad >> part) & 1);
         }
-        if (!active) continue;
-        const uint32_t kt = lds_addr(L.tile[t & 1][0]), vt = lds_addr(L.tile[t & 1][1]);
+    } else {
+        if (R == 1) prepare(std::integral_constant<int, 1>{}, std::false_type{});
+        else if (R == 2) prepare(std::integral_constant<int, 2>{}, std::false_type{});
+        else if (R == 4) prepare(std::integral_constant<int, 4>{}, std::false_type{});
+        else prepare_own();
+        clear();
+        for (int t = 0; t < ntiles; ++t) {
+            arrive(t);
+            const unsigned bad = bad_next;
+            const int t0 = p_begin + t * kTile;
+            if (t + 1 < ntiles) bad_next = issue(t + 1);
+            if (!active) continue;
 #pragma unroll 1
-        for (int u = 0; u < 3 - halves; ++u) {
-            const int sub = halves == 2 ? half : u;
-            const int s0 = t0 + 32 * sub;
-            if (s0 >= p_end) break;
-            f32x4_t s[2][NT];
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int k = 0; k < NT; ++k) s[b][k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int jj = 0; jj < 8; ++jj)
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const u32x4_t kf = lds128(kt + 16384u * sub + 8192u * b + (kaddr ^ (64u * jj)));
-#pragma unroll
-                    for (int k = 0; k < NT; ++k) s[b][k] = mfma32<KV_F16>(kf, q[k][jj], s[b][k]);
-                }
-            // softmax in base 2
-            const bool cut = s0 + 32 > p_end || (bad >> (2 * sub) & 3);   // (uniform)
-            float x[2][4];
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float v = s[b][0][i];
-#pragma unroll
-                    for (int k = 1; k < NT; ++k) v += s[b][k][i];
-                    x[b][i] = v * sc;
-                }
-            if (cut) {
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        x[b][i] = s0 + 16 * b + 4 * kb + i >= p_end ? -INFINITY
-                                  : (bad >> (2 * sub + b)) & 1     ? __builtin_nanf("")
-                                                                   : x[b][i];
-            }
-            float tm = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
-                             fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-            tm = fmaxf(tm, __shfl_xor(tm, 16, 64));
-            tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
-            if (__any(tm > m_run + kLazyMax)) {
-                const float m_new = tm > m_run + kLazyMax ? tm : m_run;
-                const float alpha = m_new == m_run ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
-                m_run = m_new;
-                d_run *= alpha;
-#pragma unroll
-                for (int dt = 0; dt < 16; ++dt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) oacc[dt][i] *= alpha;
-            }
-            const float mb = m_run - kShift<KV_F16>;
-            u32x4_t pw[NT];
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; i += 2) {
-                    const float e0 = __builtin_amdgcn_exp2f(x[b][i] - mb), e1 = __builtin_amdgcn_exp2f(x[b][i + 1] - mb);
-                    d_run += e0 + e1;
-                    uint32_t w[NT];
-                    split_terms<KV_F16, NT>(e0, e1, w);
-#pragma unroll
-                    for (int k = 0; k < NT; ++k) pw[k][2 * b + i / 2] = w[k];
-                }
-#pragma unroll
-            for (int dt = 0; dt < 16; ++dt) {
-                const uint32_t va = vt + 16384u * sub + (vaddr ^ (32u * dt));
-                const u32x2_t v0 = lds_tr(va), v1 = lds_tr(va + 8192u);
-                const u32x4_t vf = u32x4_t{v0[0], v0[1], v1[0], v1[1]};
-#pragma unroll
-                for (int k = 0; k < NT; ++k) oacc[dt] = mfma32<KV_F16>(vf, pw[k], oacc[dt]);
-            }
+            for (int sub = parts == 2 ? part : 0; sub < (parts == 2 ? part + 1 : 2); ++sub)
+                if (t0 + 32 * sub < p_end)
+                    block_step(lds_addr(L.tile[t & 1][0]), lds_addr(L.tile[t & 1][1]), t0 + 32 * sub, sub, bad);
         }
     }
-    d_run += __shfl_xor(d_run, 16, 64);
-    d_run += __shfl_xor(d_run, 32, 64);
-    // ---- the second halves handed over in LDS, one 16-byte piece a lane and dim tile
-    if (halves == 2) {   // (uniform over the workgroup)
-        __syncthreads();
-        f32x4_t* hand = reinterpret_cast<f32x4_t*>(&L) + rb * 1024;
-        if (active && half == 1) {
+    d_run = quad_sum(d_run);
+    // ---- the parts joined through LDS (16 KB a wave, in place of the tiles), by
+    // all waves, a row of 256 dims by 64 lanes: piece (dt, kb) of row n lies at
+    // 64 dt + 16 kb + (n ^ dt), so that neither side meets a bank twice
+    f32x4_t* const hand = reinterpret_cast<f32x4_t*>(L.tile);
+    __syncthreads();
+    if (active) {
+        if (NT == 3 && single) {
 #pragma unroll
-            for (int dt = 0; dt < 16; ++dt) hand[64 * dt + lane] = oacc[dt];
-            if (kb == 0) {
-                L.md[rb][n][0] = m_run;
-                L.md[rb][n][1] = d_run;
-            }
+            for (int dt = 0; dt < 16; ++dt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) oacc[dt][i] += dpp_mov<0x128>(oacc[dt][i]);
         }
-        __syncthreads();
-        if (active && half == 0) {
-            const float m1 = L.md[rb][n][0], d1 = L.md[rb][n][1];
-            const float m = fmaxf(m_run, m1);
-            // (a half without any position, or whose scores are all NaN, has maximum -inf)
-            const float f0 = m_run == m ? 1.0f : __builtin_amdgcn_exp2f(m_run - m);
-            const float f1 = m1 == m ? 1.0f : __builtin_amdgcn_exp2f(m1 - m);
-            m_run = m;
-            d_run = d_run * f0 + d1 * f1;
 #pragma unroll
-            for (int dt = 0; dt < 16; ++dt) {
-                const f32x4_t o = hand[64 * dt + lane];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) oacc[dt][i] = oacc[dt][i] * f0 + o[i] * f1;
-            }
+        for (int dt = 0; dt < 16; ++dt)
+            if (!single || n < 8) hand[1024 * wv + 64 * dt + 16 * kb + (n ^ dt)] = oacc[dt];
+        if (kb == 0) {
+            L.md[wv][n][0] = m_run;
+            L.md[wv][n][1] = d_run;
         }
     }
-    if (!active || half != 0 || 2 * rb + (n >> 3) >= count) return;
-    const size_t slot = (static_cast<size_t>(seq) * 2 + kvh) * pp.cstride + slot_c;
-    if (kb == 0) {
-        pp.m[slot * 8 + (n & 7)] = m_run - kShift<KV_F16>;
-        pp.d[slot * 8 + (n & 7)] = d_run;
-    }
-    float* o = pp.o + (slot * 8 + (n & 7)) * 256 + 4 * kb;
+    __syncthreads();
+    auto join = [&](auto pc) {
+        constexpr int PARTS = decltype(pc)::value;
+        const int rows = 8 * count;
+#pragma unroll 4
+        for (int r = wv; r < rows; r += 8) {   // row r: row r % 16 of row block r / 16
+            const int from = r >> 4, rn = r & 15, piece = 64 * (lane >> 2) + 16 * (lane & 3) + (rn ^ (lane >> 2));
+            float mk[PARTS], m = -INFINITY, d = 0.0f;
+            f32x4_t v[PARTS], o = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int dt = 0; dt < 16; ++dt) *reinterpret_cast<f32x4_t*>(o + 16 * dt) = oacc[dt];
+            for (int k = 0; k < PARTS; ++k) {
+                mk[k] = L.md[from + R * k][rn][0];
+                v[k] = hand[1024 * (from + R * k) + piece];
+            }
+#pragma unroll
+            for (int k = 0; k < PARTS; ++k) m = fmaxf(m, mk[k]);
+#pragma unroll
+            for (int k = 0; k < PARTS; ++k) {
+                // (a part without any position, or whose scores are all NaN, has maximum -inf)
+                const float f = mk[k] == m ? 1.0f : __builtin_amdgcn_exp2f(mk[k] - m);
+                d += f * L.md[from + R * k][rn][1];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] += f * v[k][i];
+            }
+            const size_t slot = (static_cast<size_t>(lead + (r >> 3)) * 2 + kvh) * pp.cstride + slot_c;
+            if (lane == 0) {
+                pp.m[slot * 8 + (r & 7)] = m - kShift<KV_F16>;
+                pp.d[slot * 8 + (r & 7)] = d;
+            }
+            *reinterpret_cast<f32x4_t*>(pp.o + (slot * 8 + (r & 7)) * 256 + 4 * lane) = o;
+        }
+    };
+    if (single) join(std::integral_constant<int, 4>{});
+    else if (parts == 2) join(std::integral_constant<int, 2>{});
+    else join(std::integral_constant<int, 1>{});
 }
 
 // ---- combine ----------------------------------------------------------------------------
@@ -585,11 +841,13 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
 // grid (16 q heads x DS dim blocks, batch), 512 threads, 256 / DS dims a
 // workgroup: chunk weights one thread a chunk; 8 DS streams of float4 lanes,
 // stream s adding chunks s, s + 8 DS, ... in order, then the streams in a fixed
-// order (results do not depend on timing). The (m, d) of every slot and the
-// gate are requested before the split is known, and a stream's first four rows
-// before the weights; every load is unconditional, its index clamped.
+// order (results do not depend on timing). The (m, d) of every slot, the
+// gate, and the number of partials (which the partial launch leaves, so that
+// the split is not derived again) are requested together, and a stream's first
+// four rows before the weights; every load is unconditional, its index clamped.
 template <int IN_DT, int OUT_DT, int DS>
-__global__ __launch_bounds__(512) void gqa_paged_combine_kernel(const void* __restrict__ q_gate, PagedSeqs a,
+__global__ __launch_bounds__(512) void gqa_paged_combine_kernel(const void* __restrict__ q_gate,
+                                                                const int32_t* __restrict__ positions, int max_ctx,
                                                                 PagedPartials pp, void* __restrict__ out) {
     constexpr int kDims = 256 / DS, kLanes = 64 / DS, kStreams = 8 * DS, kRound = 4;
     __shared__ float es[kGqaMaxChunks], red[16];
@@ -603,16 +861,12 @@ __global__ __launch_bounds__(512) void gqa_paged_combine_kernel(const void* __re
     const float m_slot = pp.m[(base + ts) * 8 + hl];
     const float d_slot = pp.d[(base + ts) * 8 + hl];
     const float gate = elem<IN_DT>::load(q_gate, qi * 512 + 256 + d0 + min(t, kDims - 1));
-    const LanePlan p0 = lane_plan(a, 0, lane);
-    const int ch = chunk_length(a, p0, lane);
-    const LanePlan mine = seq < 64 ? p0 : lane_plan(a, seq & ~63, lane);
-    const int len = __builtin_amdgcn_readlane(mine.len, seq & 63);
-    const int shared = __builtin_amdgcn_readlane(mine.shared, seq & 63);
-    if (len == 0) {   // (uniform over the workgroup)
+    const int pos = positions[seq], listed = pp.count[seq];
+    if (pos < 0 || pos >= max_ctx) {   // (uniform over the workgroup)
         if (t < kDims) elem<OUT_DT>::store(out, qi * 256 + d0 + t, __builtin_nanf(""));
         return;
     }
-    const int nc = chunks_of(shared, ch) + chunks_of(len - shared, ch);   // <= cstride
+    const int nc = min(listed, pp.cstride);
     const int sid = wave * DS + lane / kLanes, f = lane % kLanes;
     const float4* pr = reinterpret_cast<const float4*>(pp.o + (base * 8 + hl) * 256 + d0) + f;
     float4 v[kRound];
@@ -671,7 +925,7 @@ hipError_t launch_gqa_decode_paged(qff_ctx* ctx, hipStream_t stream, const qff_g
                      kv->table_cols};
     const int cap = gqa_chunk_cap(ctx->cfg, batch);
     const PagedSeqs a{positions, group, shared_len, batch, kv->table_cols << lg, ctx->num_cu / 2, cap};
-    const PagedPartials pp{ctx->gqa_m, ctx->gqa_d, ctx->gqa_o, cap};
+    const PagedPartials pp{ctx->gqa_m, ctx->gqa_d, ctx->gqa_o, ctx->gqa_nc, cap};
     const RopeFreqs rf = rope_freqs(p->rope_theta);
     const bool f16 = p->kv_f16 != 0, in16 = in_dtype == QFF_BF16, out16 = out_dtype == QFF_BF16;
     {
@@ -695,8 +949,8 @@ hipError_t launch_gqa_decode_paged(qff_ctx* ctx, hipStream_t stream, const qff_g
     const int ds = batch <= 8 ? 4 : 1;   // small batches split each head's dims over four workgroups
     const dim3 cgrid(16 * ds, batch);
 #define QFF_COMB(I, O)                                                                                       \
-    if (ds == 4) gqa_paged_combine_kernel<I, O, 4><<<cgrid, 512, 0, stream>>>(q_gate, a, pp, out);           \
-    else gqa_paged_combine_kernel<I, O, 1><<<cgrid, 512, 0, stream>>>(q_gate, a, pp, out)
+    if (ds == 4) gqa_paged_combine_kernel<I, O, 4><<<cgrid, 512, 0, stream>>>(q_gate, positions, a.max_ctx, pp, out);           \
+    else gqa_paged_combine_kernel<I, O, 1><<<cgrid, 512, 0, stream>>>(q_gate, positions, a.max_ctx, pp, out)
     if (in16) {
         if (out16) { QFF_COMB(1, 1); } else { QFF_COMB(1, 0); }
     } else {

@@ -36,6 +36,7 @@ struct qff_ctx {
     float* gqa_m = nullptr;       // [gqa_slots(cfg) * 8]
     float* gqa_d = nullptr;       // same
     float* gqa_o = nullptr;       // [gqa_slots(cfg) * 8 * 256]
+    int32_t* gqa_nc = nullptr;    // paged decode: partials of each sequence [max_batch]
     // Full-attention prefill: normed, rotated q as bf16 [T][16][256].
     uint16_t* gqa_qb = nullptr;
     uint16_t* gqa_kv16 = nullptr;   // fp16 copy of a bf16 K cache for prefill: [max_ctx][2][256]
@@ -97,7 +98,7 @@ constexpr int kQ4SkSlots = 4096;       // (row tile, slice) partials of the spli
 constexpr int kSchedChunkLocal = 0;    // slot of the DeltaNet chunk-local pass
 
 struct WorkspaceLayout {
-    size_t gqa_m, gqa_d, gqa_o;
+    size_t gqa_m, gqa_d, gqa_o, gqa_nc;
     size_t gqa_qb, gqa_kv16, gqa_vt, q4_x16, q4_fm, q4_sk_part, pf_o, pf_md, dn_arrive, sched, kimg, qop, top, pop, gates, bv;
     size_t total;
 };
