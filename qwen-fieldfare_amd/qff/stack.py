@@ -15,7 +15,8 @@ its attention output back into it (Runner:1034-1040, 1162-1166):
 
 The residual stream and every intermediate are fp32, as the reference keeps
 them (hiddenBuf0/1, qkvOutBuf, ... are float buffers, Runner:346-401); the KV
-caches are bf16. Layers take the tensors Checkpoint.deltanet_layer /
+caches are bf16, one flat cache per sequence or, with a PageTable, pages of one
+pool per layer, which sequences that share a prefix hold together. Layers take the tensors Checkpoint.deltanet_layer /
 gqa_layer return, so a stack can come from a checkpoint or from synthetic
 weights of the same layout.
 """
@@ -39,15 +40,24 @@ class AttentionStack:
     attention); the kind follows l % 4 == 3 unless `kinds` says otherwise.
     States: DeltaNet conv [B, 8192, 4] / ssm [B, 32, 128, 128] fp32, full
     attention K / V caches [B, max_ctx, 2, 256] bf16; pass them in `states`
-    or get zero states."""
+    or get zero states.
+
+    With `pages` (a PageTable of `batch` slots), full attention keeps k_pages /
+    v_pages [num_pages, page_size, 2, 256] instead, slot b of the table is
+    sequence b, and sequences can be filled a prompt slice at a time (prefill),
+    forked, released and compacted. Before each decode step, captured or not,
+    reserve() gives the new tokens their places."""
 
     def __init__(self, ctx: ops.Context, layers, batch: int, max_ctx: int, states=None, kinds=None,
-                 eps: float = 1e-6, device="cuda"):
+                 eps: float = 1e-6, device="cuda", pages=None):
         self.ctx = ctx
         self.layers = list(layers)
         self.B = batch
         self.max_ctx = max_ctx
         self.eps = eps
+        self.pages = pages
+        if pages is not None and len(pages.lengths) != batch:
+            raise ValueError(f"the page table must have {batch} slots")
         self.kinds = list(kinds) if kinds is not None else \
             ["gqa" if is_full_attention(l) else "dn" for l in range(len(self.layers))]
         if states is None:
@@ -56,6 +66,10 @@ class AttentionStack:
                 if kind == "dn":
                     states.append({"conv_state": torch.zeros(batch, 8192, 4, device=device),
                                    "ssm_state": torch.zeros(batch, 32, 128, 128, device=device)})
+                elif pages is not None:
+                    shape = (len(pages.refs), pages.page_size, 2, 256)
+                    states.append({k: torch.zeros(shape, dtype=torch.bfloat16, device=device)
+                                   for k in ("k_pages", "v_pages")})
                 else:
                     states.append({"k_cache": torch.zeros(batch, max_ctx, 2, 256, dtype=torch.bfloat16,
                                                           device=device),
@@ -86,9 +100,14 @@ class AttentionStack:
         else:
             ops.q4_norm_matmul_parts(ctx, L["in_proj"], x, L["in_norm_w"], eps,
                                      outs=(self.qg, self.kn, self.vn))
-            ops.gqa_decode(ctx, L["params"], self.qg.view(B, 16, 512), self.kn.view(B, 2, 256),
-                           self.vn.view(B, 2, 256), S["k_cache"], S["v_cache"], positions, out=self.att,
-                           eps=eps)
+            new = (self.qg.view(B, 16, 512), self.kn.view(B, 2, 256), self.vn.view(B, 2, 256))
+            if self.pages is None:
+                ops.gqa_decode(ctx, L["params"], *new, S["k_cache"], S["v_cache"], positions, out=self.att,
+                               eps=eps)
+            else:
+                P = self.pages
+                ops.gqa_decode_shared(ctx, L["params"], *new, S["k_pages"], S["v_pages"], P.table, positions,
+                                      P.group, P.shared_len, out=self.att, eps=eps)
             ops.q4_matmul_parts(ctx, [L["out_proj"]], self.att.view(B, 4096), outs=(x,), residuals=(x,))
 
     def decode_step(self, x: torch.Tensor, positions: torch.Tensor):
@@ -99,6 +118,82 @@ class AttentionStack:
             raise ValueError(f"x must be float32 [{self.B}, {HIDDEN}]")
         for l in range(len(self.layers)):
             self.layer_step(l, x, positions)
+
+    # ---- sequences of a paged stack ------------------------------------------
+
+    def _copy_pages(self, src, dst):
+        pools = [S[k] for kind, S in zip(self.kinds, self.states) if kind == "gqa" for k in ("k_pages", "v_pages")]
+        if src and pools:
+            ops.pages_copy(self.ctx, pools, src, dst)
+
+    def reserve(self, positions):
+        """Places for one decode step's tokens: positions[b] is the new token's
+        position in slot b, negative for a slot that takes no part. Pages that a
+        slot shares and is about to write are copied. Where the pool runs out
+        (OutOfPages), the slots before that one have theirs."""
+        copies = []
+        try:
+            for b, p in enumerate(positions):
+                if p >= 0:
+                    copies += self.pages.reserve(b, p, p + 1)
+        finally:
+            self._copy_pages([s for s, _ in copies], [d for _, d in copies])
+            self.pages.sync()
+
+    def prefill(self, slot: int, x: torch.Tensor, start: int = 0):
+        """A prompt slice of T tokens of one slot through every layer: x [T, 2048]
+        fp32 (the residual stream, in place) at positions start .. start + T - 1;
+        start 0 begins a sequence (zero recurrent states)."""
+        if x.dtype != torch.float32 or x.dim() != 2 or x.shape[1] != HIDDEN:
+            raise ValueError(f"x must be float32 [T, {HIDDEN}]")
+        P, T, ctx, eps = self.pages, x.shape[0], self.ctx, self.eps
+        if T > ctx.cfg.max_prefill_tokens or start + T > ctx.cfg.max_ctx:
+            raise ValueError(f"{T} tokens from {start}: the context takes slices of {ctx.cfg.max_prefill_tokens} up to "
+                             f"position {ctx.cfg.max_ctx}")
+        copies = P.reserve(slot, start, start + T)
+        self._copy_pages([s for s, _ in copies], [d for _, d in copies])
+        P.sync()
+        for kind, L, S in zip(self.kinds, self.layers, self.states):
+            y = ops.q4_norm_matmul_parts(ctx, L["in_proj"], x, L["in_norm_w"], eps)
+            if kind == "dn":
+                conv, ssm = S["conv_state"][slot], S["ssm_state"][slot]
+                if start == 0:
+                    conv.zero_()
+                    ssm.zero_()
+                core = ops.deltanet_prefill(ctx, L["params"], y[0], y[1], y[3], y[2], conv, ssm, out_dtype=torch.float32,
+                                            eps=eps)
+            else:
+                core = ops.gqa_prefill_paged(ctx, L["params"], y[0].view(T, 16, 512), y[1].view(T, 2, 256),
+                                             y[2].view(T, 2, 256), S["k_pages"], S["v_pages"], P.table[slot],
+                                             start_pos=start, out_dtype=torch.float32, eps=eps).view(T, 4096)
+            ops.q4_matmul_parts(ctx, [L["out_proj"]], core, outs=(x,), residuals=(x,))
+
+    def fork(self, src: int, dsts):
+        """Slots `dsts` (empty) go on from where slot src stands: its pages are
+        held by all, its recurrent states copied. Neighbouring slots read what
+        they share once."""
+        dsts = list(dsts)
+        if src in dsts or len(set(dsts)) < len(dsts) or any(self.pages.lengths[d] for d in dsts):
+            raise ValueError("a fork goes into empty slots")
+        for d in dsts:
+            self.pages.fork(src, d)
+        recurrent = [S for kind, S in zip(self.kinds, self.states) if kind == "dn"]
+        if dsts and recurrent:
+            for k in ("conv_state", "ssm_state"):
+                ops.pages_copy(self.ctx, [S[k] for S in recurrent], [src] * len(dsts), dsts)
+        self.pages.sync()
+
+    def release(self, slot: int):
+        """Ends a slot's sequence; pages that no other slot holds are free again."""
+        self.pages.release(slot)
+        self.pages.sync()
+
+    def compact(self) -> int:
+        """Moves the pages in use to the front of every pool; returns their
+        number."""
+        self._copy_pages(*self.pages.compact())
+        self.pages.sync()
+        return int((self.pages.refs > 0).sum())
 
 
 def random_q4(rows: int, cols: int, gen: torch.Generator, device="cuda"):
