@@ -493,8 +493,9 @@ int qff_gqa_prefill_paged(qff_ctx* ctx, qff_stream_t stream, const qff_gqa_param
 }
 
 // Every index inside the pools, no page written twice, none both read and
-// written: the pairs may then be copied in any order.
-static int page_pairs_status(qff_ctx* ctx, int num_pages, const int32_t* src, const int32_t* dst, int n) {
+// written: the pairs may then be copied in any order. *once: no source twice.
+static int page_pairs_status(qff_ctx* ctx, int num_pages, const int32_t* src, const int32_t* dst, int n,
+                             bool* once) {
     for (int i = 0; i < n; ++i)
         if (src[i] < 0 || src[i] >= num_pages || dst[i] < 0 || dst[i] >= num_pages) return QFF_ERR_INVALID_ARG;
     const size_t words = (static_cast<size_t>(num_pages) + 63) / 64;
@@ -506,16 +507,19 @@ static int page_pairs_status(qff_ctx* ctx, int num_pages, const int32_t* src, co
         }
     }
     uint64_t* bits = ctx->page_bits.data();
-    bool ok = true;
-    for (int i = 0; i < n; ++i) {
-        uint64_t& w = bits[dst[i] >> 6];
-        const uint64_t bit = 1ull << (dst[i] & 63);
-        if (w & bit) ok = false;
+    auto mark = [&](int32_t page) {   // whether it was marked before
+        uint64_t& w = bits[page >> 6];
+        const uint64_t bit = 1ull << (page & 63);
+        const bool was = (w & bit) != 0;
         w |= bit;
-    }
-    for (int i = 0; i < n; ++i)
-        if (bits[src[i] >> 6] >> (src[i] & 63) & 1) ok = false;
-    for (int i = 0; i < n; ++i) bits[dst[i] >> 6] = 0;
+        return was;
+    };
+    bool ok = true;
+    for (int i = 0; i < n; ++i) ok &= !mark(dst[i]);
+    for (int i = 0; i < n; ++i) ok &= !(bits[src[i] >> 6] >> (src[i] & 63) & 1);
+    *once = true;
+    for (int i = 0; i < n; ++i) *once &= !mark(src[i]);
+    for (int i = 0; i < n; ++i) bits[dst[i] >> 6] = bits[src[i] >> 6] = 0;
     return ok ? QFF_OK : QFF_ERR_INVALID_ARG;
 }
 
@@ -527,10 +531,11 @@ int qff_pages_copy(qff_ctx* ctx, qff_stream_t stream, void* const* pools, int np
         if (!pools[i] || !aligned16(pools[i])) return QFF_ERR_INVALID_ARG;
     if (page_bytes % 16 != 0 || page_bytes > (size_t{1} << 31)) return QFF_ERR_UNSUPPORTED;
     if (n == 0) return QFF_OK;
-    if (const int st = page_pairs_status(ctx, num_pages, src, dst, n)) return st;
+    bool once = false;
+    if (const int st = page_pairs_status(ctx, num_pages, src, dst, n, &once)) return st;
     const OnDevice on(ctx->device);
     if (!on.ok) return QFF_ERR_HIP;
-    QFF_CHECK_HIP(launch_pages_copy(ctx, stream, pools, npools, page_bytes, src, dst, n));
+    QFF_CHECK_HIP(launch_pages_copy(ctx, stream, pools, npools, page_bytes, src, dst, n, once));
     return QFF_OK;
 }
 

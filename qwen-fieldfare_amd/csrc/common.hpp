@@ -161,4 +161,9 @@ __device__ __forceinline__ void dma16(const char* base, uint32_t voff, uint32_t 
     asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "{m0}"(lds) : "memory");
 }
 
+// The same, non-temporal: for streams that no later read finds cached.
+__device__ __forceinline__ void dma16_nt(const char* base, uint32_t voff, uint32_t lds) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(voff), "s"(base), "{m0}"(lds) : "memory");
+}
+
 }  // namespace qff

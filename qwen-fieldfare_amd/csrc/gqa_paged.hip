@@ -114,8 +114,18 @@ __device__ __forceinline__ int items_of(const LanePlan& p, int ch, int lane) {
     return chunks_of(p.own(), ch) + (p.first == lane ? chunks_of(p.shared, ch) : 0);
 }
 
-// The chunk length, whole tiles.
-__device__ __forceinline__ int chunk_length(const PagedSeqs& a, const LanePlan& p0, int lane) {
+// The call's chunk length, whole tiles, and whether it reads so much that
+// nothing of it can still be cached when it is read again (half of the 256 MB
+// that lie in front of HBM): its tiles are then copied non-temporally. 32
+// sequences of up to 32K (1.1 GB) 200 -> 182 us; 8 of up to 8K (75 MB, which a
+// loop over three such calls finds cached) 21.6 -> 22.5.
+struct Chunk {
+    int len;
+    bool stream;
+};
+constexpr int kStreamTiles = 1024;   // of one kv head, 64 KB each
+
+__device__ __forceinline__ Chunk chunk_length(const PagedSeqs& a, const LanePlan& p0, int lane) {
     long long tiles = 0;
     int streams = 0, longest = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
@@ -135,7 +145,8 @@ __device__ __forceinline__ int chunk_length(const PagedSeqs& a, const LanePlan& 
     }
     ch = max(max(ch, 1), (longest + (a.cap - 2) * kTile - 1) / ((a.cap - 2) * kTile));
     // (the same in every lane; the compiler has to know, for the scalar addresses that follow from it)
-    return __builtin_amdgcn_readfirstlane(ch * kTile);
+    return Chunk{__builtin_amdgcn_readfirstlane(ch * kTile),
+                 __builtin_amdgcn_readfirstlane(static_cast<int>(tiles >= kStreamTiles)) != 0};
 }
 
 // Workgroup item g: the sequence that holds it (-1: past the last), the item's
@@ -323,7 +334,8 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
     const int wv = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
     const int kvh = blockIdx.x & 1;
     const LanePlan p0 = lane_plan(a, 0, lane);
-    const int ch = chunk_length(a, p0, lane);
+    const Chunk chunk = chunk_length(a, p0, lane);
+    const int ch = chunk.len;
     LanePlan plan;
     int item;
     const int found = find_item(a, p0, ch, static_cast<int>(blockIdx.x >> 1), lane, item, plan);
@@ -337,6 +349,7 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
     const bool has_new = !pfx && p_end == plan.len;
     const int slot_c = pfx ? c : npfx + c;
     const int ntiles = (p_end - p_begin + kTile - 1) / kTile;
+    const bool stream = chunk.stream && !pfx;   // (a long prefix is read by every block of its group)
     const int mask = (1 << kv.lg) - 1;
     const int32_t* row = kv.table + static_cast<size_t>(lead) * kv.cols;
     const int last_entry = (p_end - 1) >> kv.lg;
@@ -359,8 +372,16 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
             const int entry = p >> kv.lg;
             const size_t at = (((static_cast<size_t>(win.of(entry)) << kv.lg) + (p & mask) + 2 * wv) * 2 + kvh) * 512;
             bad |= (win.is_bad(entry) ? 1u : 0u) << i;
-            dma16(reinterpret_cast<const char*>(kv.k) + at, lt, lds_addr(&L.tile[t & 1][0][(16 * i + 2 * wv) * 256]));
-            dma16(reinterpret_cast<const char*>(kv.v) + at, lt, lds_addr(&L.tile[t & 1][1][(16 * i + 2 * wv) * 256]));
+            const char *k = reinterpret_cast<const char*>(kv.k) + at, *v = reinterpret_cast<const char*>(kv.v) + at;
+            const uint32_t lk = lds_addr(&L.tile[t & 1][0][(16 * i + 2 * wv) * 256]);
+            const uint32_t lv = lds_addr(&L.tile[t & 1][1][(16 * i + 2 * wv) * 256]);
+            if (stream) {
+                dma16_nt(k, lt, lk);
+                dma16_nt(v, lt, lv);
+            } else {
+                dma16(k, lt, lk);
+                dma16(v, lt, lv);
+            }
         }
         return bad;
     };

@@ -196,7 +196,7 @@ hipError_t launch_gqa_decode_paged(qff_ctx* ctx, hipStream_t stream, const qff_g
                                    const int32_t* positions, const int32_t* group, const int32_t* shared_len,
                                    void* out, qff_dtype out_dtype, int batch);
 hipError_t launch_pages_copy(qff_ctx* ctx, hipStream_t stream, void* const* pools, int npools, size_t page_bytes,
-                             const int32_t* src, const int32_t* dst, int n);
+                             const int32_t* src, const int32_t* dst, int n, bool once);   // once: no source twice
 hipError_t launch_q4_dequant(hipStream_t stream, const uint32_t* w, const void* scales,
                              const void* biases, qff_dtype sb_dtype, float* out, int rows, int cols);
 hipError_t launch_q4_matmul(qff_ctx* ctx, hipStream_t stream, const uint32_t* w, const void* scales,

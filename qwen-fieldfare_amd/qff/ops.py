@@ -43,7 +43,7 @@ def _pack(layout: struct.Struct, pointers, *fields) -> bytes:
         return layout.pack(*pointers, *(f if isinstance(f, int) else ctypes.c_float(f).value for f in fields))
 
 
-_BLOCKS = (ctypes.POINTER(DeltaNetParams), ctypes.POINTER(GqaParams), ctypes.POINTER(Q4Part), ctypes.POINTER(KvPages))
+_BLOCKS = (ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(DeltaNetParams), ctypes.POINTER(GqaParams), ctypes.POINTER(Q4Part), ctypes.POINTER(KvPages))
 
 
 class _Calls:
@@ -52,7 +52,7 @@ class _Calls:
     def __init__(self, L):
         for name in ("qff_q4_matmul", "qff_q4_matmul_parts", "qff_q4_norm_matmul_parts", "qff_router_top8",
                      "qff_deltanet_decode", "qff_deltanet_prefill", "qff_gqa_decode", "qff_gqa_prefill",
-                     "qff_gqa_decode_paged", "qff_gqa_decode_shared", "qff_gqa_prefill_paged"):
+                     "qff_gqa_decode_paged", "qff_gqa_decode_shared", "qff_gqa_prefill_paged", "qff_pages_copy"):
             fn = L[name]   # a new function object: the typed one of lib() stays as it is
             fn.argtypes = [ctypes.c_void_p if t in _BLOCKS else t for t in getattr(L, name).argtypes]
             fn.restype = ctypes.c_int
@@ -466,20 +466,22 @@ def pages_copy(ctx: Context, pools, src, dst) -> None:
     multiple of 16): K and V pools, or DeltaNet states with one page per
     sequence. src, dst: page numbers, as lists or int32 host tensors; a
     destination may be neither repeated nor a source."""
-    pools = list(pools)
-    if not pools:
+    n = len(pools)
+    if not n:
         raise ValueError("at least one pool")
     s, d = _host_i32("src", src), _host_i32("dst", dst)
     if s.numel() != d.numel():
         raise ValueError("src and dst must have the same length")
-    pages = pools[0].shape[0]
-    size = pools[0].numel() * pools[0].element_size() // max(pages, 1)
+    first = pools[0]
+    shape, dtype = first.shape, first.dtype
+    pages, size = shape[0], first.nbytes // max(shape[0], 1)
     for p in pools:
-        if p.shape[0] != pages or p.numel() * p.element_size() != pages * size:
+        if (p.shape != shape or p.dtype != dtype) and (p.shape[0] != pages or p.nbytes != first.nbytes):
             raise ValueError("pools must have the same number of pages and bytes per page")
-    arr = (ctypes.c_void_p * len(pools))(*(_ptr_on(ctx, "a pool", p) for p in pools))
-    check("qff_pages_copy", lib().qff_pages_copy(ctx.handle, _stream_of(ctx), arr, len(pools), size, pages,
-                                                 s.data_ptr(), d.data_ptr(), s.numel()))
+    arr = struct.pack(f"{n}P", *[_ptr_on(ctx, "a pool", p) for p in pools])
+    st = _hot().qff_pages_copy(ctx.handle, _stream_of(ctx), arr, n, size, pages, s.data_ptr(), d.data_ptr(), s.numel())
+    if st:
+        raise QffError("qff_pages_copy", st)
 
 
 __all__ = ["Context", "QffError", "q4_dequant", "q4_matmul", "deltanet_decode", "deltanet_prefill",
