@@ -47,7 +47,7 @@ WorkspaceLayout workspace_layout(const qff_ctx_cfg& cfg) {
     L.gqa_m = take(S * 8 * sizeof(float));
     L.gqa_d = take(S * 8 * sizeof(float));
     L.gqa_o = take(S * 8 * 256 * sizeof(float));
-    L.gqa_nc = take(B * sizeof(int32_t));
+    L.gqa_nc = take(std::max(B, static_cast<size_t>(kPagedTokensMax)) * sizeof(int32_t));
     L.gqa_qb = take(T * 16 * 256 * sizeof(uint16_t));
     L.gqa_kv16 = take(static_cast<size_t>(cfg.max_ctx) * 512 * sizeof(uint16_t));
     L.gqa_vt = take(static_cast<size_t>((cfg.max_ctx + 63) / 64) * 64 * 512 * sizeof(uint16_t));
@@ -487,8 +487,7 @@ int qff_gqa_prefill_paged(qff_ctx* ctx, qff_stream_t stream, const qff_gqa_param
     if (T > ctx->cfg.max_prefill_tokens || end > ctx->cfg.max_ctx) return QFF_ERR_WORKSPACE;
     const OnDevice on(ctx->device);
     if (!on.ok) return QFF_ERR_HIP;
-    QFF_CHECK_HIP(launch_gqa_prefill(ctx, stream, p, q_gate, k, v, in_dtype, kv->k, kv->v, kv, start_pos, out,
-                                     out_dtype, T));
+    QFF_CHECK_HIP(launch_gqa_prefill_paged(ctx, stream, p, q_gate, k, v, in_dtype, kv, start_pos, out, out_dtype, T));
     return QFF_OK;
 }
 

@@ -27,6 +27,7 @@
 // three of bf16 or two of fp16 (error 2e-7 to 7e-7 of the exact output, where
 // two bf16 terms leave 6e-6). fp16 weights are scaled by 2^7 (kShift), so that
 // weights down to 2^-21 of the row's largest keep all bits of their first term.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.hpp"
@@ -61,6 +62,14 @@ struct PagedSeqs {
     int batch, max_ctx;
     int slots;   // workgroups of one round, per kv head
     int cap;     // chunks allowed per sequence
+};
+
+// A prompt slice instead of a batch: T tokens of one sequence from position
+// `start` (appended before), a block of 16 after the other, each over all
+// positions up to its last token's in chunks of ch.
+struct PagedTokens {
+    int start, T, ch;
+    __device__ __host__ int end(int blk) const { return start + (16 * blk + 16 < T ? 16 * blk + 16 : T); }
 };
 
 // Sequence b0 + lane: its length, the shared positions of its block, the
@@ -324,34 +333,53 @@ struct PartLds {
 
 __device__ __forceinline__ int tile_swz(int r) { return ((r & 7) << 1) | ((r >> 3) & 1); }
 
-template <int IN_DT, int KV_F16, int NT>
+template <int IN_DT, int KV_F16, int NT, bool TOKENS>
 __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
     const void* __restrict__ q_gate, const void* __restrict__ k_new, const void* __restrict__ v_new,
     const float* __restrict__ q_norm_w, const float* __restrict__ k_norm_w, RopeFreqs rf, float scale, float eps,
-    PagedKv kv, PagedSeqs a, PagedPartials pp) {
+    PagedKv kv, PagedSeqs a, PagedTokens tk, PagedPartials pp) {
     __shared__ __attribute__((aligned(1024))) PartLds L;
     const int lane = threadIdx.x & 63;
     const int wv = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
     const int kvh = blockIdx.x & 1;
-    const LanePlan p0 = lane_plan(a, 0, lane);
-    const Chunk chunk = chunk_length(a, p0, lane);
-    const int ch = chunk.len;
-    LanePlan plan;
-    int item;
-    const int found = find_item(a, p0, ch, static_cast<int>(blockIdx.x >> 1), lane, item, plan);
-    if (found < 0) return;   // (uniform over the workgroup)
-    // the block's shared chunks come first among its first sequence's items
-    const int lead = found, npfx = chunks_of(plan.shared, ch);
-    const bool pfx = found == plan.first && item < npfx;
-    const int c = pfx ? item : item - (found == plan.first ? npfx : 0);
-    const int count = pfx ? plan.count : 1;
-    const int p_begin = (pfx ? 0 : plan.shared) + c * ch, p_end = min(pfx ? plan.shared : plan.len, p_begin + ch);
-    const bool has_new = !pfx && p_end == plan.len;
-    const int slot_c = pfx ? c : npfx + c;
+    int lead, count, p_begin, p_end, slot_c, cut_from;   // cut_from: no row's limit lies before it
+    bool has_new = false, stream = false;
+    LanePlan plan{};
+    if constexpr (TOKENS) {
+        int c = static_cast<int>(blockIdx.x >> 1), blk = 0, nc;
+        while (c >= (nc = chunks_of(tk.end(blk), tk.ch))) {   // (the grid is their sum)
+            c -= nc;
+            ++blk;
+        }
+        lead = 16 * blk;
+        count = min(kBlkSeqs, tk.T - lead);
+        p_begin = c * tk.ch;
+        p_end = min(tk.end(blk), p_begin + tk.ch);
+        slot_c = c;
+        cut_from = min(p_end, tk.start + lead + 1);
+        if (c == 0 && kvh == 0 && static_cast<int>(threadIdx.x) < count) pp.count[lead + threadIdx.x] = nc;
+    } else {
+        const LanePlan p0 = lane_plan(a, 0, lane);
+        const Chunk chunk = chunk_length(a, p0, lane);
+        const int ch = chunk.len;
+        int item;
+        lead = find_item(a, p0, ch, static_cast<int>(blockIdx.x >> 1), lane, item, plan);
+        if (lead < 0) return;   // (uniform over the workgroup)
+        // the block's shared chunks come first among its first sequence's items
+        const int npfx = chunks_of(plan.shared, ch);
+        const bool pfx = lead == plan.first && item < npfx;
+        const int c = pfx ? item : item - (lead == plan.first ? npfx : 0);
+        count = pfx ? plan.count : 1;
+        p_begin = (pfx ? 0 : plan.shared) + c * ch;
+        p_end = min(pfx ? plan.shared : plan.len, p_begin + ch);
+        has_new = !pfx && p_end == plan.len;
+        slot_c = pfx ? c : npfx + c;
+        cut_from = p_end;
+        stream = chunk.stream && !pfx;   // (a long prefix is read by every block of its group)
+    }
     const int ntiles = (p_end - p_begin + kTile - 1) / kTile;
-    const bool stream = chunk.stream && !pfx;   // (a long prefix is read by every block of its group)
     const int mask = (1 << kv.lg) - 1;
-    const int32_t* row = kv.table + static_cast<size_t>(lead) * kv.cols;
+    const int32_t* row = kv.table + (TOKENS ? 0 : static_cast<size_t>(lead) * kv.cols);
     const int last_entry = (p_end - 1) >> kv.lg;
     PageWindow win;
 
@@ -393,6 +421,9 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
     const int rb = wv & (R - 1), part = wv / R;
     const bool active = part < parts && rb < nrb;
     const int seq = lead + min(2 * rb + (n >> 3), count - 1);   // of the lane's q row
+    // the lane's row sees positions before lim
+    const int lim = TOKENS ? min(p_end, tk.start + seq + 1) : p_end;
+    auto position_of = [&](int s) { return TOKENS ? tk.start + s : a.positions[s]; };
 
     // ---- q rows: RMS norm, rotation, terms, by all waves together and handed to
     // the waves that use them through the second stage's LDS, in the operand
@@ -421,12 +452,12 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
         }
         load4<0>(q_norm_w, dim0, &w[0]);
         load4<0>(q_norm_w, dim1, &w[4]);
-        if constexpr (ONE) {   // (waves other than 4 and 5 do not use them)
+        if constexpr (ONE && !TOKENS) {   // (waves other than 4 and 5 do not use them)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 kx[i] = elem<IN_DT>::load(wv == 5 ? v_new : k_new, (static_cast<size_t>(lead) * 2 + kvh) * 256 + 4 * lane + i);
         }
-        int pos_a = a.positions[lead + min(2 * min(wv, RR - 1) + (lane >> 5), count - 1)];
+        int pos_a = position_of(lead + min(2 * min(wv, RR - 1) + (lane >> 5), count - 1));
         float freq = rf.f[lane & 31];   // (a load: the arguments lie in memory)
         // (consumed here, so that no load is moved behind the copies, whose
         // requests a later wait for it would wait for too)
@@ -437,7 +468,7 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
 #pragma unroll
             for (int r = 0; r < RR; ++r) asm volatile("" : "+v"(x[r][e]));
         }
-        if constexpr (ONE) asm volatile("" : "+v"(kx[0]), "+v"(kx[1]), "+v"(kx[2]), "+v"(kx[3]));
+        if constexpr (ONE && !TOKENS) asm volatile("" : "+v"(kx[0]), "+v"(kx[1]), "+v"(kx[2]), "+v"(kx[3]));
         win.set(p_begin >> kv.lg, entry0, kv.num_pages);
         bad_next = issue(0);
         // cos, sin of angle l % 32 of row block wv's sequence l / 32
@@ -506,7 +537,7 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
             }
             if (r0 + kAtOnce < RR) __syncthreads();
         }
-        if constexpr (ONE) {
+        if constexpr (ONE && !TOKENS) {
             if (has_new && (wv == 4 || wv == 5)) {
                 // dims 4 lane .. + 3; the rotation's partner of dim d < 32 is d + 32, 8 lanes on
                 if (wv == 4) {
@@ -543,7 +574,7 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
         const size_t qbase = (static_cast<size_t>(seq) * 16 + kvh * 8 + (n & 7)) * 512 + 8 * kb;
 #pragma unroll
         for (int jj = 0; jj < 8; ++jj) load8<IN_DT>(q_gate, qbase + 32 * jj, x[jj]);
-        int pos_a = a.positions[lead + min(2 * rb + (lane >> 5), count - 1)];
+        int pos_a = position_of(lead + min(2 * rb + (lane >> 5), count - 1));
         float freq = rf.f[lane & 31], w[8][8];
 #pragma unroll
         for (int jj = 0; jj < 8; ++jj) load8<0>(q_norm_w, 32 * jj + 8 * kb, w[jj]);
@@ -631,6 +662,8 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
                 for (int i = 0; i < 4; ++i) oacc[dt][i] *= alpha;
         }
     };
+    // what the weights' exponents count from; a token's row that sees none of the positions so far keeps weights of 0
+    auto base_of = [&] { return TOKENS && m_run == -INFINITY ? 0.0f : m_run - kShift<KV_F16>; };
     // 32 positions (s0 ..) of a block's row block; sub: which half of the tile
     auto block_step = [&](uint32_t kt, uint32_t vt, int s0, int sub, unsigned bad) {
         const uint32_t ka = kt + 16384u * sub + kaddr, va0 = vt + 16384u * sub + vaddr;   // (tiles lie at multiples of 32 KB)
@@ -676,18 +709,18 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
                 for (int k = 1; k < NT; ++k) v += s[b][k][i];
                 x[b][i] = v * sc;
             }
-        if (s0 + 32 > p_end || (bad >> (2 * sub) & 3)) {   // (uniform)
+        if (s0 + 32 > cut_from || (bad >> (2 * sub) & 3)) {   // (uniform)
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    x[b][i] = s0 + 16 * b + 4 * kb + i >= p_end ? -INFINITY
+                    x[b][i] = s0 + 16 * b + 4 * kb + i >= lim ? -INFINITY
                               : (bad >> (2 * sub + b)) & 1     ? __builtin_nanf("")
                                                                : x[b][i];
         }
         raise(fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
                     fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3]))));
-        const float mb = m_run - kShift<KV_F16>;
+        const float mb = base_of();
         u32x4_t pw[NT];
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -738,7 +771,7 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
                 x[i] = s0 + 4 * kb + i >= p_end ? -INFINITY : bad ? __builtin_nanf("") : x[i];
         }
         raise(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
-        const float mb = m_run - kShift<KV_F16>;
+        const float mb = base_of();
         uint32_t w0[NT], w1[NT];
         const float e0 = __builtin_amdgcn_exp2f(x[0] - mb), e1 = __builtin_amdgcn_exp2f(x[1] - mb);
         const float e2 = __builtin_amdgcn_exp2f(x[2] - mb), e3 = __builtin_amdgcn_exp2f(x[3] - mb);
@@ -758,6 +791,22 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
     };
+    // four dims of row r of tile t: 4 lane .. + 3 of K (0) or V (1)
+    auto tile_at = [&](int t, int which, int r) {
+        return reinterpret_cast<u32x2_t*>(&L.tile[t & 1][which][r * 256 + 8 * ((lane >> 1) ^ tile_swz(r)) + 4 * (lane & 1)]);
+    };
+    // V's rows from .. to - 1 of the last tile, behind the last position (the page may hold any bit pattern there)
+    auto clear_behind = [&](int t, int from, int to) {
+        for (int z = from + wv; z < to; z += 8) *tile_at(t, 1, z) = u32x2_t{0u, 0u};
+        __syncthreads();
+    };
+    // (a page outside the pool is read as page 0: rows that do not see it give V's rows weights of 0)
+    auto clear_bad = [&](int t, unsigned bad) {
+        if (!TOKENS || bad == 0) return;
+        for (int z = wv; z < kTile; z += 8)
+            if ((bad >> (z >> 4)) & 1) *tile_at(t, 1, z) = u32x2_t{0u, 0u};
+        __syncthreads();
+    };
     if (single) {
         prepare(std::integral_constant<int, 1>{}, std::true_type{});
         clear();
@@ -767,17 +816,12 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
             const int t0 = p_begin + t * kTile;
             if (t + 1 < ntiles) {
                 bad_next = issue(t + 1);
-            } else if (has_new) {
-                // the new token's row, and zeros behind it in the 16 positions it is among
-                const int r = plan.len - 1 - t0, end = (r | 15) + 1;
-                auto at = [&](int which, int rr) {
-                    return reinterpret_cast<u32x2_t*>(
-                        &L.tile[t & 1][which][rr * 256 + 8 * ((lane >> 1) ^ tile_swz(rr)) + 4 * (lane & 1)]);
-                };
-                if (wv == 4 || wv == 5) *at(wv - 4, r) = fresh;
-                for (int z = r + 1 + wv; z < end; z += 8) *at(1, z) = u32x2_t{0u, 0u};
-                __syncthreads();
+            } else if (TOKENS || has_new) {
+                const int r = p_end - t0;
+                if (!TOKENS && (wv == 4 || wv == 5)) *tile_at(t, wv - 4, r - 1) = fresh;   // the new token's row
+                clear_behind(t, r, (r + 15) & ~15);
             }
+            clear_bad(t, bad);
             if (active && t0 + 16 * part < p_end)
                 single_step(lds_addr(L.tile[t & 1][0]), lds_addr(L.tile[t & 1][1]), t0 + 16 * part, (bad >> part) & 1);
         }
@@ -792,6 +836,8 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
             const unsigned bad = bad_next;
             const int t0 = p_begin + t * kTile;
             if (t + 1 < ntiles) bad_next = issue(t + 1);
+            else if (TOKENS) clear_behind(t, p_end - t0, (p_end - t0 + 31) & ~31);
+            clear_bad(t, bad);
             if (!active) continue;
 #pragma unroll 1
             for (int sub = parts == 2 ? part : 0; sub < (parts == 2 ? part + 1 : 2); ++sub)
@@ -882,7 +928,7 @@ __global__ __launch_bounds__(512) void gqa_paged_combine_kernel(const void* __re
     const float m_slot = pp.m[(base + ts) * 8 + hl];
     const float d_slot = pp.d[(base + ts) * 8 + hl];
     const float gate = elem<IN_DT>::load(q_gate, qi * 512 + 256 + d0 + min(t, kDims - 1));
-    const int pos = positions[seq], listed = pp.count[seq];
+    const int pos = positions ? positions[seq] : 0, listed = pp.count[seq];
     if (pos < 0 || pos >= max_ctx) {   // (uniform over the workgroup)
         if (t < kDims) elem<OUT_DT>::store(out, qi * 256 + d0 + t, __builtin_nanf(""));
         return;
@@ -935,49 +981,143 @@ __global__ __launch_bounds__(512) void gqa_paged_combine_kernel(const void* __re
     }
 }
 
+// ---- append ------------------------------------------------------------------------------
+//
+// A prompt slice's k (RMS norm, rotation) and v rows into their pages: one
+// wave per (token, kv head), lane l dims 4 l .. + 3. Rows whose page lies
+// outside the pool are dropped.
+template <int IN_DT, int KV_F16>
+__global__ __launch_bounds__(256) void gqa_paged_append_kernel(const void* __restrict__ k, const void* __restrict__ v,
+                                                               const float* __restrict__ k_norm_w, RopeFreqs rf,
+                                                               float eps, PagedKv kv, int start, int T) {
+    const int lane = threadIdx.x & 63, unit = static_cast<int>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    if (unit >= 2 * T) return;
+    const int pos = start + (unit >> 1);
+    const int page = kv.table[pos >> kv.lg];
+    float x[4], y[4], ss = 0.0f;
+    load4<IN_DT>(k, static_cast<size_t>(unit) * 256 + 4 * lane, x);
+    load4<IN_DT>(v, static_cast<size_t>(unit) * 256 + 4 * lane, y);
+    float c, s;
+    sincosf(static_cast<float>(pos) * rf.f[lane & 31], &s, &c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ss += x[i] * x[i];
+    const float inv = 1.0f / sqrtf(group_sum<64>(ss) / 256.0f + eps);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = x[i] * inv * k_norm_w[4 * lane + i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {   // the partner of dim d < 32 is d + 32, 8 lanes on
+        const float up = __shfl_down(x[i], 8, 64), dn = __shfl_up(x[i], 8, 64);
+        const float ci = __shfl(c, (4 * lane + i) & 31, 64), si = __shfl(s, (4 * lane + i) & 31, 64);
+        const int d = 4 * lane + i;
+        if (d < 64) x[i] = d < 32 ? x[i] * ci - up * si : x[i] * ci + dn * si;
+    }
+    if (page < 0 || page >= kv.num_pages) return;
+    uint32_t k0[1], k1[1], v0[1], v1[1];
+    split_terms<KV_F16, 1>(x[0], x[1], k0);
+    split_terms<KV_F16, 1>(x[2], x[3], k1);
+    split_terms<KV_F16, 1>(y[0], y[1], v0);
+    split_terms<KV_F16, 1>(y[2], y[3], v1);
+    const size_t off = (((static_cast<size_t>(page) << kv.lg) + (pos & ((1 << kv.lg) - 1))) * 2 + (unit & 1)) * 256 + 4 * lane;
+    *reinterpret_cast<u32x2_t*>(kv.k + off) = u32x2_t{k0[0], k1[0]};
+    *reinterpret_cast<u32x2_t*>(kv.v + off) = u32x2_t{v0[0], v1[0]};
+}
+
 // ---- launch ---------------------------------------------------------------------------
 
-hipError_t launch_gqa_decode_paged(qff_ctx* ctx, hipStream_t stream, const qff_gqa_params* p, const void* q_gate,
-                                   const void* k_new, const void* v_new, qff_dtype in_dtype, const qff_kv_pages* kv,
-                                   const int32_t* positions, const int32_t* group, const int32_t* shared_len,
-                                   void* out, qff_dtype out_dtype, int batch) {
-    const int lg = __builtin_ctz(static_cast<unsigned>(kv->page_size));
-    const PagedKv pk{static_cast<uint16_t*>(kv->k), static_cast<uint16_t*>(kv->v), kv->table, kv->num_pages, lg,
-                     kv->table_cols};
-    const int cap = gqa_chunk_cap(ctx->cfg, batch);
-    const PagedSeqs a{positions, group, shared_len, batch, kv->table_cols << lg, ctx->num_cu / 2, cap};
-    const PagedPartials pp{ctx->gqa_m, ctx->gqa_d, ctx->gqa_o, ctx->gqa_nc, cap};
+static PagedKv paged_kv(const qff_kv_pages* kv) {
+    return PagedKv{static_cast<uint16_t*>(kv->k), static_cast<uint16_t*>(kv->v), kv->table, kv->num_pages,
+                   __builtin_ctz(static_cast<unsigned>(kv->page_size)), kv->table_cols};
+}
+
+// The partial launch (a batch's step, or a slice's tokens) and the combine of
+// `rows` sequences or tokens.
+static void launch_partials(qff_ctx* ctx, hipStream_t stream, const qff_gqa_params* p, const void* q_gate,
+                            const void* k_new, const void* v_new, qff_dtype in_dtype, const PagedKv& pk,
+                            const PagedSeqs* a, const PagedTokens& tk, const PagedPartials& pp, int grid, void* out,
+                            qff_dtype out_dtype, int rows) {
     const RopeFreqs rf = rope_freqs(p->rope_theta);
     const bool f16 = p->kv_f16 != 0, in16 = in_dtype == QFF_BF16, out16 = out_dtype == QFF_BF16;
     {
-        ProfScope prof(ctx, stream, "gqa_paged_partial");
-        // a round of workgroups, and one more for each stream of positions (a
-        // sequence's own, a block's shared ones) that rounding up can add
-        const int grid = 2 * (a.slots + batch + (group ? batch / 2 : 0));
-#define QFF_PART(I, F, N)                                                                                        \
-    gqa_paged_partial_kernel<I, F, N><<<grid, 512, 0, stream>>>(q_gate, k_new, v_new, p->q_norm_w, p->k_norm_w, rf, \
-                                                                p->scale, p->eps, pk, a, pp)
+        ProfScope prof(ctx, stream, a ? "gqa_paged_partial" : "gqa_paged_prefill_partial");
+        const PagedSeqs none{};
+#define QFF_PART1(I, F, N, TOK)                                                                                     \
+    gqa_paged_partial_kernel<I, F, N, TOK><<<grid, 512, 0, stream>>>(q_gate, k_new, v_new, p->q_norm_w, p->k_norm_w, rf, \
+                                                                     p->scale, p->eps, pk, a ? *a : none, tk, pp)
+#define QFF_PART(I, F, N) \
+    if (a) QFF_PART1(I, F, N, false); else QFF_PART1(I, F, N, true)
         if (f16) {
-            if (in16) QFF_PART(1, 1, 2); else QFF_PART(0, 1, 2);
+            if (in16) { QFF_PART(1, 1, 2); } else { QFF_PART(0, 1, 2); }
         } else if (out16) {
-            if (in16) QFF_PART(1, 0, 2); else QFF_PART(0, 0, 2);
+            if (in16) { QFF_PART(1, 0, 2); } else { QFF_PART(0, 0, 2); }
         } else {
-            if (in16) QFF_PART(1, 0, 3); else QFF_PART(0, 0, 3);
+            if (in16) { QFF_PART(1, 0, 3); } else { QFF_PART(0, 0, 3); }
         }
 #undef QFF_PART
+#undef QFF_PART1
     }
-    ProfScope prof(ctx, stream, "gqa_paged_combine");
-    const int ds = batch <= 8 ? 4 : 1;   // small batches split each head's dims over four workgroups
-    const dim3 cgrid(16 * ds, batch);
-#define QFF_COMB(I, O)                                                                                       \
-    if (ds == 4) gqa_paged_combine_kernel<I, O, 4><<<cgrid, 512, 0, stream>>>(q_gate, positions, a.max_ctx, pp, out);           \
-    else gqa_paged_combine_kernel<I, O, 1><<<cgrid, 512, 0, stream>>>(q_gate, positions, a.max_ctx, pp, out)
+    ProfScope prof(ctx, stream, a ? "gqa_paged_combine" : "gqa_paged_prefill_combine");
+    const int ds = rows <= 8 ? 4 : 1;   // few rows: each head's dims split over four workgroups
+    const dim3 cgrid(16 * ds, rows);
+    const int32_t* positions = a ? a->positions : nullptr;
+    const int max_ctx = a ? a->max_ctx : 1;
+#define QFF_COMB(I, O)                                                                                             \
+    if (ds == 4) gqa_paged_combine_kernel<I, O, 4><<<cgrid, 512, 0, stream>>>(q_gate, positions, max_ctx, pp, out); \
+    else gqa_paged_combine_kernel<I, O, 1><<<cgrid, 512, 0, stream>>>(q_gate, positions, max_ctx, pp, out)
     if (in16) {
         if (out16) { QFF_COMB(1, 1); } else { QFF_COMB(1, 0); }
     } else {
         if (out16) { QFF_COMB(0, 1); } else { QFF_COMB(0, 0); }
     }
 #undef QFF_COMB
+}
+
+hipError_t launch_gqa_decode_paged(qff_ctx* ctx, hipStream_t stream, const qff_gqa_params* p, const void* q_gate,
+                                   const void* k_new, const void* v_new, qff_dtype in_dtype, const qff_kv_pages* kv,
+                                   const int32_t* positions, const int32_t* group, const int32_t* shared_len,
+                                   void* out, qff_dtype out_dtype, int batch) {
+    const PagedKv pk = paged_kv(kv);
+    const int cap = gqa_chunk_cap(ctx->cfg, batch);
+    const PagedSeqs a{positions, group, shared_len, batch, kv->table_cols << pk.lg, ctx->num_cu / 2, cap};
+    const PagedPartials pp{ctx->gqa_m, ctx->gqa_d, ctx->gqa_o, ctx->gqa_nc, cap};
+    // a round of workgroups, and one more for each stream of positions (a
+    // sequence's own, a block's shared ones) that rounding up can add
+    const int grid = 2 * (a.slots + batch + (group ? batch / 2 : 0));
+    launch_partials(ctx, stream, p, q_gate, k_new, v_new, in_dtype, pk, &a, PagedTokens{}, pp, grid, out, out_dtype, batch);
+    return hipGetLastError();
+}
+
+// Slices of at most kPagedTokensMax tokens can take the decode's kernels (see launch_gqa_prefill_paged).
+hipError_t launch_gqa_prefill_paged(qff_ctx* ctx, hipStream_t stream, const qff_gqa_params* p, const void* q_gate,
+                                    const void* k, const void* v, qff_dtype in_dtype, const qff_kv_pages* kv,
+                                    int start, void* out, qff_dtype out_dtype, int T) {
+    const int cap = static_cast<int>(std::min<long long>(kGqaMaxChunks, ctx->pf_slots / T));
+    if (T > kPagedTokensMax || cap < 4)
+        return launch_gqa_prefill(ctx, stream, p, q_gate, k, v, in_dtype, kv->k, kv->v, kv, start, out, out_dtype, T);
+    const PagedKv pk = paged_kv(kv);
+    {
+        ProfScope prof(ctx, stream, "gqa_paged_append");
+        const RopeFreqs rf = rope_freqs(p->rope_theta);
+        const int blocks = (2 * T + 3) / 4;
+#define QFF_APP(I, F) gqa_paged_append_kernel<I, F><<<blocks, 256, 0, stream>>>(k, v, p->k_norm_w, rf, p->eps, pk, start, T)
+        if (p->kv_f16) {
+            if (in_dtype == QFF_BF16) QFF_APP(1, 1); else QFF_APP(0, 1);
+        } else {
+            if (in_dtype == QFF_BF16) QFF_APP(1, 0); else QFF_APP(0, 0);
+        }
+#undef QFF_APP
+    }
+    // the least chunk length that needs no second round of workgroups, and no more partials than there is room for
+    PagedTokens tk{start, T, kTile};
+    const int blks = (T + 15) / 16, slots = ctx->num_cu / 2;
+    auto items = [&] {
+        int n = 0;
+        for (int b = 0; b < blks; ++b) n += (tk.end(b) + tk.ch - 1) / tk.ch;
+        return n;
+    };
+    while ((items() > slots && tk.ch < start + T) || (start + T + tk.ch - 1) / tk.ch > cap) tk.ch += kTile;
+    // partials where the sharing prefill keeps its own: m and d [T][2][cap][8], o [T][2][cap][8][256]
+    const PagedPartials pp{ctx->pf_md, ctx->pf_md + static_cast<size_t>(T) * 16 * cap, ctx->pf_o, ctx->gqa_nc, cap};
+    launch_partials(ctx, stream, p, q_gate, k, v, in_dtype, pk, nullptr, tk, pp, 2 * items(), out, out_dtype, T);
     return hipGetLastError();
 }
 

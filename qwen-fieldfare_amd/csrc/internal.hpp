@@ -36,7 +36,7 @@ struct qff_ctx {
     float* gqa_m = nullptr;       // [gqa_slots(cfg) * 8]
     float* gqa_d = nullptr;       // same
     float* gqa_o = nullptr;       // [gqa_slots(cfg) * 8 * 256]
-    int32_t* gqa_nc = nullptr;    // paged decode: partials of each sequence [max_batch]
+    int32_t* gqa_nc = nullptr;    // paged decode: partials of each sequence or token [max_batch, kPagedTokensMax at least]
     // Full-attention prefill: normed, rotated q as bf16 [T][16][256].
     uint16_t* gqa_qb = nullptr;
     uint16_t* gqa_kv16 = nullptr;   // fp16 copy of a bf16 K cache for prefill: [max_ctx][2][256]
@@ -195,6 +195,11 @@ hipError_t launch_gqa_decode_paged(qff_ctx* ctx, hipStream_t stream, const qff_g
                                    const void* k_new, const void* v_new, qff_dtype in_dtype, const qff_kv_pages* kv,
                                    const int32_t* positions, const int32_t* group, const int32_t* shared_len,
                                    void* out, qff_dtype out_dtype, int batch);
+// Prefill into pages: a short slice on the decode's kernels, a long one as launch_gqa_prefill.
+constexpr int kPagedTokensMax = 128;   // of the former
+hipError_t launch_gqa_prefill_paged(qff_ctx* ctx, hipStream_t stream, const qff_gqa_params* p, const void* q_gate,
+                                    const void* k, const void* v, qff_dtype in_dtype, const qff_kv_pages* kv,
+                                    int start, void* out, qff_dtype out_dtype, int T);
 hipError_t launch_pages_copy(qff_ctx* ctx, hipStream_t stream, void* const* pools, int npools, size_t page_bytes,
                              const int32_t* src, const int32_t* dst, int n, bool once);   // once: no source twice
 hipError_t launch_q4_dequant(hipStream_t stream, const uint32_t* w, const void* scales,

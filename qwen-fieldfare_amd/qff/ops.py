@@ -9,6 +9,7 @@ here only when the caller does not pass them.
 from __future__ import annotations
 
 import ctypes
+import operator
 import struct
 
 import torch
@@ -453,6 +454,9 @@ def gqa_prefill_paged(ctx: Context, params: dict, q_gate, k, v, k_pages, v_pages
     return out
 
 
+_nbytes = operator.attrgetter("nbytes")
+
+
 def _host_i32(name, x) -> torch.Tensor:
     t = x if isinstance(x, torch.Tensor) else torch.tensor(x, dtype=_i32)
     if t.is_cuda or t.dtype != _i32 or t.dim() != 1 or not t.is_contiguous():
@@ -472,13 +476,15 @@ def pages_copy(ctx: Context, pools, src, dst) -> None:
     s, d = _host_i32("src", src), _host_i32("dst", dst)
     if s.numel() != d.numel():
         raise ValueError("src and dst must have the same length")
-    first = pools[0]
-    shape, dtype = first.shape, first.dtype
-    pages, size = shape[0], first.nbytes // max(shape[0], 1)
-    for p in pools:
-        if (p.shape != shape or p.dtype != dtype) and (p.shape[0] != pages or p.nbytes != first.nbytes):
-            raise ValueError("pools must have the same number of pages and bytes per page")
-    arr = struct.pack(f"{n}P", *[_ptr_on(ctx, "a pool", p) for p in pools])
+    # (whole-list checks: one by one they take as long as the launch for a model's twenty pools)
+    pages, size = pools[0].shape[0], pools[0].nbytes
+    if set(map(_nbytes, pools)) != {size} or {p.shape[0] for p in pools} != {pages}:
+        raise ValueError("pools must have the same number of pages and bytes per page")
+    size //= max(pages, 1)
+    if set(map(torch.Tensor.get_device, pools)) != {ctx.device} or not all(map(torch.Tensor.is_contiguous, pools)):
+        for p in pools:
+            _ptr_on(ctx, "a pool", p)   # (names what is wrong)
+    arr = struct.pack(f"{n}P", *map(torch.Tensor.data_ptr, pools))
     st = _hot().qff_pages_copy(ctx.handle, _stream_of(ctx), arr, n, size, pages, s.data_ptr(), d.data_ptr(), s.numel())
     if st:
         raise QffError("qff_pages_copy", st)

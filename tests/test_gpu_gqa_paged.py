@@ -13,8 +13,9 @@ Tolerances. fp32 outputs: a score is a sum of 256 products taken in 24 steps
 sqrt(24) 3 2^-24 = 9e-7, that of a softmax weight sqrt(2) of it, and an output
 row's, relative to its 2-norm, the same: 1.3e-6; the bar is four times that,
 5e-6. bf16 outputs: half a step, 2^-8 of the value, and 1e-4 of the row's rms
-for the scores' two-term q and weights (2^-16 each). Prefill: the same launches
-as qff_gqa_prefill after the pages are gathered, so the same bits."""
+for the scores' two-term q and weights (2^-16 each). Prefill: slices of more
+than 128 tokens take the launches of qff_gqa_prefill after the pages are
+gathered, so the same bits; shorter ones the decode's kernels and tolerances."""
 import numpy as np
 import pytest
 import torch
@@ -369,7 +370,7 @@ def test_calls_on_a_side_stream(hip, ctx):
 
 # -------------------------------------------------------------------- prefill
 
-@pytest.mark.parametrize("start,T", [(0, 1), (0, 64), (0, 700), (1, 1), (63, 2), (64, 33), (900, 33), (2011, 300), (3000, 1024)])
+@pytest.mark.parametrize("start,T", [(0, 129), (0, 700), (5, 130), (63, 192), (2011, 300), (3000, 1024)])
 @pytest.mark.parametrize("io,kv,out,page", [("f32", "bf16", "bf16", 16), ("bf16", "f16", "f32", 64), ("bf16", "bf16", "bf16", 256),
                                             ("f32", "f16", "bf16", 32)])
 def test_prefill_paged_is_the_flat_one(hip, ctx, start, T, io, kv, out, page):
@@ -397,6 +398,48 @@ def test_prefill_paged_is_the_flat_one(hip, ctx, start, T, io, kv, out, page):
         assert same_bits(pool, want)
 
 
+@pytest.mark.parametrize("start,T", [(0, 1), (0, 2), (0, 17), (0, 128), (1, 1), (15, 1), (63, 2), (64, 33), (900, 33), (897, 16),
+                                     (2000, 5), (3000, 100), (3968, 128), (4095, 1)])
+@pytest.mark.parametrize("io,kv,out,page", [("f32", "bf16", "f32", 16), ("bf16", "f16", "bf16", 64), ("bf16", "bf16", "bf16", 256),
+                                            ("f32", "f16", "f32", 32)])
+def test_prefill_paged_short(hip, ctx, start, T, io, kv, out, page):
+    """Short slices: blocks of 16 tokens and less, chunks that begin past a
+    token's own position, pages that end inside a tile, NaN in every row that
+    holds no position."""
+    import qff
+    c = Case([start + T], page, io, kv, seed=start + T)
+    g = torch.Generator(device=DEV).manual_seed(T)
+    qg, k, v = (_randn(g, T, *s, dtype=DT[io]) for s in ((16, 512), (2, 256), (2, 256)))
+    for i in range(start, start + T):   # (Case wrote what precedes its last position)
+        at = int(c.table_np[0, i // page])
+        c.kp[at, i % page] = float("nan")
+        c.vp[at, i % page] = float("nan")
+    kb, vb = c.before()
+    got = qff.gqa_prefill_paged(ctx, c.p, qg, k, v, c.kp, c.vp, c.table[0], start_pos=start, out_dtype=DT[out])
+    pos = torch.arange(start, start + T, dtype=torch.int32, device=DEV)
+    want_k = R.rope_norm(k, c.p["k_norm_w"], pos)
+    at, r = c.table[0].long()[pos // page], (pos % page).long()
+    assert torch.equal(c.vp[at, r], v.to(c.kv))
+    step = torch.maximum(want_k.abs() * 2.0 ** (-7 if c.kv == torch.bfloat16 else -10), torch.full_like(want_k, 2.0 ** -18))
+    assert ((c.kp[at, r].double() - want_k).abs() <= step).all()
+    assert_near(got, R.attend(c.p, qg, c.kp, c.vp, c.table[0], pos))
+    kb[at, r], vb[at, r] = c.kp[at, r], c.vp[at, r]
+    assert same_bits(kb, c.kp) and same_bits(vb, c.vp)
+
+
+def test_prefill_paged_short_in_a_small_context(hip):
+    """A context whose partial rows hold few chunks."""
+    import qff
+    small = qff.Context(max_batch=1, max_ctx=2048, max_prefill_tokens=64)
+    c = Case([1900], 16, "f32", "bf16", seed=3)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    qg, k, v = _randn(g, 64, 16, 512), _randn(g, 64, 2, 256), _randn(g, 64, 2, 256)
+    out = qff.gqa_prefill_paged(small, c.p, qg, k, v, c.kp, c.vp, c.table[0], start_pos=1836, out_dtype=torch.float32)
+    pos = torch.arange(1836, 1900, dtype=torch.int32, device=DEV)
+    assert_near(out, R.attend(c.p, qg, c.kp, c.vp, c.table[0], pos))
+    small.close()
+
+
 def test_prefill_paged_against_64_bits(hip, ctx):
     """fp16 operands: 3e-4 of the row (four times it here), and the output's
     own rounding."""
@@ -412,29 +455,29 @@ def test_prefill_paged_against_64_bits(hip, ctx):
     assert rel <= 1.2e-3, float(rel)
 
 
-def test_prefill_pages_outside_the_pool(hip, ctx):
+@pytest.mark.parametrize("T", [100, 129])
+def test_prefill_pages_outside_the_pool(hip, ctx, T):
     """Rows that see a position without a page are NaN, rows before it are not."""
     import qff
     g = torch.Generator(device=DEV).manual_seed(2)
-    T, start = 100, 70
+    start = 170 - T
     p = _params(g)
     qg, k, v = _randn(g, T, 16, 512), _randn(g, T, 2, 256), _randn(g, T, 2, 256)
-    kp, vp = _randn(g, 8, 16, 2, 256, dtype=torch.bfloat16), _randn(g, 8, 16, 2, 256, dtype=torch.bfloat16)
     for entry, first in ((8, 128), (2, 0)):    # positions 128 .. 143, or cached ones
-        kp2, vp2 = torch.cat([kp, kp]), torch.cat([vp, vp])
-        table = torch.arange(11, dtype=torch.int32, device=DEV)
-        table[entry] = 16
-        kb, vb = kp2.clone(), vp2.clone()
-        out = qff.gqa_prefill_paged(ctx, p, qg, k, v, kp2, vp2, table, start_pos=start)
+        kp, vp = _randn(g, 13, 16, 2, 256, dtype=torch.bfloat16), _randn(g, 13, 16, 2, 256, dtype=torch.bfloat16)
+        kp[0], vp[0] = float("nan"), float("nan")     # nobody's
+        table = torch.arange(1, 12, dtype=torch.int32, device=DEV)
+        table[entry] = 13
+        kb, vb = kp.clone(), vp.clone()
+        out = qff.gqa_prefill_paged(ctx, p, qg, k, v, kp, vp, table, start_pos=start)
         nan = torch.isnan(out).all(dim=2).all(dim=1)
         assert torch.equal(nan, torch.arange(start, start + T, device=DEV) >= first)
         assert not torch.isnan(out[~nan]).any()
-        rows = [q for q in range(start, start + T) if q // 16 != entry]
-        for q in rows:
-            kb[q // 16, q % 16], vb[q // 16, q % 16] = kp2[q // 16, q % 16], vp2[q // 16, q % 16]
-        assert same_bits(kb, kp2)
-        assert same_bits(vb, vp2)
-        assert torch.equal(vp2[10, 0], v[160 - start].bfloat16())
+        for q in range(start, start + T):
+            if q // 16 != entry:
+                kb[1 + q // 16, q % 16], vb[1 + q // 16, q % 16] = kp[1 + q // 16, q % 16], vp[1 + q // 16, q % 16]
+        assert same_bits(kb, kp) and same_bits(vb, vp)
+        assert torch.equal(vp[11, 0], v[160 - start].bfloat16())
 
 
 def test_prefill_captured(hip, ctx):

@@ -9,7 +9,11 @@ to its 2-norm; the paged one's within 5e-6), so an attention layer's output
 differs by 1.1e-5 at most; the out-projection and the recurrent layers pass a
 relative difference on without growing it by more than their condition, for
 which 10 is allowed: 1.1e-4 of the step's largest residual update. Prompt
-slices run the same kernels on the same rows: the same bits."""
+slices of more than 128 tokens run the same kernels on the same rows: the same
+bits. Shorter ones take the decode's kernels on pages, where the flat prefill's
+fp16 operands leave 3e-4 of a row: with two attention layers and the same
+allowance of 10, 6.1e-3 of the slice's largest update. The flat stack then goes
+on from the paged one's state, so that the steps are compared by themselves."""
 import pytest
 import torch
 
@@ -56,6 +60,24 @@ def _flat_prefill(st, slot, x, start):
                                    S["k_cache"][slot], S["v_cache"][slot], start_pos=start, out_dtype=torch.float32,
                                    eps=st.eps).view(T, 4096)
         ops.q4_matmul_parts(st.ctx, [L["out_proj"]], core, outs=(x,), residuals=(x,))
+
+
+def _prefill(paged, flat, slot, x, start):
+    """A slice of both, compared; the flat one takes over the paged one's state."""
+    a, b = x.clone(), x.clone()
+    paged.prefill(slot, a, start)
+    _flat_prefill(flat, slot, b, start)
+    if x.shape[0] > 128:
+        assert torch.equal(a, b)
+    assert float((a - b).abs().max() / (b - x).abs().max()) <= 6.1e-3
+    n = paged.pages.lengths[slot]
+    at = paged.pages.table[slot, :-(-n // PAGE)].long()
+    for kind, S, F in zip(paged.kinds, paged.states, flat.states):
+        if kind == "gqa":
+            F["k_cache"][slot, :n] = S["k_pages"][at].flatten(0, 1)[:n]
+            F["v_cache"][slot, :n] = S["v_pages"][at].flatten(0, 1)[:n]
+        else:
+            F["conv_state"][slot], F["ssm_state"][slot] = S["conv_state"][slot], S["ssm_state"][slot]
 
 
 def _flat_fork(st, src, dsts):
@@ -111,11 +133,7 @@ def test_prefill_then_decode(model):
         at = 0
         for T in (n - n // 3, n // 3):
             if T:
-                x = torch.randn(T, 2048, device=DEV, generator=g)
-                a, b = x.clone(), x.clone()
-                paged.prefill(s, a, at)
-                _flat_prefill(flat, s, b, at)
-                assert torch.equal(a, b)
+                _prefill(paged, flat, s, torch.randn(T, 2048, device=DEV, generator=g), at)
                 at += T
     for step in range(3):
         _step(paged, flat, g, [n + step if n else -1 for n in lens])
@@ -129,14 +147,8 @@ def test_fork_decode_release_compact(model, captured):
     child's pages are used again; a compaction in between changes nothing."""
     paged, flat = _stacks(model)
     g = torch.Generator(device=DEV).manual_seed(2)
-    x = torch.randn(300, 2048, device=DEV, generator=g)
-    b = x.clone()
-    paged.prefill(0, x)
-    _flat_prefill(flat, 0, b, 0)
-    other = torch.randn(90, 2048, device=DEV, generator=g)
-    b = other.clone()
-    paged.prefill(5, other)
-    _flat_prefill(flat, 5, b, 0)
+    _prefill(paged, flat, 0, torch.randn(300, 2048, device=DEV, generator=g), 0)
+    _prefill(paged, flat, 5, torch.randn(90, 2048, device=DEV, generator=g), 0)
     graph = None
     if captured:
         graph = {"x": torch.zeros(SLOTS, 2048, device=DEV), "pos": torch.full((SLOTS,), -1, dtype=torch.int32, device=DEV)}
