@@ -846,61 +846,105 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
         }
     }
     d_run = quad_sum(d_run);
-    // ---- the parts joined through LDS (16 KB a wave, in place of the tiles), by
-    // all waves, a row of 256 dims by 64 lanes: piece (dt, kb) of row n lies at
-    // 64 dt + 16 kb + (n ^ dt), so that neither side meets a bank twice
+    // ---- the parts of a row joined through LDS, in place of the tiles
     f32x4_t* const hand = reinterpret_cast<f32x4_t*>(L.tile);
-    __syncthreads();
-    if (active) {
-        if (NT == 3 && single) {
+    auto slot_of = [&](int s) { return (static_cast<size_t>(s) * 2 + kvh) * pp.cstride + slot_c; };
+    if (single) {
+        // 8 rows, each by one wave whole (256 dims by 64 lanes): piece (dt, kb) of
+        // row n lies at 64 dt + 16 kb + (n ^ dt) of its part's 16 KB, so that
+        // neither side meets a bank twice
+        __syncthreads();
+        if (active) {
+            if (NT == 3) {
+#pragma unroll
+                for (int dt = 0; dt < 16; ++dt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) oacc[dt][i] += dpp_mov<0x128>(oacc[dt][i]);
+            }
 #pragma unroll
             for (int dt = 0; dt < 16; ++dt)
+                if (n < 8) hand[1024 * wv + 64 * dt + 16 * kb + (n ^ dt)] = oacc[dt];
+            if (kb == 0) {
+                L.md[wv][n][0] = m_run;
+                L.md[wv][n][1] = d_run;
+            }
+        }
+        __syncthreads();
+        const int piece = 64 * (lane >> 2) + 16 * (lane & 3) + (wv ^ (lane >> 2));
+        float mk[4], m = -INFINITY, d = 0.0f;
+        f32x4_t v[4], o = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) oacc[dt][i] += dpp_mov<0x128>(oacc[dt][i]);
+        for (int k = 0; k < 4; ++k) {
+            mk[k] = L.md[k][wv][0];
+            v[k] = hand[1024 * k + piece];
         }
 #pragma unroll
-        for (int dt = 0; dt < 16; ++dt)
-            if (!single || n < 8) hand[1024 * wv + 64 * dt + 16 * kb + (n ^ dt)] = oacc[dt];
-        if (kb == 0) {
-            L.md[wv][n][0] = m_run;
-            L.md[wv][n][1] = d_run;
+        for (int k = 0; k < 4; ++k) m = fmaxf(m, mk[k]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            // (a part without any position, or whose scores are all NaN, has maximum -inf)
+            const float f = mk[k] == m ? 1.0f : __builtin_amdgcn_exp2f(mk[k] - m);
+            d += f * L.md[k][wv][1];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] += f * v[k][i];
         }
+        const size_t at = slot_of(lead) * 8 + wv;
+        if (lane == 0) {
+            pp.m[at] = m - kShift<KV_F16>;
+            pp.d[at] = d;
+        }
+        *reinterpret_cast<f32x4_t*>(pp.o + at * 256 + 4 * lane) = o;
+        return;
     }
-    __syncthreads();
-    auto join = [&](auto pc) {
-        constexpr int PARTS = decltype(pc)::value;
-        const int rows = 8 * count;
-#pragma unroll 4
-        for (int r = wv; r < rows; r += 8) {   // row r: row r % 16 of row block r / 16
-            const int from = r >> 4, rn = r & 15, piece = 64 * (lane >> 2) + 16 * (lane & 3) + (rn ^ (lane >> 2));
-            float mk[PARTS], m = -INFINITY, d = 0.0f;
-            f32x4_t v[PARTS], o = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 0; k < PARTS; ++k) {
-                mk[k] = L.md[from + R * k][rn][0];
-                v[k] = hand[1024 * (from + R * k) + piece];
-            }
-#pragma unroll
-            for (int k = 0; k < PARTS; ++k) m = fmaxf(m, mk[k]);
-#pragma unroll
-            for (int k = 0; k < PARTS; ++k) {
-                // (a part without any position, or whose scores are all NaN, has maximum -inf)
-                const float f = mk[k] == m ? 1.0f : __builtin_amdgcn_exp2f(mk[k] - m);
-                d += f * L.md[from + R * k][rn][1];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] += f * v[k][i];
-            }
-            const size_t slot = (static_cast<size_t>(lead + (r >> 3)) * 2 + kvh) * pp.cstride + slot_c;
-            if (lane == 0) {
-                pp.m[slot * 8 + (r & 7)] = m - kShift<KV_F16>;
-                pp.d[slot * 8 + (r & 7)] = d;
-            }
-            *reinterpret_cast<f32x4_t*>(pp.o + (slot * 8 + (r & 7)) * 256 + 4 * lane) = o;
+    // a block's rows: two parts each finish half of the dims with the other's
+    // sums (dim tiles 8 part ..); without parts a wave has the whole row
+    const bool mine = active && 2 * rb + (n >> 3) < count;
+    const size_t at = slot_of(seq) * 8 + (n & 7);
+    float* const po = pp.o + at * 256 + 4 * kb;
+    auto store_md = [&](float m, float d) {
+        if (mine && kb == 0) {
+            pp.m[at] = m - kShift<KV_F16>;
+            pp.d[at] = d;
         }
     };
-    if (single) join(std::integral_constant<int, 4>{});
-    else if (parts == 2) join(std::integral_constant<int, 2>{});
-    else join(std::integral_constant<int, 1>{});
+    if (parts == 1) {
+        store_md(m_run, d_run);
+        if (mine) {
+#pragma unroll
+            for (int dt = 0; dt < 16; ++dt) *reinterpret_cast<f32x4_t*>(po + 16 * dt) = oacc[dt];
+        }
+        return;
+    }
+    __syncthreads();
+    auto exchange = [&](auto pc) {
+        constexpr int P = decltype(pc)::value;
+        if (active) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) hand[512 * wv + 64 * c + lane] = oacc[8 * (1 - P) + c];
+            if (kb == 0) {
+                L.md[wv][n][0] = m_run;
+                L.md[wv][n][1] = d_run;
+            }
+        }
+        __syncthreads();
+        if (!mine) return;
+        const int partner = P == 0 ? wv + R : wv - R;
+        const float m1 = L.md[partner][n][0], m = fmaxf(m_run, m1);
+        // (a part without any position, or whose scores are all NaN, has maximum -inf)
+        const float f0 = m_run == m ? 1.0f : __builtin_amdgcn_exp2f(m_run - m);
+        const float f1 = m1 == m ? 1.0f : __builtin_amdgcn_exp2f(m1 - m);
+        if (P == 0) store_md(m, d_run * f0 + L.md[partner][n][1] * f1);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            const f32x4_t v = hand[512 * partner + 64 * c + lane];
+            f32x4_t o;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = oacc[8 * P + c][i] * f0 + v[i] * f1;
+            *reinterpret_cast<f32x4_t*>(po + 16 * (8 * P + c)) = o;
+        }
+    };
+    if (part == 1) exchange(std::integral_constant<int, 1>{});
+    else exchange(std::integral_constant<int, 0>{});
 }
 
 // ---- combine ----------------------------------------------------------------------------
