@@ -385,9 +385,12 @@ int qff_gqa_decode_shared(qff_ctx* ctx, qff_stream_t stream, const qff_gqa_param
 
 /* qff_gqa_prefill on a paged cache: T consecutive tokens of one sequence at
  * positions start_pos .. start_pos + T - 1, whose pages the one row of
- * kv->table names. Arguments, precision and limits otherwise as
- * qff_gqa_prefill (QFF_ERR_INVALID_ARG when start_pos + T exceeds table_cols *
- * page_size); q_gate and out are 16-byte aligned. */
+ * kv->table names. Arguments and limits otherwise as qff_gqa_prefill
+ * (QFF_ERR_INVALID_ARG when start_pos + T exceeds table_cols * page_size); q_gate,
+ * out and the norm weights are 16-byte aligned. Slices of up to 128 tokens (bf16
+ * outputs of an fp16 cache), 42 (fp32 outputs of a bf16 cache) or 64 (others) have
+ * qff_gqa_decode_paged's precision, longer ones the fp16 operands of
+ * qff_gqa_prefill. */
 int qff_gqa_prefill_paged(qff_ctx* ctx, qff_stream_t stream, const qff_gqa_params* p,
                           const void* q_gate, const void* k, const void* v, qff_dtype in_dtype,
                           const qff_kv_pages* kv, int start_pos, void* out, qff_dtype out_dtype,

@@ -23,10 +23,12 @@
 // Both products run on 16x16x32 MFMAs in the cache's type, in which K and V
 // are exact. q and the softmax weights enter as NT terms of that type (hi,
 // the rest rounded again, ...): two bf16 terms carry 16 bits and two fp16
-// terms 22, three bf16 terms 24. bf16 outputs take two terms; fp32 outputs
-// three of bf16 or two of fp16 (error 2e-7 to 7e-7 of the exact output, where
-// two bf16 terms leave 6e-6). fp16 weights are scaled by 2^7 (kShift), so that
-// weights down to 2^-21 of the row's largest keep all bits of their first term.
+// terms 22, three bf16 terms 24. fp32 outputs take three of bf16 or two of fp16
+// (error 2e-7 to 7e-7 of the exact output, where two bf16 terms leave 6e-6);
+// bf16 outputs, whose own rounding is 1.7e-3, two of bf16 (one would add as
+// much again) or one of fp16 (3e-4; 32 sequences over 32K 54.6 us, with two
+// 65). fp16 weights are scaled by 2^7 (kShift), so that weights down to 2^-21
+// of the row's largest keep all bits of their first term.
 #include <algorithm>
 #include <type_traits>
 
@@ -1073,6 +1075,9 @@ static PagedKv paged_kv(const qff_kv_pages* kv) {
                    __builtin_ctz(static_cast<unsigned>(kv->page_size)), kv->table_cols};
 }
 
+// Terms of q and of the weights.
+static int paged_terms(bool kv_f16, bool out16) { return kv_f16 ? (out16 ? 1 : 2) : (out16 ? 2 : 3); }
+
 // The partial launch (a batch's step, or a slice's tokens) and the combine of
 // `rows` sequences or tokens.
 static void launch_partials(qff_ctx* ctx, hipStream_t stream, const qff_gqa_params* p, const void* q_gate,
@@ -1089,9 +1094,12 @@ static void launch_partials(qff_ctx* ctx, hipStream_t stream, const qff_gqa_para
                                                                      p->scale, p->eps, pk, a ? *a : none, tk, pp)
 #define QFF_PART(I, F, N) \
     if (a) QFF_PART1(I, F, N, false); else QFF_PART1(I, F, N, true)
-        if (f16) {
+        const int terms = paged_terms(f16, out16);
+        if (terms == 1) {
+            if (in16) { QFF_PART(1, 1, 1); } else { QFF_PART(0, 1, 1); }
+        } else if (f16) {
             if (in16) { QFF_PART(1, 1, 2); } else { QFF_PART(0, 1, 2); }
-        } else if (out16) {
+        } else if (terms == 2) {
             if (in16) { QFF_PART(1, 0, 2); } else { QFF_PART(0, 0, 2); }
         } else {
             if (in16) { QFF_PART(1, 0, 3); } else { QFF_PART(0, 0, 3); }
@@ -1130,12 +1138,22 @@ hipError_t launch_gqa_decode_paged(qff_ctx* ctx, hipStream_t stream, const qff_g
     return hipGetLastError();
 }
 
-// Slices of at most kPagedTokensMax tokens can take the decode's kernels (see launch_gqa_prefill_paged).
+// A slice of few tokens takes the decode's kernels: blocks of 16 tokens read the
+// pages as they are, where the other path first copies the whole cache (K as
+// fp16, V transposed). Its products take a pass for each term, so the rule is
+// tokens x terms <= 128 (us per call, this / the other path, from position 0,
+// 2000, 20000, 60000):
+//   bf16 cache and outputs (two terms)  8 tokens 16 / 20, 19 / 26, 26 / 45, 37 / 82
+//                                      64 tokens 20 / 23, 32 / 34, 63 / 64, 132 / 136
+//                                      96 tokens 22 / 25, 34 / 34, 81 / 75, 188 / 164
+//   fp16 cache, bf16 outputs (one)    128 tokens 23 / 24, 33 / 35, 79 / 99, 179 / 197
+//   bf16 cache, fp32 outputs (three)   32 tokens 18 / 23, 29 / 30, 50 / 56, 98 / 103
+//                                      64 tokens 21 / 23, 34 / 34, 73 / 67, 164 / 133
 hipError_t launch_gqa_prefill_paged(qff_ctx* ctx, hipStream_t stream, const qff_gqa_params* p, const void* q_gate,
                                     const void* k, const void* v, qff_dtype in_dtype, const qff_kv_pages* kv,
                                     int start, void* out, qff_dtype out_dtype, int T) {
     const int cap = static_cast<int>(std::min<long long>(kGqaMaxChunks, ctx->pf_slots / T));
-    if (T > kPagedTokensMax || cap < 4)
+    if (T * paged_terms(p->kv_f16 != 0, out_dtype == QFF_BF16) > kPagedTokensMax || cap < 4)
         return launch_gqa_prefill(ctx, stream, p, q_gate, k, v, in_dtype, kv->k, kv->v, kv, start, out, out_dtype, T);
     const PagedKv pk = paged_kv(kv);
     {
