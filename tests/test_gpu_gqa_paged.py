@@ -439,16 +439,17 @@ def test_prefill_paged_short(hip, ctx, start, T, io, kv, out, page):
     assert same_bits(kb, c.kp) and same_bits(vb, c.vp)
 
 
-def test_prefill_paged_short_in_a_small_context(hip):
+@pytest.mark.parametrize("kv,out", [("bf16", "f32"), ("bf16", "bf16"), ("f16", "bf16")])
+def test_prefill_paged_short_in_a_small_context(hip, kv, out):
     """A context whose partial rows hold few chunks."""
     import qff
     small = qff.Context(max_batch=1, max_ctx=2048, max_prefill_tokens=64)
-    c = Case([1900], 16, "f32", "bf16", seed=3)
+    c = Case([1900], 16, "f32", kv, seed=3)
     g = torch.Generator(device=DEV).manual_seed(3)
     qg, k, v = _randn(g, 64, 16, 512), _randn(g, 64, 2, 256), _randn(g, 64, 2, 256)
-    out = qff.gqa_prefill_paged(small, c.p, qg, k, v, c.kp, c.vp, c.table[0], start_pos=1836, out_dtype=torch.float32)
+    got = qff.gqa_prefill_paged(small, c.p, qg, k, v, c.kp, c.vp, c.table[0], start_pos=1836, out_dtype=DT[out])
     pos = torch.arange(1836, 1900, dtype=torch.int32, device=DEV)
-    assert_near(out, R.attend(c.p, qg, c.kp, c.vp, c.table[0], pos))
+    assert_near(got, R.attend(c.p, qg, c.kp, c.vp, c.table[0], pos), "", c.kv, fp16_operands=out == "f32")
     small.close()
 
 
