@@ -328,7 +328,7 @@ struct PagedPartials {
 // (what the page holds there may be any bit pattern).
 struct PartLds {
     uint16_t tile[2][2][kTile * 256];   // stage, K / V
-    float md[8][16][2];                 // per wave and row (m, d)
+    float md[8][16][2], mdw[8][32][2];  // per wave and row (m, d), rows 16 or 32 to a wave
     __attribute__((aligned(16))) float sq[4][16][8];   // sums of squares: row block, row, slice of 32 dims
     __attribute__((aligned(16))) float2 turn[4][64];   // row block, angle of the two sequences: cos, sin
 };
@@ -370,7 +370,13 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
         // the block's shared chunks come first among its first sequence's items
         const int npfx = chunks_of(plan.shared, ch);
         const bool pfx = lead == plan.first && item < npfx;
-        const int c = pfx ? item : item - (lead == plan.first ? npfx : 0);
+        int c = pfx ? item : item - (lead == plan.first ? npfx : 0);
+        if (pfx && npfx >= 4) {
+            // rotated so that c = g modulo 4 (but for the last few): the blocks of a
+            // group then read a chunk on the same one of the 8 XCDs, through one L2
+            c += (static_cast<int>(blockIdx.x >> 1) - item) & 3;
+            if (c >= npfx) c -= npfx;
+        }
         count = pfx ? plan.count : 1;
         p_begin = (pfx ? 0 : plan.shared) + c * ch;
         p_end = min(pfx ? plan.shared : plan.len, p_begin + ch);
@@ -385,40 +391,45 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
     const int last_entry = (p_end - 1) >> kv.lg;
     PageWindow win;
 
-    // tile t into stage t & 1: wave wv copies rows 2 wv + 16 i, + 1 of K and V,
-    // i < 4; 16 positions past the chunk's end repeat its last ones (masked;
-    // finite, or zeroed behind the new token). Returns the tile's bad pages as
-    // bits i.
-    auto issue = [&](int t) -> unsigned {
-        const int t0 = p_begin + t * kTile;
-        if ((min(t0 + kTile, p_end) - 1) >> kv.lg > win.base + 63)
-            win.set(t0 >> kv.lg, PageWindow::entry(row, t0 >> kv.lg, last_entry, lane), kv.num_pages);
-        unsigned bad = 0;
+    // the page window to hold tiles from .. to (at most two, 128 positions)
+    auto window = [&](int from, int to) {
+        if ((min(p_begin + (to + 1) * kTile, p_end) - 1) >> kv.lg > win.base + 63) {
+            const int first = (p_begin + from * kTile) >> kv.lg;
+            win.set(first, PageWindow::entry(row, first, last_entry, lane), kv.num_pages);
+        }
+    };
+    // Part i < 4 of tile t into stage t & 1, K or V or both: wave wv copies rows 16 i +
+    // 2 wv, + 1; 16 positions past the chunk's end repeat its last ones (masked;
+    // finite, or zeroed behind the new token). Returns bit i if their page is bad.
+    auto issue_part = [&](int t, int i, bool with_k, bool with_v) -> unsigned {
         const int h = lane >> 5;
         const uint32_t lt = 1024u * h + 16u * ((lane & 31) ^ (2 * h) ^ tile_swz(2 * wv & 15));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int p = min(t0 + 16 * i, (p_end - 1) & ~15);
-            const int entry = p >> kv.lg;
-            const size_t at = (((static_cast<size_t>(win.of(entry)) << kv.lg) + (p & mask) + 2 * wv) * 2 + kvh) * 512;
-            bad |= (win.is_bad(entry) ? 1u : 0u) << i;
-            const char *k = reinterpret_cast<const char*>(kv.k) + at, *v = reinterpret_cast<const char*>(kv.v) + at;
-            const uint32_t lk = lds_addr(&L.tile[t & 1][0][(16 * i + 2 * wv) * 256]);
-            const uint32_t lv = lds_addr(&L.tile[t & 1][1][(16 * i + 2 * wv) * 256]);
-            if (stream) {
-                dma16_nt(k, lt, lk);
-                dma16_nt(v, lt, lv);
-            } else {
-                dma16(k, lt, lk);
-                dma16(v, lt, lv);
-            }
+        const int p = min(p_begin + t * kTile + 16 * i, (p_end - 1) & ~15);
+        const int entry = p >> kv.lg;
+        const size_t at = (((static_cast<size_t>(win.of(entry)) << kv.lg) + (p & mask) + 2 * wv) * 2 + kvh) * 512;
+        const char *k = reinterpret_cast<const char*>(kv.k) + at, *v = reinterpret_cast<const char*>(kv.v) + at;
+        const uint32_t lk = lds_addr(&L.tile[t & 1][0][(16 * i + 2 * wv) * 256]);
+        const uint32_t lv = lds_addr(&L.tile[t & 1][1][(16 * i + 2 * wv) * 256]);
+        if (stream) {
+            if (with_k) dma16_nt(k, lt, lk);
+            if (with_v) dma16_nt(v, lt, lv);
+        } else {
+            if (with_k) dma16(k, lt, lk);
+            if (with_v) dma16(v, lt, lv);
         }
+        return (win.is_bad(entry) ? 1u : 0u) << i;
+    };
+    auto issue = [&](int t, bool with_k, bool with_v) -> unsigned {
+        unsigned bad = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bad |= issue_part(t, i, with_k, with_v);
         return bad;
     };
     const int n = lane & 15, kb = lane >> 4;
     const int nrb = (count + 1) / 2;
     const int R = nrb <= 1 ? 1 : nrb <= 2 ? 2 : nrb <= 4 ? 4 : 8;
     const bool single = count == 1;
+    const bool wide = NT == 1 && R == 8;   // rows 32 to a wave, see below
     const int parts = single ? 4 : R == 8 ? 1 : 2;   // of a tile's positions, one a wave
     const int rb = wv & (R - 1), part = wv / R;
     const bool active = part < parts && rb < nrb;
@@ -472,7 +483,7 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
         }
         if constexpr (ONE && !TOKENS) asm volatile("" : "+v"(kx[0]), "+v"(kx[1]), "+v"(kx[2]), "+v"(kx[3]));
         win.set(p_begin >> kv.lg, entry0, kv.num_pages);
-        bad_next = issue(0);
+        bad_next = issue(0, true, true);
         // cos, sin of angle l % 32 of row block wv's sequence l / 32
         if (wv < RR) {
             float s, c2;
@@ -586,7 +597,7 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
 #pragma unroll
             for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(x[jj][e]), "+v"(w[jj][e]));
         win.set(p_begin >> kv.lg, entry0, kv.num_pages);
-        bad_next = issue(0);
+        bad_next = issue(0, true, !wide);
         float cl, sl, cs[8], sn[8], ss = 0.0f;   // lane l: angle l % 32 of the row block's sequence l / 32
         sincosf(static_cast<float>(pos_a) * freq, &sl, &cl);
 #pragma unroll
@@ -809,6 +820,224 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
             if ((bad >> (z >> 4)) & 1) *tile_at(t, 1, z) = u32x2_t{0u, 0u};
         __syncthreads();
     };
+    // One term, more than eight sequences: the rows go 32 to a wave on 32x32x16
+    // MFMAs, each half of a tile's positions with its own four waves, so that
+    // every K or V operand read feeds 32 rows instead of 16 (with 16 the LDS reads
+    // alone, 512 KB a tile of which the transposed half runs at half rate, take
+    // longer than the products: 3.3 us a tile). Scores S^T = K Q^T of a
+    // tile run interleaved with O^T += V^T P^T of the tile before; a lane's score
+    // and output registers belong to its one q row. With more terms neither q nor
+    // a further accumulator fits beside O^T's 128 registers; on one wave a SIMD
+    // with 512 registers two terms took 67 us where sixteen rows a wave take 61.
+    auto wide_block = [&] {
+        const int rn = lane & 31, h = lane >> 5, r32 = wv & 3, side = wv >> 2;
+        const int sq = lead + min(4 * r32 + (rn >> 3), count - 1);   // of the lane's q row
+        const int limit = TOKENS ? min(p_end, tk.start + sq + 1) : p_end;
+        u32x4_t qw[16];   // B of a 32x32x16 product: column rn, dims 16 u + 8 h + e
+        {
+            // from the 16-row operands that each wave prepared, through the second stage:
+            // piece of dims 16 u + 8 h .. of row r at 64 u + 32 h + r of its 32 rows'
+            u32x4_t* const hand = reinterpret_cast<u32x4_t*>(L.tile[1]);
+#pragma unroll
+            for (int jj = 0; jj < 8; ++jj)
+                hand[1024 * (wv >> 1) + 64 * (2 * jj + (kb >> 1)) + 32 * (kb & 1) + 16 * (wv & 1) + n] = q[0][jj];
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < 16; ++u) qw[u] = hand[1024 * r32 + 64 * u + lane];
+        }
+        float m_w = -INFINITY, d_w = 0.0f;
+        // O^T: register i of dim tile dt has dim 128 (dt / 4) + 16 (dt % 4) + 64 (i / 8) +
+        // 8 (i / 4 % 2) + 4 h + i % 4: a tile's two halves lie 64 dims apart, so that the
+        // transposed reads of 32 lanes (4 rows of each half) meet no bank twice
+        f32x16_t ow[8];
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) ow[dt][i] = 0.0f;
+        // K operand of step u: row rn of the half, piece 2 u + h. V^T operand of a dim
+        // tile and 16 positions: rows 4 h + l % 16 / 4 and 8 on, dims 64 (l / 16 % 2) +
+        // 4 (l % 4) .. + 3 of the tile's, whose transposed reads give a lane's dim the
+        // positions in the order the score registers hold them (slot 8 h + 4 j + i of a
+        // step: position 8 j + 4 h + i)
+        const uint32_t kw = 512u * rn + 16u * (h ^ tile_swz(rn)) + 16384u * side;
+        const int vrow = 4 * h + ((lane & 15) >> 2);
+        const uint32_t vw = 512u * vrow + 16u * ((8 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ tile_swz(vrow)) + 8u * (lane & 1) +
+                            16384u * side;
+        u32x4_t pw[2];   // weights of the tile before, per 16 positions
+        f32x16_t s;
+        unsigned bad_k = 0;
+        // iteration t: scores of tile t (WS), O^T += V^T P^T of tile t - 1 (WV)
+        auto iter = [&](auto ws, auto wvv, int t) {
+            constexpr bool WS = decltype(ws)::value, WV = decltype(wvv)::value;
+            arrive(t);
+            const unsigned bad_v = bad_k;
+            if constexpr (WS) {
+                if (t + 1 < ntiles) window(t, t + 1);
+                bad_k = 0;
+            }
+            if constexpr (WV) {
+                if (TOKENS && !WS) clear_behind(t - 1, p_end - (p_begin + (t - 1) * kTile), kTile);
+                clear_bad(t - 1, bad_v);
+            }
+            const uint32_t ka = lds_addr(L.tile[t & 1][0]) + kw, va = lds_addr(L.tile[(t + 1) & 1][1]) + vw;
+            u32x4_t kf[4];
+            u32x2_t vf[4][2];
+            auto k_read = [&](int u) { kf[u % 4] = lds128(at_xor(ka, 32u * u)); };
+            auto v_read = [&](int u) {   // dim tile u % 8, 16 positions u / 8
+                const uint32_t dims = 32u * (u & 3) + 256u * (u >> 2 & 1);
+                vf[u % 4][0] = lds_tr(at_xor(va, dims) + 8192u * (u >> 3));
+                vf[u % 4][1] = lds_tr(at_xor(va ^ 16u, dims) + 8192u * (u >> 3) + 4096u);   // 8 rows on
+            };
+            if constexpr (WS) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+                for (int u = 0; u < 3; ++u) k_read(u);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < 16; ++u) {
+                    if (u + 3 < 16) k_read(u + 3);
+                    else if constexpr (WV) v_read(u - 13);
+                    s = mfma_32x32x16_f16(kf[u % 4], qw[u], s);
+                    // the next copies, one at a time
+                    if (u % 2 == 0 && u < 8) {
+                        if (t + 1 < ntiles) issue_part(t + 1, u / 2, true, false);
+                    } else if (u % 2 == 0) {
+                        bad_k |= issue_part(t, (u - 8) / 2, false, true);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] *= sc;
+                const int s0 = p_begin + t * kTile + 32 * side;
+                const unsigned bad = bad_k >> (2 * side) & 3;
+                if (s0 + 32 > cut_from || bad) {   // (uniform)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        s[i] = s0 + 8 * (i >> 2) + 4 * h + (i & 3) >= limit ? -INFINITY
+                               : (bad >> (i >> 3)) & 1                       ? __builtin_nanf("")
+                                                                             : s[i];
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < 3; ++u) v_read(u);
+            }
+            // PV's 16 products with the softmax of the new scores between them
+            float tm, alpha = 1.0f, mb;
+            bool raised = false;
+#pragma unroll
+            for (int u = 0; u < 16; ++u) {
+                if constexpr (WV) {
+                    if (u + 3 < 16) v_read(u + 3);
+                    ow[u & 7] = mfma_32x32x16_f16(u32x4_t{vf[u % 4][0][0], vf[u % 4][0][1], vf[u % 4][1][0], vf[u % 4][1][1]},
+                                                  pw[u >> 3], ow[u & 7]);
+                }
+                if constexpr (WS) {
+                    if (u < 4) {
+                        const float m4 = fmaxf(fmaxf(s[4 * u], s[4 * u + 1]), fmaxf(s[4 * u + 2], s[4 * u + 3]));
+                        tm = u == 0 ? m4 : fmaxf(tm, m4);
+                    } else if (u == 4) {
+                        const auto h2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(tm), __float_as_uint(tm), false, false);
+                        tm = fmaxf(__uint_as_float(h2[0]), __uint_as_float(h2[1]));
+                        raised = __any(tm > m_w + kLazyMax);
+                        if (raised) {
+                            const float m_new = tm > m_w + kLazyMax ? tm : m_w;
+                            alpha = m_new == m_w ? 1.0f : __builtin_amdgcn_exp2f(m_w - m_new);
+                            m_w = m_new;
+                            d_w *= alpha;
+                        }
+                        // (a half behind the chunk's end, or before a token's first position, gives weights of 0)
+                        mb = m_w == -INFINITY ? 0.0f : m_w - kShift<KV_F16>;
+                    } else if (u < 13) {
+                        const int i = 2 * (u - 5);
+                        s[i] = __builtin_amdgcn_exp2f(s[i] - mb);
+                        s[i + 1] = __builtin_amdgcn_exp2f(s[i + 1] - mb);
+                        d_w += s[i] + s[i + 1];
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if constexpr (WS) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) pw[i >> 2][i & 3] = pack_f16x2(s[2 * i], s[2 * i + 1]);
+                if (raised) {
+#pragma unroll
+                    for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) ow[dt][i] *= alpha;
+                }
+            }
+        };
+        iter(std::true_type{}, std::false_type{}, 0);
+        for (int t = 1; t < ntiles; ++t) iter(std::true_type{}, std::true_type{}, t);
+        iter(std::false_type{}, std::true_type{}, ntiles);
+        const auto h2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(d_w), __float_as_uint(d_w), false, false);
+        d_w = __uint_as_float(h2[0]) + __uint_as_float(h2[1]);
+        // each side finishes half of a row's dims (dim tiles 4 side ..) with the other's
+        // sums. Two pieces of four dims change places between rows 0-15 and 16-31,
+        // so that a store writes 64 bytes of 16 rows instead of 32 bytes of 32.
+        int l = lane;   // (opaque: computed ahead of the loop, the addresses would cost it registers)
+        asm volatile("" : "+v"(l));
+        auto slot_row = [&](int s) { return ((static_cast<size_t>(s) * 2 + kvh) * pp.cstride + slot_c) * 8 + (l & 7); };
+        const int s_lo = lead + 4 * r32 + ((l >> 3) & 1), n_out = 8 * ((l >> 4) & 1) + 4 * (l >> 5);
+        const bool mine_lo = s_lo < lead + count, mine_hi = s_lo + 2 < lead + count;
+        float* const po_lo = pp.o + slot_row(mine_lo ? s_lo : lead) * 256 + n_out;
+        float* const po_hi = pp.o + slot_row(mine_hi ? s_lo + 2 : lead) * 256 + n_out;
+        f32x4_t* const hand = reinterpret_cast<f32x4_t*>(L.tile);   // 16 KB a wave, one piece a lane and index
+        __syncthreads();
+        auto exchange = [&](auto pc) {
+            constexpr int P = decltype(pc)::value;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    hand[1024 * wv + 64 * (4 * c + j) + lane] =
+                        f32x4_t{ow[4 * (1 - P) + c][4 * j], ow[4 * (1 - P) + c][4 * j + 1], ow[4 * (1 - P) + c][4 * j + 2],
+                                ow[4 * (1 - P) + c][4 * j + 3]};
+            if (h == 0) {
+                L.mdw[wv][rn][0] = m_w;
+                L.mdw[wv][rn][1] = d_w;
+            }
+            __syncthreads();
+            const int partner = wv ^ 4;
+            const float m1 = L.mdw[partner][rn][0], m = fmaxf(m_w, m1);
+            const float f0 = m_w == m ? 1.0f : __builtin_amdgcn_exp2f(m_w - m);
+            const float f1 = m1 == m ? 1.0f : __builtin_amdgcn_exp2f(m1 - m);
+            if (P == 0 && l < 32 && 4 * r32 + (l >> 3) < count) {
+                const size_t at = slot_row(lead + 4 * r32 + (l >> 3));
+                pp.m[at] = m - kShift<KV_F16>;
+                pp.d[at] = d_w * f0 + L.mdw[partner][rn][1] * f1;
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int j = 0; j < 4; j += 2) {
+                    const f32x4_t v0 = hand[1024 * partner + 64 * (4 * c + j) + lane];
+                    const f32x4_t v1 = hand[1024 * partner + 64 * (4 * c + j + 1) + lane];
+                    f32x4_t lo, hi;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const auto r = __builtin_amdgcn_permlane16_swap(
+                            __float_as_uint(ow[4 * P + c][4 * j + i] * f0 + v0[i] * f1),
+                            __float_as_uint(ow[4 * P + c][4 * j + 4 + i] * f0 + v1[i] * f1), false, false);
+                        lo[i] = __uint_as_float(r[0]);
+                        hi[i] = __uint_as_float(r[1]);
+                    }
+                    const int dim = 128 * P + 16 * c + 32 * j;
+                    if (mine_lo) *reinterpret_cast<f32x4_t*>(po_lo + dim) = lo;
+                    if (mine_hi) *reinterpret_cast<f32x4_t*>(po_hi + dim) = hi;
+                }
+        };
+        if (side == 1) exchange(std::integral_constant<int, 1>{});
+        else exchange(std::integral_constant<int, 0>{});
+    };
+    if constexpr (NT == 1) {
+        if (wide) {
+            prepare_own();
+            wide_block();
+            return;
+        }
+    }
     if (single) {
         prepare(std::integral_constant<int, 1>{}, std::true_type{});
         clear();
@@ -817,7 +1046,8 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
             const unsigned bad = bad_next;
             const int t0 = p_begin + t * kTile;
             if (t + 1 < ntiles) {
-                bad_next = issue(t + 1);
+                window(t + 1, t + 1);
+                bad_next = issue(t + 1, true, true);
             } else if (TOKENS || has_new) {
                 const int r = p_end - t0;
                 if (!TOKENS && (wv == 4 || wv == 5)) *tile_at(t, wv - 4, r - 1) = fresh;   // the new token's row
@@ -831,14 +1061,16 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
         if (R == 1) prepare(std::integral_constant<int, 1>{}, std::false_type{});
         else if (R == 2) prepare(std::integral_constant<int, 2>{}, std::false_type{});
         else if (R == 4) prepare(std::integral_constant<int, 4>{}, std::false_type{});
-        else prepare_own();
+        else if constexpr (NT > 1) prepare_own();
         clear();
         for (int t = 0; t < ntiles; ++t) {
             arrive(t);
             const unsigned bad = bad_next;
             const int t0 = p_begin + t * kTile;
-            if (t + 1 < ntiles) bad_next = issue(t + 1);
-            else if (TOKENS) clear_behind(t, p_end - t0, (p_end - t0 + 31) & ~31);
+            if (t + 1 < ntiles) {
+                window(t + 1, t + 1);
+                bad_next = issue(t + 1, true, true);
+            } else if (TOKENS) clear_behind(t, p_end - t0, (p_end - t0 + 31) & ~31);
             clear_bad(t, bad);
             if (!active) continue;
 #pragma unroll 1
