@@ -64,6 +64,7 @@ struct PagedSeqs {
     int batch, max_ctx;
     int slots;   // workgroups of one round, per kv head
     int cap;     // chunks allowed per sequence
+    int terms;   // of q and the weights
 };
 
 // A prompt slice instead of a batch: T tokens of one sequence from position
@@ -118,11 +119,19 @@ __device__ __forceinline__ LanePlan lane_plan(const PagedSeqs& a, int b0, int la
 }
 
 __device__ __forceinline__ int chunks_of(int n, int ch) { return (n + ch - 1) / ch; }
+// Chunk length of a sequence's own positions. A tile of a block of eight row
+// blocks costs about two of a single sequence with more than one term (3.5 us
+// from L2 to 1.1 - 2.1), so the sequences behind such a block get chunks twice
+// as long: 32 sequences on a prefix of 32K, bf16, 58.5 -> 55.8 us, of 8K with
+// fp32 outputs 36.6 -> 33.9. With one term (2.1 us) it loses, 45.5 -> 48.5.
+__device__ __forceinline__ int own_chunk(const PagedSeqs& a, const LanePlan& p, int ch) {
+    return p.shared > 0 && p.count > 8 && a.terms > 1 ? 2 * ch : ch;
+}
 
 // Workgroups (per kv head) of the sequence in this lane at chunk length ch:
 // its own chunks, and its block's shared ones in the block's first lane.
-__device__ __forceinline__ int items_of(const LanePlan& p, int ch, int lane) {
-    return chunks_of(p.own(), ch) + (p.first == lane ? chunks_of(p.shared, ch) : 0);
+__device__ __forceinline__ int items_of(const PagedSeqs& a, const LanePlan& p, int ch, int lane) {
+    return chunks_of(p.own(), own_chunk(a, p, ch)) + (p.first == lane ? chunks_of(p.shared, ch) : 0);
 }
 
 // The call's chunk length, whole tiles, and whether it reads so much that
@@ -141,8 +150,8 @@ __device__ __forceinline__ Chunk chunk_length(const PagedSeqs& a, const LanePlan
     int streams = 0, longest = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
         const LanePlan p = b0 == 0 ? p0 : lane_plan(a, b0, lane);
-        tiles += wave_sum_int(items_of(p, kTile, lane));
-        streams += wave_sum_int(items_of(p, 1 << 30, lane));
+        tiles += wave_sum_int(items_of(a, p, kTile, lane));
+        streams += wave_sum_int((p.own() > 0) + (p.first == lane && p.shared > 0));
         longest = max(longest, wave_max_int(p.len));
     }
     // sum of ceil(n / ch) is about tiles / ch + streams / 2, and at most tiles / ch + streams
@@ -150,7 +159,7 @@ __device__ __forceinline__ Chunk chunk_length(const PagedSeqs& a, const LanePlan
     int ch = static_cast<int>((tiles + free - 1) / free);
     const int sure = streams < a.slots ? static_cast<int>((tiles + a.slots - streams - 1) / (a.slots - streams)) : ch;
     if (a.batch <= 64) {
-        while (ch < sure && wave_sum_int(items_of(p0, ch * kTile, lane)) > a.slots) ch += (ch + 15) / 16;
+        while (ch < sure && wave_sum_int(items_of(a, p0, ch * kTile, lane)) > a.slots) ch += (ch + 15) / 16;
     } else {
         ch = sure;
     }
@@ -168,7 +177,7 @@ __device__ __forceinline__ int find_item(const PagedSeqs& a, const LanePlan& p0,
     c = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
         const LanePlan p = b0 == 0 ? p0 : lane_plan(a, b0, lane);
-        const int mine = items_of(p, ch, lane);
+        const int mine = items_of(a, p, ch, lane);
         const int incl = base + wave_inclusive_scan_int(mine);
         const unsigned long long hit = __ballot(incl > g);
         if (hit) {
@@ -378,8 +387,9 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
             if (c >= npfx) c -= npfx;
         }
         count = pfx ? plan.count : 1;
-        p_begin = (pfx ? 0 : plan.shared) + c * ch;
-        p_end = min(pfx ? plan.shared : plan.len, p_begin + ch);
+        const int step = pfx ? ch : own_chunk(a, plan, ch);
+        p_begin = (pfx ? 0 : plan.shared) + c * step;
+        p_end = min(pfx ? plan.shared : plan.len, p_begin + step);
         has_new = !pfx && p_end == plan.len;
         slot_c = pfx ? c : npfx + c;
         cut_from = p_end;
@@ -1361,7 +1371,8 @@ hipError_t launch_gqa_decode_paged(qff_ctx* ctx, hipStream_t stream, const qff_g
                                    void* out, qff_dtype out_dtype, int batch) {
     const PagedKv pk = paged_kv(kv);
     const int cap = gqa_chunk_cap(ctx->cfg, batch);
-    const PagedSeqs a{positions, group, shared_len, batch, kv->table_cols << pk.lg, ctx->num_cu / 2, cap};
+    const PagedSeqs a{positions, group, shared_len, batch, kv->table_cols << pk.lg, ctx->num_cu / 2, cap,
+                      paged_terms(p->kv_f16 != 0, out_dtype == QFF_BF16)};
     const PagedPartials pp{ctx->gqa_m, ctx->gqa_d, ctx->gqa_o, ctx->gqa_nc, cap};
     // a round of workgroups, and one more for each stream of positions (a
     // sequence's own, a block's shared ones) that rounding up can add
