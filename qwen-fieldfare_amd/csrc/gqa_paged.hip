@@ -26,8 +26,7 @@
 // terms 22, three bf16 terms 24. fp32 outputs take three of bf16 or two of fp16
 // (error 2e-7 to 7e-7 of the exact output, where two bf16 terms leave 6e-6);
 // bf16 outputs, whose own rounding is 1.7e-3, two of bf16 (one would add as
-// much again) or one of fp16 (3e-4; 32 sequences over 32K 54.6 us, with two
-// 65). fp16 weights are scaled by 2^7 (kShift), so that weights down to 2^-21
+// much again) or one of fp16 (3e-4; 32 sequences over 32K 45 us, with two 65). fp16 weights are scaled by 2^7 (kShift), so that weights down to 2^-21
 // of the row's largest keep all bits of their first term.
 #include <algorithm>
 #include <type_traits>
@@ -323,6 +322,7 @@ struct PagedPartials {
 //   16 q rows (two sequences x 8 heads): wave w takes row block w % R, and all
 //   64 positions where R = 8, otherwise half w / R of them. Per 32 positions a
 //   wave reads 16 KB of K and 16 KB of V operands for 32 NT MFMAs.
+//   With one term and R = 8 the rows go 32 to a wave (see wide_block).
 //   A single sequence's 8 rows: waves 0-3 take 16 positions each, the products
 //   of two terms in one MFMA (see single_step).
 // Waves beyond these only copy. In both
@@ -342,7 +342,12 @@ struct PartLds {
     __attribute__((aligned(16))) float2 turn[4][64];   // row block, angle of the two sequences: cos, sin
 };
 
-__device__ __forceinline__ int tile_swz(int r) { return ((r & 7) << 1) | ((r >> 3) & 1); }
+// 16-byte piece p of a tile's row r lies at p ^ tile_swz(r): the 16 pieces that 16
+// rows have in one column are apart, and so are those of rows 0-3 and 12-15 from
+// the next column's of rows 4-11, which b128 reads take together (with 1 in
+// place of 9 a third of the LDS cycles were conflicts, now 3-5 %; the times are
+// the same).
+__device__ __forceinline__ int tile_swz(int r) { return ((r & 7) << 1) ^ (((r >> 3) & 1) * 9); }
 
 template <int IN_DT, int KV_F16, int NT, bool TOKENS>
 __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
@@ -832,13 +837,15 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
     };
     // One term, more than eight sequences: the rows go 32 to a wave on 32x32x16
     // MFMAs, each half of a tile's positions with its own four waves, so that
-    // every K or V operand read feeds 32 rows instead of 16 (with 16 the LDS reads
-    // alone, 512 KB a tile of which the transposed half runs at half rate, take
-    // longer than the products: 3.3 us a tile). Scores S^T = K Q^T of a
-    // tile run interleaved with O^T += V^T P^T of the tile before; a lane's score
-    // and output registers belong to its one q row. With more terms neither q nor
-    // a further accumulator fits beside O^T's 128 registers; on one wave a SIMD
-    // with 512 registers two terms took 67 us where sixteen rows a wave take 61.
+    // every K or V operand read feeds 32 rows instead of 16 (256 KB of LDS reads a
+    // tile instead of 512). A tile takes 2.1 us from L2, 2.2 with 32 sequences
+    // over 32K; that call 51.4 -> 45.2 us. A lane's score and output registers
+    // belong to its one q row. Iteration t computes the scores of tile t and then O^T
+    // += V^T P^T of tile t - 1, with the softmax of the new scores between its
+    // products; K is copied a tile ahead of V. (The two waves of a SIMD in opposite
+    // order: 2.5 us.) With more terms q does not fit beside O^T's 128 registers;
+    // on one wave a SIMD with 512 registers two terms took 67 us where sixteen rows
+    // a wave take 61.
     auto wide_block = [&] {
         const int rn = lane & 31, h = lane >> 5, r32 = wv & 3, side = wv >> 2;
         const int sq = lead + min(4 * r32 + (rn >> 3), count - 1);   // of the lane's q row
@@ -896,7 +903,7 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
             auto v_read = [&](int u) {   // dim tile u % 8, 16 positions u / 8
                 const uint32_t dims = 32u * (u & 3) + 256u * (u >> 2 & 1);
                 vf[u % 4][0] = lds_tr(at_xor(va, dims) + 8192u * (u >> 3));
-                vf[u % 4][1] = lds_tr(at_xor(va ^ 16u, dims) + 8192u * (u >> 3) + 4096u);   // 8 rows on
+                vf[u % 4][1] = lds_tr(at_xor(va ^ 144u, dims) + 8192u * (u >> 3) + 4096u);   // 8 rows on
             };
             if constexpr (WS) {
 #pragma unroll
@@ -1389,7 +1396,7 @@ hipError_t launch_gqa_decode_paged(qff_ctx* ctx, hipStream_t stream, const qff_g
 //   bf16 cache and outputs (two terms)  8 tokens 16 / 20, 19 / 26, 26 / 45, 37 / 82
 //                                      64 tokens 20 / 23, 32 / 34, 63 / 64, 132 / 136
 //                                      96 tokens 22 / 25, 34 / 34, 81 / 75, 188 / 164
-//   fp16 cache, bf16 outputs (one)    128 tokens 23 / 24, 33 / 35, 79 / 99, 179 / 197
+//   fp16 cache, bf16 outputs (one)    128 tokens 24 / 24, 32 / 35, 69 / 99, 160 / 197
 //   bf16 cache, fp32 outputs (three)   32 tokens 18 / 23, 29 / 30, 50 / 56, 98 / 103
 //                                      64 tokens 21 / 23, 34 / 34, 73 / 67, 164 / 133
 hipError_t launch_gqa_prefill_paged(qff_ctx* ctx, hipStream_t stream, const qff_gqa_params* p, const void* q_gate,
