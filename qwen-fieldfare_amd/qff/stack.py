@@ -58,6 +58,7 @@ class AttentionStack:
         self.pages = pages
         if pages is not None and len(pages.lengths) != batch:
             raise ValueError(f"the page table must have {batch} slots")
+        self._parked = {}   # slot -> its recurrent states, while it sits out decode steps
         self.kinds = list(kinds) if kinds is not None else \
             ["gqa" if is_full_attention(l) else "dn" for l in range(len(self.layers))]
         if states is None:
@@ -121,6 +122,24 @@ class AttentionStack:
 
     # ---- sequences of a paged stack ------------------------------------------
 
+    def _paged(self):
+        if self.pages is None:
+            raise ValueError("the stack was made without pages")
+        return self.pages
+
+    def _recurrent(self):
+        return [S[k] for kind, S in zip(self.kinds, self.states) if kind == "dn" for k in ("conv_state", "ssm_state")]
+
+    def _park(self, slot: int):
+        """Keeps a slot's recurrent states aside: a decode step advances those of
+        every slot, and a slot without a position has no input."""
+        if slot not in self._parked:
+            self._parked[slot] = [t[slot].clone() for t in self._recurrent()]
+
+    def _unpark(self, slot: int):
+        for t, kept in zip(self._recurrent(), self._parked.pop(slot, [])):
+            t[slot].copy_(kept)
+
     def _copy_pages(self, src, dst):
         pools = [S[k] for kind, S in zip(self.kinds, self.states) if kind == "gqa" for k in ("k_pages", "v_pages")]
         if src and pools:
@@ -128,29 +147,45 @@ class AttentionStack:
 
     def reserve(self, positions):
         """Places for one decode step's tokens: positions[b] is the new token's
-        position in slot b, negative for a slot that takes no part. Pages that a
-        slot shares and is about to write are copied. Where the pool runs out
-        (OutOfPages), the slots before that one have theirs."""
-        copies = []
+        position in slot b, negative for a slot that takes no part (what it holds
+        stays as it is, for a later step or slice). Pages that a slot shares and is
+        about to write are copied; an empty slot's position 0 begins a sequence
+        (zero recurrent states). Where the pool runs out (OutOfPages), the slots
+        before that one have theirs."""
+        pages, copies = self._paged(), []
+        if len(positions) != self.B:
+            raise ValueError(f"positions must have {self.B} entries")
         try:
             for b, p in enumerate(positions):
-                if p >= 0:
-                    copies += self.pages.reserve(b, p, p + 1)
+                if p < 0:
+                    if pages.lengths[b]:
+                        self._park(b)
+                    continue
+                empty = not pages.lengths[b]
+                copies += pages.reserve(b, p, p + 1)
+                if empty:
+                    for t in self._recurrent():
+                        t[b].zero_()
+                self._unpark(b)
         finally:
             self._copy_pages([s for s, _ in copies], [d for _, d in copies])
             self.pages.sync()
 
     def prefill(self, slot: int, x: torch.Tensor, start: int = 0):
         """A prompt slice of T tokens of one slot through every layer: x [T, 2048]
-        fp32 (the residual stream, in place) at positions start .. start + T - 1;
-        start 0 begins a sequence (zero recurrent states)."""
+        fp32 (the residual stream, in place) at positions start .. start + T - 1,
+        behind those that the slot holds; start 0 begins a sequence in an empty slot
+        (zero recurrent states)."""
         if x.dtype != torch.float32 or x.dim() != 2 or x.shape[1] != HIDDEN:
             raise ValueError(f"x must be float32 [T, {HIDDEN}]")
-        P, T, ctx, eps = self.pages, x.shape[0], self.ctx, self.eps
+        P, T, ctx, eps = self._paged(), x.shape[0], self.ctx, self.eps
         if T > ctx.cfg.max_prefill_tokens or start + T > ctx.cfg.max_ctx:
             raise ValueError(f"{T} tokens from {start}: the context takes slices of {ctx.cfg.max_prefill_tokens} up to "
                              f"position {ctx.cfg.max_ctx}")
+        if start != P.lengths[slot] and "dn" in self.kinds:
+            raise ValueError(f"slot {slot} holds {P.lengths[slot]} positions: a slice follows them, or begins in a released slot")
         copies = P.reserve(slot, start, start + T)
+        self._unpark(slot)
         self._copy_pages([s for s, _ in copies], [d for _, d in copies])
         P.sync()
         for kind, L, S in zip(self.kinds, self.layers, self.states):
@@ -172,11 +207,12 @@ class AttentionStack:
         """Slots `dsts` (empty) go on from where slot src stands: its pages are
         held by all, its recurrent states copied. Neighbouring slots read what
         they share once."""
-        dsts = list(dsts)
-        if src in dsts or len(set(dsts)) < len(dsts) or any(self.pages.lengths[d] for d in dsts):
+        dsts, pages = list(dsts), self._paged()
+        if src in dsts or len(set(dsts)) < len(dsts) or any(pages.lengths[d] for d in dsts):
             raise ValueError("a fork goes into empty slots")
         for d in dsts:
-            self.pages.fork(src, d)
+            pages.fork(src, d)
+        self._unpark(src)
         recurrent = [S for kind, S in zip(self.kinds, self.states) if kind == "dn"]
         if dsts and recurrent:
             for k in ("conv_state", "ssm_state"):
@@ -185,13 +221,14 @@ class AttentionStack:
 
     def release(self, slot: int):
         """Ends a slot's sequence; pages that no other slot holds are free again."""
-        self.pages.release(slot)
+        self._paged().release(slot)
+        self._parked.pop(slot, None)
         self.pages.sync()
 
     def compact(self) -> int:
         """Moves the pages in use to the front of every pool; returns their
         number."""
-        self._copy_pages(*self.pages.compact())
+        self._copy_pages(*self._paged().compact())
         self.pages.sync()
         return int((self.pages.refs > 0).sum())
 

@@ -184,6 +184,83 @@ def test_fork_decode_release_compact(model, captured):
     _same_cache(paged, flat, [0, 1, 2, 3, 5])
 
 
+@pytest.mark.parametrize("captured", [False, True])
+def test_slots_that_sit_out_steps(model, captured):
+    """A slot between two slices of its prompt and one between two steps sit out
+    other slots' steps: they go on as if those had not been (the same kernels on
+    the same inputs: the same bits as in a stack that has them alone, but for the
+    split of the attention, 2e-5 of a step's largest update: 5e-6 for each of the two
+    attention layers of either). A parked slot is forked; a sequence begins by a step."""
+    paged, _ = _stacks(model)
+    alone, _ = _stacks(model)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    rows = lambda n: torch.randn(n, 2048, device=DEV, generator=g)
+    graph = None
+    if captured:
+        graph = {"x": torch.zeros(SLOTS, 2048, device=DEV), "pos": torch.full((SLOTS,), -1, dtype=torch.int32, device=DEV)}
+        paged.decode_step(graph["x"], graph["pos"])
+        torch.cuda.synchronize()
+        graph["graph"] = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph["graph"]):
+            paged.decode_step(graph["x"], graph["pos"])
+
+    def steps(st, positions, xs, graph=None):
+        st.reserve(positions)
+        x, pos = xs.clone(), torch.tensor(positions, dtype=torch.int32, device=DEV)
+        if graph is None:
+            st.decode_step(x, pos)
+            return x
+        graph["x"].copy_(x)
+        graph["pos"].copy_(pos)
+        graph["graph"].replay()
+        return graph["x"].clone()
+
+    def close(a, b, x):
+        assert not torch.isnan(a).any()
+        assert float((a - b).abs().max() / (b - x).abs().max()) <= 2e-5
+
+    first, second, other = rows(150), rows(140), rows(200)
+    for st in (paged, alone):
+        a, b = first.clone(), other.clone()
+        st.prefill(0, a)
+        st.prefill(3, b)
+    # slot 3 steps while slot 0 waits for its second slice
+    for i in range(3):
+        xs = rows(SLOTS)
+        got = steps(paged, [-1, -1, -1, 200 + i, -1, -1], xs, graph)
+        want = steps(alone, [-1, -1, -1, 200 + i, -1, -1], xs)
+        close(got[3], want[3], xs[3])
+    a, b = second.clone(), second.clone()
+    paged.prefill(0, a, 150)
+    lone, _ = _stacks(model)
+    c = first.clone()
+    lone.prefill(0, c)
+    lone.prefill(0, b, 150)
+    assert torch.equal(a, b)
+    with pytest.raises(ValueError):
+        paged.prefill(0, second.clone(), 150)
+    # slot 3 sits out, slot 0 steps; slot 3 is forked meanwhile; slot 5 begins by a step
+    xs = rows(SLOTS)
+    close(steps(paged, [290, -1, -1, -1, -1, -1], xs, graph)[0], steps(lone, [290, -1, -1, -1, -1, -1], xs)[0], xs[0])
+    paged.fork(3, [4])
+    alone.fork(3, [4])
+    fresh, _ = _stacks(model)
+    xs = rows(SLOTS)
+    got = steps(paged, [-1, -1, -1, 203, 203, 0], xs, graph)
+    want = steps(alone, [-1, -1, -1, 203, 203, -1], xs)
+    for s in (3, 4):
+        close(got[s], want[s], xs[s])
+    close(got[5], steps(fresh, [-1] * 5 + [0], xs)[5], xs[5])
+
+
+def test_calls_of_a_stack_without_pages(model):
+    _, flat = _stacks(model)
+    for call in (lambda: flat.reserve([-1] * SLOTS), lambda: flat.prefill(0, torch.zeros(4, 2048, device=DEV)),
+                 lambda: flat.fork(0, [1]), lambda: flat.release(0), lambda: flat.compact()):
+        with pytest.raises(ValueError):
+            call()
+
+
 def test_out_of_pages_changes_nothing(model):
     from qff.pages import OutOfPages
     paged, _ = _stacks(model, pages=3)
