@@ -387,7 +387,7 @@ int qff_gqa_decode_shared(qff_ctx* ctx, qff_stream_t stream, const qff_gqa_param
  * positions start_pos .. start_pos + T - 1, whose pages the one row of
  * kv->table names. Arguments and limits otherwise as qff_gqa_prefill
  * (QFF_ERR_INVALID_ARG when start_pos + T exceeds table_cols * page_size); q_gate,
- * out and the norm weights are 16-byte aligned. Slices of up to 128 tokens (bf16
+ * k, v, out and the norm weights are 16-byte aligned. Slices of up to 128 tokens (bf16
  * outputs of an fp16 cache), 42 (fp32 outputs of a bf16 cache) or 64 (others) have
  * qff_gqa_decode_paged's precision, longer ones the fp16 operands of
  * qff_gqa_prefill. */

@@ -480,7 +480,9 @@ int qff_gqa_prefill_paged(qff_ctx* ctx, qff_stream_t stream, const qff_gqa_param
     if (!ctx || !q_gate || !k || !v || !out) return QFF_ERR_INVALID_ARG;
     if (const int st = gqa_params_status(p)) return st;
     if (!dtype_ok(in_dtype) || !dtype_ok(out_dtype)) return QFF_ERR_INVALID_ARG;
-    if (!aligned16(q_gate) || !aligned16(out) || !aligned16(p->q_norm_w)) return QFF_ERR_INVALID_ARG;
+    if (!aligned16(q_gate) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(p->q_norm_w) ||
+        !aligned16(p->k_norm_w))
+        return QFF_ERR_INVALID_ARG;
     if (T <= 0 || start_pos < 0) return QFF_ERR_INVALID_ARG;
     if (const int st = kv_pages_status(ctx, kv)) return st;
     const long long end = static_cast<long long>(start_pos) + T;

@@ -57,6 +57,8 @@ int main() {
         EXPECT(want, qff_gqa_prefill_paged(&ctx, nullptr, &p, a, a, a, QFF_F32, &k, 0, a, QFF_F32, 65));
         EXPECT(want, qff_gqa_decode_shared(&ctx, nullptr, &p, a, a, a, QFF_F32, &k, ints, ints, ints, a, QFF_F32, 5));
     }
+    EXPECT(I, qff_gqa_prefill_paged(&ctx, nullptr, &p, a, odd, a, QFF_F32, &kv, 0, a, QFF_F32, 65));
+    EXPECT(I, qff_gqa_prefill_paged(&ctx, nullptr, &p, a, a, odd, QFF_F32, &kv, 0, a, QFF_F32, 65));
     qff_kv_pages big = kv;
     big.page_size = 8192;
     big.table_cols = 1;
