@@ -330,6 +330,34 @@ def test_decode_shared_long_prefix(hip):
     big.close()
 
 
+@pytest.mark.parametrize("kv,out", [("f16", "bf16"), ("bf16", "bf16")])
+def test_decode_shared_large_blocks_long_chunks(hip, kv, out):
+    """Four groups of 16 over 36000 positions in pages of 16: a large block's
+    chunks of more pages than a wave holds table entries at once, and what
+    follows each prefix in chunks of its own."""
+    import qff
+    big = qff.Context(max_batch=64, max_ctx=40_000, max_prefill_tokens=1)
+    c, group, shared = _groups([16] * 4, [36000, 35984, 36000 - 16 * 7, 33333], [1, 700, 90, 2000], 16, io="bf16", kv=kv, seed=16)
+    before = c.before()
+    c.check(qff.gqa_decode_shared(big, *c.args(), group, shared, out_dtype=DT[out]), before, seqs=(0, 13, 16, 33, 47, 63))
+    big.close()
+
+
+@pytest.mark.parametrize("kv,out", [("f16", "bf16"), ("bf16", "bf16"), ("bf16", "f32")])
+@pytest.mark.parametrize("where", [0, 9, 14])
+def test_decode_shared_large_blocks_pages_outside_the_pool(hip, ctx, kv, out, where):
+    """A bad entry in the prefix of a group of 12 (at its start, inside, in its
+    last tile): the whole group is NaN, the group next to it is not."""
+    import qff
+    c, group, shared = _groups([12, 11], [960, 960], [1, 70, 5], 64, io="bf16", kv=kv, seed=where)
+    c.table[0, where] = c.kp.shape[0] + 5
+    out = qff.gqa_decode_shared(ctx, *c.args(), group, shared, out_dtype=DT[out])
+    assert torch.isnan(out[:12]).all()
+    for b in (12, 17, 22):
+        assert_near(out[b], R.attend(c.p, c.qg[b:b + 1], c.kp, c.vp, c.table[b], c.pos[b:b + 1])[0], b, c.kv)
+    assert not torch.isnan(out[12:]).any()
+
+
 # --------------------------------------------------------- graphs and streams
 
 @pytest.mark.parametrize("shared", [False, True])
@@ -468,16 +496,16 @@ def test_prefill_paged_against_64_bits(hip, ctx):
     assert rel <= 1.2e-3, float(rel)
 
 
-@pytest.mark.parametrize("T", [100, 129])
-def test_prefill_pages_outside_the_pool(hip, ctx, T):
+@pytest.mark.parametrize("T,kv", [(100, "bf16"), (129, "bf16"), (60, "bf16"), (100, "f16"), (9, "f16")])
+def test_prefill_pages_outside_the_pool(hip, ctx, T, kv):
     """Rows that see a position without a page are NaN, rows before it are not."""
     import qff
     g = torch.Generator(device=DEV).manual_seed(2)
     start = 170 - T
     p = _params(g)
     qg, k, v = _randn(g, T, 16, 512), _randn(g, T, 2, 256), _randn(g, T, 2, 256)
-    for entry, first in ((8, 128), (2, 0)):    # positions 128 .. 143, or cached ones
-        kp, vp = _randn(g, 13, 16, 2, 256, dtype=torch.bfloat16), _randn(g, 13, 16, 2, 256, dtype=torch.bfloat16)
+    for entry, first in ((8, 128), (2, 0)) if T > 9 else ((2, 0),):    # positions 128 .. 143, or cached ones
+        kp, vp = _randn(g, 13, 16, 2, 256, dtype=DT[kv]), _randn(g, 13, 16, 2, 256, dtype=DT[kv])
         kp[0], vp[0] = float("nan"), float("nan")     # nobody's
         table = torch.arange(1, 12, dtype=torch.int32, device=DEV)
         table[entry] = 13
@@ -490,7 +518,7 @@ def test_prefill_pages_outside_the_pool(hip, ctx, T):
             if q // 16 != entry:
                 kb[1 + q // 16, q % 16], vb[1 + q // 16, q % 16] = kp[1 + q // 16, q % 16], vp[1 + q // 16, q % 16]
         assert same_bits(kb, kp) and same_bits(vb, vp)
-        assert torch.equal(vp[11, 0], v[160 - start].bfloat16())
+        assert start > 160 or torch.equal(vp[11, 0], v[160 - start].to(DT[kv]))
 
 
 def test_prefill_captured(hip, ctx):
