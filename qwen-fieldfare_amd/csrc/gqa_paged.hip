@@ -67,10 +67,14 @@ struct PagedSeqs {
 };
 
 // A prompt slice instead of a batch: T tokens of one sequence from position
-// `start` (appended before), a block of 16 after the other, each over all
-// positions up to its last token's in chunks of ch.
+// `start`, a block of 16 after the other, each over all positions up to its last
+// token's in chunks of ch. Their rows are appended before, or by this launch
+// where each wave has at most one (its chunk puts it into the tile as well,
+// over what the page held: a launch less, 3 tokens behind 2442 13.0 -> 11.3 us, 8
+// behind 20000 23.1 -> 21.4).
 struct PagedTokens {
     int start, T, ch;
+    __device__ __host__ bool append() const { return T <= 8; }
     __device__ __host__ int end(int blk) const { return start + (16 * blk + 16 < T ? 16 * blk + 16 : T); }
 };
 
@@ -463,14 +467,17 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
     // tile's copies, which land while q is prepared.
     u32x4_t q[NT][8];             // a block's: term, step of 32 dims
     u32x4_t qs[(NT + 1) / 2][8];   // a single sequence's: term 2 k in columns l % 16 < 8, term 2 k + 1 in the others
-    u32x2_t fresh = u32x2_t{0u, 0u};   // dims 4 lane .. + 3 of the new k (wave 4) or v (wave 5)
+    // dims 4 lane .. + 3 of the new k (wave 4) or v (wave 5); of a short slice's token wv, k and v
+    u32x2_t fresh = u32x2_t{0u, 0u}, fresh_v = u32x2_t{0u, 0u};
+    const bool append = TOKENS && tk.append() && wv < tk.T && tk.start + wv >= p_begin && tk.start + wv < p_end;
     unsigned bad_next = 0;
     auto prepare = [&](auto rr, auto one) {
         constexpr int RR = decltype(rr)::value;
         constexpr bool ONE = decltype(one)::value;   // a single sequence
         int entry0 = PageWindow::entry(row, p_begin >> kv.lg, last_entry, lane);
         const int dim0 = kb == 0 ? 4 * wv : 56 + 24 * wv + 8 * kb, dim1 = kb == 0 ? 32 + 4 * wv : dim0 + 4;
-        float x[RR][8], w[8], kx[4];
+        float x[RR][8], w[8], kx[4], vx[4], kw[4];
+        int page = 0;   // of the appended token
 #pragma unroll
         for (int r = 0; r < RR; ++r) {
             const int s = lead + min(2 * r + (n >> 3), count - 1);
@@ -484,6 +491,18 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 kx[i] = elem<IN_DT>::load(wv == 5 ? v_new : k_new, (static_cast<size_t>(lead) * 2 + kvh) * 256 + 4 * lane + i);
+        }
+        if constexpr (TOKENS) {
+            if (append) {
+                const size_t from = (static_cast<size_t>(wv) * 2 + kvh) * 256 + 4 * lane;
+                load4<IN_DT>(k_new, from, kx);
+                load4<IN_DT>(v_new, from, vx);
+                load4<0>(k_norm_w, 4 * lane, kw);
+                page = row[(tk.start + wv) >> kv.lg];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(kx[i]), "+v"(vx[i]), "+v"(kw[i]));
+                asm volatile("" : "+v"(page));
+            }
         }
         int pos_a = position_of(lead + min(2 * min(wv, RR - 1) + (lane >> 5), count - 1));
         float freq = rf.f[lane & 31];   // (a load: the arguments lie in memory)
@@ -565,6 +584,35 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
             }
             if (r0 + kAtOnce < RR) __syncthreads();
         }
+        if constexpr (TOKENS) {
+            if (append) {   // (the angles are those of the token's q row)
+                float ss = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) ss += kx[i] * kx[i];
+                const float inv = 1.0f / sqrtf(group_sum<64>(ss) / 256.0f + eps);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) kx[i] = kx[i] * inv * kw[i];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float up = __shfl_down(kx[i], 8, 64), dn = __shfl_up(kx[i], 8, 64);
+                    const int d = 4 * lane + i;
+                    const float2 cs = L.turn[wv >> 1][32 * (wv & 1) + (d & 31)];
+                    if (d < 64) kx[i] = d < 32 ? kx[i] * cs.x - up * cs.y : kx[i] * cs.x + dn * cs.y;
+                }
+                uint32_t w0[1], w1[1], w2[1], w3[1];
+                split_terms<KV_F16, 1>(kx[0], kx[1], w0);
+                split_terms<KV_F16, 1>(kx[2], kx[3], w1);
+                split_terms<KV_F16, 1>(vx[0], vx[1], w2);
+                split_terms<KV_F16, 1>(vx[2], vx[3], w3);
+                fresh = u32x2_t{w0[0], w1[0]};
+                fresh_v = u32x2_t{w2[0], w3[0]};
+                if (page >= 0 && page < kv.num_pages) {
+                    const size_t off = ((static_cast<size_t>(page) << kv.lg) + ((tk.start + wv) & mask)) * 512 + kvh * 256 + 4 * lane;
+                    *reinterpret_cast<u32x2_t*>(kv.k + off) = fresh;
+                    *reinterpret_cast<u32x2_t*>(kv.v + off) = fresh_v;
+                }
+            }
+        }
         if constexpr (ONE && !TOKENS) {
             if (has_new && (wv == 4 || wv == 5)) {
                 // dims 4 lane .. + 3; the rotation's partner of dim d < 32 is d + 32, 8 lanes on
@@ -587,7 +635,7 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
                 split_terms<KV_F16, 1>(kx[0], kx[1], w0);
                 split_terms<KV_F16, 1>(kx[2], kx[3], w1);
                 fresh = u32x2_t{w0[0], w1[0]};
-                const int page = row[last_entry];   // (the chunk ends with the new token)
+                page = row[last_entry];   // (the chunk ends with the new token)
                 if (page >= 0 && page < kv.num_pages) {   // (dropped where the page lies outside the pool)
                     const size_t off = ((static_cast<size_t>(page) << kv.lg) + ((plan.len - 1) & mask)) * 512 + kvh * 256 + 4 * lane;
                     *reinterpret_cast<u32x2_t*>((wv == 4 ? kv.k : kv.v) + off) = fresh;
@@ -822,6 +870,17 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
     // four dims of row r of tile t: 4 lane .. + 3 of K (0) or V (1)
     auto tile_at = [&](int t, int which, int r) {
         return reinterpret_cast<u32x2_t*>(&L.tile[t & 1][which][r * 256 + 8 * ((lane >> 1) ^ tile_swz(r)) + 4 * (lane & 1)]);
+    };
+    // a short slice's tokens into their rows of tile t, over what their pages held before
+    auto put_tokens = [&](int t) {
+        const int t0 = p_begin + t * kTile;
+        if (!TOKENS || !tk.append() || t0 + kTile <= tk.start) return;   // (uniform)
+        const int r = tk.start + wv - t0;
+        if (append && r >= 0 && r < kTile) {
+            *tile_at(t, 0, r) = fresh;
+            *tile_at(t, 1, r) = fresh_v;
+        }
+        __syncthreads();
     };
     // V's rows from .. to - 1 of the last tile, behind the last position (the page may hold any bit pattern there)
     auto clear_behind = [&](int t, int from, int to) {
@@ -1062,6 +1121,7 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
             arrive(t);
             const unsigned bad = bad_next;
             const int t0 = p_begin + t * kTile;
+            put_tokens(t);
             if (t + 1 < ntiles) {
                 window(t + 1, t + 1);
                 bad_next = issue(t + 1, true, true);
@@ -1084,6 +1144,7 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
             arrive(t);
             const unsigned bad = bad_next;
             const int t0 = p_begin + t * kTile;
+            put_tokens(t);
             if (t + 1 < ntiles) {
                 window(t + 1, t + 1);
                 bad_next = issue(t + 1, true, true);
@@ -1393,7 +1454,7 @@ hipError_t launch_gqa_decode_paged(qff_ctx* ctx, hipStream_t stream, const qff_g
 // fp16, V transposed). Its products take a pass for each term, so the rule is
 // tokens x terms <= 128 (us per call, this / the other path, from position 0,
 // 2000, 20000, 60000):
-//   bf16 cache and outputs (two terms)  8 tokens 16 / 20, 19 / 26, 26 / 45, 37 / 82
+//   bf16 cache and outputs (two terms)  8 tokens 15 / 20, 17 / 26, 23 / 45, 39 / 82
 //                                      64 tokens 20 / 23, 32 / 34, 63 / 64, 132 / 136
 //                                      96 tokens 22 / 25, 34 / 34, 81 / 75, 188 / 164
 //   fp16 cache, bf16 outputs (one)    128 tokens 24 / 24, 32 / 35, 69 / 99, 160 / 197
@@ -1406,7 +1467,7 @@ hipError_t launch_gqa_prefill_paged(qff_ctx* ctx, hipStream_t stream, const qff_
     if (T * paged_terms(p->kv_f16 != 0, out_dtype == QFF_BF16) > kPagedTokensMax || cap < 4)
         return launch_gqa_prefill(ctx, stream, p, q_gate, k, v, in_dtype, kv->k, kv->v, kv, start, out, out_dtype, T);
     const PagedKv pk = paged_kv(kv);
-    {
+    if (!PagedTokens{start, T, kTile}.append()) {
         ProfScope prof(ctx, stream, "gqa_paged_append");
         const RopeFreqs rf = rope_freqs(p->rope_theta);
         const int blocks = (2 * T + 3) / 4;

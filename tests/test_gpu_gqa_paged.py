@@ -436,7 +436,7 @@ def test_prefill_paged_is_the_flat_one(hip, ctx, start, T, io, kv, out, page):
         assert same_bits(pool, want)
 
 
-@pytest.mark.parametrize("start,T", [(0, 1), (0, 2), (0, 17), (0, 128), (1, 1), (15, 1), (63, 2), (64, 33), (900, 33), (897, 16),
+@pytest.mark.parametrize("start,T", [(0, 1), (0, 2), (0, 8), (60, 8), (125, 5), (1021, 7), (2047, 3), (3000, 4), (4088, 8), (0, 9), (0, 17), (0, 128), (1, 1), (15, 1), (63, 2), (64, 33), (900, 33), (897, 16),
                                      (2000, 5), (2000, 42), (2000, 43), (3000, 64), (3000, 65), (3000, 100), (3968, 128),
                                      (4095, 1)])
 @pytest.mark.parametrize("io,kv,out,page", [("f32", "bf16", "f32", 16), ("bf16", "f16", "bf16", 64), ("bf16", "bf16", "bf16", 256),
@@ -496,7 +496,7 @@ def test_prefill_paged_against_64_bits(hip, ctx):
     assert rel <= 1.2e-3, float(rel)
 
 
-@pytest.mark.parametrize("T,kv", [(100, "bf16"), (129, "bf16"), (60, "bf16"), (100, "f16"), (9, "f16")])
+@pytest.mark.parametrize("T,kv", [(100, "bf16"), (129, "bf16"), (60, "bf16"), (100, "f16"), (9, "f16"), (8, "bf16"), (5, "f16"), (1, "bf16")])
 def test_prefill_pages_outside_the_pool(hip, ctx, T, kv):
     """Rows that see a position without a page are NaN, rows before it are not."""
     import qff
