@@ -341,7 +341,8 @@ int qff_gqa_prefill(qff_ctx* ctx, qff_stream_t stream, const qff_gqa_params* p,
  * context's max_ctx, rounded up to a whole page. An entry in use that lies
  * outside 0 .. num_pages - 1 makes the outputs that see its positions NaN
  * (nothing outside the pool is read or written). A page that a call appends
- * to must belong to one sequence only. Cache rows in use are finite. */
+ * to must belong to one sequence only. Cache rows in use, and the k and v that a
+ * call appends, are finite in the cache's type. */
 typedef struct qff_kv_pages {
     void* k;
     void* v;
