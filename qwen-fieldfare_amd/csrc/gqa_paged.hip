@@ -67,15 +67,20 @@ struct PagedSeqs {
 };
 
 // A prompt slice instead of a batch: T tokens of one sequence from position
-// `start`, a block of 16 after the other, each over all positions up to its last
-// token's in chunks of ch. Their rows are appended before, or by this launch
+// `start`, a block of `per` (8 or 16) after the other, each over all positions up
+// to its last token's in chunks of ch. Their rows are appended before, or by this launch
 // where each wave has at most one (its chunk puts it into the tile as well,
 // over what the page held: a launch less, 3 tokens behind 2442 13.0 -> 11.3 us, 8
 // behind 20000 23.1 -> 21.4).
 struct PagedTokens {
-    int start, T, ch;
+    int start, T, ch, per;
     __device__ __host__ bool append() const { return T <= 8; }
-    __device__ __host__ int end(int blk) const { return start + (16 * blk + 16 < T ? 16 * blk + 16 : T); }
+    __device__ __host__ int end(int blk) const { return start + (per * blk + per < T ? per * blk + per : T); }
+    int items() const {
+        int n = 0;
+        for (int b = 0; b * per < T; ++b) n += (end(b) + ch - 1) / ch;
+        return n;
+    }
 };
 
 // Sequence b0 + lane: its length, the shared positions of its block, the
@@ -371,8 +376,8 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
             c -= nc;
             ++blk;
         }
-        lead = 16 * blk;
-        count = min(kBlkSeqs, tk.T - lead);
+        lead = tk.per * blk;
+        count = min(tk.per, tk.T - lead);
         p_begin = c * tk.ch;
         p_end = min(tk.end(blk), p_begin + tk.ch);
         slot_c = c;
@@ -1449,11 +1454,11 @@ hipError_t launch_gqa_decode_paged(qff_ctx* ctx, hipStream_t stream, const qff_g
     return hipGetLastError();
 }
 
-// A slice of few tokens takes the decode's kernels: blocks of 16 tokens read the
-// pages as they are, where the other path first copies the whole cache (K as
+// A slice of few tokens takes the decode's kernels: blocks of 8 or 16 tokens read
+// the pages as they are, where the other path first copies the whole cache (K as
 // fp16, V transposed). Its products take a pass for each term, so the rule is
-// tokens x terms <= 128 (us per call, this / the other path, from position 0,
-// 2000, 20000, 60000):
+// tokens x terms <= 128 (us per call, this in blocks of 16 / the other path, from
+// position 0, 2000, 20000, 60000):
 //   bf16 cache and outputs (two terms)  8 tokens 15 / 20, 17 / 26, 23 / 45, 39 / 82
 //                                      64 tokens 20 / 23, 32 / 34, 63 / 64, 132 / 136
 //                                      96 tokens 22 / 25, 34 / 34, 81 / 75, 188 / 164
@@ -1467,7 +1472,7 @@ hipError_t launch_gqa_prefill_paged(qff_ctx* ctx, hipStream_t stream, const qff_
     if (T * paged_terms(p->kv_f16 != 0, out_dtype == QFF_BF16) > kPagedTokensMax || cap < 4)
         return launch_gqa_prefill(ctx, stream, p, q_gate, k, v, in_dtype, kv->k, kv->v, kv, start, out, out_dtype, T);
     const PagedKv pk = paged_kv(kv);
-    if (!PagedTokens{start, T, kTile}.append()) {
+    if (!PagedTokens{start, T, kTile, 0}.append()) {
         ProfScope prof(ctx, stream, "gqa_paged_append");
         const RopeFreqs rf = rope_freqs(p->rope_theta);
         const int blocks = (2 * T + 3) / 4;
@@ -1479,18 +1484,24 @@ hipError_t launch_gqa_prefill_paged(qff_ctx* ctx, hipStream_t stream, const qff_
         }
 #undef QFF_APP
     }
-    // the least chunk length that needs no second round of workgroups, and no more partials than there is room for
-    PagedTokens tk{start, T, kTile};
-    const int blks = (T + 15) / 16, slots = ctx->num_cu / 2;
-    auto items = [&] {
-        int n = 0;
-        for (int b = 0; b < blks; ++b) n += (tk.end(b) + tk.ch - 1) / tk.ch;
-        return n;
+    // The least chunk length that needs no second round of workgroups, and no more
+    // partials than there is room for. Blocks of 8 tokens start and end sooner and
+    // spread over more workgroups, those of 16 read the pages half as often: 8
+    // where that makes chunks of at most four tiles (us with 8 / 16, bf16, 33
+    // tokens behind 900 and 5000 23.3 / 24.4, 29.2 / 33.5, 16 behind 20000 and 60000,
+    // 5 and 15 tiles, 31.1 / 32.6, 55.5 / 51.6; fp16 33 behind 20000, 13 tiles, 41 /
+    // 39, 64 behind 60000 118 / 90).
+    const int slots = ctx->num_cu / 2;
+    auto split = [&](int per) {
+        PagedTokens tk{start, T, kTile, per};
+        while ((tk.items() > slots && tk.ch < start + T) || (start + T + tk.ch - 1) / tk.ch > cap) tk.ch += kTile;
+        return tk;
     };
-    while ((items() > slots && tk.ch < start + T) || (start + T + tk.ch - 1) / tk.ch > cap) tk.ch += kTile;
+    PagedTokens tk = split(8);
+    if (tk.ch > 4 * kTile) tk = split(kBlkSeqs);
     // partials where the sharing prefill keeps its own: m and d [T][2][cap][8], o [T][2][cap][8][256]
     const PagedPartials pp{ctx->pf_md, ctx->pf_md + static_cast<size_t>(T) * 16 * cap, ctx->pf_o, ctx->gqa_nc, cap};
-    launch_partials(ctx, stream, p, q_gate, k, v, in_dtype, pk, nullptr, tk, pp, 2 * items(), out, out_dtype, T);
+    launch_partials(ctx, stream, p, q_gate, k, v, in_dtype, pk, nullptr, tk, pp, 2 * tk.items(), out, out_dtype, T);
     return hipGetLastError();
 }
 
