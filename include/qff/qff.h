@@ -372,7 +372,7 @@ int qff_gqa_decode_paged(qff_ctx* ctx, qff_stream_t stream, const qff_gqa_params
  *   shared_len  [batch] int32 device array: how many of its first positions a
  *               sequence has in common with its group. The positions before the
  *               least shared_len of a group's sequences are read through the
- *               table row of the first of them (of each 16), so all of them
+ *               table row of the first of them (of each up to 16), so all of them
  *               must hold the same K and V there (they may, and usually do, name
  *               the same pages).
  * A group's members may be at any positions; any values of the two arrays are

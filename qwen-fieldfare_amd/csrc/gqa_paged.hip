@@ -13,7 +13,7 @@
 // joined with weights 2^(m - max m).
 //
 //   partial  one workgroup per (block of sequences, kv head, chunk of
-//            positions): a group's shared positions for up to 16 of its
+//            positions): a group's shared positions for up to 8 or 16 of its
 //            sequences (128 q rows), or one sequence's own positions (8 q
 //            rows), whose last chunk appends the new token. K/V tiles go
 //            through LDS. One launch for both, so that the few long streams of
@@ -29,6 +29,7 @@
 // much again) or one of fp16 (3e-4; 32 sequences over 32K 45 us, with two 65). fp16 weights are scaled by 2^7 (kShift), so that weights down to 2^-21
 // of the row's largest keep all bits of their first term.
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "common.hpp"
@@ -42,8 +43,8 @@ namespace qff {
 // Every workgroup derives the same split from the device arrays (no host
 // sync, no atomics). `positions` give each sequence's length L (0 where the
 // position lies outside the table: no chunks, its output is NaN). With groups,
-// consecutive sequences with the same group >= 0 (and L > 0) are a run, cut
-// every 16 sequences, and at every multiple of 64 sequences, into blocks; the
+// consecutive sequences with the same group >= 0 (and L > 0) are a run, cut at
+// every multiple of 64 sequences and into even blocks of up to 8 or 16; the
 // positions before S = the least of the block's shared_len and L - 1, rounded
 // down to 16, are read through the table row of the block's first sequence for
 // all of it. Any values of the arrays give a valid split.
@@ -52,8 +53,14 @@ namespace qff {
 // so the chunk length is about the least that needs no second round of
 // workgroups where such a length exists.
 
-constexpr int kBlkSeqs = 16;    // sequences of a block
+constexpr int kBlkSeqs = 16;    // sequences of a block at most
 constexpr int kTile = 64;       // positions of a tile
+// Blocks of 8 start and end sooner and spread over more workgroups, blocks of 16
+// read the prefix half as often: 8 where that makes chunks of up to 10 tiles
+// (us with 8 / 16: 16 sequences on 6K, bf16 22.7 / 27.0, on 16K, 5 tiles, 28.1 / 31.5, fp16
+// 25.2 / 30.4, on 32K, 9 tiles, 36.5 / 40.1, 32.2 / 37.6; 32 on 16K, 9 tiles, 39.1 / 38.8,
+// 34.4 / 33.3, on 32K 59.5 / 55.2, 50.5 / 44.0).
+constexpr int kSmallTiles = 10;
 constexpr int kMinShared = 64;  // shorter shared prefixes are left to the sequences
 
 struct PagedSeqs {
@@ -91,7 +98,7 @@ struct LanePlan {
     __device__ __forceinline__ int own() const { return len - shared; }
 };
 
-__device__ __forceinline__ LanePlan lane_plan(const PagedSeqs& a, int b0, int lane) {
+__device__ __forceinline__ LanePlan lane_plan(const PagedSeqs& a, int b0, int lane, int bs) {
     const int b = b0 + lane;
     LanePlan p{0, 0, lane, 1};
     int grp = -1, sh = 0;
@@ -109,7 +116,14 @@ __device__ __forceinline__ LanePlan lane_plan(const PagedSeqs& a, int b0, int la
     const unsigned long long below = ~0ull >> (63 - lane);   // lanes 0 .. lane
     const unsigned long long runs = __ballot(lane == 0 || grp < 0 || grp != prev);
     const int run = 63 - __builtin_clzll(runs & below);
-    const unsigned long long blocks = __ballot(((lane - run) & (kBlkSeqs - 1)) == 0);
+    // blocks as even as they can be
+    const unsigned long long later = runs & ~below;
+    const int members = (later ? static_cast<int>(__builtin_ctzll(later)) : 64) - run;
+    // quotients of numbers up to 80, by reciprocals
+    auto quotient = [](int x, int y) { return static_cast<int>((static_cast<float>(x) + 0.5f) * __builtin_amdgcn_rcpf(static_cast<float>(y))); };
+    const int nblk = (members + bs - 1) / bs, size = quotient(members + nblk - 1, nblk);
+    const int at = lane - run;
+    const unsigned long long blocks = __ballot(at == quotient(at, size) * size);
     p.first = 63 - __builtin_clzll(blocks & below);
     const unsigned long long after = blocks & ~below;
     const int end = after ? static_cast<int>(__builtin_ctzll(after)) : 64;
@@ -130,8 +144,8 @@ __device__ __forceinline__ int chunks_of(int n, int ch) { return (n + ch - 1) / 
 // Chunk length of a sequence's own positions. A tile of a block of eight row
 // blocks costs about two of a single sequence with more than one term (3.5 us
 // from L2 to 1.1 - 2.1), so the sequences behind such a block get chunks twice
-// as long: 32 sequences on a prefix of 32K, bf16, 58.5 -> 55.8 us, of 8K with
-// fp32 outputs 36.6 -> 33.9. With one term (2.1 us) it loses, 45.5 -> 48.5.
+// as long: 32 sequences on a prefix of 32K, bf16, 58.5 -> 55.8 us. With one term
+// (2.1 us) it loses, 45.5 -> 48.5.
 __device__ __forceinline__ int own_chunk(const PagedSeqs& a, const LanePlan& p, int ch) {
     return p.shared > 0 && p.count > 8 && a.terms > 1 ? 2 * ch : ch;
 }
@@ -142,7 +156,7 @@ __device__ __forceinline__ int items_of(const PagedSeqs& a, const LanePlan& p, i
     return chunks_of(p.own(), own_chunk(a, p, ch)) + (p.first == lane ? chunks_of(p.shared, ch) : 0);
 }
 
-// The call's chunk length, whole tiles, and whether it reads so much that
+// The call's chunk length, whole tiles (0: the call has more than `most`), and whether it reads so much that
 // nothing of it can still be cached when it is read again (half of the 256 MB
 // that lie in front of HBM): its tiles are then copied non-temporally. 32
 // sequences of up to 32K (1.1 GB) 200 -> 182 us; 8 of up to 8K (75 MB, which a
@@ -153,15 +167,16 @@ struct Chunk {
 };
 constexpr int kStreamTiles = 1024;   // of one kv head, 64 KB each
 
-__device__ __forceinline__ Chunk chunk_length(const PagedSeqs& a, const LanePlan& p0, int lane) {
+__device__ __forceinline__ Chunk chunk_length(const PagedSeqs& a, const LanePlan& p0, int lane, int bs, int most) {
     long long tiles = 0;
     int streams = 0, longest = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
-        const LanePlan p = b0 == 0 ? p0 : lane_plan(a, b0, lane);
+        const LanePlan p = b0 == 0 ? p0 : lane_plan(a, b0, lane, bs);
         tiles += wave_sum_int(items_of(a, p, kTile, lane));
         streams += wave_sum_int((p.own() > 0) + (p.first == lane && p.shared > 0));
         longest = max(longest, wave_max_int(p.len));
     }
+    if (__builtin_amdgcn_readfirstlane(static_cast<int>(tiles > most))) return Chunk{0, false};
     // sum of ceil(n / ch) is about tiles / ch + streams / 2, and at most tiles / ch + streams
     const int free = max(a.slots - streams / 2, (a.slots + 1) / 2);
     int ch = static_cast<int>((tiles + free - 1) / free);
@@ -179,12 +194,12 @@ __device__ __forceinline__ Chunk chunk_length(const PagedSeqs& a, const LanePlan
 
 // Workgroup item g: the sequence that holds it (-1: past the last), the item's
 // number among the sequence's, its plan (first: as a sequence).
-__device__ __forceinline__ int find_item(const PagedSeqs& a, const LanePlan& p0, int ch, int g, int lane, int& c,
+__device__ __forceinline__ int find_item(const PagedSeqs& a, const LanePlan& p0, int ch, int g, int lane, int bs, int& c,
                                          LanePlan& plan) {
     int base = 0;
     c = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
-        const LanePlan p = b0 == 0 ? p0 : lane_plan(a, b0, lane);
+        const LanePlan p = b0 == 0 ? p0 : lane_plan(a, b0, lane, bs);
         const int mine = items_of(a, p, ch, lane);
         const int incl = base + wave_inclusive_scan_int(mine);
         const unsigned long long hit = __ballot(incl > g);
@@ -384,11 +399,17 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
         cut_from = min(p_end, tk.start + lead + 1);
         if (c == 0 && kvh == 0 && static_cast<int>(threadIdx.x) < count) pp.count[lead + threadIdx.x] = nc;
     } else {
-        const LanePlan p0 = lane_plan(a, 0, lane);
-        const Chunk chunk = chunk_length(a, p0, lane);
+        int bs = kBlkSeqs / 2;
+        LanePlan p0 = lane_plan(a, 0, lane, bs);
+        Chunk chunk = chunk_length(a, p0, lane, bs, a.group ? kSmallTiles * a.slots : INT_MAX);
+        if (chunk.len == 0) {   // (uniform)
+            bs = kBlkSeqs;
+            p0 = lane_plan(a, 0, lane, bs);
+            chunk = chunk_length(a, p0, lane, bs, INT_MAX);
+        }
         const int ch = chunk.len;
         int item;
-        lead = find_item(a, p0, ch, static_cast<int>(blockIdx.x >> 1), lane, item, plan);
+        lead = find_item(a, p0, ch, static_cast<int>(blockIdx.x >> 1), lane, bs, item, plan);
         if (lead < 0) return;   // (uniform over the workgroup)
         // the block's shared chunks come first among its first sequence's items
         const int npfx = chunks_of(plan.shared, ch);
