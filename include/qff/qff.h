@@ -356,8 +356,10 @@ typedef struct qff_kv_pages {
  * k and v appended to the page of position positions[b] in row b of the
  * table, which already names it. A position outside 0 .. table_cols *
  * page_size - 1 (a padded slot) gives a NaN row and touches no page. q_gate and
- * the norm weights are 16-byte aligned. fp32 outputs are within about 1e-6 of
- * the exact result (bf16 outputs: their own rounding). */
+ * the norm weights are 16-byte aligned. Errors grow with the scores, of rms s
+ * (at least 1 here): fp32 outputs are within about 1e-6 s of the exact row,
+ * relative to its norm; bf16 outputs add 4e-6 s (bf16 cache) or 1e-6 s (fp16) to
+ * their own rounding. */
 int qff_gqa_decode_paged(qff_ctx* ctx, qff_stream_t stream, const qff_gqa_params* p,
                          const void* q_gate, const void* k_new, const void* v_new,
                          qff_dtype in_dtype, const qff_kv_pages* kv, const int32_t* positions,
@@ -388,10 +390,9 @@ int qff_gqa_decode_shared(qff_ctx* ctx, qff_stream_t stream, const qff_gqa_param
  * positions start_pos .. start_pos + T - 1, whose pages the one row of
  * kv->table names. Arguments and limits otherwise as qff_gqa_prefill
  * (QFF_ERR_INVALID_ARG when start_pos + T exceeds table_cols * page_size); q_gate,
- * k, v, out and the norm weights are 16-byte aligned. Slices of up to 128 tokens (bf16
- * outputs of an fp16 cache), 42 (fp32 outputs of a bf16 cache) or 64 (others) have
- * qff_gqa_decode_paged's precision, longer ones the fp16 operands of
- * qff_gqa_prefill. */
+ * k, v, out and the norm weights are 16-byte aligned. Slices of up to 42 tokens (fp32
+ * outputs of a bf16 cache) or 64 (others) have qff_gqa_decode_paged's precision,
+ * longer ones the fp16 operands of qff_gqa_prefill. */
 int qff_gqa_prefill_paged(qff_ctx* ctx, qff_stream_t stream, const qff_gqa_params* p,
                           const void* q_gate, const void* k, const void* v, qff_dtype in_dtype,
                           const qff_kv_pages* kv, int start_pos, void* out, qff_dtype out_dtype,

@@ -23,11 +23,15 @@
 // Both products run on 16x16x32 MFMAs in the cache's type, in which K and V
 // are exact. q and the softmax weights enter as NT terms of that type (hi,
 // the rest rounded again, ...): two bf16 terms carry 16 bits and two fp16
-// terms 22, three bf16 terms 24. fp32 outputs take three of bf16 or two of fp16
-// (error 2e-7 to 7e-7 of the exact output, where two bf16 terms leave 6e-6);
-// bf16 outputs, whose own rounding is 1.7e-3, two of bf16 (one would add as
-// much again) or one of fp16 (3e-4; 32 sequences over 32K 45 us, with two 65). fp16 weights are scaled by 2^7 (kShift), so that weights down to 2^-21
-// of the row's largest keep all bits of their first term.
+// terms 22, three bf16 terms 24. What q's terms leave out shows in proportion to
+// the scores. fp32 outputs take three terms of bf16 or two of fp16 (error 2e-7 to
+// 7e-7 of a row at scores of rms 1, where two bf16 terms leave 6e-6). bf16
+// outputs, whose own rounding is 1.7e-3, take two of either: two bf16 terms leave 3e-6
+// at scores of rms 1 and 9e-5 in the worst row at 25; one fp16 term would leave
+// 3e-4 and 7e-3, more than the output's rounding once trained norm weights spread
+// the scores (a 64-bit emulation over 4096 positions). fp16
+// weights are scaled by 2^7 (kShift), so that weights down to 2^-21 of the row's
+// largest keep all bits of their first term.
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -70,7 +74,6 @@ struct PagedSeqs {
     int batch, max_ctx;
     int slots;   // workgroups of one round, per kv head
     int cap;     // chunks allowed per sequence
-    int terms;   // of q and the weights
 };
 
 // A prompt slice instead of a batch: T tokens of one sequence from position
@@ -142,18 +145,15 @@ __device__ __forceinline__ LanePlan lane_plan(const PagedSeqs& a, int b0, int la
 
 __device__ __forceinline__ int chunks_of(int n, int ch) { return (n + ch - 1) / ch; }
 // Chunk length of a sequence's own positions. A tile of a block of eight row
-// blocks costs about two of a single sequence with more than one term (3.5 us
-// from L2 to 1.1 - 2.1), so the sequences behind such a block get chunks twice
-// as long: 32 sequences on a prefix of 32K, bf16, 58.5 -> 55.8 us. With one term
-// (2.1 us) it loses, 45.5 -> 48.5.
-__device__ __forceinline__ int own_chunk(const PagedSeqs& a, const LanePlan& p, int ch) {
-    return p.shared > 0 && p.count > 8 && a.terms > 1 ? 2 * ch : ch;
-}
+// blocks costs about two of a single sequence (3.5 us from L2 to 1.1 - 2.1), so
+// the sequences behind such a block get chunks twice as long: 32 sequences on a
+// prefix of 32K, bf16, 58.5 -> 55.8 us.
+__device__ __forceinline__ int own_chunk(const LanePlan& p, int ch) { return p.shared > 0 && p.count > 8 ? 2 * ch : ch; }
 
 // Workgroups (per kv head) of the sequence in this lane at chunk length ch:
 // its own chunks, and its block's shared ones in the block's first lane.
-__device__ __forceinline__ int items_of(const PagedSeqs& a, const LanePlan& p, int ch, int lane) {
-    return chunks_of(p.own(), own_chunk(a, p, ch)) + (p.first == lane ? chunks_of(p.shared, ch) : 0);
+__device__ __forceinline__ int items_of(const LanePlan& p, int ch, int lane) {
+    return chunks_of(p.own(), own_chunk(p, ch)) + (p.first == lane ? chunks_of(p.shared, ch) : 0);
 }
 
 // The call's chunk length, whole tiles (0: the call has more than `most`), and whether it reads so much that
@@ -172,7 +172,7 @@ __device__ __forceinline__ Chunk chunk_length(const PagedSeqs& a, const LanePlan
     int streams = 0, longest = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
         const LanePlan p = b0 == 0 ? p0 : lane_plan(a, b0, lane, bs);
-        tiles += wave_sum_int(items_of(a, p, kTile, lane));
+        tiles += wave_sum_int(items_of(p, kTile, lane));
         streams += wave_sum_int((p.own() > 0) + (p.first == lane && p.shared > 0));
         longest = max(longest, wave_max_int(p.len));
     }
@@ -182,7 +182,7 @@ __device__ __forceinline__ Chunk chunk_length(const PagedSeqs& a, const LanePlan
     int ch = static_cast<int>((tiles + free - 1) / free);
     const int sure = streams < a.slots ? static_cast<int>((tiles + a.slots - streams - 1) / (a.slots - streams)) : ch;
     if (a.batch <= 64) {
-        while (ch < sure && wave_sum_int(items_of(a, p0, ch * kTile, lane)) > a.slots) ch += (ch + 15) / 16;
+        while (ch < sure && wave_sum_int(items_of(p0, ch * kTile, lane)) > a.slots) ch += (ch + 15) / 16;
     } else {
         ch = sure;
     }
@@ -200,7 +200,7 @@ __device__ __forceinline__ int find_item(const PagedSeqs& a, const LanePlan& p0,
     c = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
         const LanePlan p = b0 == 0 ? p0 : lane_plan(a, b0, lane, bs);
-        const int mine = items_of(a, p, ch, lane);
+        const int mine = items_of(p, ch, lane);
         const int incl = base + wave_inclusive_scan_int(mine);
         const unsigned long long hit = __ballot(incl > g);
         if (hit) {
@@ -346,7 +346,6 @@ struct PagedPartials {
 //   16 q rows (two sequences x 8 heads): wave w takes row block w % R, and all
 //   64 positions where R = 8, otherwise half w / R of them. Per 32 positions a
 //   wave reads 16 KB of K and 16 KB of V operands for 32 NT MFMAs.
-//   With one term and R = 8 the rows go 32 to a wave (see wide_block).
 //   A single sequence's 8 rows: waves 0-3 take 16 positions each, the products
 //   of two terms in one MFMA (see single_step).
 // Waves beyond these only copy. In both
@@ -361,7 +360,7 @@ struct PagedPartials {
 // (what the page holds there may be any bit pattern).
 struct PartLds {
     uint16_t tile[2][2][kTile * 256];   // stage, K / V
-    float md[8][16][2], mdw[8][32][2];  // per wave and row (m, d), rows 16 or 32 to a wave
+    float md[8][16][2];                 // per wave and row: m, d
     __attribute__((aligned(16))) float sq[4][16][8];   // sums of squares: row block, row, slice of 32 dims
     __attribute__((aligned(16))) float2 turn[4][64];   // row block, angle of the two sequences: cos, sin
 };
@@ -422,7 +421,7 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
             if (c >= npfx) c -= npfx;
         }
         count = pfx ? plan.count : 1;
-        const int step = pfx ? ch : own_chunk(a, plan, ch);
+        const int step = pfx ? ch : own_chunk(plan, ch);
         p_begin = (pfx ? 0 : plan.shared) + c * step;
         p_end = min(pfx ? plan.shared : plan.len, p_begin + step);
         has_new = !pfx && p_end == plan.len;
@@ -436,45 +435,43 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
     const int last_entry = (p_end - 1) >> kv.lg;
     PageWindow win;
 
-    // the page window to hold tiles from .. to (at most two, 128 positions)
-    auto window = [&](int from, int to) {
-        if ((min(p_begin + (to + 1) * kTile, p_end) - 1) >> kv.lg > win.base + 63) {
-            const int first = (p_begin + from * kTile) >> kv.lg;
+    // the page window to hold tile t
+    auto window = [&](int t) {
+        if ((min(p_begin + (t + 1) * kTile, p_end) - 1) >> kv.lg > win.base + 63) {
+            const int first = (p_begin + t * kTile) >> kv.lg;
             win.set(first, PageWindow::entry(row, first, last_entry, lane), kv.num_pages);
         }
     };
-    // Part i < 4 of tile t into stage t & 1, K or V or both: wave wv copies rows 16 i +
-    // 2 wv, + 1; 16 positions past the chunk's end repeat its last ones (masked;
+    // K and V of tile t into stage t & 1: in round i wave wv copies rows 16 i + 2 wv,
+    // + 1; 16 positions past the chunk's end repeat its last ones (masked;
     // finite, or zeroed behind the new token). Returns bit i if their page is bad.
-    auto issue_part = [&](int t, int i, bool with_k, bool with_v) -> unsigned {
+    auto issue = [&](int t) -> unsigned {
         const int h = lane >> 5;
         const uint32_t lt = 1024u * h + 16u * ((lane & 31) ^ (2 * h) ^ tile_swz(2 * wv & 15));
-        const int p = min(p_begin + t * kTile + 16 * i, (p_end - 1) & ~15);
-        const int entry = p >> kv.lg;
-        const size_t at = (((static_cast<size_t>(win.of(entry)) << kv.lg) + (p & mask) + 2 * wv) * 2 + kvh) * 512;
-        const char *k = reinterpret_cast<const char*>(kv.k) + at, *v = reinterpret_cast<const char*>(kv.v) + at;
-        const uint32_t lk = lds_addr(&L.tile[t & 1][0][(16 * i + 2 * wv) * 256]);
-        const uint32_t lv = lds_addr(&L.tile[t & 1][1][(16 * i + 2 * wv) * 256]);
-        if (stream) {
-            if (with_k) dma16_nt(k, lt, lk);
-            if (with_v) dma16_nt(v, lt, lv);
-        } else {
-            if (with_k) dma16(k, lt, lk);
-            if (with_v) dma16(v, lt, lv);
-        }
-        return (win.is_bad(entry) ? 1u : 0u) << i;
-    };
-    auto issue = [&](int t, bool with_k, bool with_v) -> unsigned {
         unsigned bad = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) bad |= issue_part(t, i, with_k, with_v);
+        for (int i = 0; i < 4; ++i) {
+            const int p = min(p_begin + t * kTile + 16 * i, (p_end - 1) & ~15);
+            const int entry = p >> kv.lg;
+            const size_t at = (((static_cast<size_t>(win.of(entry)) << kv.lg) + (p & mask) + 2 * wv) * 2 + kvh) * 512;
+            const char *k = reinterpret_cast<const char*>(kv.k) + at, *v = reinterpret_cast<const char*>(kv.v) + at;
+            const uint32_t lk = lds_addr(&L.tile[t & 1][0][(16 * i + 2 * wv) * 256]);
+            const uint32_t lv = lds_addr(&L.tile[t & 1][1][(16 * i + 2 * wv) * 256]);
+            if (stream) {
+                dma16_nt(k, lt, lk);
+                dma16_nt(v, lt, lv);
+            } else {
+                dma16(k, lt, lk);
+                dma16(v, lt, lv);
+            }
+            bad |= (win.is_bad(entry) ? 1u : 0u) << i;
+        }
         return bad;
     };
     const int n = lane & 15, kb = lane >> 4;
     const int nrb = (count + 1) / 2;
     const int R = nrb <= 1 ? 1 : nrb <= 2 ? 2 : nrb <= 4 ? 4 : 8;
     const bool single = count == 1;
-    const bool wide = NT == 1 && R == 8;   // rows 32 to a wave, see below
     const int parts = single ? 4 : R == 8 ? 1 : 2;   // of a tile's positions, one a wave
     const int rb = wv & (R - 1), part = wv / R;
     const bool active = part < parts && rb < nrb;
@@ -543,7 +540,7 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
         }
         if constexpr (ONE && !TOKENS) asm volatile("" : "+v"(kx[0]), "+v"(kx[1]), "+v"(kx[2]), "+v"(kx[3]));
         win.set(p_begin >> kv.lg, entry0, kv.num_pages);
-        bad_next = issue(0, true, true);
+        bad_next = issue(0);
         // cos, sin of angle l % 32 of row block wv's sequence l / 32
         if (wv < RR) {
             float s, c2;
@@ -686,7 +683,7 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
 #pragma unroll
             for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(x[jj][e]), "+v"(w[jj][e]));
         win.set(p_begin >> kv.lg, entry0, kv.num_pages);
-        bad_next = issue(0, true, !wide);
+        bad_next = issue(0);
         float cl, sl, cs[8], sn[8], ss = 0.0f;   // lane l: angle l % 32 of the row block's sequence l / 32
         sincosf(static_cast<float>(pos_a) * freq, &sl, &cl);
 #pragma unroll
@@ -880,7 +877,7 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
         d_run += (e0 + e1) + (e2 + e3);
         split_terms<KV_F16, NT>(e0, e1, w0);
         split_terms<KV_F16, NT>(e2, e3, w1);
-        u32x4_t pw = u32x4_t{w0[0], w1[0], NT > 1 ? w0[NT > 1] : 0u, NT > 1 ? w1[NT > 1] : 0u};
+        u32x4_t pw = u32x4_t{w0[0], w1[0], w0[1], w1[1]};
         if (n >= 8) pw = NT == 3 ? u32x4_t{w0[NT - 1], w1[NT - 1], 0u, 0u} : u32x4_t{0u, 0u, 0u, 0u};
 #pragma unroll
         for (int dt = 0; dt < 16; ++dt) {
@@ -920,226 +917,6 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
             if ((bad >> (z >> 4)) & 1) *tile_at(t, 1, z) = u32x2_t{0u, 0u};
         __syncthreads();
     };
-    // One term, more than eight sequences: the rows go 32 to a wave on 32x32x16
-    // MFMAs, each half of a tile's positions with its own four waves, so that
-    // every K or V operand read feeds 32 rows instead of 16 (256 KB of LDS reads a
-    // tile instead of 512). A tile takes 2.1 us from L2, 2.2 with 32 sequences
-    // over 32K; that call 51.4 -> 45.2 us. A lane's score and output registers
-    // belong to its one q row. Iteration t computes the scores of tile t and then O^T
-    // += V^T P^T of tile t - 1, with the softmax of the new scores between its
-    // products; K is copied a tile ahead of V. (The two waves of a SIMD in opposite
-    // order: 2.5 us.) With more terms q does not fit beside O^T's 128 registers;
-    // on one wave a SIMD with 512 registers two terms took 67 us where sixteen rows
-    // a wave take 61.
-    auto wide_block = [&] {
-        const int rn = lane & 31, h = lane >> 5, r32 = wv & 3, side = wv >> 2;
-        const int sq = lead + min(4 * r32 + (rn >> 3), count - 1);   // of the lane's q row
-        const int limit = TOKENS ? min(p_end, tk.start + sq + 1) : p_end;
-        u32x4_t qw[16];   // B of a 32x32x16 product: column rn, dims 16 u + 8 h + e
-        {
-            // from the 16-row operands that each wave prepared, through the second stage:
-            // piece of dims 16 u + 8 h .. of row r at 64 u + 32 h + r of its 32 rows'
-            u32x4_t* const hand = reinterpret_cast<u32x4_t*>(L.tile[1]);
-#pragma unroll
-            for (int jj = 0; jj < 8; ++jj)
-                hand[1024 * (wv >> 1) + 64 * (2 * jj + (kb >> 1)) + 32 * (kb & 1) + 16 * (wv & 1) + n] = q[0][jj];
-            __syncthreads();
-#pragma unroll
-            for (int u = 0; u < 16; ++u) qw[u] = hand[1024 * r32 + 64 * u + lane];
-        }
-        float m_w = -INFINITY, d_w = 0.0f;
-        // O^T: register i of dim tile dt has dim 128 (dt / 4) + 16 (dt % 4) + 64 (i / 8) +
-        // 8 (i / 4 % 2) + 4 h + i % 4: a tile's two halves lie 64 dims apart, so that the
-        // transposed reads of 32 lanes (4 rows of each half) meet no bank twice
-        f32x16_t ow[8];
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) ow[dt][i] = 0.0f;
-        // K operand of step u: row rn of the half, piece 2 u + h. V^T operand of a dim
-        // tile and 16 positions: rows 4 h + l % 16 / 4 and 8 on, dims 64 (l / 16 % 2) +
-        // 4 (l % 4) .. + 3 of the tile's, whose transposed reads give a lane's dim the
-        // positions in the order the score registers hold them (slot 8 h + 4 j + i of a
-        // step: position 8 j + 4 h + i)
-        const uint32_t kw = 512u * rn + 16u * (h ^ tile_swz(rn)) + 16384u * side;
-        const int vrow = 4 * h + ((lane & 15) >> 2);
-        const uint32_t vw = 512u * vrow + 16u * ((8 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ tile_swz(vrow)) + 8u * (lane & 1) +
-                            16384u * side;
-        u32x4_t pw[2];   // weights of the tile before, per 16 positions
-        f32x16_t s;
-        unsigned bad_k = 0;
-        // iteration t: scores of tile t (WS), O^T += V^T P^T of tile t - 1 (WV)
-        auto iter = [&](auto ws, auto wvv, int t) {
-            constexpr bool WS = decltype(ws)::value, WV = decltype(wvv)::value;
-            arrive(t);
-            const unsigned bad_v = bad_k;
-            if constexpr (WS) {
-                if (t + 1 < ntiles) window(t, t + 1);
-                bad_k = 0;
-            }
-            if constexpr (WV) {
-                if (TOKENS && !WS) clear_behind(t - 1, p_end - (p_begin + (t - 1) * kTile), kTile);
-                clear_bad(t - 1, bad_v);
-            }
-            const uint32_t ka = lds_addr(L.tile[t & 1][0]) + kw, va = lds_addr(L.tile[(t + 1) & 1][1]) + vw;
-            u32x4_t kf[4];
-            u32x2_t vf[4][2];
-            auto k_read = [&](int u) { kf[u % 4] = lds128(at_xor(ka, 32u * u)); };
-            auto v_read = [&](int u) {   // dim tile u % 8, 16 positions u / 8
-                const uint32_t dims = 32u * (u & 3) + 256u * (u >> 2 & 1);
-                vf[u % 4][0] = lds_tr(at_xor(va, dims) + 8192u * (u >> 3));
-                vf[u % 4][1] = lds_tr(at_xor(va ^ 144u, dims) + 8192u * (u >> 3) + 4096u);   // 8 rows on
-            };
-            if constexpr (WS) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = 0.0f;
-#pragma unroll
-                for (int u = 0; u < 3; ++u) k_read(u);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int u = 0; u < 16; ++u) {
-                    if (u + 3 < 16) k_read(u + 3);
-                    else if constexpr (WV) v_read(u - 13);
-                    s = mfma_32x32x16_f16(kf[u % 4], qw[u], s);
-                    // the next copies, one at a time
-                    if (u % 2 == 0 && u < 8) {
-                        if (t + 1 < ntiles) issue_part(t + 1, u / 2, true, false);
-                    } else if (u % 2 == 0) {
-                        bad_k |= issue_part(t, (u - 8) / 2, false, true);
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] *= sc;
-                const int s0 = p_begin + t * kTile + 32 * side;
-                const unsigned bad = bad_k >> (2 * side) & 3;
-                if (s0 + 32 > cut_from || bad) {   // (uniform)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        s[i] = s0 + 8 * (i >> 2) + 4 * h + (i & 3) >= limit ? -INFINITY
-                               : (bad >> (i >> 3)) & 1                       ? __builtin_nanf("")
-                                                                             : s[i];
-                }
-            } else {
-#pragma unroll
-                for (int u = 0; u < 3; ++u) v_read(u);
-            }
-            // PV's 16 products with the softmax of the new scores between them
-            float tm, alpha = 1.0f, mb;
-            bool raised = false;
-#pragma unroll
-            for (int u = 0; u < 16; ++u) {
-                if constexpr (WV) {
-                    if (u + 3 < 16) v_read(u + 3);
-                    ow[u & 7] = mfma_32x32x16_f16(u32x4_t{vf[u % 4][0][0], vf[u % 4][0][1], vf[u % 4][1][0], vf[u % 4][1][1]},
-                                                  pw[u >> 3], ow[u & 7]);
-                }
-                if constexpr (WS) {
-                    if (u < 4) {
-                        const float m4 = fmaxf(fmaxf(s[4 * u], s[4 * u + 1]), fmaxf(s[4 * u + 2], s[4 * u + 3]));
-                        tm = u == 0 ? m4 : fmaxf(tm, m4);
-                    } else if (u == 4) {
-                        const auto h2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(tm), __float_as_uint(tm), false, false);
-                        tm = fmaxf(__uint_as_float(h2[0]), __uint_as_float(h2[1]));
-                        raised = __any(tm > m_w + kLazyMax);
-                        if (raised) {
-                            const float m_new = tm > m_w + kLazyMax ? tm : m_w;
-                            alpha = m_new == m_w ? 1.0f : __builtin_amdgcn_exp2f(m_w - m_new);
-                            m_w = m_new;
-                            d_w *= alpha;
-                        }
-                        // (a half behind the chunk's end, or before a token's first position, gives weights of 0)
-                        mb = m_w == -INFINITY ? 0.0f : m_w - kShift<KV_F16>;
-                    } else if (u < 13) {
-                        const int i = 2 * (u - 5);
-                        s[i] = __builtin_amdgcn_exp2f(s[i] - mb);
-                        s[i + 1] = __builtin_amdgcn_exp2f(s[i + 1] - mb);
-                        d_w += s[i] + s[i + 1];
-                    }
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            if constexpr (WS) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) pw[i >> 2][i & 3] = pack_f16x2(s[2 * i], s[2 * i + 1]);
-                if (raised) {
-#pragma unroll
-                    for (int dt = 0; dt < 8; ++dt)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) ow[dt][i] *= alpha;
-                }
-            }
-        };
-        iter(std::true_type{}, std::false_type{}, 0);
-        for (int t = 1; t < ntiles; ++t) iter(std::true_type{}, std::true_type{}, t);
-        iter(std::false_type{}, std::true_type{}, ntiles);
-        const auto h2 = __builtin_amdgcn_permlane32_swap(__float_as_uint(d_w), __float_as_uint(d_w), false, false);
-        d_w = __uint_as_float(h2[0]) + __uint_as_float(h2[1]);
-        // each side finishes half of a row's dims (dim tiles 4 side ..) with the other's
-        // sums. Two pieces of four dims change places between rows 0-15 and 16-31,
-        // so that a store writes 64 bytes of 16 rows instead of 32 bytes of 32.
-        int l = lane;   // (opaque: computed ahead of the loop, the addresses would cost it registers)
-        asm volatile("" : "+v"(l));
-        auto slot_row = [&](int s) { return ((static_cast<size_t>(s) * 2 + kvh) * pp.cstride + slot_c) * 8 + (l & 7); };
-        const int s_lo = lead + 4 * r32 + ((l >> 3) & 1), n_out = 8 * ((l >> 4) & 1) + 4 * (l >> 5);
-        const bool mine_lo = s_lo < lead + count, mine_hi = s_lo + 2 < lead + count;
-        float* const po_lo = pp.o + slot_row(mine_lo ? s_lo : lead) * 256 + n_out;
-        float* const po_hi = pp.o + slot_row(mine_hi ? s_lo + 2 : lead) * 256 + n_out;
-        f32x4_t* const hand = reinterpret_cast<f32x4_t*>(L.tile);   // 16 KB a wave, one piece a lane and index
-        __syncthreads();
-        auto exchange = [&](auto pc) {
-            constexpr int P = decltype(pc)::value;
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    hand[1024 * wv + 64 * (4 * c + j) + lane] =
-                        f32x4_t{ow[4 * (1 - P) + c][4 * j], ow[4 * (1 - P) + c][4 * j + 1], ow[4 * (1 - P) + c][4 * j + 2],
-                                ow[4 * (1 - P) + c][4 * j + 3]};
-            if (h == 0) {
-                L.mdw[wv][rn][0] = m_w;
-                L.mdw[wv][rn][1] = d_w;
-            }
-            __syncthreads();
-            const int partner = wv ^ 4;
-            const float m1 = L.mdw[partner][rn][0], m = fmaxf(m_w, m1);
-            const float f0 = m_w == m ? 1.0f : __builtin_amdgcn_exp2f(m_w - m);
-            const float f1 = m1 == m ? 1.0f : __builtin_amdgcn_exp2f(m1 - m);
-            if (P == 0 && l < 32 && 4 * r32 + (l >> 3) < count) {
-                const size_t at = slot_row(lead + 4 * r32 + (l >> 3));
-                pp.m[at] = m - kShift<KV_F16>;
-                pp.d[at] = d_w * f0 + L.mdw[partner][rn][1] * f1;
-            }
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-                for (int j = 0; j < 4; j += 2) {
-                    const f32x4_t v0 = hand[1024 * partner + 64 * (4 * c + j) + lane];
-                    const f32x4_t v1 = hand[1024 * partner + 64 * (4 * c + j + 1) + lane];
-                    f32x4_t lo, hi;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const auto r = __builtin_amdgcn_permlane16_swap(
-                            __float_as_uint(ow[4 * P + c][4 * j + i] * f0 + v0[i] * f1),
-                            __float_as_uint(ow[4 * P + c][4 * j + 4 + i] * f0 + v1[i] * f1), false, false);
-                        lo[i] = __uint_as_float(r[0]);
-                        hi[i] = __uint_as_float(r[1]);
-                    }
-                    const int dim = 128 * P + 16 * c + 32 * j;
-                    if (mine_lo) *reinterpret_cast<f32x4_t*>(po_lo + dim) = lo;
-                    if (mine_hi) *reinterpret_cast<f32x4_t*>(po_hi + dim) = hi;
-                }
-        };
-        if (side == 1) exchange(std::integral_constant<int, 1>{});
-        else exchange(std::integral_constant<int, 0>{});
-    };
-    if constexpr (NT == 1) {
-        if (wide) {
-            prepare_own();
-            wide_block();
-            return;
-        }
-    }
     if (single) {
         prepare(std::integral_constant<int, 1>{}, std::true_type{});
         clear();
@@ -1149,8 +926,8 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
             const int t0 = p_begin + t * kTile;
             put_tokens(t);
             if (t + 1 < ntiles) {
-                window(t + 1, t + 1);
-                bad_next = issue(t + 1, true, true);
+                window(t + 1);
+                bad_next = issue(t + 1);
             } else if (TOKENS || has_new) {
                 const int r = p_end - t0;
                 if (!TOKENS && (wv == 4 || wv == 5)) *tile_at(t, wv - 4, r - 1) = fresh;   // the new token's row
@@ -1164,7 +941,7 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
         if (R == 1) prepare(std::integral_constant<int, 1>{}, std::false_type{});
         else if (R == 2) prepare(std::integral_constant<int, 2>{}, std::false_type{});
         else if (R == 4) prepare(std::integral_constant<int, 4>{}, std::false_type{});
-        else if constexpr (NT > 1) prepare_own();
+        else prepare_own();
         clear();
         for (int t = 0; t < ntiles; ++t) {
             arrive(t);
@@ -1172,8 +949,8 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
             const int t0 = p_begin + t * kTile;
             put_tokens(t);
             if (t + 1 < ntiles) {
-                window(t + 1, t + 1);
-                bad_next = issue(t + 1, true, true);
+                window(t + 1);
+                bad_next = issue(t + 1);
             } else if (TOKENS) clear_behind(t, p_end - t0, (p_end - t0 + 31) & ~31);
             clear_bad(t, bad);
             if (!active) continue;
@@ -1412,7 +1189,7 @@ static PagedKv paged_kv(const qff_kv_pages* kv) {
 }
 
 // Terms of q and of the weights.
-static int paged_terms(bool kv_f16, bool out16) { return kv_f16 ? (out16 ? 1 : 2) : (out16 ? 2 : 3); }
+static int paged_terms(bool kv_f16, bool out16) { return kv_f16 || out16 ? 2 : 3; }
 
 // The partial launch (a batch's step, or a slice's tokens) and the combine of
 // `rows` sequences or tokens.
@@ -1430,12 +1207,9 @@ static void launch_partials(qff_ctx* ctx, hipStream_t stream, const qff_gqa_para
                                                                      p->scale, p->eps, pk, a ? *a : none, tk, pp)
 #define QFF_PART(I, F, N) \
     if (a) QFF_PART1(I, F, N, false); else QFF_PART1(I, F, N, true)
-        const int terms = paged_terms(f16, out16);
-        if (terms == 1) {
-            if (in16) { QFF_PART(1, 1, 1); } else { QFF_PART(0, 1, 1); }
-        } else if (f16) {
+        if (f16) {
             if (in16) { QFF_PART(1, 1, 2); } else { QFF_PART(0, 1, 2); }
-        } else if (terms == 2) {
+        } else if (paged_terms(f16, out16) == 2) {
             if (in16) { QFF_PART(1, 0, 2); } else { QFF_PART(0, 0, 2); }
         } else {
             if (in16) { QFF_PART(1, 0, 3); } else { QFF_PART(0, 0, 3); }
@@ -1465,8 +1239,7 @@ hipError_t launch_gqa_decode_paged(qff_ctx* ctx, hipStream_t stream, const qff_g
                                    void* out, qff_dtype out_dtype, int batch) {
     const PagedKv pk = paged_kv(kv);
     const int cap = gqa_chunk_cap(ctx->cfg, batch);
-    const PagedSeqs a{positions, group, shared_len, batch, kv->table_cols << pk.lg, ctx->num_cu / 2, cap,
-                      paged_terms(p->kv_f16 != 0, out_dtype == QFF_BF16)};
+    const PagedSeqs a{positions, group, shared_len, batch, kv->table_cols << pk.lg, ctx->num_cu / 2, cap};
     const PagedPartials pp{ctx->gqa_m, ctx->gqa_d, ctx->gqa_o, ctx->gqa_nc, cap};
     // a round of workgroups, and one more for each stream of positions (a
     // sequence's own, a block's shared ones) that rounding up can add
@@ -1483,14 +1256,13 @@ hipError_t launch_gqa_decode_paged(qff_ctx* ctx, hipStream_t stream, const qff_g
 //   bf16 cache and outputs (two terms)  8 tokens 15 / 20, 17 / 26, 23 / 45, 39 / 82
 //                                      64 tokens 20 / 23, 32 / 34, 63 / 64, 132 / 136
 //                                      96 tokens 22 / 25, 34 / 34, 81 / 75, 188 / 164
-//   fp16 cache, bf16 outputs (one)    128 tokens 24 / 24, 32 / 35, 69 / 99, 160 / 197
 //   bf16 cache, fp32 outputs (three)   32 tokens 18 / 23, 29 / 30, 50 / 56, 98 / 103
 //                                      64 tokens 21 / 23, 34 / 34, 73 / 67, 164 / 133
 hipError_t launch_gqa_prefill_paged(qff_ctx* ctx, hipStream_t stream, const qff_gqa_params* p, const void* q_gate,
                                     const void* k, const void* v, qff_dtype in_dtype, const qff_kv_pages* kv,
                                     int start, void* out, qff_dtype out_dtype, int T) {
     const int cap = static_cast<int>(std::min<long long>(kGqaMaxChunks, ctx->pf_slots / T));
-    if (T * paged_terms(p->kv_f16 != 0, out_dtype == QFF_BF16) > kPagedTokensMax || cap < 4)
+    if (T * paged_terms(p->kv_f16 != 0, out_dtype == QFF_BF16) > 2 * kPagedTokensMax || cap < 4)
         return launch_gqa_prefill(ctx, stream, p, q_gate, k, v, in_dtype, kv->k, kv->v, kv, start, out, out_dtype, T);
     const PagedKv pk = paged_kv(kv);
     if (!PagedTokens{start, T, kTile, 0}.append()) {

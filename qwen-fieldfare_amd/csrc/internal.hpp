@@ -196,7 +196,7 @@ hipError_t launch_gqa_decode_paged(qff_ctx* ctx, hipStream_t stream, const qff_g
                                    const int32_t* positions, const int32_t* group, const int32_t* shared_len,
                                    void* out, qff_dtype out_dtype, int batch);
 // Prefill into pages: a short slice on the decode's kernels, a long one as launch_gqa_prefill.
-constexpr int kPagedTokensMax = 128;   // tokens of the former
+constexpr int kPagedTokensMax = 64;   // tokens of the former
 hipError_t launch_gqa_prefill_paged(qff_ctx* ctx, hipStream_t stream, const qff_gqa_params* p, const void* q_gate,
                                     const void* k, const void* v, qff_dtype in_dtype, const qff_kv_pages* kv,
                                     int start, void* out, qff_dtype out_dtype, int T);
