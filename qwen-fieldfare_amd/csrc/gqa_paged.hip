@@ -1261,8 +1261,9 @@ hipError_t launch_gqa_decode_paged(qff_ctx* ctx, hipStream_t stream, const qff_g
 hipError_t launch_gqa_prefill_paged(qff_ctx* ctx, hipStream_t stream, const qff_gqa_params* p, const void* q_gate,
                                     const void* k, const void* v, qff_dtype in_dtype, const qff_kv_pages* kv,
                                     int start, void* out, qff_dtype out_dtype, int T) {
-    const int cap = static_cast<int>(std::min<long long>(kGqaMaxChunks, ctx->pf_slots / T));
-    if (T * paged_terms(p->kv_f16 != 0, out_dtype == QFF_BF16) > 2 * kPagedTokensMax || cap < 4)
+    // (a slice's precision follows from its tokens and types alone: a context of few
+    // partial rows gives fewer chunks, pf_slots(cfg) at least one a token)
+    if (T * paged_terms(p->kv_f16 != 0, out_dtype == QFF_BF16) > 2 * kPagedTokensMax)
         return launch_gqa_prefill(ctx, stream, p, q_gate, k, v, in_dtype, kv->k, kv->v, kv, start, out, out_dtype, T);
     const PagedKv pk = paged_kv(kv);
     if (!PagedTokens{start, T, kTile, 0}.append()) {
@@ -1284,7 +1285,7 @@ hipError_t launch_gqa_prefill_paged(qff_ctx* ctx, hipStream_t stream, const qff_
     // tokens behind 900 and 5000 23.3 / 24.4, 29.2 / 33.5, 16 behind 20000 and 60000,
     // 5 and 15 tiles, 31.1 / 32.6, 55.5 / 51.6; fp16 33 behind 20000, 13 tiles, 41 /
     // 39, 64 behind 60000 118 / 90).
-    const int slots = ctx->num_cu / 2;
+    const int slots = ctx->num_cu / 2, cap = static_cast<int>(std::min<long long>(kGqaMaxChunks, ctx->pf_slots / T));
     auto split = [&](int per) {
         PagedTokens tk{start, T, kTile, per};
         while ((tk.items() > slots && tk.ch < start + T) || (start + T + tk.ch - 1) / tk.ch > cap) tk.ch += kTile;

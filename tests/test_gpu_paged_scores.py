@@ -79,3 +79,21 @@ def test_short_slices_at_score_magnitudes(hip, ctx, io, kv, out, start, T, s):
     got = qff.gqa_prefill_paged(ctx, c.p, qg, k, v, c.kp, c.vp, c.table[0], start_pos=start, out_dtype=DT[out])
     pos = torch.arange(start, start + T, dtype=torch.int32, device=DEV)
     assert_near(got, R.attend(c.p, qg, c.kp, c.vp, c.table[0], pos), kv, s)
+
+
+@pytest.mark.parametrize("max_ctx,start,T", [(512, 448, 64), (512, 470, 42), (200, 130, 64), (100, 41, 42), (100, 3, 9), (64, 62, 2)])
+@pytest.mark.parametrize("io,kv,out", TYPES)
+def test_short_slices_in_contexts_of_few_partials(hip, io, kv, out, max_ctx, start, T):
+    """A slice's precision depends on its tokens and types, not on how many
+    partial rows its context has: one to three chunks a token here."""
+    import qff
+    if T * (3 if (kv, out) == ("bf16", "f32") else 2) > 128:
+        T = 42
+    small = qff.Context(max_batch=1, max_ctx=max_ctx, max_prefill_tokens=64)
+    c = Case([start + T], 16, io, kv, seed=T)
+    g = torch.Generator(device=DEV).manual_seed(T)
+    qg, k, v = (_randn(g, T, *shape, dtype=DT[io]) for shape in ((16, 512), (2, 256), (2, 256)))
+    got = qff.gqa_prefill_paged(small, c.p, qg, k, v, c.kp, c.vp, c.table[0], start_pos=start, out_dtype=DT[out])
+    pos = torch.arange(start, start + T, dtype=torch.int32, device=DEV)
+    assert_near(got, R.attend(c.p, qg, c.kp, c.vp, c.table[0], pos), kv, 1)
+    small.close()
