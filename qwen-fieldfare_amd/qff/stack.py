@@ -56,8 +56,13 @@ class AttentionStack:
         self.max_ctx = max_ctx
         self.eps = eps
         self.pages = pages
-        if pages is not None and len(pages.lengths) != batch:
-            raise ValueError(f"the page table must have {batch} slots")
+        if pages is not None:
+            # (here, and not by the first call that finds out with its positions reserved)
+            if len(pages.lengths) != batch or batch > ctx.cfg.max_batch:
+                raise ValueError(f"the page table must have {batch} slots, and the context's max_batch as many")
+            if pages.cols > -(-ctx.cfg.max_ctx // pages.page_size):
+                raise ValueError(f"the page table's rows of {pages.cols * pages.page_size} positions exceed the context's "
+                                 f"max_ctx of {ctx.cfg.max_ctx}")
         self._parked = {}   # slot -> its recurrent states, while it sits out decode steps
         self.kinds = list(kinds) if kinds is not None else \
             ["gqa" if is_full_attention(l) else "dn" for l in range(len(self.layers))]
@@ -175,9 +180,11 @@ class AttentionStack:
         """A prompt slice of T tokens of one slot through every layer: x [T, 2048]
         fp32 (the residual stream, in place) at positions start .. start + T - 1,
         behind those that the slot holds; start 0 begins a sequence in an empty slot
-        (zero recurrent states)."""
+        (zero recurrent states). A refused call changes nothing."""
         if x.dtype != torch.float32 or x.dim() != 2 or x.shape[1] != HIDDEN:
             raise ValueError(f"x must be float32 [T, {HIDDEN}]")
+        if x.get_device() != self.ctx.device or not x.is_contiguous():
+            raise ValueError(f"x must be contiguous, on the context's device, cuda:{self.ctx.device}")
         P, T, ctx, eps = self._paged(), x.shape[0], self.ctx, self.eps
         if T > ctx.cfg.max_prefill_tokens or start + T > ctx.cfg.max_ctx:
             raise ValueError(f"{T} tokens from {start}: the context takes slices of {ctx.cfg.max_prefill_tokens} up to "
