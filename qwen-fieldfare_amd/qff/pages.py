@@ -111,6 +111,21 @@ class PageTable:
         self.lengths[slot] = 0
         self._dirty = True
 
+    def truncate(self, slot: int, end: int) -> None:
+        """Slot `slot` holds its first `end` positions only: a reservation taken
+        back, or tokens that are given up. Pages behind them that no other slot
+        holds are free again."""
+        if not 0 <= end <= self.lengths[slot]:
+            raise ValueError(f"slot {slot} holds {self.lengths[slot]} positions, not {end}")
+        if end == self.lengths[slot]:
+            return
+        row, keep = self._rows[slot], -(-end // self.page_size)
+        for page in self.pages_of(slot)[keep:]:
+            self._drop(page)
+        row[keep:] = -1
+        self.lengths[slot] = end
+        self._dirty = True
+
     def compact(self) -> tuple[list[int], list[int]]:
         """Moves the pages in use to the front of the pools: returns sources
         and destinations (disjoint) of the copies to make in every pool. Pages

@@ -25,6 +25,7 @@ from __future__ import annotations
 import torch
 
 from . import ops
+from .pages import OutOfPages
 
 HIDDEN = 2048
 
@@ -153,13 +154,21 @@ class AttentionStack:
     def reserve(self, positions):
         """Places for one decode step's tokens: positions[b] is the new token's
         position in slot b, negative for a slot that takes no part (what it holds
-        stays as it is, for a later step or slice). Pages that a slot shares and is
-        about to write are copied; an empty slot's position 0 begins a sequence
-        (zero recurrent states). Where the pool runs out (OutOfPages), the slots
-        before that one have theirs."""
+        stays as it is, for a later step or slice). Each follows those that the slot
+        holds (it may lie among them in a stack without recurrent layers, whose
+        states cannot go back). Pages that a slot shares and is about to write are
+        copied; an empty slot's position 0 begins a sequence (zero recurrent
+        states). Where the pool runs out (OutOfPages), no slot holds a position more
+        than before; the copies made for the slots before that one stay theirs."""
         pages, copies = self._paged(), []
         if len(positions) != self.B:
             raise ValueError(f"positions must have {self.B} entries")
+        held = list(pages.lengths)
+        for b, p in enumerate(positions):
+            if p > held[b] or 0 <= p < held[b] and "dn" in self.kinds:
+                raise ValueError(f"slot {b} holds {held[b]} positions: position {p} does not follow them")
+            if p >= pages.cols * pages.page_size:
+                raise ValueError(f"slot {b}: position {p} does not fit {pages.cols} pages")
         try:
             for b, p in enumerate(positions):
                 if p < 0:
@@ -172,6 +181,10 @@ class AttentionStack:
                     for t in self._recurrent():
                         t[b].zero_()
                 self._unpark(b)
+        except OutOfPages:
+            for b, n in enumerate(held):
+                pages.truncate(b, n)
+            raise
         finally:
             self._copy_pages([s for s, _ in copies], [d for _, d in copies])
             self.pages.sync()

@@ -70,3 +70,84 @@ def test_a_table_that_the_context_cannot_serve_is_refused_at_once():
     with pytest.raises(ValueError, match="slots"):
         AttentionStack(_ctx(), [], SLOTS + 1, 256, states=[], kinds=[], device="cpu", pages=table)
     _stack(ctx=_ctx(max_ctx=250))    # 256 positions in whole pages
+
+
+def _copy(st, monkeypatch):
+    """The page copies of the stack, on the host."""
+    def pages_copy(ctx, pools, src, dst):
+        for pool in pools:
+            for s, d in zip(src, dst):
+                pool[d] = pool[s]
+    monkeypatch.setattr("qff.stack.ops.pages_copy", pages_copy)
+
+
+def _hold(st, slot, n):
+    """Slot `slot` holds n positions, as a prompt's slices leave it."""
+    st.pages.reserve(slot, 0, n)
+    st.pages.sync()
+
+
+@pytest.mark.parametrize("positions", [[20, -1, 7, -1], [20, -1, 4, -1], [20, -1, 5, 1], [20, -1, 5, 256], [20, 3, 5, -1]])
+def test_a_step_follows_what_each_slot_holds(positions):
+    """A position before the end would advance recurrent states twice, one past
+    it leaves a hole: refused with no slot changed, the ones before it neither."""
+    st = _stack()
+    _hold(st, 0, 20)
+    _hold(st, 2, 5)
+    before = _snapshot(st)
+    with pytest.raises(ValueError):
+        st.reserve(positions)
+    assert _same(before, _snapshot(st)) and not st._parked
+    st.reserve([20, -1, 5, 0])
+    assert st.pages.lengths == [21, 0, 6, 1]
+
+
+def test_a_stack_without_recurrent_layers_may_go_back(monkeypatch):
+    st = _stack(kinds=("gqa",))
+    _copy(st, monkeypatch)
+    _hold(st, 0, 20)
+    st.reserve([18, -1, -1, -1])
+    assert st.pages.lengths == [20, 0, 0, 0]
+
+
+@pytest.mark.parametrize("kinds", [("dn", "gqa"), ("gqa",)])
+def test_out_of_pages_takes_the_steps_positions_back(monkeypatch, kinds):
+    """Slot 0 would begin a page, slot 1 copy a shared one, slot 2 find none
+    free: none counts its position, and the same step goes through once there is
+    room, with states as they were."""
+    st = _stack(kinds=kinds, pages=4)
+    _copy(st, monkeypatch)
+    _hold(st, 0, 16)
+    _hold(st, 1, 5)
+    st.pages.fork(1, 2)
+    st.pages.sync()
+    states = [t.clone() for t in st._recurrent()]
+    first = st.pages.pages_of(1)[0]
+    _hold(st, 3, 2)                     # (one page is left)
+    with pytest.raises(OutOfPages):
+        st.reserve([16, 5, 5, -1])      # slot 0 takes it, slot 1 is refused
+    assert st.pages.lengths == [16, 5, 5, 2] and st.pages.free_pages == 1
+    assert [st.pages.pages_of(s) for s in (1, 2)] == [[first], [first]]
+    st.reserve([-1, 5, -1, -1])         # sits out: the position it did not get is not counted
+    assert st.pages.lengths == [16, 6, 5, 2]
+    with pytest.raises(OutOfPages):
+        st.reserve([16, 6, 5, -1])
+    assert st.pages.lengths == [16, 6, 5, 2]
+    st.release(3)
+    st.reserve([16, 6, 5, -1])
+    assert st.pages.lengths == [17, 7, 6, 0]
+    assert all(torch.equal(a, b) for a, b in zip(states, st._recurrent()))
+
+
+def test_a_sequence_that_could_not_begin_begins_later(monkeypatch):
+    """Position 0 of an empty slot, taken back: the slot is empty again, and the
+    next try begins with zero states."""
+    st = _stack(pages=2)
+    _copy(st, monkeypatch)
+    _hold(st, 1, 16)
+    with pytest.raises(OutOfPages):
+        st.reserve([0, 16, -1, -1])
+    assert st.pages.lengths == [0, 16, 0, 0] and st.pages.free_pages == 1
+    st._recurrent()[0][0] = 7.0         # (what steps leave in a slot without a position)
+    st.reserve([0, -1, -1, -1])
+    assert all(not t[0].any() for t in st._recurrent())

@@ -152,3 +152,25 @@ def test_refusals():
     with pytest.raises(ValueError):
         t.fork(0, 0)
     assert t.compact() == ([], [])
+
+
+def test_truncate_is_what_reserving_less_leaves():
+    t = PageTable(10, 16, 3, 128, device="cpu")
+    t.reserve(0, 0, 50)
+    t.fork(0, 1)
+    for slot, end in ((0, 51), (0, -1), (2, 1)):
+        with pytest.raises(ValueError):
+            t.truncate(slot, end)
+    t.truncate(0, 50)                       # all of it: nothing changes
+    assert t.pages_of(0) == [0, 1, 2, 3]
+    t.truncate(0, 32)                       # pages 2 and 3 are slot 1's alone
+    assert t.pages_of(0) == [0, 1] and t.lengths == [32, 50, 0] and t.free_pages == 6
+    assert t.refs[:4].tolist() == [2, 2, 1, 1]
+    t.truncate(1, 33)
+    assert t.pages_of(1) == [0, 1, 2] and t.free_pages == 7
+    t.sync()
+    assert t.table.tolist() == t._rows.tolist() and t.group.tolist() == [-1, -1, -1] and t._rows[1, 3] == -1
+    t.truncate(1, 0)
+    assert t.pages_of(1) == [] and t.refs[:3].tolist() == [1, 1, 0]
+    assert t.reserve(1, 0, 16) == [] and t.lengths == [32, 16, 0]
+    _consistent(t)
