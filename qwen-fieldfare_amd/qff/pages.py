@@ -53,7 +53,13 @@ class PageTable:
     def free_pages(self) -> int:
         return len(self._free)
 
+    def check_slot(self, slot: int) -> None:
+        """Refuses what is no slot's number (a negative one would be another slot's)."""
+        if not 0 <= slot < len(self.lengths):
+            raise IndexError(f"slot {slot} of {len(self.lengths)}")
+
     def pages_of(self, slot: int) -> list[int]:
+        self.check_slot(slot)
         return [int(p) for p in self._rows[slot, :-(-self.lengths[slot] // self.page_size)]]
 
     def _take(self) -> int:
@@ -71,6 +77,7 @@ class PageTable:
         it pages of its own for them. Returns the (source, destination) pages to
         copy in every pool first, for pages it shared and that hold positions it
         keeps. Positions before start must be there already."""
+        self.check_slot(slot)
         if not 0 <= start < end or start > self.lengths[slot]:
             raise ValueError(f"positions {start} .. {end - 1} do not follow the {self.lengths[slot]} that slot {slot} holds")
         if end > self.cols * self.page_size:
@@ -94,6 +101,8 @@ class PageTable:
 
     def fork(self, src: int, dst: int) -> None:
         """Slot dst (empty) gets what slot src holds; no page is copied."""
+        self.check_slot(src)
+        self.check_slot(dst)
         if src == dst or self.lengths[dst]:
             raise ValueError(f"slot {dst} must be empty")
         n = -(-self.lengths[src] // self.page_size)
@@ -115,6 +124,7 @@ class PageTable:
         """Slot `slot` holds its first `end` positions only: a reservation taken
         back, or tokens that are given up. Pages behind them that no other slot
         holds are free again."""
+        self.check_slot(slot)
         if not 0 <= end <= self.lengths[slot]:
             raise ValueError(f"slot {slot} holds {self.lengths[slot]} positions, not {end}")
         if end == self.lengths[slot]:

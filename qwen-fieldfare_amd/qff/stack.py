@@ -199,6 +199,7 @@ class AttentionStack:
         if x.get_device() != self.ctx.device or not x.is_contiguous():
             raise ValueError(f"x must be contiguous, on the context's device, cuda:{self.ctx.device}")
         P, T, ctx, eps = self._paged(), x.shape[0], self.ctx, self.eps
+        P.check_slot(slot)
         if T > ctx.cfg.max_prefill_tokens or start + T > ctx.cfg.max_ctx:
             raise ValueError(f"{T} tokens from {start}: the context takes slices of {ctx.cfg.max_prefill_tokens} up to "
                              f"position {ctx.cfg.max_ctx}")
@@ -228,6 +229,8 @@ class AttentionStack:
         held by all, its recurrent states copied. Neighbouring slots read what
         they share once."""
         dsts, pages = list(dsts), self._paged()
+        for s in (src, *dsts):
+            pages.check_slot(s)
         if src in dsts or len(set(dsts)) < len(dsts) or any(pages.lengths[d] for d in dsts):
             raise ValueError("a fork goes into empty slots")
         for d in dsts:

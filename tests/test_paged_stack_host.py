@@ -151,3 +151,18 @@ def test_a_sequence_that_could_not_begin_begins_later(monkeypatch):
     st._recurrent()[0][0] = 7.0         # (what steps leave in a slot without a position)
     st.reserve([0, -1, -1, -1])
     assert all(not t[0].any() for t in st._recurrent())
+
+
+@pytest.mark.parametrize("slot", [-1, -SLOTS, SLOTS])
+def test_what_is_no_slots_number_is_refused(slot):
+    """A negative number would be another slot's pages, and not its parked states."""
+    st = _stack(ctx=_ctx(device=-1))
+    _hold(st, 3, 40)
+    before = _snapshot(st)
+    P = st.pages
+    for call in (lambda: st.prefill(slot, torch.zeros(4, 2048)), lambda: st.release(slot), lambda: st.fork(slot, [1]),
+                 lambda: st.fork(3, [0, slot]), lambda: P.reserve(slot, 0, 1), lambda: P.release(slot), lambda: P.fork(slot, 0),
+                 lambda: P.fork(3, slot), lambda: P.truncate(slot, 0), lambda: P.pages_of(slot)):
+        with pytest.raises(IndexError):
+            call()
+        assert _same(before, _snapshot(st))
