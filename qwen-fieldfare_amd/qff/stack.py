@@ -123,6 +123,11 @@ class AttentionStack:
         in each sequence; full-attention layers append there)."""
         if x.dtype != torch.float32 or tuple(x.shape) != (self.B, HIDDEN):
             raise ValueError(f"x must be float32 [{self.B}, {HIDDEN}]")
+        # (here, and not by the first full-attention layer, with recurrent states advanced before it)
+        if positions.dtype != torch.int32 or positions.numel() != self.B:
+            raise TypeError(f"positions must be int32 [{self.B}]")
+        if positions.device != x.device or not positions.is_contiguous():
+            raise ValueError("positions must be contiguous, on x's device")
         for l in range(len(self.layers)):
             self.layer_step(l, x, positions)
 

@@ -166,3 +166,20 @@ def test_what_is_no_slots_number_is_refused(slot):
         with pytest.raises(IndexError):
             call()
         assert _same(before, _snapshot(st))
+
+
+@pytest.mark.parametrize("positions,error", [(torch.zeros(SLOTS), TypeError), (torch.zeros(SLOTS, dtype=torch.int64), TypeError),
+                                             (torch.zeros(SLOTS - 1, dtype=torch.int32), TypeError),
+                                             (torch.zeros(2 * SLOTS, dtype=torch.int32)[::2], ValueError),
+                                             (torch.zeros(SLOTS, dtype=torch.int32, device="meta"), ValueError)])
+def test_a_step_is_refused_before_its_first_layer(monkeypatch, positions, error):
+    """A full-attention layer behind recurrent ones would refuse these positions
+    with the states before it advanced."""
+    st = _stack(ctx=_ctx(device=-1))
+    ran = []
+    monkeypatch.setattr(st, "layer_step", lambda l, x, pos: ran.append(l))
+    with pytest.raises(error):
+        st.decode_step(torch.zeros(SLOTS, 2048), positions)
+    assert not ran
+    st.decode_step(torch.zeros(SLOTS, 2048), torch.zeros(SLOTS, dtype=torch.int32))
+    assert ran == [0, 1]
