@@ -81,3 +81,143 @@ def test_kv_pages_block_matches_the_structure():
     from qff._lib import KvPages
     f = (0x1122334455667788, 0x1122334455667799, 0x11223344556677aa, 3, 64, 17)
     assert ops._P_KV.pack(*f) == bytes(KvPages(*f)) and ops._P_KV.size == ctypes.sizeof(KvPages)
+
+
+class _Calls:
+    """In the library's place: takes every call, and remembers their names."""
+
+    def __init__(self):
+        self.made = []
+
+    def __getattr__(self, name):
+        return lambda *args: self.made.append(name) or 0
+
+
+@pytest.fixture
+def on_host(monkeypatch):
+    """(context, calls): host tensors lie on this context's device (-1), so that
+    nothing but the check in question can refuse a call."""
+    from qff import ops
+    calls = _Calls()
+    monkeypatch.setattr(ops, "_hot", lambda: calls)
+    monkeypatch.setattr(ops, "_stream_of", lambda ctx: 0)
+    return types.SimpleNamespace(device=-1, handle=None), calls
+
+
+def _each_call(ops, ctx, a):
+    """The decode, the shared decode and the prefill of these arguments."""
+    B = a["positions"].numel()
+    yield "qff_gqa_decode_paged", lambda: ops.gqa_decode_paged(ctx, **a)
+    ints = torch.zeros(B, dtype=torch.int32)
+    yield "qff_gqa_decode_shared", lambda: ops.gqa_decode_shared(ctx, **a, group=ints, shared_len=ints)
+    one = {k: a[k] for k in ("params", "q_gate", "k_pages", "v_pages") if k in a} | {"k": a["k_new"], "v": a["v_new"], "table": a["table"][0]}
+    yield "qff_gqa_prefill_paged", lambda: ops.gqa_prefill_paged(ctx, **one, **({"out": a["out"]} if "out" in a else {}))
+
+
+def test_wrappers_pass_on_what_they_check(on_host):
+    from qff import ops
+    ctx, calls = on_host
+    for kv in (torch.bfloat16, torch.float16):
+        for name, call in _each_call(ops, ctx, _args(kv=kv)):
+            assert call().shape == (2, 16, 256) and calls.made[-1] == name
+    ops.pages_copy(ctx, [torch.zeros(4, 16)], [0], [1])
+    assert calls.made[-1] == "qff_pages_copy"
+
+
+_BF, _NORMS = torch.bfloat16, "q_norm_w and k_norm_w must have 256"
+
+
+@pytest.mark.parametrize("change,error,match", [
+    ({"k_pages": torch.zeros(4, 16, 2, 256)}, TypeError, "KV caches must both"),
+    ({"v_pages": torch.zeros(4, 16, 2, 256, dtype=torch.float16)}, TypeError, "KV caches must both"),
+    ({"k_new": torch.zeros(2, 2, 256, dtype=_BF)}, TypeError, "share q_gate's dtype"),
+    ({"v_new": torch.zeros(2, 2, 256, dtype=_BF)}, TypeError, "share q_gate's dtype"),
+    ({"v_pages": torch.zeros(3, 16, 2, 256, dtype=_BF)}, ValueError, "k_pages and v_pages must be"),     # fewer pages than K's
+    ({"v_pages": torch.zeros(5, 16, 2, 256, dtype=_BF)}, ValueError, "k_pages and v_pages must be"),
+    ({"v_pages": torch.zeros(4, 8, 2, 256, dtype=_BF)}, ValueError, "k_pages and v_pages must be"),
+    ({"k_pages": torch.zeros(4, 16, 256, 2, dtype=_BF), "v_pages": torch.zeros(4, 16, 256, 2, dtype=_BF)}, ValueError, "k_pages and v_pages must be"),
+    ({"k_pages": torch.zeros(64, 2, 256, dtype=_BF), "v_pages": torch.zeros(64, 2, 256, dtype=_BF)}, ValueError, "k_pages and v_pages must be"),
+    ({"q_gate": torch.zeros(2, 16, 511)}, ValueError, "q_gate must be"),
+    ({"k_new": torch.zeros(3, 2, 256)}, ValueError, "q_gate must be"),
+    ({"v_new": torch.zeros(2, 2, 255)}, ValueError, "q_gate must be"),
+    ({"params": {"q_norm_w": torch.ones(255), "k_norm_w": torch.ones(256)}}, ValueError, _NORMS),
+    ({"params": {"q_norm_w": torch.ones(256), "k_norm_w": torch.ones(128)}}, ValueError, _NORMS),
+    ({"params": {"q_norm_w": torch.ones(256, dtype=_BF), "k_norm_w": torch.ones(256)}}, TypeError, "q_norm_w must be torch.float32"),
+    ({"table": torch.zeros(2, 2, dtype=torch.int64)}, TypeError, "the page table must be torch.int32"),
+    ({"out": torch.zeros(1, 16, 256)}, ValueError, "out must be"),
+    ({"out": torch.zeros(2, 16, 512)[:, :, ::2]}, ValueError, "out must be contiguous"),
+    ({"out": torch.zeros(2, 16, 256, dtype=torch.float64)}, TypeError, "unsupported dtype"),
+    ({"q_gate": torch.zeros(2, 16, 1024)[:, :, ::2]}, ValueError, "q_gate must be contiguous"),
+    ({"k_new": torch.zeros(2, 2, 512)[:, :, ::2]}, ValueError, "k must be contiguous"),
+    ({"v_new": torch.zeros(2, 2, 512)[:, :, ::2]}, ValueError, "v must be contiguous"),
+    ({"k_pages": torch.zeros(8, 16, 2, 256, dtype=_BF)[::2]}, ValueError, "k_pages must be contiguous"),
+    ({"v_pages": torch.zeros(8, 16, 2, 256, dtype=_BF)[::2]}, ValueError, "v_pages must be contiguous")])
+def test_each_wrapper_check_by_itself(on_host, change, error, match):
+    """What the wrapper lets through without this one check, it refuses with
+    the check's own message, in all three calls; nothing reaches the library."""
+    from qff import ops
+    ctx, calls = on_host
+    for name, call in _each_call(ops, ctx, {**_args(), **change}):
+        with pytest.raises(error, match=match):
+            call()
+    assert not calls.made
+
+
+def test_table_and_sequence_checks_by_themselves(on_host):
+    from qff import ops
+    ctx, calls = on_host
+    a = _args()
+    ints = lambda *n: torch.zeros(*n, dtype=torch.int32)   # noqa: E731
+    for table in (ints(3, 2), ints(1, 2), ints(2), ints(2, 2, 1)):
+        with pytest.raises(ValueError, match=r"the page table must be \[2, entries\]"):
+            ops.gqa_decode_paged(ctx, **{**a, "table": table})
+    with pytest.raises(ValueError, match="the page table must be contiguous"):
+        ops.gqa_decode_paged(ctx, **{**a, "table": ints(2, 4)[:, ::2]})
+    for positions in (ints(1), ints(3)):
+        with pytest.raises(ValueError, match="positions must be"):
+            ops.gqa_decode_paged(ctx, **{**a, "positions": positions})
+    with pytest.raises(TypeError, match="positions must be torch.int32"):
+        ops.gqa_decode_paged(ctx, **{**a, "positions": torch.zeros(2, dtype=torch.int64)})
+    for more in ({"group": ints(1), "shared_len": ints(2)}, {"group": ints(2), "shared_len": ints(3)}):
+        with pytest.raises(ValueError, match="positions, group and shared_len must be"):
+            ops.gqa_decode_shared(ctx, **a, **more)
+    for name in ("group", "shared_len"):
+        with pytest.raises(TypeError, match=f"{name} must be torch.int32"):
+            ops.gqa_decode_shared(ctx, **a, **{"group": ints(2), "shared_len": ints(2), name: torch.zeros(2)})
+    one = {"params": a["params"], "q_gate": a["q_gate"], "k": a["k_new"], "v": a["v_new"], "k_pages": a["k_pages"], "v_pages": a["v_pages"]}
+    for table in (ints(2, 2), ints(1, 1, 2)):
+        with pytest.raises(ValueError, match=r"the page table must be \[1, entries\]"):
+            ops.gqa_prefill_paged(ctx, **one, table=table)
+    with pytest.raises(TypeError, match="the page table must be torch.int32"):
+        ops.gqa_prefill_paged(ctx, **one, table=torch.zeros(2, dtype=torch.int64))
+    assert not calls.made
+    # another device than the context's
+    far = types.SimpleNamespace(device=0, handle=None)
+    for name, call in _each_call(ops, far, a):
+        with pytest.raises(ValueError, match="must live on the context's device, cuda:0"):
+            call()
+    assert not calls.made
+
+
+def test_copy_wrapper_checks_by_themselves(on_host):
+    from qff import ops
+    ctx, calls = on_host
+    pool = torch.zeros(4, 16)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)   # noqa: E731
+    for pools, src, dst, error, match in (
+            ([], [0], [1], ValueError, "at least one pool"),
+            ([pool], [0, 1], [2], ValueError, "src and dst must have the same length"),
+            ([pool], [0], [], ValueError, "src and dst must have the same length"),
+            ([pool, pool[:3]], [0], [1], ValueError, "the same number of pages"),
+            ([pool, torch.zeros(4, 12)], [0], [1], ValueError, "the same number of pages"),
+            ([pool, torch.zeros(8, 8)], [0], [1], ValueError, "the same number of pages"),     # as many bytes, other pages
+            ([pool, torch.zeros(4, 32)[:, ::2]], [0], [1], ValueError, "a pool must be contiguous"),
+            ([pool], torch.tensor([0]), i32(1), TypeError, "src must be"),
+            ([pool], i32(0), torch.tensor([1]), TypeError, "dst must be"),
+            ([pool], i32(0)[None], i32(1), TypeError, "src must be"),
+            ([pool], i32(0, 0, 1, 1)[::2], i32(2, 3), TypeError, "src must be")):
+        with pytest.raises(error, match=match):
+            ops.pages_copy(ctx, pools, src, dst)
+    with pytest.raises(ValueError, match="must live on the context's device, cuda:0"):
+        ops.pages_copy(types.SimpleNamespace(device=0, handle=None), [pool], [0], [1])
+    assert not calls.made
