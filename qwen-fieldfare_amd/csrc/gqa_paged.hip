@@ -57,8 +57,8 @@ namespace qff {
 // so the chunk length is about the least that needs no second round of
 // workgroups where such a length exists.
 
-constexpr int kBlkSeqs = 16;    // sequences of a block at most
-constexpr int kTile = 64;       // positions of a tile
+constexpr int kBlkSeqs = kPagedBlk;   // sequences of a block at most
+constexpr int kTile = kPagedTile;   // positions of a tile
 // Blocks of 8 start and end sooner and spread over more workgroups, blocks of 16
 // read the prefix half as often: 8 where that makes chunks of up to 10 tiles
 // (us with 8 / 16: 16 sequences on 6K, bf16 22.7 / 27.0, on 16K, 5 tiles, 28.1 / 31.5, fp16
@@ -74,23 +74,6 @@ struct PagedSeqs {
     int batch, max_ctx;
     int slots;   // workgroups of one round, per kv head
     int cap;     // chunks allowed per sequence
-};
-
-// A prompt slice instead of a batch: T tokens of one sequence from position
-// `start`, a block of `per` (8 or 16) after the other, each over all positions up
-// to its last token's in chunks of ch. Their rows are appended before, or by this launch
-// where each wave has at most one (its chunk puts it into the tile as well,
-// over what the page held: a launch less, 3 tokens behind 2442 13.0 -> 11.3 us, 8
-// behind 20000 23.1 -> 21.4).
-struct PagedTokens {
-    int start, T, ch, per;
-    __device__ __host__ bool append() const { return T <= 8; }
-    __device__ __host__ int end(int blk) const { return start + (per * blk + per < T ? per * blk + per : T); }
-    int items() const {
-        int n = 0;
-        for (int b = 0; b * per < T; ++b) n += (end(b) + ch - 1) / ch;
-        return n;
-    }
 };
 
 // Sequence b0 + lane: its length, the shared positions of its block, the
@@ -1266,7 +1249,7 @@ hipError_t launch_gqa_prefill_paged(qff_ctx* ctx, hipStream_t stream, const qff_
     if (T * paged_terms(p->kv_f16 != 0, out_dtype == QFF_BF16) > 2 * kPagedTokensMax)
         return launch_gqa_prefill(ctx, stream, p, q_gate, k, v, in_dtype, kv->k, kv->v, kv, start, out, out_dtype, T);
     const PagedKv pk = paged_kv(kv);
-    if (!PagedTokens{start, T, kTile, 0}.append()) {
+    if (!PagedTokens{start, T, kTile, kBlkSeqs}.append()) {
         ProfScope prof(ctx, stream, "gqa_paged_append");
         const RopeFreqs rf = rope_freqs(p->rope_theta);
         const int blocks = (2 * T + 3) / 4;
@@ -1278,21 +1261,8 @@ hipError_t launch_gqa_prefill_paged(qff_ctx* ctx, hipStream_t stream, const qff_
         }
 #undef QFF_APP
     }
-    // The least chunk length that needs no second round of workgroups, and no more
-    // partials than there is room for. Blocks of 8 tokens start and end sooner and
-    // spread over more workgroups, those of 16 read the pages half as often: 8
-    // where that makes chunks of at most four tiles (us with 8 / 16, bf16, 33
-    // tokens behind 900 and 5000 23.3 / 24.4, 29.2 / 33.5, 16 behind 20000 and 60000,
-    // 5 and 15 tiles, 31.1 / 32.6, 55.5 / 51.6; fp16 33 behind 20000, 13 tiles, 41 /
-    // 39, 64 behind 60000 118 / 90).
-    const int slots = ctx->num_cu / 2, cap = static_cast<int>(std::min<long long>(kGqaMaxChunks, ctx->pf_slots / T));
-    auto split = [&](int per) {
-        PagedTokens tk{start, T, kTile, per};
-        while ((tk.items() > slots && tk.ch < start + T) || (start + T + tk.ch - 1) / tk.ch > cap) tk.ch += kTile;
-        return tk;
-    };
-    PagedTokens tk = split(8);
-    if (tk.ch > 4 * kTile) tk = split(kBlkSeqs);
+    const int cap = static_cast<int>(std::min<long long>(kGqaMaxChunks, ctx->pf_slots / T));
+    const PagedTokens tk = paged_tokens_split(start, T, ctx->num_cu / 2, cap);
     // partials where the sharing prefill keeps its own: m and d [T][2][cap][8], o [T][2][cap][8][256]
     const PagedPartials pp{ctx->pf_md, ctx->pf_md + static_cast<size_t>(T) * 16 * cap, ctx->pf_o, ctx->gqa_nc, cap};
     launch_partials(ctx, stream, p, q_gate, k, v, in_dtype, pk, nullptr, tk, pp, 2 * tk.items(), out, out_dtype, T);

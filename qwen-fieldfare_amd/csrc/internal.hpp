@@ -197,6 +197,39 @@ hipError_t launch_gqa_decode_paged(qff_ctx* ctx, hipStream_t stream, const qff_g
                                    void* out, qff_dtype out_dtype, int batch);
 // Prefill into pages: a short slice on the decode's kernels, a long one as launch_gqa_prefill.
 constexpr int kPagedTokensMax = 64;   // tokens of the former
+constexpr int kPagedTile = 64, kPagedBlk = 16;   // positions of a tile; sequences or tokens of a block at most
+
+// A prompt slice instead of a batch: T tokens of one sequence from position
+// `start`, a block of `per` (8 or 16) after the other, each over all positions up
+// to its last token's in chunks of ch. Their rows are appended before, or by this launch
+// where each wave has at most one (its chunk puts it into the tile as well,
+// over what the page held: a launch less, 3 tokens behind 2442 13.0 -> 11.3 us, 8
+// behind 20000 23.1 -> 21.4).
+struct PagedTokens {
+    int start, T, ch, per;
+    __device__ __host__ bool append() const { return T <= 8; }
+    __device__ __host__ int end(int blk) const { return start + (per * blk + per < T ? per * blk + per : T); }
+    int items() const {
+        int n = 0;
+        for (int b = 0; b * per < T; ++b) n += (end(b) + ch - 1) / ch;
+        return n;
+    }
+};
+// The least chunk length that needs no second round of workgroups (`slots` a kv
+// head), and no more than the cap partials a token that there is room for. Blocks of 8
+// tokens start and end sooner and spread over more workgroups, those of 16 read
+// the pages half as often: 8 where that makes chunks of at most four tiles (us
+// with 8 / 16, bf16, 33 tokens behind 900 and 5000 23.3 / 24.4, 29.2 / 33.5, 16
+// behind 20000 and 60000, 5 and 15 tiles, 31.1 / 32.6, 55.5 / 51.6).
+inline PagedTokens paged_tokens_split(int start, int T, int slots, int cap) {
+    auto split = [&](int per) {
+        PagedTokens tk{start, T, kPagedTile, per};
+        while ((tk.items() > slots && tk.ch < start + T) || (start + T + tk.ch - 1) / tk.ch > cap) tk.ch += kPagedTile;
+        return tk;
+    };
+    const PagedTokens tk = split(kPagedBlk / 2);
+    return tk.ch > 4 * kPagedTile ? split(kPagedBlk) : tk;
+}
 hipError_t launch_gqa_prefill_paged(qff_ctx* ctx, hipStream_t stream, const qff_gqa_params* p, const void* q_gate,
                                     const void* k, const void* v, qff_dtype in_dtype, const qff_kv_pages* kv,
                                     int start, void* out, qff_dtype out_dtype, int T);

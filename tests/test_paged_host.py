@@ -221,3 +221,44 @@ def test_copy_wrapper_checks_by_themselves(on_host):
     with pytest.raises(ValueError, match="must live on the context's device, cuda:0"):
         ops.pages_copy(types.SimpleNamespace(device=0, handle=None), [pool], [0], [1])
     assert not calls.made
+
+
+def _program(tmp_path, name):
+    """A C++ program of tests/host_checks over the library, built with g++."""
+    from qff._lib import LIB_PATH
+    exe, rocm = str(tmp_path / name), os.environ.get("ROCM_PATH", "/opt/rocm")
+    r = subprocess.run(["g++", "-std=c++17", "-O1", "-D__HIP_PLATFORM_AMD__", "-w", "-I" + os.path.join(rocm, "include"),
+                        "-I" + os.path.join(ROOT, "include"), "-I" + os.path.join(ROOT, "qwen-fieldfare_amd", "csrc"),
+                        os.path.join(ROOT, "tests", "host_checks", name + ".cpp"), LIB_PATH, "-L" + os.path.join(rocm, "lib"),
+                        "-lamdhip64", "-Wl,-rpath," + os.path.dirname(LIB_PATH), "-Wl,-rpath," + os.path.join(rocm, "lib"),
+                        "-o", exe], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-2000:]
+    return exe
+
+
+def test_split_of_short_slices(tmp_path):
+    """The shapes that tests/test_gpu_paged_blocks.py means for blocks of 16 tokens
+    take them; for slices of any length behind any history, in contexts of few
+    partial rows too, the split keeps to its workgroups and partial rows."""
+    import random
+
+    import test_gpu_paged_blocks as blocks
+    import qff
+    qff.lib()
+    exe = _program(tmp_path, "paged_split")
+    C, P = blocks.CONTEXT["max_ctx"], blocks.CONTEXT["max_prefill_tokens"]
+    tokens = list(blocks.BLOCKS_OF_16)
+    assert sum(t <= 42 for _, t in tokens) >= 5    # (as many tokens as three terms take)
+    rng = random.Random(1)
+    more = []
+    for _ in range(3000):
+        t = rng.randint(1, 64)
+        c = int(2 ** rng.uniform(7, 17))
+        more.append((c, rng.choice([t, 64, 8192]), rng.randint(0, max(0, c - t)), t))
+    r = subprocess.run([exe], input="\n".join(" ".join(map(str, x)) for x in [(C, P, s, t) for s, t in tokens] + more),
+                       capture_output=True, text=True)
+    assert r.returncode == 0, [line for line in r.stdout.splitlines() if "BAD" in line][:5]
+    lines = r.stdout.splitlines()
+    assert len(lines) == len(tokens) + len(more)
+    for shape, line in zip(tokens, lines):
+        assert line.split()[0] == "16", (shape, line)
