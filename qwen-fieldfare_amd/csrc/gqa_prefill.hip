@@ -157,11 +157,12 @@ __global__ __launch_bounds__(64 * kPrepWaves) void gqa_prefill_prep_kernel(
     blk -= pg.vt_blocks;
     if (blk < pg.k16_blocks) {
         // the fp16 copy of K cache rows 0 .. start - 1 (both kv heads); NaN where a page has no row
-        const int i = blk * 512 + static_cast<int>(threadIdx.x);
-        if (i < start * 64) {
-            const size_t o = static_cast<size_t>(i) * 8;
+        // (64 pieces a row: their numbers pass 32 bits from 2^25 rows on)
+        const size_t i = static_cast<size_t>(blk) * 512 + threadIdx.x;
+        if (i < static_cast<size_t>(start) * 64) {
+            const size_t o = i * 8;
             if constexpr (PAGED) {
-                const long long r = at.row(i >> 6);
+                const long long r = at.row(static_cast<int>(i >> 6));
                 u32x4_t w = u32x4_t{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
                 if (r >= 0) {
                     w = *reinterpret_cast<const u32x4_t*>(k_cache + r * 512 + 8 * (i & 63));
@@ -754,7 +755,7 @@ hipError_t launch_gqa_prefill(qff_ctx* ctx, hipStream_t stream, const qff_gqa_pa
         PrepGrid pg;
         pg.vt_stride = (ctx->cfg.max_ctx + kPfKT - 1) / kPfKT;   // tiles per kv head
         pg.vt_blocks = 2 * ((start_pos + T + kPfKT - 1) / kPfKT);
-        pg.k16_blocks = copy_k ? (start_pos * 64 + 511) / 512 : 0;
+        pg.k16_blocks = copy_k ? (start_pos + 7) / 8 : 0;   // 8 rows a workgroup
         // a wave per round where the tokens do not fill the chip: its time is
         // then one round's chain of load, reduction and store instead of three
         // (us per call at 16, 500, 1000, 8192 tokens from position 0: 22.5,
