@@ -51,16 +51,6 @@ namespace qff {
 constexpr int kPfQB = 16;       // query tokens per workgroup
 constexpr int kPfKT = 64;       // K/V positions per tile
 
-// The transposed fp16 copy of V, per kv head and 64-position tile a
-// [256 dims][64 slots] block (the tile's 32 KB contiguous, tiles of one kv
-// head ntile_stride apart). Within each 16 slots, slot 8h + 4j + i holds
-// position 8j + 4h + i (bits 2 and 3 swapped): the order in which the
-// attention's O^T = V^T P^T operand runs over positions, so a lane's eight
-// positions are one 16-byte piece. Positions before start come from the
-// cache, start .. start + T - 1 from the step's v (rounded to the cache's
-// type first, exactly as the prep workgroups store them, so the copy holds
-// the cache's values), later ones are zero. A workgroup of 512 threads
-// stages one tile through LDS.
 // Where position p's row lies: row p of a flat cache, or row p % page of pool
 // page table[p / page]. An entry outside the pool has no row (-1).
 template <bool PAGED>
@@ -74,6 +64,16 @@ struct KvPlace {
     }
 };
 
+// The transposed fp16 copy of V, per kv head and 64-position tile a
+// [256 dims][64 slots] block (the tile's 32 KB contiguous, tiles of one kv
+// head ntile_stride apart). Within each 16 slots, slot 8h + 4j + i holds
+// position 8j + 4h + i (bits 2 and 3 swapped): the order in which the
+// attention's O^T = V^T P^T operand runs over positions, so a lane's eight
+// positions are one 16-byte piece. Positions before start come from the
+// cache, start .. start + T - 1 from the step's v (rounded to the cache's
+// type first, exactly as the prep workgroups store them, so the copy holds
+// the cache's values), later ones are zero. A workgroup of 512 threads
+// stages one tile through LDS.
 __device__ __forceinline__ int vt_slot_row(int s) { return (s & ~12) | ((s & 4) << 1) | ((s & 8) >> 1); }
 
 template <int IN_DT, int KV_F16, bool PAGED>
