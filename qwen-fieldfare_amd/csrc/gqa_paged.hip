@@ -60,11 +60,11 @@ namespace qff {
 constexpr int kBlkSeqs = kPagedBlk;   // sequences of a block at most
 constexpr int kTile = kPagedTile;   // positions of a tile
 // Blocks of 8 start and end sooner and spread over more workgroups, blocks of 16
-// read the prefix half as often: 8 where that makes chunks of up to 10 tiles
-// (us with 8 / 16: 16 sequences on 6K, bf16 22.7 / 27.0, on 16K, 5 tiles, 28.1 / 31.5, fp16
-// 25.2 / 30.4, on 32K, 9 tiles, 36.5 / 40.1, 32.2 / 37.6; 32 on 16K, 9 tiles, 39.1 / 38.8,
-// 34.4 / 33.3, on 32K 59.5 / 55.2, 50.5 / 44.0).
-constexpr int kSmallTiles = 10;
+// read the prefix half as often: 8 where that makes chunks of up to
+// kPagedSmallTiles (us with 8 / 16, bf16 outputs of a bf16 cache, an fp16 one within 2 %:
+// 16 sequences on 6K 23.4 / 26.5, on 32K, 9 tiles, 38.5 / 41.7; 32 on 16K, 10 tiles,
+// 39.8 / 40.7; 24 on 32K, 13 tiles, 47.5 / 53.4; 32 on 24K, 14 tiles, 48.0 / 47.2, on
+// 32K 58.4 / 56.4; fp32 outputs 24 on 32K 55.6 / 62.5, 32 on 24K 56.3 / 54.3).
 constexpr int kMinShared = 64;  // shorter shared prefixes are left to the sequences
 
 struct PagedSeqs {
@@ -383,7 +383,7 @@ __global__ __launch_bounds__(512) void gqa_paged_partial_kernel(
     } else {
         int bs = kBlkSeqs / 2;
         LanePlan p0 = lane_plan(a, 0, lane, bs);
-        Chunk chunk = chunk_length(a, p0, lane, bs, a.group ? kSmallTiles * a.slots : INT_MAX);
+        Chunk chunk = chunk_length(a, p0, lane, bs, a.group ? kPagedSmallTiles * a.slots : INT_MAX);
         if (chunk.len == 0) {   // (uniform)
             bs = kBlkSeqs;
             p0 = lane_plan(a, 0, lane, bs);

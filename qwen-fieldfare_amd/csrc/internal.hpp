@@ -198,6 +198,7 @@ hipError_t launch_gqa_decode_paged(qff_ctx* ctx, hipStream_t stream, const qff_g
 // Prefill into pages: a short slice on the decode's kernels, a long one as launch_gqa_prefill.
 constexpr int kPagedTokensMax = 64;   // tokens of the former
 constexpr int kPagedTile = 64, kPagedBlk = 16;   // positions of a tile; sequences or tokens of a block at most
+constexpr int kPagedSmallTiles = 13;   // longest chunks, in tiles, that blocks of half as many are taken for
 
 // A prompt slice instead of a batch: T tokens of one sequence from position
 // `start`, a block of `per` (8 or 16) after the other, each over all positions up
@@ -218,9 +219,11 @@ struct PagedTokens {
 // The least chunk length that needs no second round of workgroups (`slots` a kv
 // head), and no more than the cap partials a token that there is room for. Blocks of 8
 // tokens start and end sooner and spread over more workgroups, those of 16 read
-// the pages half as often: 8 where that makes chunks of at most four tiles (us
-// with 8 / 16, bf16, 33 tokens behind 900 and 5000 23.3 / 24.4, 29.2 / 33.5, 16
-// behind 20000 and 60000, 5 and 15 tiles, 31.1 / 32.6, 55.5 / 51.6).
+// the pages half as often: 8 where that makes chunks of up to kPagedSmallTiles (us
+// with 8 / 16, bf16: behind 20000 16 tokens, 5 tiles, 31.4 / 33.3, 24, 8 tiles, 35.3 /
+// 39.1, 33, 13 tiles, 45.8 / 47.9, 42, 15 tiles, 48.1 / 47.9, 64, 20 tiles, 57.0 / 56.7;
+// behind 60000 9, 15 tiles, 50.2 / 45.8, 64 134.7 / 126.3. It loses 1 us for 64 behind
+// 5000, 5 tiles, 34.7 / 33.6; an fp16 cache and fp32 outputs alike).
 inline PagedTokens paged_tokens_split(int start, int T, int slots, int cap) {
     auto split = [&](int per) {
         PagedTokens tk{start, T, kPagedTile, per};
@@ -228,7 +231,7 @@ inline PagedTokens paged_tokens_split(int start, int T, int slots, int cap) {
         return tk;
     };
     const PagedTokens tk = split(kPagedBlk / 2);
-    return tk.ch > 4 * kPagedTile ? split(kPagedBlk) : tk;
+    return tk.ch > kPagedSmallTiles * kPagedTile ? split(kPagedBlk) : tk;
 }
 hipError_t launch_gqa_prefill_paged(qff_ctx* ctx, hipStream_t stream, const qff_gqa_params* p, const void* q_gate,
                                     const void* k, const void* v, qff_dtype in_dtype, const qff_kv_pages* kv,

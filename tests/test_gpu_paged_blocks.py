@@ -1,6 +1,6 @@
 """Prompt slices on pages whose blocks are of 16 tokens, which the split takes
-where blocks of 8 would need long chunks (which shapes do is checked on the
-host: tests/test_paged_host.py). Tolerances as in tests/test_gpu_paged_scores.py,
+where blocks of 8 would need long chunks, and of 8 in the longest they get
+(which shapes take which is checked on the host: tests/test_paged_host.py). Tolerances as in tests/test_gpu_paged_scores.py,
 at scores of rms 1."""
 import pytest
 import torch
@@ -12,10 +12,11 @@ from test_gpu_paged_scores import assert_near
 
 pytestmark = pytest.mark.gpu
 
-CONTEXT = {"max_ctx": 24000, "max_prefill_tokens": 128}
+CONTEXT = {"max_ctx": 62000, "max_prefill_tokens": 128}
 # (start, tokens): whole and partial last blocks, one block and four, cached positions that end
 # inside a tile and a page, at their ends, and slices that begin there
-BLOCKS_OF_16 = [(20000, 9), (19999, 16), (8000, 33), (12011, 25), (5999, 42), (5056, 64), (6001, 57)]
+BLOCKS_OF_16 = [(60000, 9), (59999, 16), (26000, 33), (34011, 25), (19999, 42), (14080, 64), (16001, 57)]
+BLOCKS_OF_8 = [(20000, 9), (19999, 16), (8000, 33), (12011, 25), (5999, 42), (5056, 64), (6001, 57)]   # long chunks of these
 TYPES = [("f32", "bf16", "f32", 16), ("bf16", "bf16", "bf16", 256), ("bf16", "f16", "bf16", 64), ("f32", "f16", "f32", 32)]
 
 
@@ -60,9 +61,9 @@ def _tokens(T, kv, out):
     return min(T, 42) if (kv, out) == ("bf16", "f32") else T
 
 
-@pytest.mark.parametrize("start,T", BLOCKS_OF_16)
+@pytest.mark.parametrize("start,T", BLOCKS_OF_16 + BLOCKS_OF_8)
 @pytest.mark.parametrize("io,kv,out,page", TYPES)
-def test_blocks_of_16_tokens(hip, ctx, start, T, io, kv, out, page):
+def test_blocks_of_16_tokens_and_long_chunks_of_8(hip, ctx, start, T, io, kv, out, page):
     import qff
     T = _tokens(T, kv, out)
     c, qg, k, v, pos, at, r = _slice(start, T, page, io, kv, seed=T)
@@ -72,10 +73,12 @@ def test_blocks_of_16_tokens(hip, ctx, start, T, io, kv, out, page):
     assert_near(got, R.attend(c.p, qg, c.kp, c.vp, c.table[0], pos), kv, 1)
 
 
-@pytest.mark.parametrize("start,T,where", [(20000, 9, 0), (19999, 16, 20000), (8000, 33, 8016), (12011, 25, 12011), (5999, 42, 3000),
+@pytest.mark.parametrize("start,T,where", [(60000, 9, 0), (59999, 16, 60000), (26000, 33, 26016), (34011, 25, 34011), (19999, 42, 3000),
+                                           (19999, 42, 20032), (14080, 64, 14095), (14080, 64, 14128), (14080, 64, 14143),
+                                           (20000, 9, 0), (19999, 16, 20000), (8000, 33, 8016), (12011, 25, 12011), (5999, 42, 3000),
                                            (5999, 42, 6032), (5056, 64, 5071), (5056, 64, 5104), (5056, 64, 5119)])
 @pytest.mark.parametrize("io,kv,out,page", [(io, kv, out, 16) for io, kv, out, _ in TYPES])
-def test_blocks_of_16_tokens_pages_outside_the_pool(hip, ctx, start, T, where, io, kv, out, page):
+def test_pages_outside_the_pool_in_long_chunks(hip, ctx, start, T, where, io, kv, out, page):
     """The page of position `where` lies outside the pool: tokens that see it are
     NaN, those before it are right, and its rows are dropped."""
     import qff

@@ -77,7 +77,7 @@ def test_shared_decode_rescaled_large_blocks(hip, ctx, io, kv, out):
     _check(c, qff.gqa_decode_shared(ctx, *c.args(), group, shared, out_dtype=DT[out]), kv, seqs=(0, 1, 7, 15, 16, 21, 27))
 
 
-@pytest.mark.parametrize("start,T", [(700, 5), (130, 8), (1000, 40), (0, 42), (64, 17), (8000, 33), (20000, 9), (5999, 42)])
+@pytest.mark.parametrize("start,T", [(700, 5), (130, 8), (1000, 40), (0, 42), (64, 17), (8000, 33), (20000, 9), (5999, 42), (26000, 33), (19999, 42)])
 @pytest.mark.parametrize("io,kv,out", TYPES)
 def test_short_slices_rescaled(hip, ctx, io, kv, out, start, T):
     """Blocks of 8 and 16 tokens; the slice's own k rows are peaks of the tokens

@@ -247,8 +247,8 @@ def test_split_of_short_slices(tmp_path):
     qff.lib()
     exe = _program(tmp_path, "paged_split")
     C, P = blocks.CONTEXT["max_ctx"], blocks.CONTEXT["max_prefill_tokens"]
-    tokens = list(blocks.BLOCKS_OF_16)
-    assert sum(t <= 42 for _, t in tokens) >= 5    # (as many tokens as three terms take)
+    tokens = blocks.BLOCKS_OF_16 + blocks.BLOCKS_OF_8
+    assert sum(t <= 42 for _, t in blocks.BLOCKS_OF_16) >= 5    # (as many tokens as three terms take)
     rng = random.Random(1)
     more = []
     for _ in range(3000):
@@ -261,4 +261,4 @@ def test_split_of_short_slices(tmp_path):
     lines = r.stdout.splitlines()
     assert len(lines) == len(tokens) + len(more)
     for shape, line in zip(tokens, lines):
-        assert line.split()[0] == "16", (shape, line)
+        assert line.split()[0] == ("16" if shape in blocks.BLOCKS_OF_16 else "8"), (shape, line)
