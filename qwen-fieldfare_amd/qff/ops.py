@@ -110,7 +110,8 @@ class Context:
                  max_prefill_tokens: int = 8192):
         self.device = device
         h = ctypes.c_void_p()
-        cfg = CtxCfg(max_batch, max_ctx, max_prefill_tokens)
+        # (zeros stand for the defaults, as in the library; cfg holds what applies)
+        cfg = CtxCfg(max_batch or 32, max_ctx or 65536, max_prefill_tokens or 8192)
         check("qff_ctx_create", lib().qff_ctx_create(ctypes.byref(h), device, ctypes.byref(cfg)))
         self.handle = h
         self.cfg = cfg

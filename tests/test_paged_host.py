@@ -262,3 +262,15 @@ def test_split_of_short_slices(tmp_path):
     assert len(lines) == len(tokens) + len(more)
     for shape, line in zip(tokens, lines):
         assert line.split()[0] == ("16" if shape in blocks.BLOCKS_OF_16 else "8"), (shape, line)
+
+
+def test_a_contexts_limits_hold_what_zeros_stand_for(monkeypatch):
+    """What checks against ctx.cfg see is what the library applies."""
+    from qff import ops
+    made = []
+    monkeypatch.setattr(ops, "lib", lambda: types.SimpleNamespace(qff_ctx_create=lambda h, device, cfg: made.append(cfg) or 0))
+    for args, want in (((0, 0, 0, 0), (32, 65536, 8192)), ((0, 4, 0, 16), (4, 65536, 16)), ((0,), (32, 65536, 8192))):
+        c = ops.Context(*args)
+        assert (c.cfg.max_batch, c.cfg.max_ctx, c.cfg.max_prefill_tokens) == want
+        c.handle = None
+    assert len(made) == 3
