@@ -97,3 +97,45 @@ def test_short_slices_in_contexts_of_few_partials(hip, io, kv, out, max_ctx, sta
     pos = torch.arange(start, start + T, dtype=torch.int32, device=DEV)
     assert_near(got, R.attend(c.p, qg, c.kp, c.vp, c.table[0], pos), kv, 1)
     small.close()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("io,kv,out", TYPES)
+def test_a_row_without_a_value_leaves_the_others(hip, ctx, io, kv, out, bad):
+    """q, and the gate, of single sequences or tokens NaN or infinite, next to
+    others in a wave, a block and a row block: those keep their bits."""
+    import qff
+    c, group, shared = _groups([2, 12, 1, 8, 3], [900, 2000, 30, 1100, 3000], [1, 40, 300], 64, io=io, kv=kv, seed=5)
+    start = [t.clone() for t in (c.kp, c.vp)]
+    rows, gates = [0, 3, 9, 14, 17, 25], [1, 5]
+    for call, more in ((qff.gqa_decode_paged, ()), (qff.gqa_decode_shared, (group, shared))):
+        c.kp.copy_(start[0])
+        c.vp.copy_(start[1])
+        want = call(ctx, *c.args(), *more, out_dtype=DT[out])
+        qg = c.qg.clone()
+        for i, b in enumerate(rows):
+            qg[b, (5 * i) % 16, 31 * i] = bad
+        for b in gates:
+            qg[b, 2, 300] = float("nan")
+        c.kp.copy_(start[0])
+        c.vp.copy_(start[1])
+        got = call(ctx, c.p, qg, *c.args()[2:], *more, out_dtype=DT[out])
+        for i, b in enumerate(rows):
+            assert torch.isnan(got[b, (5 * i) % 16]).all()
+            want[b, (5 * i) % 16] = got[b, (5 * i) % 16] = 0
+        for b in gates:
+            assert torch.isnan(got[b, 2, 44])
+            want[b, 2, 44] = got[b, 2, 44] = 0
+        assert torch.equal(got, want)
+    T = 40
+    c = Case([700 + T], 16, io, kv, seed=T)
+    qg, k, v = (_randn(torch.Generator(device=DEV).manual_seed(T), T, *s, dtype=DT[io]) for s in ((16, 512), (2, 256), (2, 256)))
+    run = lambda q: qff.gqa_prefill_paged(ctx, c.p, q, k, v, c.kp, c.vp, c.table[0], start_pos=700, out_dtype=DT[out])   # noqa: E731
+    want, other = run(qg), qg.clone()
+    for t in (0, 7, 8, 39):
+        other[t, t % 16, t] = bad
+    got = run(other)
+    for t in (0, 7, 8, 39):
+        assert torch.isnan(got[t, t % 16]).all()
+        want[t, t % 16] = got[t, t % 16] = 0
+    assert torch.equal(got, want)
