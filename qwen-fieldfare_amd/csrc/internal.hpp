@@ -236,6 +236,13 @@ inline PagedTokens paged_tokens_split(int start, int T, int slots, int cap) {
 hipError_t launch_gqa_prefill_paged(qff_ctx* ctx, hipStream_t stream, const qff_gqa_params* p, const void* q_gate,
                                     const void* k, const void* v, qff_dtype in_dtype, const qff_kv_pages* kv,
                                     int start, void* out, qff_dtype out_dtype, int T);
+constexpr int kCopyPairs = 448, kCopyThreads = 256;   // pairs that a launch's arguments hold; threads of a workgroup
+constexpr size_t kCopySeg = 16384;                    // bytes that one copies
+// Pairs of a launch: a grid has fewer than 2^32 work-items (256 GB copied in a pool).
+inline int copy_pairs(size_t page_bytes) {
+    const size_t groups = ((size_t{1} << 32) - 1) / kCopyThreads, segs = (page_bytes + kCopySeg - 1) / kCopySeg;
+    return static_cast<int>(groups / segs < kCopyPairs ? groups / segs : kCopyPairs);
+}
 hipError_t launch_pages_copy(qff_ctx* ctx, hipStream_t stream, void* const* pools, int npools, size_t page_bytes,
                              const int32_t* src, const int32_t* dst, int n, bool once);   // once: no source twice
 hipError_t launch_q4_dequant(hipStream_t stream, const uint32_t* w, const void* scales,

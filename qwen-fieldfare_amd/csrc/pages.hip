@@ -11,7 +11,8 @@
 // cache (106 with ordinary stores, 110 with non-temporal loads too). The pairs
 // travel in the kernel's arguments (no upload, no workspace; a captured
 // call replays the pairs it was captured with), as many as 4 KB of arguments
-// hold with the pool addresses: more go in further launches.
+// hold with the pool addresses and a launch takes work-items for: more go in
+// further launches.
 #include <algorithm>
 
 #include "common.hpp"
@@ -20,8 +21,7 @@
 
 namespace qff {
 
-constexpr int kCopyPools = 32, kCopyPairs = 448;
-constexpr size_t kCopySeg = 16384;   // bytes per workgroup
+constexpr int kCopyPools = 32;
 
 struct CopyArgs {
     char* pools[kCopyPools];
@@ -32,7 +32,7 @@ struct CopyArgs {
 static_assert(sizeof(CopyArgs) <= 4096 - 64, "kernel arguments");
 
 template <bool ONCE>
-__global__ __launch_bounds__(256) void pages_copy_kernel(const CopyArgs a) {
+__global__ __launch_bounds__(kCopyThreads) void pages_copy_kernel(const CopyArgs a) {
     const int pair = static_cast<int>(blockIdx.x) / a.segs, seg = static_cast<int>(blockIdx.x) - pair * a.segs;
     char* pool = a.pools[blockIdx.y];
     const char* from = pool + static_cast<size_t>(a.src[pair]) * a.page_bytes;
@@ -55,16 +55,17 @@ hipError_t launch_pages_copy(qff_ctx* ctx, hipStream_t stream, void* const* pool
     CopyArgs a;
     a.page_bytes = page_bytes;
     a.segs = static_cast<int>((page_bytes + kCopySeg - 1) / kCopySeg);
-    for (int i0 = 0; i0 < n; i0 += kCopyPairs) {
-        const int pairs = std::min(kCopyPairs, n - i0);
+    const int most = copy_pairs(page_bytes);
+    for (int i0 = 0; i0 < n; i0 += most) {
+        const int pairs = std::min(most, n - i0);
         std::copy(src + i0, src + i0 + pairs, a.src);
         std::copy(dst + i0, dst + i0 + pairs, a.dst);
         for (int p0 = 0; p0 < npools; p0 += kCopyPools) {
             const int count = std::min(kCopyPools, npools - p0);
             for (int p = 0; p < count; ++p) a.pools[p] = static_cast<char*>(pools[p0 + p]);
             const dim3 grid(pairs * a.segs, count);
-            if (once) pages_copy_kernel<true><<<grid, 256, 0, stream>>>(a);
-            else pages_copy_kernel<false><<<grid, 256, 0, stream>>>(a);
+            if (once) pages_copy_kernel<true><<<grid, kCopyThreads, 0, stream>>>(a);
+            else pages_copy_kernel<false><<<grid, kCopyThreads, 0, stream>>>(a);
         }
     }
     return hipGetLastError();

@@ -274,3 +274,10 @@ def test_a_contexts_limits_hold_what_zeros_stand_for(monkeypatch):
         assert (c.cfg.max_batch, c.cfg.max_ctx, c.cfg.max_prefill_tokens) == want
         c.handle = None
     assert len(made) == 3
+
+
+def test_copy_launches_stay_within_a_grid(tmp_path):
+    import qff
+    qff.lib()
+    r = subprocess.run([_program(tmp_path, "copy_launches")], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout[-1000:]
