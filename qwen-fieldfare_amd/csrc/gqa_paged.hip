@@ -1234,13 +1234,14 @@ hipError_t launch_gqa_decode_paged(qff_ctx* ctx, hipStream_t stream, const qff_g
 // A slice of few tokens takes the decode's kernels: blocks of 8 or 16 tokens read
 // the pages as they are, where the other path first copies the whole cache (K as
 // fp16, V transposed). Its products take a pass for each term, so the rule is
-// tokens x terms <= 128 (us per call, this in blocks of 16 / the other path, from
-// position 0, 2000, 20000, 60000):
-//   bf16 cache and outputs (two terms)  8 tokens 15 / 20, 17 / 26, 23 / 45, 39 / 82
-//                                      64 tokens 20 / 23, 32 / 34, 63 / 64, 132 / 136
-//                                      96 tokens 22 / 25, 34 / 34, 81 / 75, 188 / 164
-//   bf16 cache, fp32 outputs (three)   32 tokens 18 / 23, 29 / 30, 50 / 56, 98 / 103
-//                                      64 tokens 21 / 23, 34 / 34, 73 / 67, 164 / 133
+// tokens x terms <= 128 (us per call, this / the other path, behind 0, 2000, 20000
+// and 60000 positions):
+//   two terms    9 tokens 16 / 24, 20 / 26, 28 / 45, 46 / 86
+//               64 tokens 18 / 23, 29 / 34, 57 / 61, 126 / 134
+//               96 tokens 22 / 25, 34 / 34, 81 / 75, 188 / 164
+//   three terms 33 tokens 18 / 23, 26 / 30, 51 / 55, 115 / 117
+//               42 tokens 19 / 23, 27 / 31, 55 / 56, 126 / 118
+//               64 tokens 19 / 23, 31 / 34, 67 / 61, 161 / 134
 hipError_t launch_gqa_prefill_paged(qff_ctx* ctx, hipStream_t stream, const qff_gqa_params* p, const void* q_gate,
                                     const void* k, const void* v, qff_dtype in_dtype, const qff_kv_pages* kv,
                                     int start, void* out, qff_dtype out_dtype, int T) {

@@ -122,8 +122,8 @@ class PageTable:
 
     def truncate(self, slot: int, end: int) -> None:
         """Slot `slot` holds its first `end` positions only: a reservation taken
-        back, or tokens that are given up. Pages behind them that no other slot
-        holds are free again."""
+        back, or tokens that are given up (recurrent states are the caller's). Pages
+        behind them that no other slot holds are free again."""
         self.check_slot(slot)
         if not 0 <= end <= self.lengths[slot]:
             raise ValueError(f"slot {slot} holds {self.lengths[slot]} positions, not {end}")
