@@ -358,7 +358,7 @@ typedef struct qff_kv_pages {
  * page_size - 1 (a padded slot) gives a NaN row and touches no page. q_gate and
  * the norm weights are 16-byte aligned. Errors grow with the scores, of rms s
  * (at least 1 here): fp32 outputs are within about 1e-6 s of the exact row,
- * relative to its norm; bf16 outputs add 4e-6 s (bf16 cache) or 1e-6 s (fp16) to
+ * relative to its norm; bf16 outputs add about 5e-6 s (bf16 cache) or 1e-6 s (fp16) to
  * their own rounding. */
 int qff_gqa_decode_paged(qff_ctx* ctx, qff_stream_t stream, const qff_gqa_params* p,
                          const void* q_gate, const void* k_new, const void* v_new,
