@@ -443,7 +443,9 @@ def gqa_prefill_paged(ctx: Context, params: dict, q_gate, k, v, k_pages, v_pages
                       out_dtype=torch.bfloat16, theta=1e7, scale=1.0 / 16, eps=1e-6):
     """gqa_prefill on a paged cache: T tokens of one sequence at positions
     start_pos .. start_pos + T - 1, appended to the pages its row of the table
-    (int32 [entries]) names -> out [T,16,256]."""
+    (int32 [entries]) names -> out [T,16,256]. Up to 42 tokens (fp32 outputs of a
+    bf16 cache) or 64 (others) have gqa_decode_paged's precision, longer slices
+    gqa_prefill's fp16 operands."""
     T = q_gate.shape[0]
     prm, qp, kp, vp, code, kv = _paged_args(ctx, params, q_gate, k, v, k_pages, v_pages,
                                             table[None] if table.dim() == 1 else table, 1, T, theta, scale, eps)
