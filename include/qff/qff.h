@@ -206,6 +206,102 @@ int qff_router_top8(qff_ctx* ctx, qff_stream_t stream, const uint32_t* w,
                     const void* x, qff_dtype x_dtype, float* logits,
                     int32_t* indices, float* scores, int experts, int cols, int batch);
 
+/* ------------------------------------------------------------ expert block */
+
+/* Affine-Q4 matrices of one shape [rows, cols], one behind another (a single
+ * one where the call says so): w [n][rows][cols/8], scales and biases
+ * [n][rows][cols/64], as in qff_q4_dequant, w 16-byte aligned. */
+typedef struct qff_q4_matrices {
+    const uint32_t* w;
+    const void* scales;
+    const void* biases;
+} qff_q4_matrices;
+
+/* A layer's expert weights: the routed experts' matrices, and those of the
+ * shared expert that every token goes through (w NULL: the layer has none).
+ * A call reads the matrices it needs and no others. 1 <= experts <= 512;
+ * hidden and inter are multiples of 64, up to 4096. */
+typedef struct qff_moe_weights {
+    qff_q4_matrices gate, up;                 /* [experts][inter, hidden] */
+    qff_q4_matrices down;                     /* [experts][hidden, inter] */
+    qff_q4_matrices shared_gate, shared_up;   /* [inter, hidden]          */
+    qff_q4_matrices shared_down;              /* [hidden, inter]          */
+    qff_dtype sb_dtype;                       /* of scales and biases: QFF_BF16 or QFF_F16 */
+    int experts, hidden, inter;
+} qff_moe_weights;
+
+/* RMSNorm of each token, y[m, c] = x[m, c] * rsqrt(mean_c x[m, c]^2 + eps) *
+ * norm_w[c], and with `gate` (not NULL: one affine-Q8 row [1, cols] as in
+ * qff_q8_dequant, scales and biases of gate_sb) the shared expert's
+ * coefficient coef[m] = sigmoid(sum_c gate[c] y[m, c]) from the unrounded y.
+ * Replaces qwen_rmsnorm_f32 (deltanet.metal:18-53) where the router and the
+ * experts read the normalised rows. x [tokens, cols] of x_dtype, y of y_dtype,
+ * norm_w [cols] of norm_dtype (each F32 or BF16), coef [tokens] fp32. y may be
+ * x. cols is a multiple of 64, up to 8192; x, y, norm_w and gate->w are
+ * 16-byte aligned. tokens may be 0. */
+int qff_rms_norm(qff_ctx* ctx, qff_stream_t stream, const void* x, qff_dtype x_dtype,
+                 const void* norm_w, qff_dtype norm_dtype, float eps, const qff_q4_matrices* gate,
+                 qff_dtype gate_sb, void* y, qff_dtype y_dtype, float* coef, int cols, int tokens);
+
+/* The first half of the expert block, every token through its experts:
+ *   h[m, j] = silu(x[m] Wg^T) * (x[m] Wu^T),  silu(a) = a / (1 + e^-a),
+ * with the matrices of expert indices[m, j] for j < top and, where the layer
+ * has a shared expert (p->shared_gate), its own for j = top. Replaces the
+ * staged / cached gate-up-SiLU kernels of deltanet.metal:904-1114, 1212-1832
+ * over expert matrices that are resident. An index outside 0 .. experts - 1 (a
+ * padded token, an expert held elsewhere) leaves its row of h as it was; the
+ * same index may occur twice in a token.
+ *   x       [tokens, hidden] of x_dtype (F32 or BF16), finite
+ *   indices [tokens, top] int32 device array, 1 <= top <= 16
+ *   h       [tokens, top + shared, inter] of h_dtype (F32, BF16 or F16; what
+ *           exceeds fp16 becomes infinite there)
+ * x and h are 16-byte aligned. Nibbles, scales and biases enter the products
+ * exactly, an fp32 x as three bf16 terms; from 33 tokens on, where h is BF16 or
+ * F16, the products run on fp16 operands (qff_moe_down says how). tokens may be 0;
+ * QFF_ERR_WORKSPACE above the larger of max_batch and max_prefill_tokens. */
+int qff_moe_gate_up(qff_ctx* ctx, qff_stream_t stream, const qff_moe_weights* p, const void* x,
+                    qff_dtype x_dtype, const int32_t* indices, int top, void* h, qff_dtype h_dtype,
+                    int tokens);
+
+/* The second half:
+ *   y[m] = residual[m] + sum_{j < top} scores[m, j] h[m, j] Wd^T
+ *          (+ coef[m] h[m, top] Wsd^T with a shared expert, p->shared_down),
+ * summed in fp32 in the order of j. Replaces the down-accumulate and combine
+ * kernels of deltanet.metal:904-1114, 1212-1832, 1985-2227. Pairs whose index lies
+ * outside 0 .. experts - 1 add nothing, whatever h holds there.
+ *   h        [tokens, top + shared, inter] of h_dtype (F32, BF16 or F16), finite
+ *   scores   [tokens, top] fp32, coef [tokens] fp32 (NULL: 1)
+ *   residual [tokens, hidden] of y_dtype, or NULL; may be y
+ *   y        [tokens, hidden] of y_dtype (F32 or BF16)
+ * h, residual and y are 16-byte aligned. tokens and errors as above. */
+int qff_moe_down(qff_ctx* ctx, qff_stream_t stream, const qff_moe_weights* p, const void* h,
+                 qff_dtype h_dtype, const int32_t* indices, const float* scores, int top,
+                 const float* coef, const void* residual, void* y, qff_dtype y_dtype, int tokens);
+
+/* ---------------------------------------------------------------- sampling */
+
+/* The next token of each sequence from its logits l [batch, vocab] (F32 or
+ * BF16). With t = temperature[b] > 0 the tokens, in descending order of l and
+ * equal ones by index, weigh e_i = exp((l_i - l_max) / t), held as whole numbers of
+ * 2^-44. Kept are the first of that order which pass all of
+ *   top_k[b] > 0   the first top_k
+ *   min_p[b] > 0   e_i >= min_p
+ *   top_p[b] < 1   what the top_k's tokens before it weigh is less than
+ *                  top_p of what all of the top_k's weigh,
+ * the first always. Of the kept ones, in the order of their indices, the token is
+ * the first whose running sum exceeds floor(u[b] * sum), u in [0, 1) (values
+ * outside count as the nearest inside); probs[b] = its weight over the sum.
+ * t <= 0 or NaN: the first of the order, probs 1. A NaN logit counts as -inf, a row
+ * of nothing else gives token -1 and probs 0; infinite logits share all weight.
+ * Arithmetic is in fp64 and integers: results depend on no order of sums. The
+ * arrays temperature, top_k, top_p and min_p may each be NULL: 1, off, off, off.
+ * probs may be NULL. Counterpart of QwenLogitSelector (Runtime/Generation/
+ * QwenGenerationSupport.swift:228-362), which runs on the host.
+ * 1 <= vocab <= 262144. batch may be 0; QFF_ERR_WORKSPACE above max_batch. */
+int qff_sample(qff_ctx* ctx, qff_stream_t stream, const void* logits, qff_dtype dtype, const float* u,
+               const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+               int32_t* tokens, float* probs, int vocab, int batch);
+
 /* ---------------------------------------------------------------- DeltaNet */
 
 /* Per-layer constants of a Gated DeltaNet layer (fp32, device pointers),

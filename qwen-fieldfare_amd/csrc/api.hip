@@ -5,6 +5,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <new>
 
 #include "common.hpp"
@@ -70,6 +71,16 @@ WorkspaceLayout workspace_layout(const qff_ctx_cfg& cfg) {
     L.pop = take(NC * 32 * 2 * 6 * 512 * sizeof(uint16_t));
     L.gates = take(NC * 32 * 4 * 64 * sizeof(float));
     L.bv = take(NC * 32 * 64 * 128 * sizeof(float));
+    L.moe_off = take((kMoeMaxExperts + 1) * sizeof(int));
+    L.moe_list = take(static_cast<size_t>(moe_tokens(cfg)) * kMoeMaxTop * sizeof(int));
+    L.moe_part = take(moe_part_bytes(cfg));
+    L.sm_range = take(B * kSampleChunks * sizeof(float2));
+    L.sm_mass = take(B * kSampleChunks * kSampleBins * sizeof(unsigned long long));
+    L.sm_count = take(B * kSampleChunks * kSampleBins * sizeof(uint32_t));
+    L.sm_cut = take(B * sizeof(SampleCut));
+    L.sm_base = take(B * kSampleChunks * sizeof(unsigned long long));
+    L.sm_listed = take(B * kSampleChunks * sizeof(int));
+    L.sm_list = take(B * kSampleVocab * sizeof(int32_t));
     L.total = off;
     return L;
 }
@@ -189,6 +200,17 @@ int qff_ctx_create(qff_ctx** out, int device, const qff_ctx_cfg* cfg) {
     c->pf_slots = pf_slots(c->cfg);
     c->sched = reinterpret_cast<unsigned*>(base + L.sched);
     c->num_cu = prop.multiProcessorCount;
+    c->moe_off = reinterpret_cast<int*>(base + L.moe_off);
+    c->moe_list = reinterpret_cast<int*>(base + L.moe_list);
+    c->moe_part = base + L.moe_part;
+    c->moe_part_bytes = moe_part_bytes(c->cfg);
+    c->sample = SampleWork{reinterpret_cast<float2*>(base + L.sm_range),
+                           reinterpret_cast<unsigned long long*>(base + L.sm_mass),
+                           reinterpret_cast<uint32_t*>(base + L.sm_count),
+                           reinterpret_cast<SampleCut*>(base + L.sm_cut),
+                           reinterpret_cast<unsigned long long*>(base + L.sm_base),
+                           reinterpret_cast<int*>(base + L.sm_listed),
+                           reinterpret_cast<int32_t*>(base + L.sm_list)};
     c->dn_arrive = reinterpret_cast<unsigned*>(base + L.dn_arrive);
     if (hipMemset(c->sched, 0, 2 * kSchedSlots * sizeof(unsigned)) != hipSuccess ||
         hipMemset(c->dn_arrive, 0, static_cast<size_t>(c->cfg.max_batch) * 16 * sizeof(unsigned)) != hipSuccess) {
@@ -538,6 +560,89 @@ int qff_pages_copy(qff_ctx* ctx, qff_stream_t stream, void* const* pools, int np
     const OnDevice on(ctx->device);
     if (!on.ok) return QFF_ERR_HIP;
     QFF_CHECK_HIP(launch_pages_copy(ctx, stream, pools, npools, page_bytes, src, dst, n, once));
+    return QFF_OK;
+}
+
+// (where a call has no tokens its tensors need no addresses)
+static bool given(const void* p, bool needed) { return aligned16(p) && (p || !needed); }
+
+int qff_rms_norm(qff_ctx* ctx, qff_stream_t stream, const void* x, qff_dtype x_dtype, const void* norm_w,
+                 qff_dtype norm_dtype, float eps, const qff_q4_matrices* gate, qff_dtype gate_sb, void* y,
+                 qff_dtype y_dtype, float* coef, int cols, int tokens) {
+    if (!ctx || tokens < 0 || cols <= 0 || !(eps >= 0.0f)) return QFF_ERR_INVALID_ARG;
+    if (!dtype_ok(x_dtype) || !dtype_ok(norm_dtype) || !dtype_ok(y_dtype)) return QFF_ERR_INVALID_ARG;
+    const bool any = tokens > 0;
+    if (!given(x, any) || !given(y, any) || !given(norm_w, true)) return QFF_ERR_INVALID_ARG;
+    if (gate && (!given(gate->w, true) || !gate->scales || !gate->biases || (any && !coef))) return QFF_ERR_INVALID_ARG;
+    if (gate && gate_sb != QFF_BF16 && gate_sb != QFF_F16) return QFF_ERR_INVALID_ARG;
+    if (cols % 64 != 0 || cols > 8192) return QFF_ERR_UNSUPPORTED;
+    if (!any) return QFF_OK;
+    const OnDevice on(ctx->device);
+    if (!on.ok) return QFF_ERR_HIP;
+    QFF_CHECK_HIP(launch_rms_norm(ctx, stream, x, x_dtype, norm_w, norm_dtype, eps, gate, gate_sb, y, y_dtype, coef, cols,
+                                  tokens));
+    return QFF_OK;
+}
+
+static bool q4_matrices_ok(const qff_q4_matrices& q) { return given(q.w, true) && q.scales && q.biases; }
+
+// What both halves of the expert block check: `own` the matrices they need.
+static int moe_status(const qff_ctx* ctx, const qff_moe_weights* p, std::initializer_list<const qff_q4_matrices*> own,
+                      std::initializer_list<const qff_q4_matrices*> shared, const int32_t* indices, int top, int tokens) {
+    if (!ctx || !p || tokens < 0 || (tokens > 0 && !indices)) return QFF_ERR_INVALID_ARG;
+    if (p->sb_dtype != QFF_BF16 && p->sb_dtype != QFF_F16) return QFF_ERR_INVALID_ARG;
+    for (const qff_q4_matrices* q : own)
+        if (!q4_matrices_ok(*q)) return QFF_ERR_INVALID_ARG;
+    const bool has = (*shared.begin())->w != nullptr;
+    for (const qff_q4_matrices* q : shared)
+        if ((q->w != nullptr) != has || (has && !q4_matrices_ok(*q))) return QFF_ERR_INVALID_ARG;
+    if (p->experts <= 0 || top <= 0 || p->hidden <= 0 || p->inter <= 0) return QFF_ERR_INVALID_ARG;
+    if (p->experts > kMoeMaxExperts || top > kMoeMaxTop || p->hidden % 64 != 0 || p->hidden > 4096 || p->inter % 64 != 0 ||
+        p->inter > 4096)
+        return QFF_ERR_UNSUPPORTED;
+    if (tokens > moe_tokens(ctx->cfg)) return QFF_ERR_WORKSPACE;
+    return QFF_OK;
+}
+
+int qff_moe_gate_up(qff_ctx* ctx, qff_stream_t stream, const qff_moe_weights* p, const void* x, qff_dtype x_dtype,
+                    const int32_t* indices, int top, void* h, qff_dtype h_dtype, int tokens) {
+    if (!p || !dtype_ok(x_dtype) || !dtype_ok(h_dtype, true)) return QFF_ERR_INVALID_ARG;
+    if (const int st = moe_status(ctx, p, {&p->gate, &p->up}, {&p->shared_gate, &p->shared_up}, indices, top, tokens))
+        return st;
+    if (!given(x, tokens > 0) || !given(h, tokens > 0)) return QFF_ERR_INVALID_ARG;
+    if (tokens == 0) return QFF_OK;
+    const OnDevice on(ctx->device);
+    if (!on.ok) return QFF_ERR_HIP;
+    QFF_CHECK_HIP(launch_moe_gate_up(ctx, stream, p, x, x_dtype, indices, top, h, h_dtype, tokens));
+    return QFF_OK;
+}
+
+int qff_moe_down(qff_ctx* ctx, qff_stream_t stream, const qff_moe_weights* p, const void* h, qff_dtype h_dtype,
+                 const int32_t* indices, const float* scores, int top, const float* coef, const void* residual, void* y,
+                 qff_dtype y_dtype, int tokens) {
+    if (!p || !dtype_ok(h_dtype, true) || !dtype_ok(y_dtype)) return QFF_ERR_INVALID_ARG;
+    if (const int st = moe_status(ctx, p, {&p->down}, {&p->shared_down}, indices, top, tokens)) return st;
+    if (!given(h, tokens > 0) || !given(y, tokens > 0) || !aligned16(residual) || (tokens > 0 && !scores))
+        return QFF_ERR_INVALID_ARG;
+    if (tokens == 0) return QFF_OK;
+    const OnDevice on(ctx->device);
+    if (!on.ok) return QFF_ERR_HIP;
+    QFF_CHECK_HIP(launch_moe_down(ctx, stream, p, h, h_dtype, indices, scores, top, coef, residual, y, y_dtype, tokens));
+    return QFF_OK;
+}
+
+int qff_sample(qff_ctx* ctx, qff_stream_t stream, const void* logits, qff_dtype dtype, const float* u,
+               const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p, int32_t* tokens,
+               float* probs, int vocab, int batch) {
+    if (!ctx || !dtype_ok(dtype) || batch < 0 || vocab <= 0) return QFF_ERR_INVALID_ARG;
+    if (batch > 0 && (!logits || !u || !tokens)) return QFF_ERR_INVALID_ARG;
+    if (vocab > kSampleVocab) return QFF_ERR_UNSUPPORTED;
+    if (batch > ctx->cfg.max_batch) return QFF_ERR_WORKSPACE;
+    if (batch == 0) return QFF_OK;
+    const OnDevice on(ctx->device);
+    if (!on.ok) return QFF_ERR_HIP;
+    QFF_CHECK_HIP(launch_sample(ctx, stream, logits, dtype, u, temperature, top_k, top_p, min_p, tokens, probs, vocab,
+                                batch));
     return QFF_OK;
 }
 

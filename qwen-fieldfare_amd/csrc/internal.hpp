@@ -26,6 +26,24 @@ struct qff_dn_bufs {
     float* bv;        // per (chunk, value head): beta V [64][128] in the state pass's lane order
 };
 
+// Sampling: what its launches hand on, per row of up to kSampleChunks chunks.
+constexpr int kSampleChunks = 64, kSampleBins = 64, kSampleVocab = 262144;
+struct SampleCut {
+    unsigned long long total, mass_before;   // weight of the row, and of the bins before lo
+    int count_before;                        // tokens of those
+    int lo, hi;                              // the bins that hold the borders; lo > hi: none
+    bool by_count, by_mass;                  // top-k, top-p cut something off
+};
+struct SampleWork {
+    float2* range;                  // [max_batch][chunks] largest, least finite logit
+    unsigned long long* bin_mass;   // [max_batch][chunks][bins]
+    uint32_t* bin_count;            // same
+    SampleCut* cut;                 // [max_batch]
+    unsigned long long* base;       // [max_batch][chunks] weight kept of the bins before lo
+    int* listed;                    // [max_batch][chunks] tokens listed of the others
+    int32_t* list;                  // [max_batch][vocab], a chunk's from its first token's place on
+};
+
 struct qff_ctx {
     int device = 0;
     qff_ctx_cfg cfg{};
@@ -62,6 +80,14 @@ struct qff_ctx {
     // DeltaNet decode: per (sequence, key head) arrival counters [max_batch][16],
     // zero between launches (the second arrival resets its counter).
     unsigned* dn_arrive = nullptr;
+    // Expert block: where each expert's pairs begin [kMoeMaxExperts + 1], the
+    // pairs [moe_tokens(cfg)][kMoeMaxTop], and rows of pairs between the down
+    // products and their sum.
+    int* moe_off = nullptr;
+    int* moe_list = nullptr;
+    void* moe_part = nullptr;
+    size_t moe_part_bytes = 0;
+    SampleWork sample{};
     // Work-queue counters of the persistent kernels, zero between launches
     // (each launch's last workgroup resets its pair); kSchedSlots pairs.
     unsigned* sched = nullptr;
@@ -97,9 +123,26 @@ constexpr int kSchedSlots = 8;         // work-queue counter pairs in the contex
 constexpr int kQ4SkSlots = 4096;       // (row tile, slice) partials of the split decode-batch Q4 product
 constexpr int kSchedChunkLocal = 0;    // slot of the DeltaNet chunk-local pass
 
+constexpr int kMoeMaxExperts = 512, kMoeMaxTop = 16;
+// Tokens of an expert-block call at most, and the bytes for the rows of its
+// pairs: nine rows of 2048 values in two bytes a token, in four for up to 256
+// tokens, and one token of any shape. A call takes its tokens in as many slices as that needs.
+inline int moe_tokens(const qff_ctx_cfg& cfg) {
+    const int n = cfg.max_batch > cfg.max_prefill_tokens ? cfg.max_batch : cfg.max_prefill_tokens;
+    return n < 1 << 26 ? n : 1 << 26;   // (a pair's code is 32 times its token)
+}
+inline size_t moe_part_bytes(const qff_ctx_cfg& cfg) {
+    const size_t n = static_cast<size_t>(moe_tokens(cfg)), row = 9 * 2048;
+    const size_t most = n * row * 2 > (n < 256 ? n : 256) * row * 4 ? n * row * 2 : (n < 256 ? n : 256) * row * 4;
+    const size_t one = static_cast<size_t>(kMoeMaxTop + 1) * 4096 * 4;
+    return most > one ? most : one;
+}
+
 struct WorkspaceLayout {
     size_t gqa_m, gqa_d, gqa_o, gqa_nc;
     size_t gqa_qb, gqa_kv16, gqa_vt, q4_x16, q4_fm, q4_sk_part, pf_o, pf_md, dn_arrive, sched, kimg, qop, top, pop, gates, bv;
+    size_t moe_off, moe_list, moe_part;
+    size_t sm_range, sm_mass, sm_count, sm_cut, sm_base, sm_listed, sm_list;
     size_t total;
 };
 WorkspaceLayout workspace_layout(const qff_ctx_cfg& cfg);
@@ -268,6 +311,17 @@ hipError_t launch_q8_dequant(hipStream_t stream, const uint32_t* w, const void* 
 hipError_t launch_router_top8(qff_ctx* ctx, hipStream_t stream, const uint32_t* w, const void* scales,
                               const void* biases, qff_dtype sb_dtype, const void* x, qff_dtype x_dtype,
                               float* logits, int32_t* indices, float* scores, int experts, int cols, int batch);
+hipError_t launch_rms_norm(qff_ctx* ctx, hipStream_t stream, const void* x, qff_dtype x_dtype, const void* norm_w,
+                           qff_dtype norm_dtype, float eps, const qff_q4_matrices* gate, qff_dtype gate_sb, void* y,
+                           qff_dtype y_dtype, float* coef, int cols, int tokens);
+hipError_t launch_moe_gate_up(qff_ctx* ctx, hipStream_t stream, const qff_moe_weights* w, const void* x, qff_dtype x_dtype,
+                              const int32_t* indices, int top, void* h, qff_dtype h_dtype, int tokens);
+hipError_t launch_moe_down(qff_ctx* ctx, hipStream_t stream, const qff_moe_weights* w, const void* h, qff_dtype h_dtype,
+                           const int32_t* indices, const float* scores, int top, const float* coef, const void* residual,
+                           void* y, qff_dtype y_dtype, int tokens);
+hipError_t launch_sample(qff_ctx* ctx, hipStream_t stream, const void* logits, qff_dtype dtype, const float* u,
+                         const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                         int32_t* tokens, float* probs, int vocab, int batch);
 constexpr int kQ4GemmMinBatch = 33;   // batches at least this large take the tiled GEMM
 hipError_t launch_kv_append(hipStream_t stream, const float* k, const float* v, void* k_cache,
                             void* v_cache, qff_dtype cache_dtype, int pos, int max_seq);

@@ -43,6 +43,16 @@ class KvPages(ctypes.Structure):
     _fields_ = [("k", _vp), ("v", _vp), ("table", _vp), ("num_pages", _i), ("page_size", _i), ("table_cols", _i)]
 
 
+class Q4Matrices(ctypes.Structure):
+    _fields_ = [("w", _vp), ("scales", _vp), ("biases", _vp)]
+
+
+class MoeWeights(ctypes.Structure):
+    _fields_ = [("gate", Q4Matrices), ("up", Q4Matrices), ("down", Q4Matrices), ("shared_gate", Q4Matrices),
+                ("shared_up", Q4Matrices), ("shared_down", Q4Matrices), ("sb_dtype", _i), ("experts", _i), ("hidden", _i),
+                ("inter", _i)]
+
+
 Q4_MAX_PARTS = 8
 
 
@@ -80,6 +90,10 @@ SIGNATURES = {
     "qff_gqa_prefill_paged": [_vp, _vp, ctypes.POINTER(GqaParams), _vp, _vp, _vp, _i, ctypes.POINTER(KvPages), _i,
                               _vp, _i, _i],
     "qff_pages_copy": [_vp, _vp, ctypes.POINTER(_vp), _i, ctypes.c_size_t, _i, _vp, _vp, _i],
+    "qff_rms_norm": [_vp, _vp, _vp, _i, _vp, _i, _f, ctypes.POINTER(Q4Matrices), _i, _vp, _i, _vp, _i, _i],
+    "qff_moe_gate_up": [_vp, _vp, ctypes.POINTER(MoeWeights), _vp, _i, _vp, _i, _vp, _i, _i],
+    "qff_moe_down": [_vp, _vp, ctypes.POINTER(MoeWeights), _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _i],
+    "qff_sample": [_vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i],
     "qff_kv_append": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i],
     "qff_attention_gate": [_vp, _vp, _vp, _vp, _vp, _i],
     "qff_profile_enable": [_vp, _i],

@@ -14,8 +14,8 @@ import struct
 
 import torch
 
-from ._lib import (BF16, F16, F32, Q4_MAX_PARTS, CtxCfg, DeltaNetParams, GqaParams, KvPages, Q4Part, QffError,
-                   check, lib)
+from ._lib import (BF16, F16, F32, Q4_MAX_PARTS, CtxCfg, DeltaNetParams, GqaParams, KvPages, MoeWeights, Q4Matrices,
+                   Q4Part, QffError, check, lib)
 
 _DT = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 _TORCH = {F32: torch.float32, BF16: torch.bfloat16, F16: torch.float16}
@@ -31,6 +31,9 @@ _P_DN = struct.Struct("PPPPf4x")
 _P_GQA = struct.Struct("PPfiffi4x")
 _P_KV = struct.Struct("PPPiii4x")
 _P_Q4 = [struct.Struct("PPPi4xPi4xP" * n) for n in range(Q4_MAX_PARTS + 1)]
+_P_Q4M = struct.Struct("PPP")
+_P_MOE = struct.Struct("18P4i")
+assert _P_Q4M.size == ctypes.sizeof(Q4Matrices) and _P_MOE.size == ctypes.sizeof(MoeWeights)
 assert _P_DN.size == ctypes.sizeof(DeltaNetParams) and _P_GQA.size == ctypes.sizeof(GqaParams)
 assert _P_Q4[1].size == ctypes.sizeof(Q4Part) and _P_KV.size == ctypes.sizeof(KvPages)
 
@@ -44,7 +47,8 @@ def _pack(layout: struct.Struct, pointers, *fields) -> bytes:
         return layout.pack(*pointers, *(f if isinstance(f, int) else ctypes.c_float(f).value for f in fields))
 
 
-_BLOCKS = (ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(DeltaNetParams), ctypes.POINTER(GqaParams), ctypes.POINTER(Q4Part), ctypes.POINTER(KvPages))
+_BLOCKS = (ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(DeltaNetParams), ctypes.POINTER(GqaParams), ctypes.POINTER(Q4Part), ctypes.POINTER(KvPages),
+           ctypes.POINTER(Q4Matrices), ctypes.POINTER(MoeWeights))
 
 
 class _Calls:
@@ -53,7 +57,8 @@ class _Calls:
     def __init__(self, L):
         for name in ("qff_q4_matmul", "qff_q4_matmul_parts", "qff_q4_norm_matmul_parts", "qff_router_top8",
                      "qff_deltanet_decode", "qff_deltanet_prefill", "qff_gqa_decode", "qff_gqa_prefill",
-                     "qff_gqa_decode_paged", "qff_gqa_decode_shared", "qff_gqa_prefill_paged", "qff_pages_copy"):
+                     "qff_gqa_decode_paged", "qff_gqa_decode_shared", "qff_gqa_prefill_paged", "qff_pages_copy",
+                     "qff_rms_norm", "qff_moe_gate_up", "qff_moe_down", "qff_sample"):
             fn = L[name]   # a new function object: the typed one of lib() stays as it is
             fn.argtypes = [ctypes.c_void_p if t in _BLOCKS else t for t in getattr(L, name).argtypes]
             fn.restype = ctypes.c_int
@@ -493,6 +498,192 @@ def pages_copy(ctx: Context, pools, src, dst) -> None:
         raise QffError("qff_pages_copy", st)
 
 
+# ---- the expert block and the next token ---------------------------------------
+
+def _matrix(ctx: Context, name: str, q, bits: int, shape=None):
+    """(w, scales, biases) of affine-quantized matrices on the context's device:
+    their addresses, once shapes and types are what the library reads."""
+    w, s, b = q
+    cols = w.shape[-1] * (32 // bits)
+    if w.dtype != _i32 and w.dtype != torch.uint32:
+        raise TypeError(f"{name}: the words must be int32")
+    if s.dtype != b.dtype or s.dtype not in (_bf16, _f16):
+        raise TypeError(f"{name}: scales and biases must both be bfloat16 or both float16")
+    if cols % 64 or s.shape != (*w.shape[:-1], cols // 64) or b.shape != s.shape:
+        raise ValueError(f"{name}: scales and biases must be [.., cols / 64] of [.., {cols}]")
+    if shape is not None and (*w.shape[:-1], cols) != shape:
+        raise ValueError(f"{name} must be {list(shape)}")
+    return _ptr_on(ctx, name, w), _ptr_on(ctx, name + "'s scales", s), _ptr_on(ctx, name + "'s biases", b)
+
+
+class ExpertWeights:
+    """A layer's expert weights, each as (words, scales, biases) of affine-Q4
+    matrices: gate, up [experts, inter, hidden], down [experts, hidden, inter] and
+    the shared expert's [inter, hidden], [hidden, inter] (None: there is none).
+    moe_gate_up needs gate and up, moe_down needs down; what only the other needs
+    may be None. The tensors are kept and stay where they are."""
+
+    def __init__(self, gate=None, up=None, down=None, shared_gate=None, shared_up=None, shared_down=None):
+        self.matrices = (gate, up, down, shared_gate, shared_up, shared_down)
+        if gate is None and down is None:
+            raise ValueError("either gate and up or down")
+        if (gate is None) != (up is None) or (shared_gate is None) != (shared_up is None):
+            raise ValueError("gate and up come together")
+        if shared_gate is not None and gate is None or shared_down is not None and down is None:
+            raise ValueError("a shared expert's matrices stand beside the routed experts'")
+        if gate is not None and down is not None and (shared_gate is None) != (shared_down is None):
+            raise ValueError("a shared expert has all three matrices")
+        w = (gate if gate is not None else down)[0]
+        if w.dim() != 3:
+            raise ValueError("the experts' words must be [experts, rows, cols / 8]")
+        rows, cols = w.shape[1], w.shape[2] * 8
+        self.experts = w.shape[0]
+        self.inter, self.hidden = (rows, cols) if gate is not None else (cols, rows)
+        self.dtype = next(q[1].dtype for q in self.matrices if q is not None)
+        self._packed = None   # (context's device, parameter block): made by the first call, checked there
+
+    def _block(self, ctx: Context) -> bytes:
+        if self._packed is not None and self._packed[0] == ctx.device:
+            return self._packed[1]
+        up, down = (self.inter, self.hidden), (self.hidden, self.inter)
+        flat = []
+        for name, q, shape in zip(("gate", "up", "down", "shared_gate", "shared_up", "shared_down"), self.matrices,
+                                  [(self.experts, *s) for s in (up, up, down)] + [up, up, down]):
+            if q is not None and q[1].dtype != self.dtype:
+                raise TypeError("all scales and biases must have one type")
+            flat += _matrix(ctx, name, q, 4, shape) if q is not None else (0, 0, 0)
+        block = _P_MOE.pack(*flat, _DT[self.dtype], self.experts, self.hidden, self.inter)
+        self._packed = (ctx.device, block)
+        return block
+
+
+def _indices(ctx: Context, indices, tokens: int) -> int:
+    if indices.dim() != 2 or indices.shape[0] != tokens:
+        raise ValueError(f"indices must be [{tokens}, top]")
+    return _ptr_on(ctx, "indices", indices, _i32)
+
+
+def rms_norm(ctx: Context, x: torch.Tensor, norm_w: torch.Tensor, eps: float = 1e-6, gate=None, out=None, out_dtype=None,
+             coef=None):
+    """RMSNorm of each row of x [tokens, cols] (f32 or bf16) with weight norm_w
+    [cols] -> out (x's type unless out or out_dtype says otherwise; may be x). With
+    `gate`, one affine-Q8 row (words [1, cols / 4], scales, biases [1, cols / 64]),
+    (out, coef): coef [tokens] f32 = sigmoid(<gate, normed row>)."""
+    if x.dim() != 2 or norm_w.numel() != x.shape[1]:
+        raise ValueError("x must be [tokens, cols] and norm_w have cols entries")
+    n, cols = x.shape
+    if out is None:
+        out = torch.empty(n, cols, dtype=out_dtype or x.dtype, device=x.device)
+    elif out.shape != x.shape:
+        raise ValueError(f"out must be [{n}, {cols}]")
+    block, sb, cp = 0, BF16, 0
+    if gate is not None:
+        block, sb = _P_Q4M.pack(*_matrix(ctx, "gate", gate, 8, (1, cols))), _code(gate[1])
+        if coef is None:
+            coef = torch.empty(n, dtype=_f32, device=x.device)
+        elif coef.numel() != n:
+            raise ValueError(f"coef must be [{n}]")
+        cp = _ptr_on(ctx, "coef", coef, _f32)
+    st = _hot().qff_rms_norm(ctx.handle, _stream_of(ctx), _ptr_on(ctx, "x", x), _code(x), _ptr_on(ctx, "norm_w", norm_w),
+                             _code(norm_w), eps, block, sb, _ptr_on(ctx, "out", out), _code(out), cp, cols, n)
+    if st:
+        raise QffError("qff_rms_norm", st)
+    return out if gate is None else (out, coef)
+
+
+def moe_gate_up(ctx: Context, experts: ExpertWeights, x: torch.Tensor, indices: torch.Tensor, out=None,
+                out_dtype=torch.float32) -> torch.Tensor:
+    """Every token through its experts' gate and up projections: x [tokens, hidden]
+    (f32 or bf16), indices int32 [tokens, top] -> silu(x Wg^T) * (x Wu^T) [tokens,
+    top (+ 1, the shared expert), inter] (f32, bf16 or f16). An index that is no
+    expert's leaves its row as it was (a new tensor's: undefined)."""
+    n = x.shape[0]
+    if experts.matrices[0] is None:
+        raise ValueError("the weights have no gate and up matrices")
+    if x.dim() != 2 or x.shape[1] != experts.hidden:
+        raise ValueError(f"x must be [tokens, {experts.hidden}]")
+    block, ip = experts._block(ctx), _indices(ctx, indices, n)
+    shape = (n, indices.shape[1] + (experts.matrices[3] is not None), experts.inter)
+    if out is None:
+        out = torch.empty(shape, dtype=out_dtype, device=x.device)
+    elif out.shape != shape:
+        raise ValueError(f"out must be {list(shape)}")
+    st = _hot().qff_moe_gate_up(ctx.handle, _stream_of(ctx), block, _ptr_on(ctx, "x", x), _code(x), ip, indices.shape[1],
+                                _ptr_on(ctx, "out", out), _code(out), n)
+    if st:
+        raise QffError("qff_moe_gate_up", st)
+    return out
+
+
+def moe_down(ctx: Context, experts: ExpertWeights, h: torch.Tensor, indices: torch.Tensor, scores: torch.Tensor, coef=None,
+             residual=None, out=None, out_dtype=torch.float32) -> torch.Tensor:
+    """The experts' down projections of h [tokens, top (+ 1), inter] (f32, bf16 or
+    f16), weighted with scores f32 [tokens, top] (the shared expert's row with coef f32
+    [tokens], or 1) and summed on top of residual [tokens, hidden] (out's type; may be
+    out) -> [tokens, hidden] (f32 or bf16)."""
+    n = h.shape[0]
+    if experts.matrices[2] is None:
+        raise ValueError("the weights have no down matrices")
+    block, ip = experts._block(ctx), _indices(ctx, indices, n)
+    if h.shape != (n, indices.shape[1] + (experts.matrices[5] is not None), experts.inter):
+        raise ValueError(f"h must be [{n}, {indices.shape[1] + (experts.matrices[5] is not None)}, {experts.inter}]")
+    if scores.shape != indices.shape:
+        raise ValueError(f"scores must be {list(indices.shape)}")
+    if out is None:
+        out = torch.empty(n, experts.hidden, dtype=out_dtype, device=h.device)
+    elif out.shape != (n, experts.hidden):
+        raise ValueError(f"out must be [{n}, {experts.hidden}]")
+    cp = rp = 0
+    if coef is not None:
+        if coef.numel() != n:
+            raise ValueError(f"coef must be [{n}]")
+        cp = _ptr_on(ctx, "coef", coef, _f32)
+    if residual is not None:
+        if residual.shape != out.shape or residual.dtype != out.dtype:
+            raise ValueError("a residual must match its output's dtype and shape")
+        rp = _ptr_on(ctx, "residual", residual)
+    st = _hot().qff_moe_down(ctx.handle, _stream_of(ctx), block, _ptr_on(ctx, "h", h), _code(h), ip,
+                             _ptr_on(ctx, "scores", scores, _f32), indices.shape[1], cp, rp, _ptr_on(ctx, "out", out),
+                             _code(out), n)
+    if st:
+        raise QffError("qff_moe_down", st)
+    return out
+
+
+def _per_row(ctx: Context, name: str, t, n: int, dtype) -> int:
+    if t is None:
+        return 0
+    if t.numel() != n:
+        raise ValueError(f"{name} must be [{n}]")
+    return _ptr_on(ctx, name, t, dtype)
+
+
+def sample(ctx: Context, logits: torch.Tensor, u: torch.Tensor, temperature=None, top_k=None, top_p=None, min_p=None,
+           out=None, prob=None):
+    """The next token of each sequence: logits [batch, vocab] (f32 or bf16), u f32
+    [batch] in [0, 1) the random numbers; temperature, top_p, min_p f32 [batch] and
+    top_k int32 [batch] on the device, or None (1, 1, 0 and 0, which filter
+    nothing). Returns (tokens int32 [batch], what the drawn one had as its chance,
+    f32 [batch]). temperature 0 takes the largest logit."""
+    if logits.dim() != 2:
+        raise ValueError("logits must be [batch, vocab]")
+    n, vocab = logits.shape
+    if out is None:
+        out = torch.empty(n, dtype=_i32, device=logits.device)
+    if prob is None:
+        prob = torch.empty(n, dtype=_f32, device=logits.device)
+    if u is None:
+        raise TypeError("u must be float32 random numbers")
+    st = _hot().qff_sample(ctx.handle, _stream_of(ctx), _ptr_on(ctx, "logits", logits), _code(logits),
+                           _per_row(ctx, "u", u, n, _f32), _per_row(ctx, "temperature", temperature, n, _f32),
+                           _per_row(ctx, "top_k", top_k, n, _i32), _per_row(ctx, "top_p", top_p, n, _f32),
+                           _per_row(ctx, "min_p", min_p, n, _f32), _per_row(ctx, "out", out, n, _i32),
+                           _per_row(ctx, "prob", prob, n, _f32), vocab, n)
+    if st:
+        raise QffError("qff_sample", st)
+    return out, prob
+
+
 __all__ = ["Context", "QffError", "q4_dequant", "q4_matmul", "deltanet_decode", "deltanet_prefill",
            "gqa_decode", "gqa_prefill", "gqa_decode_paged", "gqa_decode_shared", "gqa_prefill_paged", "pages_copy",
-           "BF16", "F16", "F32"]
+           "ExpertWeights", "rms_norm", "moe_gate_up", "moe_down", "sample", "BF16", "F16", "F32"]
