@@ -71,9 +71,12 @@ WorkspaceLayout workspace_layout(const qff_ctx_cfg& cfg) {
     L.pop = take(NC * 32 * 2 * 6 * 512 * sizeof(uint16_t));
     L.gates = take(NC * 32 * 4 * 64 * sizeof(float));
     L.bv = take(NC * 32 * 64 * 128 * sizeof(float));
-    L.moe_off = take((kMoeMaxExperts + 1) * sizeof(int));
+    L.moe_off = take(sizeof(int));
+    L.moe_tiles = take(moe_tiles(cfg) * 16);
     L.moe_list = take(static_cast<size_t>(moe_tokens(cfg)) * kMoeMaxTop * sizeof(int));
+    L.moe_xs = take(moe_part_bytes(cfg) / 16);
     L.moe_part = take(moe_part_bytes(cfg));
+    L.moe_exps = take(moe_part_bytes(cfg) / 32);
     L.sm_range = take(B * kSampleChunks * sizeof(float2));
     L.sm_mass = take(B * kSampleChunks * kSampleBins * sizeof(unsigned long long));
     L.sm_count = take(B * kSampleChunks * kSampleBins * sizeof(uint32_t));
@@ -202,7 +205,10 @@ int qff_ctx_create(qff_ctx** out, int device, const qff_ctx_cfg* cfg) {
     c->num_cu = prop.multiProcessorCount;
     c->moe_off = reinterpret_cast<int*>(base + L.moe_off);
     c->moe_list = reinterpret_cast<int*>(base + L.moe_list);
+    c->moe_tiles = base + L.moe_tiles;
+    c->moe_xs = reinterpret_cast<float*>(base + L.moe_xs);
     c->moe_part = base + L.moe_part;
+    c->moe_exps = reinterpret_cast<float*>(base + L.moe_exps);
     c->moe_part_bytes = moe_part_bytes(c->cfg);
     c->sample = SampleWork{reinterpret_cast<float2*>(base + L.sm_range),
                            reinterpret_cast<unsigned long long*>(base + L.sm_mass),

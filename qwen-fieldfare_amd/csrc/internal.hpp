@@ -80,12 +80,16 @@ struct qff_ctx {
     // DeltaNet decode: per (sequence, key head) arrival counters [max_batch][16],
     // zero between launches (the second arrival resets its counter).
     unsigned* dn_arrive = nullptr;
-    // Expert block: where each expert's pairs begin [kMoeMaxExperts + 1], the
-    // pairs [moe_tokens(cfg)][kMoeMaxTop], and rows of pairs between the down
-    // products and their sum.
+    // Expert block: the tiles of a call's pairs [moe_tiles(cfg)] (int4) and their
+    // number, the pairs expert by expert [moe_tokens(cfg)][kMoeMaxTop]; factors and
+    // group sums of the products' rows (moe_part_bytes / 16); rows of pairs between
+    // the down products and their sum, and the exponents of 16-bit ones (/ 32).
     int* moe_off = nullptr;
+    void* moe_tiles = nullptr;
     int* moe_list = nullptr;
+    float* moe_xs = nullptr;
     void* moe_part = nullptr;
+    float* moe_exps = nullptr;
     size_t moe_part_bytes = 0;
     SampleWork sample{};
     // Work-queue counters of the persistent kernels, zero between launches
@@ -138,10 +142,15 @@ inline size_t moe_part_bytes(const qff_ctx_cfg& cfg) {
     return most > one ? most : one;
 }
 
+// Tiles of 32 pairs or more of any call: every expert's last one may be smaller.
+inline size_t moe_tiles(const qff_ctx_cfg& cfg) {
+    return static_cast<size_t>(moe_tokens(cfg)) * (kMoeMaxTop + 1) / 32 + kMoeMaxExperts + 2;
+}
+
 struct WorkspaceLayout {
     size_t gqa_m, gqa_d, gqa_o, gqa_nc;
     size_t gqa_qb, gqa_kv16, gqa_vt, q4_x16, q4_fm, q4_sk_part, pf_o, pf_md, dn_arrive, sched, kimg, qop, top, pop, gates, bv;
-    size_t moe_off, moe_list, moe_part;
+    size_t moe_off, moe_tiles, moe_list, moe_xs, moe_part, moe_exps;
     size_t sm_range, sm_mass, sm_count, sm_cut, sm_base, sm_listed, sm_list;
     size_t total;
 };

@@ -293,13 +293,17 @@ __global__ __launch_bounds__(64 * kOneWaves) void moe_down_one_kernel(MoeArgs p,
 
 // ---- several tokens of one expert ------------------------------------------------
 
-// Which pairs each expert has, for calls of many: one workgroup counts them,
-// sums the counts up and writes the pairs expert by expert (in no fixed order
-// within one: a pair's sums do not depend on its place).
+// Which pairs each expert has, and the tiles of up to `most` (a multiple of 32)
+// that they make: one workgroup counts the pairs, sums the counts up and writes the
+// pairs expert by expert (in no fixed order within one: a pair's sums do not
+// depend on its place). An expert's tiles share its pairs evenly, in multiples of
+// 32; the shared expert, number `experts`, has every token.
 constexpr int kPlanThreads = 1024;
+static_assert(kMoeMaxExperts < kPlanThreads, "an expert a thread");
 __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* __restrict__ indices, int experts, int top,
-                                                                int tokens, int* __restrict__ off, int* __restrict__ list) {
-    __shared__ int cnt[kMoeMaxExperts], at[kMoeMaxExperts], wsum[kPlanThreads / 64];
+                                                                int tokens, int shared, int most, int* __restrict__ count,
+                                                                int4* __restrict__ tiles, int* __restrict__ list) {
+    __shared__ int cnt[kMoeMaxExperts], at[kMoeMaxExperts], wsum[2][kPlanThreads / 64];
     const int t = threadIdx.x, n = tokens * top;
     if (t < kMoeMaxExperts) cnt[t] = 0;
     __syncthreads();
@@ -308,16 +312,29 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* _
         if (e >= 0 && e < experts) atomicAdd(&cnt[e], 1);
     }
     __syncthreads();
-    const int own = t < experts ? cnt[t] : 0;
-    const int incl = wave_inclusive_scan_int(own);
-    if ((t & 63) == 63) wsum[t >> 6] = incl;
+    const int own = t < experts ? cnt[t] : t == experts && shared ? tokens : 0;
+    const int own_tiles = (own + most - 1) / most;
+    const int incl = wave_inclusive_scan_int(t < experts ? own : 0), incl_tiles = wave_inclusive_scan_int(own_tiles);
+    if ((t & 63) == 63) {
+        wsum[0][t >> 6] = incl;
+        wsum[1][t >> 6] = incl_tiles;
+    }
     __syncthreads();
-    int before = incl - own;
-    for (int w = 0; w < t >> 6; ++w) before += wsum[w];
-    if (t < experts) {
-        off[t] = before;
-        at[t] = before;
-        if (t == experts - 1) off[experts] = before + own;
+    int before = incl - own, tile = incl_tiles - own_tiles;
+    for (int w = 0; w < t >> 6; ++w) {
+        before += wsum[0][w];
+        tile += wsum[1][w];
+    }
+    if (t < experts) at[t] = before;
+    if (t == experts) {
+        *count = tile + own_tiles;
+        before = 0;   // (its pairs are the tokens themselves)
+    }
+    if (own_tiles > 0) {
+        const int each = ((own + own_tiles - 1) / own_tiles + 31) / 32 * 32;
+        // (rounded up, the last tiles may have fewer or none)
+        for (int k = 0; k < own_tiles; ++k)
+            tiles[tile + k] = make_int4(t, before + k * each, min(each, max(own - k * each, 0)), 0);
     }
     __syncthreads();
     for (int i = t; i < n; i += kPlanThreads) {
@@ -327,7 +344,8 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* _
 }
 
 constexpr int kRowsWaves = 8;
-constexpr int kRowsScan = 1024;   // pairs of a call that each workgroup looks through by itself
+constexpr int kRowsTokens = 32;   // tokens of a call at most
+constexpr int kRowsScan = kRowsTokens * kMoeMaxTop;   // whose pairs each workgroup looks through by itself
 
 // 16 RT rows of one expert's matrices against its tokens, 16 at a time: WK waves
 // over K times RT row tiles. Outputs leave through `store(acc.., row, code)`.
@@ -337,8 +355,7 @@ struct RowsKernel {
     static constexpr int kRed = WK * kRt * MATS * 16 * 17;
 
     template <class Store>
-    static __device__ __forceinline__ void run(const MoeArgs& p, const int* __restrict__ off, const int* __restrict__ plan,
-                                               float* lds, Store&& store) {
+    static __device__ __forceinline__ void run(const MoeArgs& p, float* lds, Store&& store) {
         constexpr int T = XCols<X_DT>::kTerms;
         const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 15, kg = lane >> 4;
         const int wk = wave % WK, rt = wave / WK;
@@ -348,13 +365,8 @@ struct RowsKernel {
 
         __shared__ int list[kRowsScan], found;
         int n;
-        const int* from = list;
         if (shared) {
             n = p.tokens;
-        } else if (plan) {
-            const int o = off[e];
-            n = off[e + 1] - o;
-            from = plan + o;
         } else {
             if (t == 0) found = 0;
             __syncthreads();
@@ -386,7 +398,7 @@ struct RowsKernel {
 
         for (int t0 = 0; t0 < n; t0 += 16) {
             const int place = min(t0 + c, n - 1);
-            const int code = shared ? pair_code(place, p.top) : from[place];
+            const int code = shared ? pair_code(place, p.top) : list[place];
             const size_t xrow = MATS == 2 ? static_cast<size_t>(code >> 5) * p.cols
                                           : (static_cast<size_t>(code >> 5) * p.slots + (code & 31)) * p.cols;
             f32x4_t acc[MATS];
@@ -457,17 +469,16 @@ struct RowsKernel {
 #pragma unroll
                     for (int q = 0; q < WK; ++q) v[i] += red[(((q * kRt + tile) * MATS + i) * 16 + tok) * 17 + r];
                 }
-                store(v, row, shared ? pair_code(t0 + tok, p.top) : from[t0 + tok]);
+                store(v, row, shared ? pair_code(t0 + tok, p.top) : list[t0 + tok]);
             }
         }
     }
 };
 
 template <int X_DT, int SB_DT, int H_DT, int WK>
-__global__ __launch_bounds__(64 * kRowsWaves) void moe_gate_up_rows_kernel(MoeArgs p, const int* __restrict__ off,
-                                                                           const int* __restrict__ plan, void* __restrict__ h) {
+__global__ __launch_bounds__(64 * kRowsWaves) void moe_gate_up_rows_kernel(MoeArgs p, void* __restrict__ h) {
     extern __shared__ __attribute__((aligned(16))) float lds[];
-    RowsKernel<X_DT, SB_DT, 2, WK>::run(p, off, plan, lds, [&](const float (&v)[2], int row, int code) {
+    RowsKernel<X_DT, SB_DT, 2, WK>::run(p, lds, [&](const float (&v)[2], int row, int code) {
         const size_t o = (static_cast<size_t>(code >> 5) * p.slots + (code & 31)) * p.rows + row;
         elem<H_DT>::store(h, o, silu(v[0]) * v[1]);
     });
@@ -475,13 +486,11 @@ __global__ __launch_bounds__(64 * kRowsWaves) void moe_gate_up_rows_kernel(MoeAr
 
 // The weighted row of each pair, for moe_combine_kernel.
 template <int X_DT, int SB_DT, int WK>
-__global__ __launch_bounds__(64 * kRowsWaves) void moe_down_rows_kernel(MoeArgs p, const int* __restrict__ off,
-                                                                        const int* __restrict__ plan,
-                                                                        const float* __restrict__ scores,
+__global__ __launch_bounds__(64 * kRowsWaves) void moe_down_rows_kernel(MoeArgs p, const float* __restrict__ scores,
                                                                         const float* __restrict__ coef,
                                                                         float* __restrict__ part) {
     extern __shared__ __attribute__((aligned(16))) float lds[];
-    RowsKernel<X_DT, SB_DT, 1, WK>::run(p, off, plan, lds, [&](const float (&v)[1], int row, int code) {
+    RowsKernel<X_DT, SB_DT, 1, WK>::run(p, lds, [&](const float (&v)[1], int row, int code) {
         const int m = code >> 5, j = code & 31;
         const float f = j < p.top ? scores[m * p.top + j] : coef ? coef[m] : 1.0f;
         part[(static_cast<size_t>(m) * p.slots + j) * p.rows + row] = f * v[0];
@@ -508,6 +517,463 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const float* __restric
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) elem<Y_DT>::store(y, o + i, a[i]);
+}
+
+// ---- many tokens ------------------------------------------------------------------
+//
+// From 33 tokens on: the plan's tiles against the matrices on 32x32x16 fp16
+// products. A weight is s q + b = s (q - 8) + (b + 8 s); its first part is exact
+// in fp16 where the scale has 8 significant bits (bf16): q - 8 is a power of two
+// or has three bits. The nibble becomes 16 + q (its bits are the top ones of the
+// mantissa), one packed FMA (16 + q) s - 24 s gives the product without a rounding,
+// and the second part, constant over a group, meets the group's sums of x in a few
+// products at the end. An fp16 scale (11 bits) is split into its first eight bits
+// and the rest, two products a weight (WT = 2), where the output's precision needs
+// it; for bf16 outputs (q - 8) s is rounded to fp16 (WT = 1).
+// x enters as fp16 after a power-of-two shift that puts its row's largest
+// magnitude into [2^13, 2^14), for fp32 x and F32 or F16 outputs as two terms of 11
+// bits (XT = 2); fp16 rows of h are taken as they lie. s 256 and x lie inside
+// fp16's normal range for scales of 2^-22 .. 31; b + 8 s may be up to 8 in magnitude.
+// So F32 and F16 outputs are sums of exact products (up to 2^-22 of x), and
+// bf16 ones carry 11 bits an operand.
+
+// Rows of x for the tiles: XT fp16 terms [row][XT][cols] (each 8 columns in the
+// order c0, c4, c1, c5, .., the nibbles' own) and the row's factor 2^(e - 8); and
+// the sums of its groups as two fp16 terms [row][2][gp] (gp: groups rounded up to
+// 16, the rest zeros), shifted as x is, with the factor that takes them back. One
+// wave a row. COPY false (fp16 rows, used where they lie): the sums alone.
+constexpr int kX16Waves = 4;
+constexpr int kSumsPad = 16;
+template <int X_DT, int XT, bool COPY>
+__global__ __launch_bounds__(64 * kX16Waves) void moe_x16_kernel(const void* __restrict__ x, uint16_t* __restrict__ x16,
+                                                                 float2* __restrict__ fac, uint16_t* __restrict__ sums,
+                                                                 int cols, int rows) {
+    const int lane = threadIdx.x & 63, row = blockIdx.x * kX16Waves + (threadIdx.x >> 6), nb = cols / 8;
+    if (row >= rows) return;
+    constexpr int kMax = 8;   // 8-column blocks of a lane: cols <= 4096
+    float v[kMax][8], s[kMax];
+    float mx = 0.0f, ms = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kMax; ++i) {
+        s[i] = 0.0f;
+        if (64 * i >= nb) continue;
+        const int b = min(lane + 64 * i, nb - 1);
+        const size_t o = static_cast<size_t>(row) * cols + 8 * b;
+        if constexpr (X_DT == 0) {
+            const f32x4_t* q = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(x) + o);
+            const f32x4_t a = q[0], c = q[1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[i][e] = a[e];
+                v[i][4 + e] = c[e];
+            }
+        } else {
+            const u32x4_t u = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(x) + o);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint16_t w[2] = {static_cast<uint16_t>(u[e]), static_cast<uint16_t>(u[e] >> 16)};
+                v[i][2 * e] = elem<X_DT>::load(w, 0);
+                v[i][2 * e + 1] = elem<X_DT>::load(w, 1);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (COPY) mx = fmaxf(mx, fabsf(v[i][e]));
+            s[i] += v[i][e];
+        }
+        s[i] = group_sum<8>(s[i]);   // (nb is a multiple of 8: a group's eight lanes are all in or all past the end)
+        ms = fmaxf(ms, fabsf(s[i]));
+    }
+    // (exponents of at least -127 keep their powers finite for the smallest rows)
+    const auto shift = [](float m) { return m > 0.0f ? max(__builtin_amdgcn_frexp_expf(m) - 14, -127) : 0; };
+    const int e = COPY ? shift(group_max<64>(mx)) : 0, es = shift(group_max<64>(ms));
+    if (lane == 0) fac[row] = make_float2(ldexpf(1.0f, e - 8), ldexpf(1.0f, es - e - 5));
+    const float p = ldexpf(1.0f, -e), ps = ldexpf(1.0f, -es);
+    const int G = cols / 64, gp = (G + kSumsPad - 1) / kSumsPad * kSumsPad;
+    uint16_t* const so = sums + static_cast<size_t>(row) * 2 * gp;
+#pragma unroll
+    for (int i = 0; i < kMax; ++i) {
+        const int g = 8 * i + lane / 8;
+        if (g < gp && (lane & 7) == 0) {
+            uint32_t hi, lo;
+            split_f16x2(g < G ? s[i] * ps : 0.0f, 0.0f, hi, lo);
+            so[g] = static_cast<uint16_t>(hi);
+            so[gp + g] = static_cast<uint16_t>(lo);
+        }
+        if constexpr (COPY) {
+            const int b = lane + 64 * i;
+            if (64 * i >= nb || b >= nb) continue;
+            u32x4_t h, l;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (XT == 2) {
+                    uint32_t hi, lo;
+                    split_f16x2(v[i][j] * p, v[i][j + 4] * p, hi, lo);
+                    h[j] = hi;
+                    l[j] = lo;
+                } else {
+                    h[j] = pack_f16x2(v[i][j] * p, v[i][j + 4] * p);
+                }
+            }
+            uint16_t* o = x16 + static_cast<size_t>(row) * XT * cols + 8 * b;
+            *reinterpret_cast<u32x4_t*>(o) = h;
+            if constexpr (XT == 2) *reinterpret_cast<u32x4_t*>(o + cols) = l;
+        }
+    }
+}
+
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+
+// A group's scale for one row of the tile: s 256 (its first eight bits for WT = 2)
+// and the rest of it.
+template <int SB_DT, int WT>
+__device__ __forceinline__ uint32_t tile_scale(uint16_t s) {
+    const float v = 256.0f * elem<SB_DT>::load(&s, 0);
+    if constexpr (WT == 1) return f32_to_f16(v);
+    const float hi = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+    return f32_to_f16(hi) | static_cast<uint32_t>(f32_to_f16(v - hi)) << 16;
+}
+
+// Nibble word -> fp16 pairs 256 s (q - 8): the pairs (q_j, q_j+4), or with NATURAL
+// (q_2j, q_2j+1) from the even and the odd nibbles' bytes.
+template <bool EXACT, bool NATURAL>
+__device__ __forceinline__ u32x4_t q4_to_f16(uint32_t w, f16x2_t s, f16x2_t c) {
+    constexpr uint32_t k16 = 0x4C004C00u;   // 16, 16
+    u32x4_t r;
+    const uint32_t even = w & 0x0f0f0f0fu, odd = w >> 4 & 0x0f0f0f0fu;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        uint32_t e;
+        if constexpr (NATURAL) {
+            e = __builtin_amdgcn_perm(odd, even, 0x0c040c00u + 0x00010001u * j) << 6 | k16;
+        } else {
+            e = ((j < 2 ? w << (6 - 4 * j) : w >> (4 * j - 6)) & 0x03C003C0u) | k16;
+        }
+        const f16x2_t v = __builtin_bit_cast(f16x2_t, e);
+        const f16x2_t q = EXACT ? __builtin_elementwise_fma(v, s, c)
+                                : (v - f16x2_t{static_cast<_Float16>(24.0f), static_cast<_Float16>(24.0f)}) * s;
+        r[j] = __builtin_bit_cast(uint32_t, q);
+    }
+    return r;
+}
+
+constexpr int kTileRows = 256;   // weight rows of a workgroup: four waves of 64, in two row tiles of 32
+
+// What the tile kernel reads beside the weights.
+struct TileArgs {
+    const int* count;
+    const int4* tiles;
+    const int* list;
+    const uint16_t* x16;   // [row][XT][cols]
+    const float2* fac;     // [row]: of the products, of the sums' products ahead of that
+    const uint16_t* sums;  // [row][2][gp]
+};
+
+// One tile: 256 weight rows (of gate and up: 128 of each, a wave's two row tiles the
+// same rows of both) x NMT tiles of 32 tokens. As in q4.hip's large product,
+// a wave loads its own rows' words (16 bytes a row and group, a group ahead) and
+// converts them in registers; the tokens' group goes from global memory into LDS,
+// double-buffered, one barrier a group, rows swizzled so that the 32 rows of an
+// operand read meet every bank group twice.
+template <int MATS, int SB_DT, int XT, int WT, bool NATURAL, int MMT, int NMT>
+__device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, const int4 tile, const MoeMat& m0, const MoeMat& m1,
+                                         int row0, uint16_t* Xl, uint32_t* sbl, f32x16_t (&acc)[2][NMT]) {
+    constexpr bool kExact = SB_DT == 1 || WT == 2;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = lane & 31, h = lane >> 5;
+    const int G = p.cols / 64;
+    const bool shared = tile.x >= p.experts;
+    auto x_row = [&](int place) {
+        const int code = shared ? pair_code(tile.y + place, p.top) : a.list[tile.y + place];
+        return MATS == 2 ? code >> 5 : (code >> 5) * p.slots + (code & 31);
+    };
+    // staging: chunks of 8 tokens, XT NMT of them a wave; lane l the 16-byte piece l & 7 of token l >> 3, which is the
+    // token's 8-column block (l & 7) ^ ((token >> 1) & 7) of the group
+    const uint16_t* xsrc[NMT];
+#pragma unroll
+    for (int i = 0; i < NMT; ++i) {
+        const int tok = 8 * (NMT * wave + i) + (lane >> 3);
+        xsrc[i] = a.x16 + static_cast<size_t>(x_row(min(tok, tile.z - 1))) * XT * p.cols + 8 * ((lane & 7) ^ ((tok >> 1) & 7));
+    }
+    auto stage_x = [&](int buf, int g) {
+#pragma unroll
+        for (int i = 0; i < NMT; ++i)
+#pragma unroll
+            for (int x = 0; x < XT; ++x)
+                __builtin_amdgcn_global_load_lds(
+                    (const __attribute__((address_space(1))) void*)(xsrc[i] + x * p.cols + 64 * g),
+                    (__attribute__((address_space(3))) void*)(Xl + ((buf * XT + x) * 32 * MMT + 8 * (NMT * wave + i)) * 64), 16, 0,
+                    0);
+    };
+    const int wrow = MATS == 2 ? row0 + 32 * wave + r : row0 + 64 * wave + r;
+    const uint32_t* wsrc[2];
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt)
+        wsrc[rt] = (rt && MATS == 2 ? m1.w : m0.w) + static_cast<size_t>(min(wrow + (MATS == 2 ? 0 : 32 * rt), p.rows - 1)) * (p.cols / 8) + 4 * h;
+    u32x4_t wa[2][2];
+    auto fetch_w = [&](u32x4_t (&dst)[2], int g) {
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) dst[rt] = *reinterpret_cast<const u32x4_t*>(wsrc[rt] + 8 * g);
+    };
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+        for (int mt = 0; mt < NMT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[rt][mt][i] = 0.0f;
+
+    auto step = [&](int s, int g) {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        stage_x((g + 1) & 1, min(g + 1, G - 1));
+        const u32x4_t (&cur)[2] = wa[s];
+        fetch_w(wa[s ^ 1], min(g + 1, G - 1));
+        __builtin_amdgcn_sched_barrier(0);
+        f16x2_t sv[2][WT], cv[2][WT];
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) {
+            const uint32_t sc = sbl[g * kTileRows + 64 * wave + 32 * rt + r];
+#pragma unroll
+            for (int k = 0; k < WT; ++k) {
+                const uint32_t one = sc >> (16 * k) & 0xffffu;
+                sv[rt][k] = __builtin_bit_cast(f16x2_t, one | one << 16);
+                cv[rt][k] = sv[rt][k] * f16x2_t{static_cast<_Float16>(-24.0f), static_cast<_Float16>(-24.0f)};
+            }
+        }
+        const int sw = (r >> 1) & 7;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            u32x4_t A[2][WT], B[NMT][XT];
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+                for (int k = 0; k < WT; ++k) A[rt][k] = q4_to_f16<kExact, NATURAL>(cur[rt][ks], sv[rt][k], cv[rt][k]);
+#pragma unroll
+            for (int mt = 0; mt < NMT; ++mt)
+#pragma unroll
+                for (int x = 0; x < XT; ++x)
+                    B[mt][x] = *reinterpret_cast<const u32x4_t*>(Xl + (((g & 1) * XT + x) * 32 * MMT + 32 * mt + r) * 64 +
+                                                                 8 * ((4 * h + ks) ^ sw));
+#pragma unroll
+            for (int x = XT - 1; x >= 0; --x)
+#pragma unroll
+                for (int k = WT - 1; k >= 0; --k)
+#pragma unroll
+                    for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+                        for (int mt = 0; mt < NMT; ++mt) {
+                            if (x == 1 && k == 1) continue;   // (2^-19 of the product's 2^-22 part)
+                            acc[rt][mt] = mfma_32x32x16_f16(A[rt][k], B[mt][x], acc[rt][mt]);
+                        }
+        }
+    };
+    stage_x(0, 0);
+    fetch_w(wa[0], 0);
+    int g = 0;
+    for (; g + 1 < G; g += 2) {
+        step(0, g);
+        step(1, g + 1);
+    }
+    if (g < G) step(0, g);
+
+    // the groups' constant parts: (b + 8 s) 2^13 against the rows' sums, two fp16 terms each
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (the last step's copies, before LDS is anyone else's)
+    const int gp = (G + kSumsPad - 1) / kSumsPad * kSumsPad;
+    const uint16_t* S[NMT];
+    float2 fac[NMT];
+#pragma unroll
+    for (int mt = 0; mt < NMT; ++mt) {
+        const size_t row = x_row(min(32 * mt + r, tile.z - 1));
+        S[mt] = a.sums + row * 2 * gp + 8 * h;
+        fac[mt] = a.fac[row];
+    }
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt) {
+        const uint16_t* const ms = rt && MATS == 2 ? m1.s : m0.s;
+        const uint16_t* const mb = rt && MATS == 2 ? m1.b : m0.b;
+        const size_t base = static_cast<size_t>(min(wrow + (MATS == 2 ? 0 : 32 * rt), p.rows - 1)) * G;
+        f32x16_t add[NMT];
+#pragma unroll
+        for (int mt = 0; mt < NMT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) add[mt][i] = 0.0f;
+        for (int k0 = 0; k0 < G; k0 += 16) {
+            u32x4_t bh, bl;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float v[2];
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const size_t k = base + min(k0 + 8 * h + 2 * j + q, G - 1);
+                    v[q] = 8192.0f * fmaf(8.0f, elem<SB_DT>::load(ms, k), elem<SB_DT>::load(mb, k));
+                }
+                uint32_t hi, lo;
+                split_f16x2(v[0], v[1], hi, lo);
+                bh[j] = hi;
+                bl[j] = lo;
+            }
+#pragma unroll
+            for (int mt = 0; mt < NMT; ++mt) {
+                const u32x4_t xh = *reinterpret_cast<const u32x4_t*>(S[mt] + k0);
+                const u32x4_t xl = *reinterpret_cast<const u32x4_t*>(S[mt] + gp + k0);
+                add[mt] = mfma_32x32x16_f16(bl, xh, add[mt]);
+                add[mt] = mfma_32x32x16_f16(bh, xl, add[mt]);
+                add[mt] = mfma_32x32x16_f16(bh, xh, add[mt]);
+            }
+        }
+#pragma unroll
+        for (int mt = 0; mt < NMT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[rt][mt][i] = fmaf(add[mt][i], fac[mt].y, acc[rt][mt][i]) * fac[mt].x;
+    }
+}
+
+// The tile of this workgroup, its scales in LDS; body(tile, m, row0, run) where
+// there is one.
+template <int MATS, int SB_DT, int WT, class Body>
+__device__ __forceinline__ void tile_begin(const MoeArgs& p, const TileArgs& a, uint32_t* sbl, Body&& body) {
+    constexpr int kOwn = kTileRows / MATS;   // rows of each matrix
+    const int blocks = (p.rows + kOwn - 1) / kOwn, at = blockIdx.x / blocks;
+    if (at >= *a.count) return;
+    const int4 tile = a.tiles[at];
+    if (tile.z == 0) return;
+    const int row0 = kOwn * (blockIdx.x % blocks), G = p.cols / 64;
+    const bool shared = tile.x >= p.experts;
+    const MoeMat m0 = moe_matrix(p.m[0], p.sh[0], shared, tile.x, p.rows, p.cols);
+    const MoeMat m1 = MATS == 2 ? moe_matrix(p.m[1], p.sh[1], shared, tile.x, p.rows, p.cols) : m0;
+    for (int i = threadIdx.x; i < kTileRows * G; i += 256) {
+        const int q = i / G, g = i - q * G;   // row of the tile: for two matrices 32 of the first, 32 of the second, ..
+        const int row = MATS == 2 ? row0 + 32 * (q >> 6) + (q & 31) : row0 + q;
+        const uint16_t* ms = MATS == 2 && (q & 32) ? m1.s : m0.s;
+        sbl[g * kTileRows + q] = tile_scale<SB_DT, WT>(ms[static_cast<size_t>(min(row, p.rows - 1)) * G + g]);
+    }
+    body(tile, m0, m1, row0);
+}
+
+template <int MATS, int SB_DT, int XT, int WT, bool NATURAL, int MMT, class Out>
+__device__ __forceinline__ void tile_kernel(const MoeArgs& p, const TileArgs& a, Out&& out) {
+    __shared__ __attribute__((aligned(16))) uint16_t Xl[2 * XT * 32 * MMT * 64];
+    extern __shared__ __attribute__((aligned(16))) uint32_t sbl[];   // [G][256]
+    tile_begin<MATS, SB_DT, WT>(p, a, sbl, [&](const int4& tile, const MoeMat& m0, const MoeMat& m1, int row0) {
+        auto run = [&](auto n) {
+            constexpr int NMT = decltype(n)::value;
+            f32x16_t acc[2][NMT];
+            tile_run<MATS, SB_DT, XT, WT, NATURAL, MMT, NMT>(p, a, tile, m0, m1, row0, Xl, sbl, acc);
+            const int lane = threadIdx.x & 63;
+#pragma unroll
+            for (int mt = 0; mt < NMT; ++mt) {
+                const int tok = 32 * mt + (lane & 31);
+                if (tok >= tile.z) continue;
+                const bool shared = tile.x >= p.experts;
+                const int code = shared ? pair_code(tile.y + tok, p.top) : a.list[tile.y + tok];
+                out(acc[0][mt], acc[1][mt], row0, code);
+            }
+        };
+        const int nmt = (tile.z + 31) / 32;
+        if constexpr (MMT >= 4) {
+            if (nmt == 4) return run(std::integral_constant<int, 4>{});
+            if (nmt == 3) return run(std::integral_constant<int, 3>{});
+        }
+        if constexpr (MMT >= 2) {
+            if (nmt == 2) return run(std::integral_constant<int, 2>{});
+        }
+        run(std::integral_constant<int, 1>{});
+    });
+}
+
+// (a lane's rows of a 32 x 32 tile: 8 j + 4 h .. + 3, its token the column)
+template <int SB_DT, int XT, int WT, int H_DT, int MMT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void moe_gate_up_tile_kernel(MoeArgs p, TileArgs a,
+                                                                                                       void* __restrict__ h) {
+    tile_kernel<2, SB_DT, XT, WT, false, MMT>(p, a, [&](const f32x16_t& g, const f32x16_t& u, int row0, int code) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const size_t base = (static_cast<size_t>(code >> 5) * p.slots + (code & 31)) * p.rows;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int row = row0 + 32 * wave + 8 * j + 4 * (lane >> 5);
+            if (row >= p.rows) continue;
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = silu(g[4 * j + i]) * u[4 * j + i];
+            if constexpr (H_DT == 0) {
+                *reinterpret_cast<f32x4_t*>(static_cast<float*>(h) + base + row) = f32x4_t{v[0], v[1], v[2], v[3]};
+            } else if constexpr (H_DT == 1) {
+                *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(h) + base + row) =
+                    u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+            } else {
+                *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(h) + base + row) =
+                    u32x2_t{pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3])};
+            }
+        }
+    });
+}
+
+// The pairs' weighted rows: fp32, or (HALF) fp16 relative to the power of two above
+// the largest of each 64, whose exponents stand in `exps` [pair][rows / 64].
+template <int SB_DT, int XT, int WT, bool NATURAL, bool HALF, int MMT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void moe_down_tile_kernel(
+    MoeArgs p, TileArgs a, const float* __restrict__ scores, const float* __restrict__ coef, void* __restrict__ part,
+    float* __restrict__ exps) {
+    tile_kernel<1, SB_DT, XT, WT, NATURAL, MMT>(p, a, [&](const f32x16_t& a0, const f32x16_t& a1, int row0, int code) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = code >> 5, s = code & 31;
+        const float f = s < p.top ? scores[m * p.top + s] : coef ? coef[m] : 1.0f;
+        const size_t pair = static_cast<size_t>(m) * p.slots + s;
+        const int block = row0 + 64 * wave;
+        if (block >= p.rows) return;   // (rows come in multiples of 64)
+        float k = 1.0f;
+        if constexpr (HALF) {
+            float mx = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fmaxf(fabsf(a0[i]), fabsf(a1[i])));
+            mx *= fabsf(f);
+            // the other half of the token's rows lies 32 lanes on (both are here: they share the token)
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const int e = mx > 0.0f ? max(__builtin_amdgcn_frexp_expf(mx) - 15, -126) : 0;
+            k = ldexpf(1.0f, -e);
+            if (lane < 32) exps[pair * (p.rows / 64) + block / 64] = ldexpf(1.0f, e);
+        }
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const size_t o = pair * p.rows + block + 32 * rt + 8 * j + 4 * (lane >> 5);
+                f32x4_t v;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = (rt ? a1[4 * j + i] : a0[4 * j + i]) * f * k;
+                if constexpr (HALF)
+                    *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(part) + o) =
+                        u32x2_t{pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3])};
+                else
+                    *reinterpret_cast<f32x4_t*>(static_cast<float*>(part) + o) = v;
+            }
+    });
+}
+
+// y[m] = residual[m] + the rows of its pairs, in their order: a thread 8 columns.
+template <int Y_DT>
+__global__ __launch_bounds__(256) void moe_combine_half_kernel(const uint16_t* __restrict__ part, const float* __restrict__ exps,
+                                                               const int32_t* __restrict__ indices, int experts, int top,
+                                                               int slots, const void* residual, void* y, int rows) {
+    const int m = blockIdx.y, r = 8 * (blockIdx.x * 256 + threadIdx.x);
+    if (r >= rows) return;
+    const size_t o = static_cast<size_t>(m) * rows + r;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = residual ? elem<Y_DT>::load(residual, o + i) : 0.0f;
+    for (int j = 0; j < slots; ++j) {
+        const int e = j < top ? indices[m * top + j] : 0;
+        if (e < 0 || (j < top && e >= experts)) continue;
+        const size_t pair = static_cast<size_t>(m) * slots + j;
+        const u32x4_t u = *reinterpret_cast<const u32x4_t*>(part + pair * rows + r);
+        const float k = exps[pair * (rows / 64) + r / 64];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = fmaf(f16_to_f32(static_cast<uint16_t>(u[i])), k, v[2 * i]);
+            v[2 * i + 1] = fmaf(f16_to_f32(static_cast<uint16_t>(u[i] >> 16)), k, v[2 * i + 1]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) elem<Y_DT>::store(y, o + i, v[i]);
 }
 
 MoeMat moe_mat(const qff_q4_matrices& q) {
@@ -541,6 +1007,68 @@ void with_sb(qff_dtype d, F&& f) {
 
 size_t dtype_size(qff_dtype d) { return d == QFF_F32 ? 4 : 2; }
 
+// A call's rows in the tiles' operand form and the plan of its pairs.
+struct Terms {
+    int x, w;   // fp16 terms of x and of a weight
+};
+Terms tile_terms(qff_dtype x, qff_dtype sb, qff_dtype out) {
+    return {x == QFF_F32 && out != QFF_BF16 ? 2 : 1, sb == QFF_F16 && out != QFF_BF16 ? 2 : 1};
+}
+// Tokens of a tile, in units of 32: as many as an expert has on average, within
+// what fits the registers and LDS.
+int tile_units(int pairs, int experts, int xt) {
+    const int avg = pairs / experts;
+    return xt == 1 && avg > 48 ? 4 : avg > 24 ? 2 : 1;
+}
+
+hipError_t moe_plan(qff_ctx* ctx, hipStream_t stream, const MoeArgs& p, bool shared, int units) {
+    ProfScope prof(ctx, stream, "moe_plan");
+    moe_plan_kernel<<<1, kPlanThreads, 0, stream>>>(p.indices, p.experts, p.top, p.tokens, shared, 32 * units, ctx->moe_off,
+                                                    static_cast<int4*>(ctx->moe_tiles), ctx->moe_list);
+    return hipGetLastError();
+}
+
+// x as fp16 terms, factors and sums of `rows` rows; fp16 x stays where it is.
+void moe_x16(qff_ctx* ctx, hipStream_t stream, const void* x, qff_dtype dtype, int xt, int cols, int rows, TileArgs& a) {
+    ProfScope prof(ctx, stream, "moe_x16");
+    float2* fac = reinterpret_cast<float2*>(ctx->moe_xs);
+    uint16_t* sums = reinterpret_cast<uint16_t*>(fac + (rows + 1) / 2 * 2);   // (16-byte aligned)
+    const int grid = (rows + kX16Waves - 1) / kX16Waves;
+#define QFF_X16(X, XT, COPY) \
+    moe_x16_kernel<X, XT, COPY><<<grid, 64 * kX16Waves, 0, stream>>>(x, ctx->q4_x16, fac, sums, cols, rows)
+    if (dtype == QFF_F16) QFF_X16(2, 1, false);
+    else if (dtype == QFF_BF16) QFF_X16(1, 1, true);
+    else if (xt == 1) QFF_X16(0, 1, true);
+    else QFF_X16(0, 2, true);
+#undef QFF_X16
+    a.x16 = dtype == QFF_F16 ? static_cast<const uint16_t*>(x) : ctx->q4_x16;
+    a.fac = fac;
+    a.sums = sums;
+}
+
+// Tokens of a slice whose `rows` rows of x each fit the workspace.
+int slice_tokens(const qff_ctx* ctx, int rows, int cols, int xt, bool copy, int tokens) {
+    size_t most = std::min<size_t>(tokens, 65535);
+    if (copy) most = std::min(most, static_cast<size_t>(ctx->q4_xs_tokens) * 8192 / (static_cast<size_t>(rows) * xt * cols * 2));
+    const size_t row = 8 + (cols / 64 + kSumsPad - 1) / kSumsPad * kSumsPad * 4;
+    return static_cast<int>(std::min(most, (moe_part_bytes(ctx->cfg) / 16 - 8) / (rows * row)));
+}
+
+unsigned tile_grid(const MoeArgs& p, bool shared, int units, int own_rows) {
+    const int most = 32 * units, pairs = p.tokens * p.top;
+    const int tiles = pairs / most + std::min(p.experts, pairs) + (shared ? (p.tokens + most - 1) / most : 0);
+    return static_cast<unsigned>(tiles) * ((p.rows + own_rows - 1) / own_rows);
+}
+
+template <int... V>
+struct Ints {};
+template <class F, int V0, int... V>
+void pick(int v, Ints<V0, V...>, F&& f) {
+    if constexpr (sizeof...(V) == 0) f(Dt<V0>{});
+    else if (v == V0) f(Dt<V0>{});
+    else pick(v, Ints<V...>{}, f);
+}
+
 }  // namespace
 
 hipError_t launch_moe_gate_up(qff_ctx* ctx, hipStream_t stream, const qff_moe_weights* w, const void* x, qff_dtype x_dtype,
@@ -559,6 +1087,7 @@ hipError_t launch_moe_gate_up(qff_ctx* ctx, hipStream_t stream, const qff_moe_we
     p.rows = w->inter;
     p.cols = w->hidden;
     p.tokens = tokens;
+    const int G = p.cols / 64;
     if (tokens * p.slots <= kOnePairs) {
         ProfScope prof(ctx, stream, "moe_gate_up_one");
         const dim3 grid(p.rows / 16, tokens * p.slots);
@@ -571,30 +1100,54 @@ hipError_t launch_moe_gate_up(qff_ctx* ctx, hipStream_t stream, const qff_moe_we
         });
         return hipGetLastError();
     }
-    const int *off = nullptr, *plan = nullptr;
-    if (tokens * top > kRowsScan) {
-        ProfScope prof(ctx, stream, "moe_plan");
-        moe_plan_kernel<<<1, kPlanThreads, 0, stream>>>(indices, p.experts, top, tokens, ctx->moe_off, ctx->moe_list);
-        off = ctx->moe_off;
-        plan = ctx->moe_list;
-    }
-    ProfScope prof(ctx, stream, "moe_gate_up_rows");
-    const int G = p.cols / 64;
-    auto launch = [&](auto X, auto S, auto H, auto K) {
-        using R = RowsKernel<X.value, S.value, 2, K.value>;
-        const dim3 grid((p.rows + R::kRows - 1) / R::kRows, p.experts + shared);
-        const size_t lds = (4 * static_cast<size_t>(G) * R::kRows + R::kRed) * sizeof(float);
-        moe_gate_up_rows_kernel<X.value, S.value, H.value, K.value>
-            <<<grid, 64 * kRowsWaves, lds, stream>>>(p, off, plan, h);
-    };
-    with_io(x_dtype, [&](auto X) {
-        with_sb(w->sb_dtype, [&](auto S) {
-            with_dtype(h_dtype, [&](auto H) {
-                if (G <= 8) launch(X, S, H, Dt<2>{});
-                else launch(X, S, H, Dt<8>{});
+    if (tokens <= kRowsTokens) {
+        ProfScope prof(ctx, stream, "moe_gate_up_rows");
+        auto launch = [&](auto X, auto S, auto H, auto K) {
+            using R = RowsKernel<X.value, S.value, 2, K.value>;
+            const dim3 grid((p.rows + R::kRows - 1) / R::kRows, p.experts + shared);
+            const size_t lds = (4 * static_cast<size_t>(G) * R::kRows + R::kRed) * sizeof(float);
+            moe_gate_up_rows_kernel<X.value, S.value, H.value, K.value><<<grid, 64 * kRowsWaves, lds, stream>>>(p, h);
+        };
+        with_io(x_dtype, [&](auto X) {
+            with_sb(w->sb_dtype, [&](auto S) {
+                with_dtype(h_dtype, [&](auto H) {
+                    if (G <= 8) launch(X, S, H, Dt<2>{});
+                    else launch(X, S, H, Dt<8>{});
+                });
             });
         });
-    });
+        return hipGetLastError();
+    }
+    const Terms tm = tile_terms(x_dtype, w->sb_dtype, h_dtype);
+    const int most = slice_tokens(ctx, 1, p.cols, tm.x, true, tokens);
+    const size_t lds = static_cast<size_t>(G) * kTileRows * sizeof(uint32_t);
+    for (int t0 = 0; t0 < tokens; t0 += most) {
+        p.tokens = std::min(most, tokens - t0);
+        p.indices = indices + static_cast<size_t>(t0) * top;
+        TileArgs a{ctx->moe_off, static_cast<const int4*>(ctx->moe_tiles), ctx->moe_list, nullptr, nullptr, nullptr};
+        moe_x16(ctx, stream, static_cast<const char*>(x) + static_cast<size_t>(t0) * p.cols * dtype_size(x_dtype), x_dtype, tm.x,
+                p.cols, p.tokens, a);
+        const int units = tile_units(p.tokens * top, p.experts, tm.x);
+        if (const hipError_t e = moe_plan(ctx, stream, p, shared, units)) return e;
+        ProfScope prof(ctx, stream, "moe_gate_up_tile");
+        const unsigned grid = tile_grid(p, shared, units, kTileRows / 2);
+        void* to = static_cast<char*>(h) + static_cast<size_t>(t0) * p.slots * p.rows * dtype_size(h_dtype);
+        auto launch = [&](auto S, auto XT, auto WT, auto H) {
+            auto go = [&](auto U) {
+                moe_gate_up_tile_kernel<S.value, XT.value, WT.value, H.value, U.value><<<grid, 256, lds, stream>>>(p, a, to);
+            };
+            if constexpr (XT.value == 1) pick(units, Ints<1, 2, 4>{}, go);
+            else pick(units, Ints<1, 2>{}, go);
+        };
+        with_sb(w->sb_dtype, [&](auto S) {
+            if (h_dtype == QFF_BF16) return launch(S, Dt<1>{}, Dt<1>{}, Dt<1>{});
+            constexpr int WT = decltype(S)::value == 2 ? 2 : 1;
+            pick(tm.x, Ints<1, 2>{}, [&](auto XT) {
+                if (h_dtype == QFF_F32) launch(S, XT, Dt<WT>{}, Dt<0>{});
+                else launch(S, XT, Dt<WT>{}, Dt<2>{});
+            });
+        });
+    }
     return hipGetLastError();
 }
 
@@ -627,9 +1180,12 @@ hipError_t launch_moe_down(qff_ctx* ctx, hipStream_t stream, const qff_moe_weigh
         });
         return hipGetLastError();
     }
-    // as many tokens at a time as the workspace has rows of pairs for
-    const size_t per = static_cast<size_t>(p.slots) * p.rows * sizeof(float);
-    const int most = static_cast<int>(std::min<size_t>({ctx->moe_part_bytes / per, static_cast<size_t>(tokens), 65535}));
+    const bool few = tokens <= kRowsTokens, half = !few && y_dtype == QFF_BF16;
+    const Terms tm = tile_terms(h_dtype, w->sb_dtype, y_dtype);
+    // as many tokens at a time as the workspace has room for
+    const size_t per = static_cast<size_t>(p.slots) * p.rows * (half ? 2 : 4);
+    int most = static_cast<int>(std::min<size_t>({ctx->moe_part_bytes / per, static_cast<size_t>(tokens), 65535}));
+    if (!few) most = std::min(most, slice_tokens(ctx, p.slots, p.cols, tm.x, h_dtype != QFF_F16, tokens));
     for (int t0 = 0; t0 < tokens; t0 += most) {
         const int n = std::min(most, tokens - t0);
         p.tokens = n;
@@ -638,22 +1194,16 @@ hipError_t launch_moe_down(qff_ctx* ctx, hipStream_t stream, const qff_moe_weigh
         const float* sc = scores + static_cast<size_t>(t0) * top;
         const float* cf = coef ? coef + t0 : nullptr;
         const size_t yo = static_cast<size_t>(t0) * p.rows * dtype_size(y_dtype);
-        const int *off = nullptr, *plan = nullptr;
-        if (n * top > kRowsScan) {
-            ProfScope prof(ctx, stream, "moe_plan");
-            moe_plan_kernel<<<1, kPlanThreads, 0, stream>>>(p.indices, p.experts, top, n, ctx->moe_off, ctx->moe_list);
-            off = ctx->moe_off;
-            plan = ctx->moe_list;
-        }
-        float* part = static_cast<float*>(ctx->moe_part);
-        {
+        const void* res = residual ? static_cast<const char*>(residual) + yo : nullptr;
+        void* to = static_cast<char*>(y) + yo;
+        if (few) {
             ProfScope prof(ctx, stream, "moe_down_rows");
             auto launch = [&](auto X, auto S, auto K) {
                 using R = RowsKernel<X.value, S.value, 1, K.value>;
                 const dim3 grid((p.rows + R::kRows - 1) / R::kRows, p.experts + shared);
                 const size_t lds = (2 * static_cast<size_t>(G) * R::kRows + R::kRed) * sizeof(float);
                 moe_down_rows_kernel<X.value, S.value, K.value>
-                    <<<grid, 64 * kRowsWaves, lds, stream>>>(p, off, plan, sc, cf, part);
+                    <<<grid, 64 * kRowsWaves, lds, stream>>>(p, sc, cf, static_cast<float*>(ctx->moe_part));
             };
             with_dtype(h_dtype, [&](auto X) {
                 with_sb(w->sb_dtype, [&](auto S) {
@@ -661,13 +1211,42 @@ hipError_t launch_moe_down(qff_ctx* ctx, hipStream_t stream, const qff_moe_weigh
                     else launch(X, S, Dt<8>{});
                 });
             });
+        } else {
+            TileArgs a{ctx->moe_off, static_cast<const int4*>(ctx->moe_tiles), ctx->moe_list, nullptr, nullptr, nullptr};
+            moe_x16(ctx, stream, p.x, h_dtype, tm.x, p.cols, n * p.slots, a);
+            const int units = tile_units(n * top, p.experts, tm.x);
+            if (const hipError_t e = moe_plan(ctx, stream, p, shared, units)) return e;
+            ProfScope prof(ctx, stream, "moe_down_tile");
+            const unsigned grid = tile_grid(p, shared, units, kTileRows);
+            const size_t lds = static_cast<size_t>(G) * kTileRows * sizeof(uint32_t);
+            auto launch = [&](auto S, auto XT, auto WT, auto NAT, auto HALF) {
+                auto go = [&](auto U) {
+                    moe_down_tile_kernel<S.value, XT.value, WT.value, NAT.value, HALF.value, U.value>
+                        <<<grid, 256, lds, stream>>>(p, a, sc, cf, ctx->moe_part, ctx->moe_exps);
+                };
+                if constexpr (XT.value == 1) pick(units, Ints<1, 2, 4>{}, go);
+                else pick(units, Ints<1, 2>{}, go);
+            };
+            with_sb(w->sb_dtype, [&](auto S) {
+                constexpr int WT = decltype(S)::value == 2 ? 2 : 1;
+                if (half) {
+                    if (h_dtype == QFF_F16) launch(S, Dt<1>{}, Dt<1>{}, Dt<1>{}, Dt<1>{});
+                    else launch(S, Dt<1>{}, Dt<1>{}, Dt<0>{}, Dt<1>{});
+                } else if (h_dtype == QFF_F16) {
+                    launch(S, Dt<1>{}, Dt<WT>{}, Dt<1>{}, Dt<0>{});
+                } else {
+                    pick(tm.x, Ints<1, 2>{}, [&](auto XT) { launch(S, XT, Dt<WT>{}, Dt<0>{}, Dt<0>{}); });
+                }
+            });
         }
         ProfScope prof(ctx, stream, "moe_combine");
-        const dim3 grid((p.rows + 1023) / 1024, n);
         with_io(y_dtype, [&](auto Y) {
-            moe_combine_kernel<Y.value><<<grid, 256, 0, stream>>>(
-                part, p.indices, p.experts, top, p.slots, residual ? static_cast<const char*>(residual) + yo : nullptr,
-                static_cast<char*>(y) + yo, p.rows);
+            if (half)
+                moe_combine_half_kernel<Y.value><<<dim3((p.rows + 2047) / 2048, n), 256, 0, stream>>>(
+                    static_cast<const uint16_t*>(ctx->moe_part), ctx->moe_exps, p.indices, p.experts, top, p.slots, res, to, p.rows);
+            else
+                moe_combine_kernel<Y.value><<<dim3((p.rows + 1023) / 1024, n), 256, 0, stream>>>(
+                    static_cast<const float*>(ctx->moe_part), p.indices, p.experts, top, p.slots, res, to, p.rows);
         });
     }
     return hipGetLastError();
