@@ -74,6 +74,7 @@ WorkspaceLayout workspace_layout(const qff_ctx_cfg& cfg) {
     L.moe_off = take(sizeof(int));
     L.moe_tiles = take(moe_tiles(cfg) * 16);
     L.moe_list = take(static_cast<size_t>(moe_tokens(cfg)) * kMoeMaxTop * sizeof(int));
+    L.moe_parts = take((static_cast<size_t>(moe_tokens(cfg)) * kMoeMaxTop / 1024 + 1) * kMoeMaxExperts * sizeof(int));
     L.moe_xs = take(moe_part_bytes(cfg) / 16);
     L.moe_part = take(moe_part_bytes(cfg));
     L.moe_exps = take(moe_part_bytes(cfg) / 32);
@@ -206,6 +207,7 @@ int qff_ctx_create(qff_ctx** out, int device, const qff_ctx_cfg* cfg) {
     c->moe_off = reinterpret_cast<int*>(base + L.moe_off);
     c->moe_list = reinterpret_cast<int*>(base + L.moe_list);
     c->moe_tiles = base + L.moe_tiles;
+    c->moe_parts = reinterpret_cast<int*>(base + L.moe_parts);
     c->moe_xs = reinterpret_cast<float*>(base + L.moe_xs);
     c->moe_part = base + L.moe_part;
     c->moe_exps = reinterpret_cast<float*>(base + L.moe_exps);

@@ -81,12 +81,14 @@ struct qff_ctx {
     // zero between launches (the second arrival resets its counter).
     unsigned* dn_arrive = nullptr;
     // Expert block: the tiles of a call's pairs [moe_tiles(cfg)] (int4) and their
-    // number, the pairs expert by expert [moe_tokens(cfg)][kMoeMaxTop]; factors and
+    // number, the pairs expert by expert [moe_tokens(cfg)][kMoeMaxTop], the counts
+    // of each 1024 of them [..][kMoeMaxExperts]; factors and
     // group sums of the products' rows (moe_part_bytes / 16); rows of pairs between
     // the down products and their sum, and the exponents of 16-bit ones (/ 32).
     int* moe_off = nullptr;
     void* moe_tiles = nullptr;
     int* moe_list = nullptr;
+    int* moe_parts = nullptr;
     float* moe_xs = nullptr;
     void* moe_part = nullptr;
     float* moe_exps = nullptr;
@@ -150,7 +152,7 @@ inline size_t moe_tiles(const qff_ctx_cfg& cfg) {
 struct WorkspaceLayout {
     size_t gqa_m, gqa_d, gqa_o, gqa_nc;
     size_t gqa_qb, gqa_kv16, gqa_vt, q4_x16, q4_fm, q4_sk_part, pf_o, pf_md, dn_arrive, sched, kimg, qop, top, pop, gates, bv;
-    size_t moe_off, moe_tiles, moe_list, moe_xs, moe_part, moe_exps;
+    size_t moe_off, moe_tiles, moe_list, moe_parts, moe_xs, moe_part, moe_exps;
     size_t sm_range, sm_mass, sm_count, sm_cut, sm_base, sm_listed, sm_list;
     size_t total;
 };

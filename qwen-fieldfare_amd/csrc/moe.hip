@@ -294,22 +294,52 @@ __global__ __launch_bounds__(64 * kOneWaves) void moe_down_one_kernel(MoeArgs p,
 // ---- several tokens of one expert ------------------------------------------------
 
 // Which pairs each expert has, and the tiles of up to `most` (a multiple of 32)
-// that they make: one workgroup counts the pairs, sums the counts up and writes the
-// pairs expert by expert (in no fixed order within one: a pair's sums do not
-// depend on its place). An expert's tiles share its pairs evenly, in multiples of
-// 32; the shared expert, number `experts`, has every token.
-constexpr int kPlanThreads = 1024;
+// that they make: the pairs are counted, the counts summed up and the pairs written
+// expert by expert (in no fixed order within one: a pair's sums do not depend on
+// its place). An expert's tiles share its pairs evenly, in multiples of 32; the
+// shared expert, number `experts`, has every token. Up to kPlanAlone pairs one
+// workgroup does it all (6 us at 4000 pairs, 69 at 65536); beyond, a workgroup for
+// each kPlanShare pairs counts its own, and each then sums up those before it.
+constexpr int kPlanThreads = 1024, kPlanShare = 1024, kPlanAlone = 4096;
 static_assert(kMoeMaxExperts < kPlanThreads, "an expert a thread");
-__global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* __restrict__ indices, int experts, int top,
-                                                                int tokens, int shared, int most, int* __restrict__ count,
-                                                                int4* __restrict__ tiles, int* __restrict__ list) {
-    __shared__ int cnt[kMoeMaxExperts], at[kMoeMaxExperts], wsum[2][kPlanThreads / 64];
-    const int t = threadIdx.x, n = tokens * top;
-    if (t < kMoeMaxExperts) cnt[t] = 0;
+
+__global__ __launch_bounds__(kPlanThreads) void moe_count_kernel(const int32_t* __restrict__ indices, int experts, int n,
+                                                                 int* __restrict__ parts) {
+    __shared__ int cnt[kMoeMaxExperts];
+    const int t = threadIdx.x, i = blockIdx.x * kPlanShare + t;
+    if (t < experts) cnt[t] = 0;
     __syncthreads();
-    for (int i = t; i < n; i += kPlanThreads) {
-        const int e = indices[i];
-        if (e >= 0 && e < experts) atomicAdd(&cnt[e], 1);
+    const int e = i < n ? indices[i] : -1;
+    if (e >= 0 && e < experts) atomicAdd(&cnt[e], 1);
+    __syncthreads();
+    if (t < experts) parts[static_cast<size_t>(blockIdx.x) * experts + t] = cnt[t];
+}
+
+__global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* __restrict__ indices, int experts, int top,
+                                                                int tokens, int shared, int most, const int* __restrict__ parts,
+                                                                int* __restrict__ count, int4* __restrict__ tiles,
+                                                                int* __restrict__ list) {
+    __shared__ int cnt[kMoeMaxExperts], at[kMoeMaxExperts], wsum[2][kPlanThreads / 64];
+    const int t = threadIdx.x, n = tokens * top, share = parts ? kPlanShare : n, i0 = blockIdx.x * share, i1 = min(i0 + share, n);
+    int mine = 0;   // pairs of expert t that other workgroups write ahead of this one's
+    if (parts) {
+        int all = 0;
+        if (t < experts) {
+#pragma unroll 8
+            for (int b = 0; b < static_cast<int>(gridDim.x); ++b) {
+                const int c = parts[static_cast<size_t>(b) * experts + t];
+                all += c;
+                mine += b < static_cast<int>(blockIdx.x) ? c : 0;
+            }
+            cnt[t] = all;
+        }
+    } else {
+        if (t < kMoeMaxExperts) cnt[t] = 0;
+        __syncthreads();
+        for (int i = i0 + t; i < i1; i += kPlanThreads) {
+            const int e = indices[i];
+            if (e >= 0 && e < experts) atomicAdd(&cnt[e], 1);
+        }
     }
     __syncthreads();
     const int own = t < experts ? cnt[t] : t == experts && shared ? tokens : 0;
@@ -325,19 +355,21 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* _
         before += wsum[0][w];
         tile += wsum[1][w];
     }
-    if (t < experts) at[t] = before;
-    if (t == experts) {
-        *count = tile + own_tiles;
-        before = 0;   // (its pairs are the tokens themselves)
-    }
-    if (own_tiles > 0) {
-        const int each = ((own + own_tiles - 1) / own_tiles + 31) / 32 * 32;
-        // (rounded up, the last tiles may have fewer or none)
-        for (int k = 0; k < own_tiles; ++k)
-            tiles[tile + k] = make_int4(t, before + k * each, min(each, max(own - k * each, 0)), 0);
+    if (t < experts) at[t] = before + mine;
+    if (blockIdx.x == 0) {
+        if (t == experts) {
+            *count = tile + own_tiles;
+            before = 0;   // (its pairs are the tokens themselves)
+        }
+        if (own_tiles > 0) {
+            const int each = ((own + own_tiles - 1) / own_tiles + 31) / 32 * 32;
+            // (rounded up, the last tiles may have fewer or none)
+            for (int k = 0; k < own_tiles; ++k)
+                tiles[tile + k] = make_int4(t, before + k * each, min(each, max(own - k * each, 0)), 0);
+        }
     }
     __syncthreads();
-    for (int i = t; i < n; i += kPlanThreads) {
+    for (int i = i0 + t; i < i1; i += kPlanThreads) {
         const int e = indices[i];
         if (e >= 0 && e < experts) list[atomicAdd(&at[e], 1)] = pair_code(i / top, i % top);
     }
@@ -626,12 +658,17 @@ typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 
 // A group's scale for one row of the tile: s 256 (its first eight bits for WT = 2)
 // and the rest of it.
+template <int WT>
+using tile_sb = std::conditional_t<WT == 1, uint16_t, uint32_t>;
 template <int SB_DT, int WT>
-__device__ __forceinline__ uint32_t tile_scale(uint16_t s) {
+__device__ __forceinline__ tile_sb<WT> tile_scale(uint16_t s) {
     const float v = 256.0f * elem<SB_DT>::load(&s, 0);
-    if constexpr (WT == 1) return f32_to_f16(v);
-    const float hi = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
-    return f32_to_f16(hi) | static_cast<uint32_t>(f32_to_f16(v - hi)) << 16;
+    if constexpr (WT == 1) {
+        return f32_to_f16(v);
+    } else {
+        const float hi = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+        return f32_to_f16(hi) | static_cast<uint32_t>(f32_to_f16(v - hi)) << 16;
+    }
 }
 
 // Nibble word -> fp16 pairs 256 s (q - 8): the pairs (q_j, q_j+4), or with NATURAL
@@ -669,6 +706,22 @@ struct TileArgs {
     const uint16_t* sums;  // [row][2][gp]
 };
 
+// Eight consecutive 16-bit values from `at` on, those past `end` the last one.
+// vec: 16-byte aligned, and `end` is a multiple of 8 further on.
+__device__ __forceinline__ u32x4_t load_u16x8(const uint16_t* __restrict__ p, int at, int end, bool vec) {
+    if (vec) return *reinterpret_cast<const u32x4_t*>(p + min(at, end - 8));
+    uint16_t v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = p[min(at + i, end - 1)];
+    u32x4_t r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = v[2 * i] | static_cast<uint32_t>(v[2 * i + 1]) << 16;
+    return r;
+}
+__device__ __forceinline__ bool sb_vec(const MoeMat& m, int G) {
+    return (G & 7) == 0 && ((reinterpret_cast<uintptr_t>(m.s) | reinterpret_cast<uintptr_t>(m.b)) & 15) == 0;
+}
+
 // One tile: 256 weight rows (of gate and up: 128 of each, a wave's two row tiles the
 // same rows of both) x NMT tiles of 32 tokens. As in q4.hip's large product,
 // a wave loads its own rows' words (16 bytes a row and group, a group ahead) and
@@ -676,14 +729,13 @@ struct TileArgs {
 // double-buffered, one barrier a group, rows swizzled so that the 32 rows of an
 // operand read meet every bank group twice.
 template <int MATS, int SB_DT, int XT, int WT, bool NATURAL, int MMT, int NMT>
-__device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, const int4 tile, const MoeMat& m0, const MoeMat& m1,
-                                         int row0, uint16_t* Xl, uint32_t* sbl, f32x16_t (&acc)[2][NMT]) {
+__device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, const MoeMat& m0, const MoeMat& m1, int row0,
+                                         const int* codes, uint16_t* Xl, const tile_sb<WT>* sbl, f32x16_t (&acc)[2][NMT], float2 (&fac)[NMT]) {
     constexpr bool kExact = SB_DT == 1 || WT == 2;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = lane & 31, h = lane >> 5;
     const int G = p.cols / 64;
-    const bool shared = tile.x >= p.experts;
     auto x_row = [&](int place) {
-        const int code = shared ? pair_code(tile.y + place, p.top) : a.list[tile.y + place];
+        const int code = codes[place];
         return MATS == 2 ? code >> 5 : (code >> 5) * p.slots + (code & 31);
     };
     // staging: chunks of 8 tokens, XT NMT of them a wave; lane l the 16-byte piece l & 7 of token l >> 3, which is the
@@ -692,7 +744,7 @@ __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, co
 #pragma unroll
     for (int i = 0; i < NMT; ++i) {
         const int tok = 8 * (NMT * wave + i) + (lane >> 3);
-        xsrc[i] = a.x16 + static_cast<size_t>(x_row(min(tok, tile.z - 1))) * XT * p.cols + 8 * ((lane & 7) ^ ((tok >> 1) & 7));
+        xsrc[i] = a.x16 + static_cast<size_t>(x_row(tok)) * XT * p.cols + 8 * ((lane & 7) ^ ((tok >> 1) & 7));
     }
     auto stage_x = [&](int buf, int g) {
 #pragma unroll
@@ -776,97 +828,126 @@ __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, co
     }
     if (g < G) step(0, g);
 
-    // the groups' constant parts: (b + 8 s) 2^13 against the rows' sums, two fp16 terms each
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (the last step's copies, before LDS is anyone else's)
+    // the groups' constant parts, (b + 8 s) 2^13 against the rows' sums, two fp16 terms each, 16 groups at a time: thread t
+    // forms row t's terms in the staging buffer (32 bytes a row and term, its halves swapped in every other four rows)
     const int gp = (G + kSumsPad - 1) / kSumsPad * kSumsPad;
+    const int own = min(MATS == 2 ? row0 + 32 * wave + (t & 31) : row0 + t, p.rows - 1);
+    const MoeMat& mm = MATS == 2 && (t & 32) ? m1 : m0;
+    const bool vec = sb_vec(m0, G) && sb_vec(m1, G);
+    const size_t base = static_cast<size_t>(own) * G;
     const uint16_t* S[NMT];
-    float2 fac[NMT];
 #pragma unroll
     for (int mt = 0; mt < NMT; ++mt) {
-        const size_t row = x_row(min(32 * mt + r, tile.z - 1));
+        const size_t row = x_row(32 * mt + r);
         S[mt] = a.sums + row * 2 * gp + 8 * h;
         fac[mt] = a.fac[row];
     }
+    for (int k0 = 0; k0 < G; k0 += 16) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (the last step's copies have landed)
+        __syncthreads();
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt) {
-        const uint16_t* const ms = rt && MATS == 2 ? m1.s : m0.s;
-        const uint16_t* const mb = rt && MATS == 2 ? m1.b : m0.b;
-        const size_t base = static_cast<size_t>(min(wrow + (MATS == 2 ? 0 : 32 * rt), p.rows - 1)) * G;
-        f32x16_t add[NMT];
-#pragma unroll
-        for (int mt = 0; mt < NMT; ++mt)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) add[mt][i] = 0.0f;
-        for (int k0 = 0; k0 < G; k0 += 16) {
+        for (int q = 0; q < 2; ++q) {
+            // (groups past the last meet sums of zero)
+            const u32x4_t s8 = load_u16x8(mm.s + base, k0 + 8 * q, G, vec), b8 = load_u16x8(mm.b + base, k0 + 8 * q, G, vec);
             u32x4_t bh, bl;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float v[2];
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const size_t k = base + min(k0 + 8 * h + 2 * j + q, G - 1);
-                    v[q] = 8192.0f * fmaf(8.0f, elem<SB_DT>::load(ms, k), elem<SB_DT>::load(mb, k));
+                for (int i = 0; i < 2; ++i) {
+                    const uint16_t sq = static_cast<uint16_t>(s8[j] >> (16 * i)), bq = static_cast<uint16_t>(b8[j] >> (16 * i));
+                    v[i] = 8192.0f * fmaf(8.0f, elem<SB_DT>::load(&sq, 0), elem<SB_DT>::load(&bq, 0));
                 }
                 uint32_t hi, lo;
                 split_f16x2(v[0], v[1], hi, lo);
                 bh[j] = hi;
                 bl[j] = lo;
             }
+            uint16_t* o = Xl + 16 * t + 8 * (q ^ (t >> 2 & 1));
+            *reinterpret_cast<u32x4_t*>(o) = bh;
+            *reinterpret_cast<u32x4_t*>(o + 16 * kTileRows) = bl;
+        }
+        __syncthreads();
 #pragma unroll
-            for (int mt = 0; mt < NMT; ++mt) {
-                const u32x4_t xh = *reinterpret_cast<const u32x4_t*>(S[mt] + k0);
-                const u32x4_t xl = *reinterpret_cast<const u32x4_t*>(S[mt] + gp + k0);
-                add[mt] = mfma_32x32x16_f16(bl, xh, add[mt]);
-                add[mt] = mfma_32x32x16_f16(bh, xl, add[mt]);
-                add[mt] = mfma_32x32x16_f16(bh, xh, add[mt]);
+        for (int mt = 0; mt < NMT; ++mt) {
+            const u32x4_t xh = *reinterpret_cast<const u32x4_t*>(S[mt] + k0);
+            const u32x4_t xl = *reinterpret_cast<const u32x4_t*>(S[mt] + gp + k0);
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt) {
+                const int q = 64 * wave + 32 * rt + r;
+                const uint16_t* o = Xl + 16 * q + 8 * (h ^ (q >> 2 & 1));
+                const u32x4_t bh = *reinterpret_cast<const u32x4_t*>(o), bl = *reinterpret_cast<const u32x4_t*>(o + 16 * kTileRows);
+                f32x16_t add;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) add[i] = 0.0f;
+                add = mfma_32x32x16_f16(bl, xh, add);
+                add = mfma_32x32x16_f16(bh, xl, add);
+                add = mfma_32x32x16_f16(bh, xh, add);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[rt][mt][i] = fmaf(add[i], fac[mt].y, acc[rt][mt][i]);
             }
         }
-#pragma unroll
-        for (int mt = 0; mt < NMT; ++mt)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[rt][mt][i] = fmaf(add[mt][i], fac[mt].y, acc[rt][mt][i]) * fac[mt].x;
     }
 }
 
-// The tile of this workgroup, its scales in LDS; body(tile, m, row0, run) where
-// there is one.
-template <int MATS, int SB_DT, int WT, class Body>
-__device__ __forceinline__ void tile_begin(const MoeArgs& p, const TileArgs& a, uint32_t* sbl, Body&& body) {
+// The tile of this workgroup, its pairs and scales in LDS; body(tile, m0, m1, row0)
+// where there is one.
+template <int MATS, int SB_DT, int WT, int MMT, class Body>
+__device__ __forceinline__ void tile_begin(const MoeArgs& p, const TileArgs& a, int* codes, tile_sb<WT>* sbl, Body&& body) {
     constexpr int kOwn = kTileRows / MATS;   // rows of each matrix
     const int blocks = (p.rows + kOwn - 1) / kOwn, at = blockIdx.x / blocks;
-    if (at >= *a.count) return;
-    const int4 tile = a.tiles[at];
-    if (tile.z == 0) return;
-    const int row0 = kOwn * (blockIdx.x % blocks), G = p.cols / 64;
+    const int count = *a.count;
+    const int4 tile = a.tiles[at];   // (stale past the count, and unused)
+    if (at >= count || tile.z == 0) return;
+    const int row0 = kOwn * (blockIdx.x % blocks), G = p.cols / 64, t = threadIdx.x;
     const bool shared = tile.x >= p.experts;
     const MoeMat m0 = moe_matrix(p.m[0], p.sh[0], shared, tile.x, p.rows, p.cols);
     const MoeMat m1 = MATS == 2 ? moe_matrix(p.m[1], p.sh[1], shared, tile.x, p.rows, p.cols) : m0;
-    for (int i = threadIdx.x; i < kTileRows * G; i += 256) {
-        const int q = i / G, g = i - q * G;   // row of the tile: for two matrices 32 of the first, 32 of the second, ..
-        const int row = MATS == 2 ? row0 + 32 * (q >> 6) + (q & 31) : row0 + q;
-        const uint16_t* ms = MATS == 2 && (q & 32) ? m1.s : m0.s;
-        sbl[g * kTileRows + q] = tile_scale<SB_DT, WT>(ms[static_cast<size_t>(min(row, p.rows - 1)) * G + g]);
+    if (t < 32 * MMT) {
+        const int k = tile.y + min(t, tile.z - 1);
+        codes[t] = shared ? pair_code(k, p.top) : a.list[k];
     }
+    // thread t: row t of the tile (of two matrices 32 of the first, 32 of the second, ..)
+    const int row = min(MATS == 2 ? row0 + 32 * (t >> 6) + (t & 31) : row0 + t, p.rows - 1);
+    const MoeMat& mm = MATS == 2 && (t & 32) ? m1 : m0;
+    const bool vec = sb_vec(m0, G) && sb_vec(m1, G);
+    const uint16_t* const src = mm.s + static_cast<size_t>(row) * G;
+    for (int g0 = 0; g0 < G; g0 += 32) {
+        u32x4_t v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k == 0 || g0 + 8 * k < G) v[k] = load_u16x8(src, g0 + 8 * k, G, vec);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int g = g0 + 8 * k + i;
+                if (g < G) sbl[g * kTileRows + t] = tile_scale<SB_DT, WT>(static_cast<uint16_t>(v[k][i / 2] >> (16 * (i & 1))));
+            }
+    }
+    __syncthreads();
     body(tile, m0, m1, row0);
 }
 
 template <int MATS, int SB_DT, int XT, int WT, bool NATURAL, int MMT, class Out>
 __device__ __forceinline__ void tile_kernel(const MoeArgs& p, const TileArgs& a, Out&& out) {
-    __shared__ __attribute__((aligned(16))) uint16_t Xl[2 * XT * 32 * MMT * 64];
-    extern __shared__ __attribute__((aligned(16))) uint32_t sbl[];   // [G][256]
-    tile_begin<MATS, SB_DT, WT>(p, a, sbl, [&](const int4& tile, const MoeMat& m0, const MoeMat& m1, int row0) {
+    constexpr int kStage = 2 * XT * 32 * MMT * 64, kConst = 2 * 16 * kTileRows;   // (the latter at the end)
+    __shared__ __attribute__((aligned(16))) uint16_t Xl[kStage > kConst ? kStage : kConst];
+    __shared__ int codes[32 * MMT];
+    extern __shared__ __attribute__((aligned(16))) char sbl_bytes[];   // [G][256]
+    tile_sb<WT>* const sbl = reinterpret_cast<tile_sb<WT>*>(sbl_bytes);
+    tile_begin<MATS, SB_DT, WT, MMT>(p, a, codes, sbl, [&](const int4& tile, const MoeMat& m0, const MoeMat& m1, int row0) {
         auto run = [&](auto n) {
             constexpr int NMT = decltype(n)::value;
             f32x16_t acc[2][NMT];
-            tile_run<MATS, SB_DT, XT, WT, NATURAL, MMT, NMT>(p, a, tile, m0, m1, row0, Xl, sbl, acc);
+            float2 fac[NMT];
+            tile_run<MATS, SB_DT, XT, WT, NATURAL, MMT, NMT>(p, a, m0, m1, row0, codes, Xl, sbl, acc, fac);
             const int lane = threadIdx.x & 63;
 #pragma unroll
             for (int mt = 0; mt < NMT; ++mt) {
                 const int tok = 32 * mt + (lane & 31);
                 if (tok >= tile.z) continue;
-                const bool shared = tile.x >= p.experts;
-                const int code = shared ? pair_code(tile.y + tok, p.top) : a.list[tile.y + tok];
-                out(acc[0][mt], acc[1][mt], row0, code);
+                out(acc[0][mt], acc[1][mt], fac[mt].x, row0, codes[tok]);
             }
         };
         const int nmt = (tile.z + 31) / 32;
@@ -885,7 +966,7 @@ __device__ __forceinline__ void tile_kernel(const MoeArgs& p, const TileArgs& a,
 template <int SB_DT, int XT, int WT, int H_DT, int MMT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void moe_gate_up_tile_kernel(MoeArgs p, TileArgs a,
                                                                                                        void* __restrict__ h) {
-    tile_kernel<2, SB_DT, XT, WT, false, MMT>(p, a, [&](const f32x16_t& g, const f32x16_t& u, int row0, int code) {
+    tile_kernel<2, SB_DT, XT, WT, false, MMT>(p, a, [&](const f32x16_t& g, const f32x16_t& u, float f, int row0, int code) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         const size_t base = (static_cast<size_t>(code >> 5) * p.slots + (code & 31)) * p.rows;
 #pragma unroll
@@ -894,7 +975,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void m
             if (row >= p.rows) continue;
             float v[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = silu(g[4 * j + i]) * u[4 * j + i];
+            for (int i = 0; i < 4; ++i) v[i] = silu(g[4 * j + i] * f) * (u[4 * j + i] * f);
             if constexpr (H_DT == 0) {
                 *reinterpret_cast<f32x4_t*>(static_cast<float*>(h) + base + row) = f32x4_t{v[0], v[1], v[2], v[3]};
             } else if constexpr (H_DT == 1) {
@@ -914,9 +995,9 @@ template <int SB_DT, int XT, int WT, bool NATURAL, bool HALF, int MMT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void moe_down_tile_kernel(
     MoeArgs p, TileArgs a, const float* __restrict__ scores, const float* __restrict__ coef, void* __restrict__ part,
     float* __restrict__ exps) {
-    tile_kernel<1, SB_DT, XT, WT, NATURAL, MMT>(p, a, [&](const f32x16_t& a0, const f32x16_t& a1, int row0, int code) {
+    tile_kernel<1, SB_DT, XT, WT, NATURAL, MMT>(p, a, [&](const f32x16_t& a0, const f32x16_t& a1, float fac, int row0, int code) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = code >> 5, s = code & 31;
-        const float f = s < p.top ? scores[m * p.top + s] : coef ? coef[m] : 1.0f;
+        const float f = fac * (s < p.top ? scores[m * p.top + s] : coef ? coef[m] : 1.0f);
         const size_t pair = static_cast<size_t>(m) * p.slots + s;
         const int block = row0 + 64 * wave;
         if (block >= p.rows) return;   // (rows come in multiples of 64)
@@ -1022,9 +1103,15 @@ int tile_units(int pairs, int experts, int xt) {
 }
 
 hipError_t moe_plan(qff_ctx* ctx, hipStream_t stream, const MoeArgs& p, bool shared, int units) {
+    const int n = p.tokens * p.top, blocks = n > kPlanAlone ? (n + kPlanShare - 1) / kPlanShare : 1;
+    int* parts = blocks > 1 ? ctx->moe_parts : nullptr;
+    if (parts) {
+        ProfScope prof(ctx, stream, "moe_count");
+        moe_count_kernel<<<blocks, kPlanThreads, 0, stream>>>(p.indices, p.experts, n, parts);
+    }
     ProfScope prof(ctx, stream, "moe_plan");
-    moe_plan_kernel<<<1, kPlanThreads, 0, stream>>>(p.indices, p.experts, p.top, p.tokens, shared, 32 * units, ctx->moe_off,
-                                                    static_cast<int4*>(ctx->moe_tiles), ctx->moe_list);
+    moe_plan_kernel<<<blocks, kPlanThreads, 0, stream>>>(p.indices, p.experts, p.top, p.tokens, shared, 32 * units, parts,
+                                                         ctx->moe_off, static_cast<int4*>(ctx->moe_tiles), ctx->moe_list);
     return hipGetLastError();
 }
 
@@ -1120,7 +1207,7 @@ hipError_t launch_moe_gate_up(qff_ctx* ctx, hipStream_t stream, const qff_moe_we
     }
     const Terms tm = tile_terms(x_dtype, w->sb_dtype, h_dtype);
     const int most = slice_tokens(ctx, 1, p.cols, tm.x, true, tokens);
-    const size_t lds = static_cast<size_t>(G) * kTileRows * sizeof(uint32_t);
+    const size_t lds = static_cast<size_t>(G) * kTileRows * 2 * tm.w;
     for (int t0 = 0; t0 < tokens; t0 += most) {
         p.tokens = std::min(most, tokens - t0);
         p.indices = indices + static_cast<size_t>(t0) * top;
@@ -1218,7 +1305,7 @@ hipError_t launch_moe_down(qff_ctx* ctx, hipStream_t stream, const qff_moe_weigh
             if (const hipError_t e = moe_plan(ctx, stream, p, shared, units)) return e;
             ProfScope prof(ctx, stream, "moe_down_tile");
             const unsigned grid = tile_grid(p, shared, units, kTileRows);
-            const size_t lds = static_cast<size_t>(G) * kTileRows * sizeof(uint32_t);
+            const size_t lds = static_cast<size_t>(G) * kTileRows * 2 * tm.w;
             auto launch = [&](auto S, auto XT, auto WT, auto NAT, auto HALF) {
                 auto go = [&](auto U) {
                     moe_down_tile_kernel<S.value, XT.value, WT.value, NAT.value, HALF.value, U.value>
