@@ -694,6 +694,7 @@ __device__ __forceinline__ u32x4_t q4_to_f16(uint32_t w, f16x2_t s, f16x2_t c) {
     return r;
 }
 
+constexpr int kXcds = 8;
 constexpr int kTileRows = 256;   // weight rows of a workgroup: four waves of 64, in two row tiles of 32
 
 // What the tile kernel reads beside the weights.
@@ -895,11 +896,15 @@ __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, co
 template <int MATS, int SB_DT, int WT, int MMT, class Body>
 __device__ __forceinline__ void tile_begin(const MoeArgs& p, const TileArgs& a, int* codes, tile_sb<WT>* sbl, Body&& body) {
     constexpr int kOwn = kTileRows / MATS;   // rows of each matrix
-    const int blocks = (p.rows + kOwn - 1) / kOwn, at = blockIdx.x / blocks;
-    const int count = *a.count;
-    const int4 tile = a.tiles[at];   // (stale past the count, and unused)
-    if (at >= count || tile.z == 0) return;
-    const int row0 = kOwn * (blockIdx.x % blocks), G = p.cols / 64, t = threadIdx.x;
+    const int blocks = (p.rows + kOwn - 1) / kOwn, items = *a.count * blocks;
+    // Workgroups go round the XCDs in turn: each XCD takes one run of the items, so that an expert's row blocks
+    // and tiles meet in one L2 (the weights are read for each tile, x for each row block).
+    const int run = (items + kXcds - 1) / kXcds, slot = blockIdx.x / kXcds;
+    const int item = static_cast<int>(blockIdx.x % kXcds) * run + slot;
+    if (slot >= run || item >= items) return;
+    const int4 tile = a.tiles[item / blocks];
+    if (tile.z == 0) return;
+    const int row0 = kOwn * (item % blocks), G = p.cols / 64, t = threadIdx.x;
     const bool shared = tile.x >= p.experts;
     const MoeMat m0 = moe_matrix(p.m[0], p.sh[0], shared, tile.x, p.rows, p.cols);
     const MoeMat m1 = MATS == 2 ? moe_matrix(p.m[1], p.sh[1], shared, tile.x, p.rows, p.cols) : m0;
@@ -1144,7 +1149,8 @@ int slice_tokens(const qff_ctx* ctx, int rows, int cols, int xt, bool copy, int 
 unsigned tile_grid(const MoeArgs& p, bool shared, int units, int own_rows) {
     const int most = 32 * units, pairs = p.tokens * p.top;
     const int tiles = pairs / most + std::min(p.experts, pairs) + (shared ? (p.tokens + most - 1) / most : 0);
-    return static_cast<unsigned>(tiles) * ((p.rows + own_rows - 1) / own_rows);
+    const unsigned items = static_cast<unsigned>(tiles) * ((p.rows + own_rows - 1) / own_rows);
+    return (items + kXcds - 1) / kXcds * kXcds;
 }
 
 template <int... V>
