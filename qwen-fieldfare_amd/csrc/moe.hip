@@ -674,9 +674,8 @@ __device__ __forceinline__ tile_sb<WT> tile_scale(uint16_t s) {
 // Nibble word -> fp16 pairs 256 s (q - 8): the pairs (q_j, q_j+4), or with NATURAL
 // (q_2j, q_2j+1) from the even and the odd nibbles' bytes.
 template <bool EXACT, bool NATURAL>
-__device__ __forceinline__ u32x4_t q4_to_f16(uint32_t w, f16x2_t s, f16x2_t c) {
-    constexpr uint32_t k16 = 0x4C004C00u;   // 16, 16
-    u32x4_t r;
+__device__ __forceinline__ u32x4_t q4_to_f16(uint32_t w, f16x2_t s, f16x2_t c, uint32_t k16) {
+    u32x4_t r;   // (k16: the fp16 pair 16, 16 in a register, for one and-or or shift-or a pair)
     const uint32_t even = w & 0x0f0f0f0fu, odd = w >> 4 & 0x0f0f0f0fu;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -723,12 +722,30 @@ __device__ __forceinline__ bool sb_vec(const MoeMat& m, int G) {
     return (G & 7) == 0 && ((reinterpret_cast<uintptr_t>(m.s) | reinterpret_cast<uintptr_t>(m.b)) & 15) == 0;
 }
 
+// Groups of x and of the weights on their way or in use: as many as LDS holds
+// beside a second workgroup.
+constexpr int tile_stages(int mmt) { return mmt == 4 ? 2 : mmt == 2 ? 3 : 4; }
+constexpr int tile_stage_bytes(int xt, int mmt) { return xt * 32 * mmt * 128 + kTileRows * 32; }
+
+// All waves here, each with at most N of its copies still under way (the copies
+// are not the compiler's own: its barrier would wait for all of them, and so
+// would its reads of LDS behind them).
+template <int N>
+__device__ __forceinline__ void meet() {
+    static_assert(N < 64, "six bits count them");
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+template <int N, class F>
+__device__ __forceinline__ void unroll(F&& f) {
+    if constexpr (N > 1) unroll<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
+}
+
 // One tile: 256 weight rows (of gate and up: 128 of each, a wave's two row tiles the
-// same rows of both) x NMT tiles of 32 tokens. As in q4.hip's large product,
-// a wave loads its own rows' words (16 bytes a row and group, a group ahead) and
-// converts them in registers; the tokens' group goes from global memory into LDS,
-// double-buffered, one barrier a group, rows swizzled so that the 32 rows of an
-// operand read meet every bank group twice.
+// same rows of both) x NMT tiles of 32 tokens. Groups of x and of the words go from
+// global memory into LDS, tile_stages of them in turn, one barrier a group; a
+// wave converts its own rows' words in registers. Rows of x are swizzled so that
+// the 32 rows of an operand read meet every bank group twice.
 template <int MATS, int SB_DT, int XT, int WT, bool NATURAL, int MMT, int NMT>
 __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, const MoeMat& m0, const MoeMat& m1, int row0,
                                          const int* codes, uint16_t* Xl, const tile_sb<WT>* sbl, f32x16_t (&acc)[2][NMT], float2 (&fac)[NMT]) {
@@ -739,34 +756,34 @@ __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, co
         const int code = codes[place];
         return MATS == 2 ? code >> 5 : (code >> 5) * p.slots + (code & 31);
     };
-    // staging: chunks of 8 tokens, XT NMT of them a wave; lane l the 16-byte piece l & 7 of token l >> 3, which is the
-    // token's 8-column block (l & 7) ^ ((token >> 1) & 7) of the group
-    const uint16_t* xsrc[NMT];
+    // A stage holds a group's x [XT][32 MMT tokens][64] and words [wave][2 row tiles][64 lanes][16 bytes]. Copies of x: 8
+    // tokens each, lane l the 16-byte piece l & 7 of token l >> 3, which is the token's 8-column block (l & 7) ^ ((token >>
+    // 1) & 7) of the group; of words: the wave's own rows', as its lanes read them back.
+    constexpr int NS = tile_stages(MMT), kStage = tile_stage_bytes(XT, MMT), kXBytes = XT * 32 * MMT * 128;
+    const uint32_t at = lds_addr(Xl);
+    uint32_t xoff[NMT], woff[2];
 #pragma unroll
     for (int i = 0; i < NMT; ++i) {
         const int tok = 8 * (NMT * wave + i) + (lane >> 3);
-        xsrc[i] = a.x16 + static_cast<size_t>(x_row(tok)) * XT * p.cols + 8 * ((lane & 7) ^ ((tok >> 1) & 7));
+        xoff[i] = (static_cast<uint32_t>(x_row(tok)) * XT * p.cols + 8 * ((lane & 7) ^ ((tok >> 1) & 7))) * 2;
     }
-    auto stage_x = [&](int buf, int g) {
-#pragma unroll
-        for (int i = 0; i < NMT; ++i)
-#pragma unroll
-            for (int x = 0; x < XT; ++x)
-                __builtin_amdgcn_global_load_lds(
-                    (const __attribute__((address_space(1))) void*)(xsrc[i] + x * p.cols + 64 * g),
-                    (__attribute__((address_space(3))) void*)(Xl + ((buf * XT + x) * 32 * MMT + 8 * (NMT * wave + i)) * 64), 16, 0,
-                    0);
-    };
     const int wrow = MATS == 2 ? row0 + 32 * wave + r : row0 + 64 * wave + r;
-    const uint32_t* wsrc[2];
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt)
-        wsrc[rt] = (rt && MATS == 2 ? m1.w : m0.w) + static_cast<size_t>(min(wrow + (MATS == 2 ? 0 : 32 * rt), p.rows - 1)) * (p.cols / 8) + 4 * h;
-    u32x4_t wa[2][2];
-    auto fetch_w = [&](u32x4_t (&dst)[2], int g) {
+    for (int rt = 0; rt < 2; ++rt) woff[rt] = static_cast<uint32_t>(min(wrow + (MATS == 2 ? 0 : 32 * rt), p.rows - 1)) * (p.cols / 2) + 16 * h;
+    auto stage = [&](int buf, int g) {
 #pragma unroll
-        for (int rt = 0; rt < 2; ++rt) dst[rt] = *reinterpret_cast<const u32x4_t*>(wsrc[rt] + 8 * g);
+        for (int x = 0; x < XT; ++x)
+#pragma unroll
+            for (int i = 0; i < NMT; ++i)
+                dma16(reinterpret_cast<const char*>(a.x16) + x * p.cols * 2 + 128 * g, xoff[i],
+                      at + buf * kStage + (x * 32 * MMT + 8 * (NMT * wave + i)) * 128);
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt)
+            dma16(reinterpret_cast<const char*>(rt && MATS == 2 ? m1.w : m0.w) + 32 * g, woff[rt],
+                  at + buf * kStage + kXBytes + (2 * wave + rt) * 1024);
     };
+    uint32_t k16 = 0x4C004C00u;
+    asm("" : "+v"(k16));
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
@@ -774,14 +791,20 @@ __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, co
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[rt][mt][i] = 0.0f;
 
-    auto step = [&](int s, int g) {
+    // group g, in stage s, has landed once only the copies of the NS - 2 groups behind it may be under way; group g + NS - 1
+    // goes where g - 1 was (past the last group, the last one again: every step copies alike)
+    constexpr int kPer = NMT * XT + 2;
+    auto step = [&](auto st, int g) {
+        constexpr int s = decltype(st)::value;
         __builtin_amdgcn_sched_barrier(0);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        stage_x((g + 1) & 1, min(g + 1, G - 1));
-        const u32x4_t (&cur)[2] = wa[s];
-        fetch_w(wa[s ^ 1], min(g + 1, G - 1));
+        meet<(NS - 2) * kPer>();
+        stage((s + NS - 1) % NS, min(g + NS - 1, G - 1));
         __builtin_amdgcn_sched_barrier(0);
+        const uint16_t* const xs = Xl + s * kStage / 2;
+        u32x4_t cur[2];
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt)
+            cur[rt] = *reinterpret_cast<const u32x4_t*>(xs + kXBytes / 2 + (2 * wave + rt) * 512 + 8 * lane);
         f16x2_t sv[2][WT], cv[2][WT];
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt) {
@@ -800,12 +823,12 @@ __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, co
 #pragma unroll
             for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
-                for (int k = 0; k < WT; ++k) A[rt][k] = q4_to_f16<kExact, NATURAL>(cur[rt][ks], sv[rt][k], cv[rt][k]);
+                for (int k = 0; k < WT; ++k) A[rt][k] = q4_to_f16<kExact, NATURAL>(cur[rt][ks], sv[rt][k], cv[rt][k], k16);
 #pragma unroll
             for (int mt = 0; mt < NMT; ++mt)
 #pragma unroll
                 for (int x = 0; x < XT; ++x)
-                    B[mt][x] = *reinterpret_cast<const u32x4_t*>(Xl + (((g & 1) * XT + x) * 32 * MMT + 32 * mt + r) * 64 +
+                    B[mt][x] = *reinterpret_cast<const u32x4_t*>(xs + (x * 32 * MMT + 32 * mt + r) * 64 +
                                                                  8 * ((4 * h + ks) ^ sw));
 #pragma unroll
             for (int x = XT - 1; x >= 0; --x)
@@ -820,14 +843,11 @@ __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, co
                         }
         }
     };
-    stage_x(0, 0);
-    fetch_w(wa[0], 0);
-    int g = 0;
-    for (; g + 1 < G; g += 2) {
-        step(0, g);
-        step(1, g + 1);
-    }
-    if (g < G) step(0, g);
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i) stage(i, min(i, G - 1));
+    for (int g = 0; g < G; g += NS) unroll<NS>([&](auto i) {
+        if (g + i.value < G) step(i, g + i.value);
+    });
 
     // the groups' constant parts, (b + 8 s) 2^13 against the rows' sums, two fp16 terms each, 16 groups at a time: thread t
     // forms row t's terms in the staging buffer (32 bytes a row and term, its halves swapped in every other four rows)
@@ -844,8 +864,7 @@ __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, co
         fac[mt] = a.fac[row];
     }
     for (int k0 = 0; k0 < G; k0 += 16) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (the last step's copies have landed)
-        __syncthreads();
+        meet<0>();   // (the last steps' copies have landed, the tile's and the terms' last reads been made)
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             // (groups past the last meet sums of zero)
@@ -917,18 +936,21 @@ __device__ __forceinline__ void tile_begin(const MoeArgs& p, const TileArgs& a, 
     const MoeMat& mm = MATS == 2 && (t & 32) ? m1 : m0;
     const bool vec = sb_vec(m0, G) && sb_vec(m1, G);
     const uint16_t* const src = mm.s + static_cast<size_t>(row) * G;
-    for (int g0 = 0; g0 < G; g0 += 32) {
+    // (LDS has room for whole eights of groups: those past the last are not read)
+    auto put = [&](int k, const u32x4_t& v) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            sbl[(8 * k + i) * kTileRows + t] = tile_scale<SB_DT, WT>(static_cast<uint16_t>(v[i / 2] >> (16 * (i & 1))));
+    };
+    if (vec && G <= 32) {
         u32x4_t v[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (k == 0 || g0 + 8 * k < G) v[k] = load_u16x8(src, g0 + 8 * k, G, vec);
+        for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const u32x4_t*>(src + min(8 * k, G - 8));
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int g = g0 + 8 * k + i;
-                if (g < G) sbl[g * kTileRows + t] = tile_scale<SB_DT, WT>(static_cast<uint16_t>(v[k][i / 2] >> (16 * (i & 1))));
-            }
+            if (8 * k < G) put(k, v[k]);
+    } else {
+        for (int k = 0; 8 * k < G; ++k) put(k, load_u16x8(src, 8 * k, G, vec));
     }
     __syncthreads();
     body(tile, m0, m1, row0);
@@ -936,7 +958,7 @@ __device__ __forceinline__ void tile_begin(const MoeArgs& p, const TileArgs& a, 
 
 template <int MATS, int SB_DT, int XT, int WT, bool NATURAL, int MMT, class Out>
 __device__ __forceinline__ void tile_kernel(const MoeArgs& p, const TileArgs& a, Out&& out) {
-    constexpr int kStage = 2 * XT * 32 * MMT * 64, kConst = 2 * 16 * kTileRows;   // (the latter at the end)
+    constexpr int kStage = tile_stages(MMT) * tile_stage_bytes(XT, MMT) / 2, kConst = 2 * 16 * kTileRows;   // (the latter at the end)
     __shared__ __attribute__((aligned(16))) uint16_t Xl[kStage > kConst ? kStage : kConst];
     __shared__ int codes[32 * MMT];
     extern __shared__ __attribute__((aligned(16))) char sbl_bytes[];   // [G][256]
@@ -1143,6 +1165,7 @@ int slice_tokens(const qff_ctx* ctx, int rows, int cols, int xt, bool copy, int 
     size_t most = std::min<size_t>(tokens, 65535);
     if (copy) most = std::min(most, static_cast<size_t>(ctx->q4_xs_tokens) * 8192 / (static_cast<size_t>(rows) * xt * cols * 2));
     const size_t row = 8 + (cols / 64 + kSumsPad - 1) / kSumsPad * kSumsPad * 4;
+    most = std::min(most, (size_t{1} << 31) / (static_cast<size_t>(rows) * cols * 2));   // (offsets of rows have 32 bits)
     return static_cast<int>(std::min(most, (moe_part_bytes(ctx->cfg) / 16 - 8) / (rows * row)));
 }
 
@@ -1213,7 +1236,7 @@ hipError_t launch_moe_gate_up(qff_ctx* ctx, hipStream_t stream, const qff_moe_we
     }
     const Terms tm = tile_terms(x_dtype, w->sb_dtype, h_dtype);
     const int most = slice_tokens(ctx, 1, p.cols, tm.x, true, tokens);
-    const size_t lds = static_cast<size_t>(G) * kTileRows * 2 * tm.w;
+    const size_t lds = static_cast<size_t>((G + 7) / 8 * 8) * kTileRows * 2 * tm.w;
     for (int t0 = 0; t0 < tokens; t0 += most) {
         p.tokens = std::min(most, tokens - t0);
         p.indices = indices + static_cast<size_t>(t0) * top;
@@ -1311,7 +1334,7 @@ hipError_t launch_moe_down(qff_ctx* ctx, hipStream_t stream, const qff_moe_weigh
             if (const hipError_t e = moe_plan(ctx, stream, p, shared, units)) return e;
             ProfScope prof(ctx, stream, "moe_down_tile");
             const unsigned grid = tile_grid(p, shared, units, kTileRows);
-            const size_t lds = static_cast<size_t>(G) * kTileRows * 2 * tm.w;
+            const size_t lds = static_cast<size_t>((G + 7) / 8 * 8) * kTileRows * 2 * tm.w;
             auto launch = [&](auto S, auto XT, auto WT, auto NAT, auto HALF) {
                 auto go = [&](auto U) {
                     moe_down_tile_kernel<S.value, XT.value, WT.value, NAT.value, HALF.value, U.value>
