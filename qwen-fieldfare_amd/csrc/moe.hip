@@ -724,7 +724,7 @@ __device__ __forceinline__ bool sb_vec(const MoeMat& m, int G) {
 
 // Groups of x and of the weights on their way or in use: as many as LDS holds
 // beside a second workgroup.
-constexpr int tile_stages(int mmt) { return mmt == 4 ? 2 : mmt == 2 ? 3 : 4; }
+constexpr int tile_stages(int xt, int mmt) { return mmt == 4 ? 2 : mmt == 2 ? 4 - xt : 5 - xt; }
 constexpr int tile_stage_bytes(int xt, int mmt) { return xt * 32 * mmt * 128 + kTileRows * 32; }
 
 // All waves here, each with at most N of its copies still under way (the copies
@@ -759,7 +759,7 @@ __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, co
     // A stage holds a group's x [XT][32 MMT tokens][64] and words [wave][2 row tiles][64 lanes][16 bytes]. Copies of x: 8
     // tokens each, lane l the 16-byte piece l & 7 of token l >> 3, which is the token's 8-column block (l & 7) ^ ((token >>
     // 1) & 7) of the group; of words: the wave's own rows', as its lanes read them back.
-    constexpr int NS = tile_stages(MMT), kStage = tile_stage_bytes(XT, MMT), kXBytes = XT * 32 * MMT * 128;
+    constexpr int NS = tile_stages(XT, MMT), kStage = tile_stage_bytes(XT, MMT), kXBytes = XT * 32 * MMT * 128;
     const uint32_t at = lds_addr(Xl);
     uint32_t xoff[NMT], woff[2];
 #pragma unroll
@@ -958,7 +958,7 @@ __device__ __forceinline__ void tile_begin(const MoeArgs& p, const TileArgs& a, 
 
 template <int MATS, int SB_DT, int XT, int WT, bool NATURAL, int MMT, class Out>
 __device__ __forceinline__ void tile_kernel(const MoeArgs& p, const TileArgs& a, Out&& out) {
-    constexpr int kStage = tile_stages(MMT) * tile_stage_bytes(XT, MMT) / 2, kConst = 2 * 16 * kTileRows;   // (the latter at the end)
+    constexpr int kStage = tile_stages(XT, MMT) * tile_stage_bytes(XT, MMT) / 2, kConst = 2 * 16 * kTileRows;   // (the latter at the end)
     __shared__ __attribute__((aligned(16))) uint16_t Xl[kStage > kConst ? kStage : kConst];
     __shared__ int codes[32 * MMT];
     extern __shared__ __attribute__((aligned(16))) char sbl_bytes[];   // [G][256]
