@@ -817,19 +817,26 @@ __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, co
             }
         }
         const int sw = (r >> 1) & 7;
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            u32x4_t A[2][WT], B[NMT][XT];
-#pragma unroll
-            for (int rt = 0; rt < 2; ++rt)
-#pragma unroll
-                for (int k = 0; k < WT; ++k) A[rt][k] = q4_to_f16<kExact, NATURAL>(cur[rt][ks], sv[rt][k], cv[rt][k], k16);
+        u32x4_t A[2][2][WT], B[2][NMT][XT];
+        auto operands = [&](int ks) {
 #pragma unroll
             for (int mt = 0; mt < NMT; ++mt)
 #pragma unroll
                 for (int x = 0; x < XT; ++x)
-                    B[mt][x] = *reinterpret_cast<const u32x4_t*>(xs + (x * 32 * MMT + 32 * mt + r) * 64 +
-                                                                 8 * ((4 * h + ks) ^ sw));
+                    B[ks & 1][mt][x] = *reinterpret_cast<const u32x4_t*>(xs + (x * 32 * MMT + 32 * mt + r) * 64 + 8 * ((4 * h + ks) ^ sw));
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+                for (int k = 0; k < WT; ++k)
+                    A[ks & 1][rt][k] = q4_to_f16<kExact, NATURAL>(cur[rt][ks], sv[rt][k], cv[rt][k], k16);
+        };
+        operands(0);
+        // the next k step's reads, then its conversions between this one's products
+        constexpr int kProducts = 2 * NMT * (XT * WT == 4 ? 3 : XT * WT), kBetween = (2 * WT * 16 + kProducts - 1) / kProducts;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (ks < 3) operands(ks + 1);
 #pragma unroll
             for (int x = XT - 1; x >= 0; --x)
 #pragma unroll
@@ -839,8 +846,15 @@ __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, co
 #pragma unroll
                         for (int mt = 0; mt < NMT; ++mt) {
                             if (x == 1 && k == 1) continue;   // (2^-19 of the product's 2^-22 part)
-                            acc[rt][mt] = mfma_32x32x16_f16(A[rt][k], B[mt][x], acc[rt][mt]);
+                            acc[rt][mt] = mfma_32x32x16_f16(A[ks & 1][rt][k], B[ks & 1][mt][x], acc[rt][mt]);
                         }
+            if (ks < 3) {
+                __builtin_amdgcn_sched_group_barrier(0x100, NMT * XT, 0);
+                unroll<kProducts>([&](auto) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, kBetween, 0);
+                });
+            }
         }
     };
 #pragma unroll
@@ -991,7 +1005,7 @@ __device__ __forceinline__ void tile_kernel(const MoeArgs& p, const TileArgs& a,
 
 // (a lane's rows of a 32 x 32 tile: 8 j + 4 h .. + 3, its token the column)
 template <int SB_DT, int XT, int WT, int H_DT, int MMT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void moe_gate_up_tile_kernel(MoeArgs p, TileArgs a,
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void moe_gate_up_tile_kernel(MoeArgs p, TileArgs a,
                                                                                                        void* __restrict__ h) {
     tile_kernel<2, SB_DT, XT, WT, false, MMT>(p, a, [&](const f32x16_t& g, const f32x16_t& u, float f, int row0, int code) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -1019,7 +1033,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void m
 // The pairs' weighted rows: fp32, or (HALF) fp16 relative to the power of two above
 // the largest of each 64, whose exponents stand in `exps` [pair][rows / 64].
 template <int SB_DT, int XT, int WT, bool NATURAL, bool HALF, int MMT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void moe_down_tile_kernel(
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void moe_down_tile_kernel(
     MoeArgs p, TileArgs a, const float* __restrict__ scores, const float* __restrict__ coef, void* __restrict__ part,
     float* __restrict__ exps) {
     tile_kernel<1, SB_DT, XT, WT, NATURAL, MMT>(p, a, [&](const f32x16_t& a0, const f32x16_t& a1, float fac, int row0, int code) {
