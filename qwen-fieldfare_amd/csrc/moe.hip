@@ -694,6 +694,7 @@ __device__ __forceinline__ u32x4_t q4_to_f16(uint32_t w, f16x2_t s, f16x2_t c, u
 }
 
 constexpr int kXcds = 8;
+constexpr int kOutRow = 272;   // bytes of LDS for a token's outputs of one wave: 64 fp32 values and a pad
 constexpr int kTileRows = 256;   // weight rows of a workgroup: four waves of 64, in two row tiles of 32
 
 // What the tile kernel reads beside the weights.
@@ -732,7 +733,7 @@ constexpr int tile_stage_bytes(int xt, int mmt) { return xt * 32 * mmt * 128 + k
 // would its reads of LDS behind them).
 template <int N>
 __device__ __forceinline__ void meet() {
-    static_assert(N < 64, "six bits count them");
+    static_assert(N < 64, "six bits count them");   // (63: any number)
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 template <int N, class F>
@@ -785,11 +786,77 @@ __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, co
     uint32_t k16 = 0x4C004C00u;
     asm("" : "+v"(k16));
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt)
+    for (int i = 0; i < NS - 1; ++i) stage(i, min(i, G - 1));
+
+    // The groups' constant parts while those copies are under way: (b + 8 s) 2^13 against the rows' sums, two fp16 terms
+    // each, 16 groups at a time. Thread t forms row t's terms in the stage that is still free (32 bytes a row and term, its
+    // halves swapped in every other four rows).
+    {
+        const int gp = (G + kSumsPad - 1) / kSumsPad * kSumsPad;
+        const int own = min(MATS == 2 ? row0 + 32 * wave + (t & 31) : row0 + t, p.rows - 1);
+        const MoeMat& mm = MATS == 2 && (t & 32) ? m1 : m0;
+        const bool vec = sb_vec(m0, G) && sb_vec(m1, G);
+        const size_t base = static_cast<size_t>(own) * G;
+        uint16_t* const terms = Xl + (NS - 1) * kStage / 2;
+        const uint16_t* S[NMT];
 #pragma unroll
-        for (int mt = 0; mt < NMT; ++mt)
+        for (int mt = 0; mt < NMT; ++mt) {
+            const size_t row = x_row(32 * mt + r);
+            S[mt] = a.sums + row * 2 * gp + 8 * h;
+            fac[mt] = a.fac[row];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[rt][mt][i] = 0.0f;
+            for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[rt][mt][i] = 0.0f;
+        }
+        for (int k0 = 0; k0 < G; k0 += 16) {
+            if (k0) meet<63>();   // (the terms before have been read)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                // (groups past the last meet sums of zero)
+                const u32x4_t s8 = load_u16x8(mm.s + base, k0 + 8 * q, G, vec), b8 = load_u16x8(mm.b + base, k0 + 8 * q, G, vec);
+                u32x4_t bh, bl;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float v[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint16_t sq = static_cast<uint16_t>(s8[j] >> (16 * i)), bq = static_cast<uint16_t>(b8[j] >> (16 * i));
+                        v[i] = 8192.0f * fmaf(8.0f, elem<SB_DT>::load(&sq, 0), elem<SB_DT>::load(&bq, 0));
+                    }
+                    uint32_t hi, lo;
+                    split_f16x2(v[0], v[1], hi, lo);
+                    bh[j] = hi;
+                    bl[j] = lo;
+                }
+                uint16_t* o = terms + 16 * t + 8 * (q ^ (t >> 2 & 1));
+                *reinterpret_cast<u32x4_t*>(o) = bh;
+                *reinterpret_cast<u32x4_t*>(o + 16 * kTileRows) = bl;
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            meet<63>();
+#pragma unroll
+            for (int mt = 0; mt < NMT; ++mt) {
+                const u32x4_t xh = *reinterpret_cast<const u32x4_t*>(S[mt] + k0);
+                const u32x4_t xl = *reinterpret_cast<const u32x4_t*>(S[mt] + gp + k0);
+#pragma unroll
+                for (int rt = 0; rt < 2; ++rt) {
+                    const int q = 64 * wave + 32 * rt + r;
+                    const uint16_t* o = terms + 16 * q + 8 * (h ^ (q >> 2 & 1));
+                    const u32x4_t bh = *reinterpret_cast<const u32x4_t*>(o), bl = *reinterpret_cast<const u32x4_t*>(o + 16 * kTileRows);
+                    acc[rt][mt] = mfma_32x32x16_f16(bl, xh, acc[rt][mt]);
+                    acc[rt][mt] = mfma_32x32x16_f16(bh, xl, acc[rt][mt]);
+                    acc[rt][mt] = mfma_32x32x16_f16(bh, xh, acc[rt][mt]);
+                }
+            }
+        }
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+            for (int mt = 0; mt < NMT; ++mt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[rt][mt][i] *= fac[mt].y;
+    }
 
     // group g, in stage s, has landed once only the copies of the NS - 2 groups behind it may be under way; group g + NS - 1
     // goes where g - 1 was (past the last group, the last one again: every step copies alike)
@@ -857,71 +924,10 @@ __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, co
             }
         }
     };
-#pragma unroll
-    for (int i = 0; i < NS - 1; ++i) stage(i, min(i, G - 1));
     for (int g = 0; g < G; g += NS) unroll<NS>([&](auto i) {
         if (g + i.value < G) step(i, g + i.value);
     });
-
-    // the groups' constant parts, (b + 8 s) 2^13 against the rows' sums, two fp16 terms each, 16 groups at a time: thread t
-    // forms row t's terms in the staging buffer (32 bytes a row and term, its halves swapped in every other four rows)
-    const int gp = (G + kSumsPad - 1) / kSumsPad * kSumsPad;
-    const int own = min(MATS == 2 ? row0 + 32 * wave + (t & 31) : row0 + t, p.rows - 1);
-    const MoeMat& mm = MATS == 2 && (t & 32) ? m1 : m0;
-    const bool vec = sb_vec(m0, G) && sb_vec(m1, G);
-    const size_t base = static_cast<size_t>(own) * G;
-    const uint16_t* S[NMT];
-#pragma unroll
-    for (int mt = 0; mt < NMT; ++mt) {
-        const size_t row = x_row(32 * mt + r);
-        S[mt] = a.sums + row * 2 * gp + 8 * h;
-        fac[mt] = a.fac[row];
-    }
-    for (int k0 = 0; k0 < G; k0 += 16) {
-        meet<0>();   // (the last steps' copies have landed, the tile's and the terms' last reads been made)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            // (groups past the last meet sums of zero)
-            const u32x4_t s8 = load_u16x8(mm.s + base, k0 + 8 * q, G, vec), b8 = load_u16x8(mm.b + base, k0 + 8 * q, G, vec);
-            u32x4_t bh, bl;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float v[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint16_t sq = static_cast<uint16_t>(s8[j] >> (16 * i)), bq = static_cast<uint16_t>(b8[j] >> (16 * i));
-                    v[i] = 8192.0f * fmaf(8.0f, elem<SB_DT>::load(&sq, 0), elem<SB_DT>::load(&bq, 0));
-                }
-                uint32_t hi, lo;
-                split_f16x2(v[0], v[1], hi, lo);
-                bh[j] = hi;
-                bl[j] = lo;
-            }
-            uint16_t* o = Xl + 16 * t + 8 * (q ^ (t >> 2 & 1));
-            *reinterpret_cast<u32x4_t*>(o) = bh;
-            *reinterpret_cast<u32x4_t*>(o + 16 * kTileRows) = bl;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int mt = 0; mt < NMT; ++mt) {
-            const u32x4_t xh = *reinterpret_cast<const u32x4_t*>(S[mt] + k0);
-            const u32x4_t xl = *reinterpret_cast<const u32x4_t*>(S[mt] + gp + k0);
-#pragma unroll
-            for (int rt = 0; rt < 2; ++rt) {
-                const int q = 64 * wave + 32 * rt + r;
-                const uint16_t* o = Xl + 16 * q + 8 * (h ^ (q >> 2 & 1));
-                const u32x4_t bh = *reinterpret_cast<const u32x4_t*>(o), bl = *reinterpret_cast<const u32x4_t*>(o + 16 * kTileRows);
-                f32x16_t add;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) add[i] = 0.0f;
-                add = mfma_32x32x16_f16(bl, xh, add);
-                add = mfma_32x32x16_f16(bh, xl, add);
-                add = mfma_32x32x16_f16(bh, xh, add);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[rt][mt][i] = fmaf(add[i], fac[mt].y, acc[rt][mt][i]);
-            }
-        }
-    }
+    meet<0>();   // (LDS is free: the last steps' copies have landed, their reads been made)
 }
 
 // The tile of this workgroup, its pairs and scales in LDS; body(tile, m0, m1, row0)
@@ -971,9 +977,12 @@ __device__ __forceinline__ void tile_begin(const MoeArgs& p, const TileArgs& a, 
 }
 
 template <int MATS, int SB_DT, int XT, int WT, bool NATURAL, int MMT, class Out>
-__device__ __forceinline__ void tile_kernel(const MoeArgs& p, const TileArgs& a, Out&& out) {
-    constexpr int kStage = tile_stages(XT, MMT) * tile_stage_bytes(XT, MMT) / 2, kConst = 2 * 16 * kTileRows;   // (the latter at the end)
-    __shared__ __attribute__((aligned(16))) uint16_t Xl[kStage > kConst ? kStage : kConst];
+__device__ __forceinline__ void tile_kernel(const MoeArgs& p, const TileArgs& a, const Out& out) {
+    // (the last stage first holds the constant parts' terms; behind the last group, all of them each wave's rows of outputs)
+    constexpr int kStage = tile_stage_bytes(XT, MMT), kConst = 64 * kTileRows;
+    constexpr int kBytes = (tile_stages(XT, MMT) - 1) * kStage + (kStage > kConst ? kStage : kConst);
+    static_assert(kBytes >= 4 * 32 * kOutRow, "32 rows of outputs a wave");
+    __shared__ __attribute__((aligned(16))) uint16_t Xl[kBytes / 2];
     __shared__ int codes[32 * MMT];
     extern __shared__ __attribute__((aligned(16))) char sbl_bytes[];   // [G][256]
     tile_sb<WT>* const sbl = reinterpret_cast<tile_sb<WT>*>(sbl_bytes);
@@ -984,11 +993,18 @@ __device__ __forceinline__ void tile_kernel(const MoeArgs& p, const TileArgs& a,
             float2 fac[NMT];
             tile_run<MATS, SB_DT, XT, WT, NATURAL, MMT, NMT>(p, a, m0, m1, row0, codes, Xl, sbl, acc, fac);
             const int lane = threadIdx.x & 63;
+            char* const rows = reinterpret_cast<char*>(Xl) + (threadIdx.x >> 6) * 32 * kOutRow;
 #pragma unroll
             for (int mt = 0; mt < NMT; ++mt) {
-                const int tok = 32 * mt + (lane & 31);
-                if (tok >= tile.z) continue;
-                out(acc[0][mt], acc[1][mt], fac[mt].x, row0, codes[tok]);
+                out.put(acc[0][mt], acc[1][mt], fac[mt].x, row0, codes[32 * mt + (lane & 31)], rows + (lane & 31) * kOutRow);
+                // a token's bytes, 16 a lane
+                constexpr int kPieces = Out::kBytes / 16, kTokens = 64 / kPieces;
+#pragma unroll
+                for (int i = 0; i < 32 / kTokens; ++i) {
+                    const int tok = kTokens * i + lane / kPieces, piece = lane % kPieces;
+                    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(rows + tok * kOutRow + 16 * piece);
+                    if (32 * mt + tok < tile.z) out.store(v, row0, codes[32 * mt + tok], piece);
+                }
             }
         };
         const int nmt = (tile.z + 31) / 32;
@@ -1003,72 +1019,90 @@ __device__ __forceinline__ void tile_kernel(const MoeArgs& p, const TileArgs& a,
     });
 }
 
-// (a lane's rows of a 32 x 32 tile: 8 j + 4 h .. + 3, its token the column)
-template <int SB_DT, int XT, int WT, int H_DT, int MMT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void moe_gate_up_tile_kernel(MoeArgs p, TileArgs a,
-                                                                                                       void* __restrict__ h) {
-    tile_kernel<2, SB_DT, XT, WT, false, MMT>(p, a, [&](const f32x16_t& g, const f32x16_t& u, float f, int row0, int code) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        const size_t base = (static_cast<size_t>(code >> 5) * p.slots + (code & 31)) * p.rows;
+// What becomes of a wave's two row tiles: put() leaves a token's kBytes in its row
+// of LDS (a lane holds rows 8 j + 4 h .. + 3 of its token, the column), store()
+// takes 16 of them to memory. (Stored from the accumulators, 16 bytes of a row at a
+// time, the pairs' rows alone took the down products of 8192 tokens 100 us.)
+template <int DT>
+__device__ __forceinline__ void put4(char* to, int at, f32x4_t v) {
+    if constexpr (DT == 0) *reinterpret_cast<f32x4_t*>(to + 4 * at) = v;
+    else if constexpr (DT == 1) *reinterpret_cast<u32x2_t*>(to + 2 * at) = u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    else *reinterpret_cast<u32x2_t*>(to + 2 * at) = u32x2_t{pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3])};
+}
+
+template <int H_DT>
+struct GateUpOut {
+    static constexpr int kSize = H_DT == 0 ? 4 : 2, kBytes = 32 * kSize;
+    const MoeArgs& p;
+    void* h;
+    __device__ __forceinline__ void put(const f32x16_t& g, const f32x16_t& u, float f, int, int, char* to) const {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int row = row0 + 32 * wave + 8 * j + 4 * (lane >> 5);
-            if (row >= p.rows) continue;
-            float v[4];
+            f32x4_t v;
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] = silu(g[4 * j + i] * f) * (u[4 * j + i] * f);
-            if constexpr (H_DT == 0) {
-                *reinterpret_cast<f32x4_t*>(static_cast<float*>(h) + base + row) = f32x4_t{v[0], v[1], v[2], v[3]};
-            } else if constexpr (H_DT == 1) {
-                *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(h) + base + row) =
-                    u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-            } else {
-                *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(h) + base + row) =
-                    u32x2_t{pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3])};
-            }
+            put4<H_DT>(to, 8 * j + 4 * (threadIdx.x >> 5 & 1), v);
         }
-    });
+    }
+    __device__ __forceinline__ void store(u32x4_t v, int row0, int code, int piece) const {
+        const int row = row0 + 32 * (threadIdx.x >> 6);
+        if (row >= p.rows) return;   // (rows come in multiples of 64)
+        const size_t at = (static_cast<size_t>(code >> 5) * p.slots + (code & 31)) * p.rows + row;
+        *reinterpret_cast<u32x4_t*>(static_cast<char*>(h) + at * kSize + 16 * piece) = v;
+    }
+};
+template <int SB_DT, int XT, int WT, int H_DT, int MMT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void moe_gate_up_tile_kernel(MoeArgs p, TileArgs a,
+                                                                                                          void* __restrict__ h) {
+    tile_kernel<2, SB_DT, XT, WT, false, MMT>(p, a, GateUpOut<H_DT>{p, h});
 }
 
 // The pairs' weighted rows: fp32, or (HALF) fp16 relative to the power of two above
-// the largest of each 64, whose exponents stand in `exps` [pair][rows / 64].
-template <int SB_DT, int XT, int WT, bool NATURAL, bool HALF, int MMT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void moe_down_tile_kernel(
-    MoeArgs p, TileArgs a, const float* __restrict__ scores, const float* __restrict__ coef, void* __restrict__ part,
-    float* __restrict__ exps) {
-    tile_kernel<1, SB_DT, XT, WT, NATURAL, MMT>(p, a, [&](const f32x16_t& a0, const f32x16_t& a1, float fac, int row0, int code) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = code >> 5, s = code & 31;
+// the largest of each 64, which stands in `exps` [pair][rows / 64].
+template <bool HALF>
+struct DownOut {
+    static constexpr int kBytes = HALF ? 128 : 256;
+    const MoeArgs& p;
+    const float* scores;
+    const float* coef;
+    void* part;
+    float* exps;
+    __device__ __forceinline__ void put(const f32x16_t& a0, const f32x16_t& a1, float fac, int row0, int code, char* to) const {
+        const int lane = threadIdx.x & 63, m = code >> 5, s = code & 31;
         const float f = fac * (s < p.top ? scores[m * p.top + s] : coef ? coef[m] : 1.0f);
-        const size_t pair = static_cast<size_t>(m) * p.slots + s;
-        const int block = row0 + 64 * wave;
-        if (block >= p.rows) return;   // (rows come in multiples of 64)
-        float k = 1.0f;
+        float k = f;
         if constexpr (HALF) {
             float mx = 0.0f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fmaxf(fabsf(a0[i]), fabsf(a1[i])));
-            mx *= fabsf(f);
-            // the other half of the token's rows lies 32 lanes on (both are here: they share the token)
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const int e = mx > 0.0f ? max(__builtin_amdgcn_frexp_expf(mx) - 15, -126) : 0;
-            k = ldexpf(1.0f, -e);
-            if (lane < 32) exps[pair * (p.rows / 64) + block / 64] = ldexpf(1.0f, e);
+            mx = fmaxf(mx, __shfl_xor(mx, 32)) * fabsf(f);   // (the other half of the token's rows lies 32 lanes on)
+            const int e = mx > 0.0f ? max(__builtin_amdgcn_frexp_expf(mx) - 15, -126) : 0, block = row0 / 64 + (threadIdx.x >> 6);
+            k = f * ldexpf(1.0f, -e);
+            if (lane < 32 && 64 * block < p.rows)
+                exps[(static_cast<size_t>(m) * p.slots + s) * (p.rows / 64) + block] = ldexpf(1.0f, e);
         }
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const size_t o = pair * p.rows + block + 32 * rt + 8 * j + 4 * (lane >> 5);
                 f32x4_t v;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = (rt ? a1[4 * j + i] : a0[4 * j + i]) * f * k;
-                if constexpr (HALF)
-                    *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(part) + o) =
-                        u32x2_t{pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3])};
-                else
-                    *reinterpret_cast<f32x4_t*>(static_cast<float*>(part) + o) = v;
+                for (int i = 0; i < 4; ++i) v[i] = (rt ? a1[4 * j + i] : a0[4 * j + i]) * k;
+                put4<HALF ? 2 : 0>(to, 32 * rt + 8 * j + 4 * (lane >> 5), v);
             }
-    });
+    }
+    __device__ __forceinline__ void store(u32x4_t v, int row0, int code, int piece) const {
+        const int row = row0 + 64 * (threadIdx.x >> 6);
+        if (row >= p.rows) return;
+        const size_t at = (static_cast<size_t>(code >> 5) * p.slots + (code & 31)) * p.rows + row;
+        *reinterpret_cast<u32x4_t*>(static_cast<char*>(part) + at * (HALF ? 2 : 4) + 16 * piece) = v;
+    }
+};
+template <int SB_DT, int XT, int WT, bool NATURAL, bool HALF, int MMT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void moe_down_tile_kernel(
+    MoeArgs p, TileArgs a, const float* __restrict__ scores, const float* __restrict__ coef, void* __restrict__ part,
+    float* __restrict__ exps) {
+    tile_kernel<1, SB_DT, XT, WT, NATURAL, MMT>(p, a, DownOut<HALF>{p, scores, coef, part, exps});
 }
 
 // y[m] = residual[m] + the rows of its pairs, in their order: a thread 8 columns.
