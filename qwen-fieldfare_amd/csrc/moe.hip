@@ -742,14 +742,61 @@ __device__ __forceinline__ void unroll(F&& f) {
     f(std::integral_constant<int, N - 1>{});
 }
 
+// Where the constant parts' terms lie in the staging buffer: in the last stage, or
+// (more than 16 groups, 32 KB at a time) from its beginning.
+__device__ __forceinline__ constexpr int tile_terms_at(int xt, int mmt, int groups) {
+    return groups <= 16 ? (tile_stages(xt, mmt) - 1) * tile_stage_bytes(xt, mmt) : 0;
+}
+
+// The constant parts' terms of groups k0 .. k0 + 31: (b + 8 s) 2^13 in two fp16
+// terms. Thread t forms row t's (of two matrices 32 rows of the first, 32 of the
+// second, ..): [16 groups][term][row][16], a row's halves swapped in every other four
+// rows. Groups past the last (which meet sums of zero) take its.
+template <int MATS>
+__device__ __forceinline__ int tile_row(const MoeArgs& p, int row0) {
+    const int t = threadIdx.x;
+    return min(MATS == 2 ? row0 + 32 * (t >> 6) + (t & 31) : row0 + t, p.rows - 1);
+}
+template <int SB_DT>
+__device__ __forceinline__ void put_terms(uint16_t* to, int k, const u32x4_t& s8, const u32x4_t& b8) {
+    const int t = threadIdx.x;
+    u32x4_t bh, bl;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float v[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint16_t sq = static_cast<uint16_t>(s8[j] >> (16 * i)), bq = static_cast<uint16_t>(b8[j] >> (16 * i));
+            v[i] = 8192.0f * fmaf(8.0f, elem<SB_DT>::load(&sq, 0), elem<SB_DT>::load(&bq, 0));
+        }
+        uint32_t hi, lo;
+        split_f16x2(v[0], v[1], hi, lo);
+        bh[j] = hi;
+        bl[j] = lo;
+    }
+    uint16_t* o = to + k / 16 * 32 * kTileRows + 16 * t + 8 * ((k / 8 & 1) ^ (t >> 2 & 1));
+    *reinterpret_cast<u32x4_t*>(o) = bh;
+    *reinterpret_cast<u32x4_t*>(o + 16 * kTileRows) = bl;
+}
+template <int MATS, int SB_DT>
+__device__ __forceinline__ void tile_terms(const MoeArgs& p, const MoeMat& m0, const MoeMat& m1, int row0, int k0, uint16_t* to) {
+    const int G = p.cols / 64;
+    const MoeMat& mm = MATS == 2 && (threadIdx.x & 32) ? m1 : m0;
+    const bool vec = sb_vec(m0, G) && sb_vec(m1, G);
+    const size_t base = static_cast<size_t>(tile_row<MATS>(p, row0)) * G;
+    for (int k = 0; k < 32 && k0 + k < (G + 15) / 16 * 16; k += 8)
+        put_terms<SB_DT>(to, k, load_u16x8(mm.s + base, k0 + k, G, vec), load_u16x8(mm.b + base, k0 + k, G, vec));
+}
+
 // One tile: 256 weight rows (of gate and up: 128 of each, a wave's two row tiles the
 // same rows of both) x NMT tiles of 32 tokens. Groups of x and of the words go from
 // global memory into LDS, tile_stages of them in turn, one barrier a group; a
 // wave converts its own rows' words in registers. Rows of x are swizzled so that
 // the 32 rows of an operand read meet every bank group twice.
-template <int MATS, int SB_DT, int XT, int WT, bool NATURAL, int MMT, int NMT>
+template <int MATS, int SB_DT, int XT, int WT, bool NATURAL, int MMT, int NMT, class Out>
 __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, const MoeMat& m0, const MoeMat& m1, int row0,
-                                         const int* codes, uint16_t* Xl, const tile_sb<WT>* sbl, f32x16_t (&acc)[2][NMT], float2 (&fac)[NMT]) {
+                                         const int* codes, uint16_t* Xl, const tile_sb<WT>* sbl, f32x16_t (&acc)[2][NMT], float2 (&fac)[NMT],
+                                         const Out& out) {
     constexpr bool kExact = SB_DT == 1 || WT == 2;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = lane & 31, h = lane >> 5;
     const int G = p.cols / 64;
@@ -785,68 +832,53 @@ __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, co
     };
     uint32_t k16 = 0x4C004C00u;
     asm("" : "+v"(k16));
-#pragma unroll
-    for (int i = 0; i < NS - 1; ++i) stage(i, min(i, G - 1));
-
-    // The groups' constant parts while those copies are under way: (b + 8 s) 2^13 against the rows' sums, two fp16 terms
-    // each, 16 groups at a time. Thread t forms row t's terms in the stage that is still free (32 bytes a row and term, its
-    // halves swapped in every other four rows).
+    // The groups' constant parts: their terms, 32 groups at a time (the first are there already), against the rows' sums.
+    // Up to 16 groups the terms lie in the last stage and the first copies are on their way meanwhile; they are asked for
+    // behind the sums, since the wait for these is the compiler's, which does not count copies.
+    const bool early = G <= 16;
     {
         const int gp = (G + kSumsPad - 1) / kSumsPad * kSumsPad;
-        const int own = min(MATS == 2 ? row0 + 32 * wave + (t & 31) : row0 + t, p.rows - 1);
-        const MoeMat& mm = MATS == 2 && (t & 32) ? m1 : m0;
-        const bool vec = sb_vec(m0, G) && sb_vec(m1, G);
-        const size_t base = static_cast<size_t>(own) * G;
-        uint16_t* const terms = Xl + (NS - 1) * kStage / 2;
         const uint16_t* S[NMT];
 #pragma unroll
         for (int mt = 0; mt < NMT; ++mt) {
             const size_t row = x_row(32 * mt + r);
             S[mt] = a.sums + row * 2 * gp + 8 * h;
             fac[mt] = a.fac[row];
+            fac[mt].x *= out.weight(codes[32 * mt + r]);
 #pragma unroll
             for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[rt][mt][i] = 0.0f;
         }
+        const uint16_t* const terms = Xl + tile_terms_at(XT, MMT, G) / 2;
         for (int k0 = 0; k0 < G; k0 += 16) {
-            if (k0) meet<63>();   // (the terms before have been read)
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                // (groups past the last meet sums of zero)
-                const u32x4_t s8 = load_u16x8(mm.s + base, k0 + 8 * q, G, vec), b8 = load_u16x8(mm.b + base, k0 + 8 * q, G, vec);
-                u32x4_t bh, bl;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float v[2];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint16_t sq = static_cast<uint16_t>(s8[j] >> (16 * i)), bq = static_cast<uint16_t>(b8[j] >> (16 * i));
-                        v[i] = 8192.0f * fmaf(8.0f, elem<SB_DT>::load(&sq, 0), elem<SB_DT>::load(&bq, 0));
-                    }
-                    uint32_t hi, lo;
-                    split_f16x2(v[0], v[1], hi, lo);
-                    bh[j] = hi;
-                    bl[j] = lo;
-                }
-                uint16_t* o = terms + 16 * t + 8 * (q ^ (t >> 2 & 1));
-                *reinterpret_cast<u32x4_t*>(o) = bh;
-                *reinterpret_cast<u32x4_t*>(o + 16 * kTileRows) = bl;
-            }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            meet<63>();
+            u32x4_t xh[NMT], xl[NMT];
 #pragma unroll
             for (int mt = 0; mt < NMT; ++mt) {
-                const u32x4_t xh = *reinterpret_cast<const u32x4_t*>(S[mt] + k0);
-                const u32x4_t xl = *reinterpret_cast<const u32x4_t*>(S[mt] + gp + k0);
+                xh[mt] = *reinterpret_cast<const u32x4_t*>(S[mt] + k0);
+                xl[mt] = *reinterpret_cast<const u32x4_t*>(S[mt] + gp + k0);
+            }
+            if (k0 && k0 % 32 == 0) {
+                __syncthreads();   // (the terms before have been read)
+                tile_terms<MATS, SB_DT>(p, m0, m1, row0, k0, Xl + tile_terms_at(XT, MMT, G) / 2);
+                __syncthreads();
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (early) {
 #pragma unroll
-                for (int rt = 0; rt < 2; ++rt) {
-                    const int q = 64 * wave + 32 * rt + r;
-                    const uint16_t* o = terms + 16 * q + 8 * (h ^ (q >> 2 & 1));
-                    const u32x4_t bh = *reinterpret_cast<const u32x4_t*>(o), bl = *reinterpret_cast<const u32x4_t*>(o + 16 * kTileRows);
-                    acc[rt][mt] = mfma_32x32x16_f16(bl, xh, acc[rt][mt]);
-                    acc[rt][mt] = mfma_32x32x16_f16(bh, xl, acc[rt][mt]);
-                    acc[rt][mt] = mfma_32x32x16_f16(bh, xh, acc[rt][mt]);
+                for (int i = 0; i < NS - 1; ++i) stage(i, min(i, G - 1));
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt) {
+                const int q = 64 * wave + 32 * rt + r;
+                const uint16_t* o = terms + k0 % 32 * 2 * kTileRows + 16 * q + 8 * (h ^ (q >> 2 & 1));
+                const u32x4_t bh = *reinterpret_cast<const u32x4_t*>(o), bl = *reinterpret_cast<const u32x4_t*>(o + 16 * kTileRows);
+#pragma unroll
+                for (int mt = 0; mt < NMT; ++mt) {
+                    acc[rt][mt] = mfma_32x32x16_f16(bl, xh[mt], acc[rt][mt]);
+                    acc[rt][mt] = mfma_32x32x16_f16(bh, xl[mt], acc[rt][mt]);
+                    acc[rt][mt] = mfma_32x32x16_f16(bh, xh[mt], acc[rt][mt]);
                 }
             }
         }
@@ -856,6 +888,11 @@ __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, co
             for (int mt = 0; mt < NMT; ++mt)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[rt][mt][i] *= fac[mt].y;
+        if (!early) {
+            meet<63>();   // (the terms have been read)
+#pragma unroll
+            for (int i = 0; i < NS - 1; ++i) stage(i, min(i, G - 1));
+        }
     }
 
     // group g, in stage s, has landed once only the copies of the NS - 2 groups behind it may be under way; group g + NS - 1
@@ -933,7 +970,7 @@ __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, co
 // The tile of this workgroup, its pairs and scales in LDS; body(tile, m0, m1, row0)
 // where there is one.
 template <int MATS, int SB_DT, int WT, int MMT, class Body>
-__device__ __forceinline__ void tile_begin(const MoeArgs& p, const TileArgs& a, int* codes, tile_sb<WT>* sbl, Body&& body) {
+__device__ __forceinline__ void tile_begin(const MoeArgs& p, const TileArgs& a, int* codes, tile_sb<WT>* sbl, uint16_t* terms, Body&& body) {
     constexpr int kOwn = kTileRows / MATS;   // rows of each matrix
     const int blocks = (p.rows + kOwn - 1) / kOwn, items = *a.count * blocks;
     // Workgroups go round the XCDs in turn: each XCD takes one run of the items, so that an expert's row blocks
@@ -951,26 +988,34 @@ __device__ __forceinline__ void tile_begin(const MoeArgs& p, const TileArgs& a, 
         const int k = tile.y + min(t, tile.z - 1);
         codes[t] = shared ? pair_code(k, p.top) : a.list[k];
     }
-    // thread t: row t of the tile (of two matrices 32 of the first, 32 of the second, ..)
-    const int row = min(MATS == 2 ? row0 + 32 * (t >> 6) + (t & 31) : row0 + t, p.rows - 1);
+    // thread t: row t's scales and the first 32 groups' terms
     const MoeMat& mm = MATS == 2 && (t & 32) ? m1 : m0;
     const bool vec = sb_vec(m0, G) && sb_vec(m1, G);
-    const uint16_t* const src = mm.s + static_cast<size_t>(row) * G;
+    const size_t base = static_cast<size_t>(tile_row<MATS>(p, row0)) * G;
     // (LDS has room for whole eights of groups: those past the last are not read)
-    auto put = [&](int k, const u32x4_t& v) {
+    auto put = [&](int k, const u32x4_t& s8, const u32x4_t& b8) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            sbl[(8 * k + i) * kTileRows + t] = tile_scale<SB_DT, WT>(static_cast<uint16_t>(v[i / 2] >> (16 * (i & 1))));
+            sbl[(8 * k + i) * kTileRows + t] = tile_scale<SB_DT, WT>(static_cast<uint16_t>(s8[i / 2] >> (16 * (i & 1))));
+        if (k < 4) put_terms<SB_DT>(terms, 8 * k, s8, b8);
     };
-    if (vec && G <= 32) {
-        u32x4_t v[4];
+    const int eights = (G + 7) / 8;
+    if (vec && G == 8) {
+        const u32x4_t s8 = *reinterpret_cast<const u32x4_t*>(mm.s + base), b8 = *reinterpret_cast<const u32x4_t*>(mm.b + base);
+        put(0, s8, b8);
+        put_terms<SB_DT>(terms, 8, s8, b8);
+    } else if (vec && G == 32) {
+        u32x4_t s8[4], b8[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const u32x4_t*>(src + min(8 * k, G - 8));
+        for (int k = 0; k < 4; ++k) {
+            s8[k] = *reinterpret_cast<const u32x4_t*>(mm.s + base + 8 * k);
+            b8[k] = *reinterpret_cast<const u32x4_t*>(mm.b + base + 8 * k);
+        }
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (8 * k < G) put(k, v[k]);
+        for (int k = 0; k < 4; ++k) put(k, s8[k], b8[k]);
     } else {
-        for (int k = 0; 8 * k < G; ++k) put(k, load_u16x8(src, 8 * k, G, vec));
+        for (int k = 0; k < eights; ++k) put(k, load_u16x8(mm.s + base, 8 * k, G, vec), load_u16x8(mm.b + base, 8 * k, G, vec));
+        if (eights < 4 && (eights & 1)) put_terms<SB_DT>(terms, 8 * eights, u32x4_t{}, u32x4_t{});   // (the half that meets sums of zero)
     }
     __syncthreads();
     body(tile, m0, m1, row0);
@@ -978,20 +1023,20 @@ __device__ __forceinline__ void tile_begin(const MoeArgs& p, const TileArgs& a, 
 
 template <int MATS, int SB_DT, int XT, int WT, bool NATURAL, int MMT, class Out>
 __device__ __forceinline__ void tile_kernel(const MoeArgs& p, const TileArgs& a, const Out& out) {
-    // (the last stage first holds the constant parts' terms; behind the last group, all of them each wave's rows of outputs)
+    // (it first holds the constant parts' terms; behind the last group, all of them each wave's rows of outputs)
     constexpr int kStage = tile_stage_bytes(XT, MMT), kConst = 64 * kTileRows;
     constexpr int kBytes = (tile_stages(XT, MMT) - 1) * kStage + (kStage > kConst ? kStage : kConst);
-    static_assert(kBytes >= 4 * 32 * kOutRow, "32 rows of outputs a wave");
+    static_assert(kBytes >= 4 * 32 * kOutRow && kBytes >= 2 * kConst, "32 rows of outputs a wave; 32 groups' terms");
     __shared__ __attribute__((aligned(16))) uint16_t Xl[kBytes / 2];
     __shared__ int codes[32 * MMT];
     extern __shared__ __attribute__((aligned(16))) char sbl_bytes[];   // [G][256]
     tile_sb<WT>* const sbl = reinterpret_cast<tile_sb<WT>*>(sbl_bytes);
-    tile_begin<MATS, SB_DT, WT, MMT>(p, a, codes, sbl, [&](const int4& tile, const MoeMat& m0, const MoeMat& m1, int row0) {
+    tile_begin<MATS, SB_DT, WT, MMT>(p, a, codes, sbl, Xl + tile_terms_at(XT, MMT, p.cols / 64) / 2, [&](const int4& tile, const MoeMat& m0, const MoeMat& m1, int row0) {
         auto run = [&](auto n) {
             constexpr int NMT = decltype(n)::value;
             f32x16_t acc[2][NMT];
             float2 fac[NMT];
-            tile_run<MATS, SB_DT, XT, WT, NATURAL, MMT, NMT>(p, a, m0, m1, row0, codes, Xl, sbl, acc, fac);
+            tile_run<MATS, SB_DT, XT, WT, NATURAL, MMT, NMT>(p, a, m0, m1, row0, codes, Xl, sbl, acc, fac, out);
             const int lane = threadIdx.x & 63;
             char* const rows = reinterpret_cast<char*>(Xl) + (threadIdx.x >> 6) * 32 * kOutRow;
 #pragma unroll
@@ -1035,6 +1080,7 @@ struct GateUpOut {
     static constexpr int kSize = H_DT == 0 ? 4 : 2, kBytes = 32 * kSize;
     const MoeArgs& p;
     void* h;
+    __device__ __forceinline__ float weight(int) const { return 1.0f; }
     __device__ __forceinline__ void put(const f32x16_t& g, const f32x16_t& u, float f, int, int, char* to) const {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -1067,9 +1113,12 @@ struct DownOut {
     const float* coef;
     void* part;
     float* exps;
-    __device__ __forceinline__ void put(const f32x16_t& a0, const f32x16_t& a1, float fac, int row0, int code, char* to) const {
+    __device__ __forceinline__ float weight(int code) const {
+        const int m = code >> 5, s = code & 31;
+        return s < p.top ? scores[m * p.top + s] : coef ? coef[m] : 1.0f;
+    }
+    __device__ __forceinline__ void put(const f32x16_t& a0, const f32x16_t& a1, float f, int row0, int code, char* to) const {
         const int lane = threadIdx.x & 63, m = code >> 5, s = code & 31;
-        const float f = fac * (s < p.top ? scores[m * p.top + s] : coef ? coef[m] : 1.0f);
         float k = f;
         if constexpr (HALF) {
             float mx = 0.0f;
