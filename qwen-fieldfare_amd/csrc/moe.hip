@@ -154,17 +154,68 @@ constexpr int kGroups = 4;   // groups of 64 columns that a wave requests at onc
 //
 // A tile is 16 weight rows against one token, x as the A operand (the same
 // token in all 16 rows) and the weights as B, so that a lane's accumulator is its
-// own weight row's sum (lane & 15) and needs that row's scale alone.
+// own weight row's sum (lane & 15) and needs that row's scale alone. A wave takes
+// 256 columns at a time: each lane splits four of them into terms, which all read
+// back from the wave's own LDS (split by every lane for itself they took more
+// instructions than the weights: gate and up of a token 13.4 us).
+constexpr int kOneWaves = 8, kChunk = 64 * kGroups;
+
+// A lane's four columns of x, and their terms in the k order.
+template <int X_DT>
+struct XFour {
+    static constexpr int kTerms = XCols<X_DT>::kTerms;
+    float v[4];
+    __device__ __forceinline__ void load(const void* x, size_t i) {
+        if constexpr (X_DT == 0) {
+            const f32x4_t f = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(x) + i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = f[k];
+        } else {
+            const u32x2_t u = *reinterpret_cast<const u32x2_t*>(static_cast<const uint16_t*>(x) + i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint16_t h = static_cast<uint16_t>(u[k / 2] >> (16 * (k & 1)));
+                v[k] = elem<X_DT>::load(&h, 0);
+            }
+        }
+    }
+    // to: [kTerms][kChunk]. Even lanes hold columns 0-3 of a word of 8 and write its first two pairs (c0, c4), (c1, c5),
+    // odd ones hold 4-7 and write the others.
+    __device__ __forceinline__ void split(uint16_t* to, int lane) const {
+        const bool odd = lane & 1;
+        float a[2], b[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float give = odd ? v[j] : v[2 + j], take = dpp_mov<0xB1>(give);   // (the neighbour's, lane ^ 1)
+            a[j] = odd ? take : v[j];
+            b[j] = odd ? v[2 + j] : take;
+        }
+#pragma unroll
+        for (int q = 0; q < kTerms; ++q) {
+            u32x2_t t;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                t[j] = pack_bf16x2(a[j], b[j]);
+                a[j] -= __uint_as_float(t[j] << 16);
+                b[j] -= __uint_as_float(t[j] & 0xffff0000u);
+            }
+            *reinterpret_cast<u32x2_t*>(to + q * kChunk + 4 * lane) = t;
+        }
+    }
+};
 
 template <int X_DT, int SB_DT, int MATS>
 struct OneStep {
     u32x4_t w[MATS][kGroups / 2];
-    XCols<X_DT> x[kGroups];
-    uint16_t s[MATS][kGroups], b[MATS][kGroups];
+    XFour<X_DT> x;
+    u32x2_t s[MATS], b[MATS];
 
-    // groups g0 .. g0 + 3 (those past the last are requested as the last and not used)
-    __device__ __forceinline__ void load(const MoeMat (&m)[MATS], const void* xp, size_t xrow, int row, int cols, int g0,
-                                         int kg) {
+    // x of groups g0 .. g0 + 3 (columns past the last are requested as the row's last four and not used)
+    __device__ __forceinline__ void load_x(const void* xp, size_t xrow, int cols, int g0, int lane) {
+        x.load(xp, xrow + min(64 * g0 + 4 * lane, cols - 4));
+    }
+    // their words, scales and biases (those past the last group are requested as the last's and not used)
+    __device__ __forceinline__ void load_w(const MoeMat (&m)[MATS], int row, int cols, int g0, int kg) {
         const int G = cols / 64;
         const size_t r = static_cast<size_t>(row);
 #pragma unroll
@@ -173,21 +224,28 @@ struct OneStep {
             for (int sp = 0; sp < kGroups / 2; ++sp)
                 w[i][sp] = *reinterpret_cast<const u32x4_t*>(m[i].w + r * (cols / 8) +
                                                              8 * min(g0 + 2 * sp + (kg >> 1), G - 1) + 4 * (kg & 1));
+            // (in one load each where rows begin on 8 bytes: two-byte ones took gate and up of a token 4 us)
+            const size_t at = r * G;
+            if ((G & 3) == 0 && ((reinterpret_cast<uintptr_t>(m[i].s) | reinterpret_cast<uintptr_t>(m[i].b)) & 7) == 0) {
+                s[i] = *reinterpret_cast<const u32x2_t*>(m[i].s + at + g0);
+                b[i] = *reinterpret_cast<const u32x2_t*>(m[i].b + at + g0);
+            } else {
 #pragma unroll
-            for (int k = 0; k < kGroups; ++k) {
-                const size_t at = r * G + min(g0 + k, G - 1);
-                s[i][k] = m[i].s[at];
-                b[i][k] = m[i].b[at];
+                for (int k = 0; k < 2; ++k) {
+                    const size_t g = at + min(g0 + 2 * k, G - 1), h = at + min(g0 + 2 * k + 1, G - 1);
+                    s[i][k] = m[i].s[g] | static_cast<uint32_t>(m[i].s[h]) << 16;
+                    b[i][k] = m[i].b[g] | static_cast<uint32_t>(m[i].b[h]) << 16;
+                }
             }
         }
-#pragma unroll
-        for (int k = 0; k < kGroups; ++k)
-            x[k].load(xp, xrow + 64 * min(g0 + k, G - 1) + 32 * (kg & 1) + 16 * (kg >> 1));
     }
-    __device__ __forceinline__ void add(float (&acc)[MATS], int groups) const {
+    // xs: the wave's own [kTerms][kChunk]
+    __device__ __forceinline__ void add(float (&acc)[MATS], int groups, uint16_t* xs, int lane) const {
         constexpr int T = XCols<X_DT>::kTerms;
+        const int kg = lane >> 4;
         const uint32_t one = q4_one();
         const u32x4_t ones{one, one, one, one};
+        x.split(xs, lane);
         uint32_t words[MATS][kGroups / 2][4];
 #pragma unroll
         for (int i = 0; i < MATS; ++i)
@@ -202,7 +260,9 @@ struct OneStep {
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
                 u32x4_t t[T];
-                x[k].terms(st, t);
+#pragma unroll
+                for (int j = 0; j < T; ++j)
+                    t[j] = *reinterpret_cast<const u32x4_t*>(xs + j * kChunk + 64 * k + 32 * (kg & 1) + 16 * (kg >> 1) + 8 * st);
 #pragma unroll
                 for (int j = T - 1; j >= 0; --j) X = mfma_16x16x32_bf16(t[j], ones, X);
 #pragma unroll
@@ -214,33 +274,35 @@ struct OneStep {
             }
 #pragma unroll
             for (int i = 0; i < MATS; ++i) {
-                const float sc = 16.0f * elem<SB_DT>::load(&s[i][k], 0), bi = elem<SB_DT>::load(&b[i][k], 0);
+                const uint16_t sk = static_cast<uint16_t>(s[i][k / 2] >> (16 * (k & 1)));
+                const uint16_t bk = static_cast<uint16_t>(b[i][k / 2] >> (16 * (k & 1)));
+                const float sc = 16.0f * elem<SB_DT>::load(&sk, 0), bi = elem<SB_DT>::load(&bk, 0);
                 acc[i] = fmaf(sc, P[i][0], fmaf(bi - sc, X[0], acc[i]));
             }
         }
     }
 };
 
-constexpr int kOneWaves = 8;
-
 // Gate and up: one workgroup per (16 rows, pair), its waves over K.
 template <int X_DT, int SB_DT, int H_DT>
 __global__ __launch_bounds__(64 * kOneWaves) void moe_gate_up_one_kernel(MoeArgs p, void* __restrict__ h) {
+    __shared__ __attribute__((aligned(16))) uint16_t xs[kOneWaves][XCols<X_DT>::kTerms * kChunk];
+    __shared__ float red[kOneWaves][2][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, kg = lane >> 4;
-    const int tok = blockIdx.y / p.slots, j = blockIdx.y % p.slots;
+    const int tok = blockIdx.y / p.slots, j = blockIdx.y % p.slots, G = p.cols / 64, row0 = 16 * blockIdx.x;
     const bool shared = j >= p.top;
     const int e = shared ? 0 : p.indices[tok * p.top + j];
+    OneStep<X_DT, SB_DT, 2> st;
+    st.load_x(p.x, static_cast<size_t>(tok) * p.cols, p.cols, kGroups * wave, lane);   // (ahead of the expert's number)
     if (e < 0 || (!shared && e >= p.experts)) return;
     const MoeMat m[2] = {moe_matrix(p.m[0], p.sh[0], shared, e, p.rows, p.cols),
                          moe_matrix(p.m[1], p.sh[1], shared, e, p.rows, p.cols)};
-    const int row0 = 16 * blockIdx.x, G = p.cols / 64;
     float acc[2] = {0.0f, 0.0f};
     for (int g0 = kGroups * wave; g0 < G; g0 += kGroups * kOneWaves) {
-        OneStep<X_DT, SB_DT, 2> st;
-        st.load(m, p.x, static_cast<size_t>(tok) * p.cols, row0 + c, p.cols, g0, kg);
-        st.add(acc, G - g0);
+        st.load_w(m, row0 + c, p.cols, g0, kg);
+        if (g0 != kGroups * wave) st.load_x(p.x, static_cast<size_t>(tok) * p.cols, p.cols, g0, lane);
+        st.add(acc, G - g0, xs[wave], lane);
     }
-    __shared__ float red[kOneWaves][2][16];
     if (lane < 16) {
         red[wave][0][lane] = acc[0];
         red[wave][1][lane] = acc[1];
@@ -263,28 +325,49 @@ template <int X_DT, int SB_DT, int Y_DT>
 __global__ __launch_bounds__(64 * kOneWaves) void moe_down_one_kernel(MoeArgs p, const float* __restrict__ scores,
                                                                       const float* __restrict__ coef, const void* residual,
                                                                       void* y) {
+    __shared__ __attribute__((aligned(16))) uint16_t xs[kOneWaves][XCols<X_DT>::kTerms * kChunk];
+    __shared__ float red[kOneWaves][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, kg = lane >> 4;
     const int tok = blockIdx.y, row0 = 16 * blockIdx.x, G = p.cols / 64, steps = (G + kGroups - 1) / kGroups;
+    const size_t o = static_cast<size_t>(tok) * p.rows + row0 + c;
+    const float res = residual ? elem<Y_DT>::load(residual, o) : 0.0f;
     float acc = 0.0f;
-    for (int it = wave; it < p.slots * steps; it += kOneWaves) {
-        const int j = it / steps, g0 = kGroups * (it - j * steps);
-        const bool shared = j >= p.top;
-        const int e = shared ? 0 : p.indices[tok * p.top + j];
-        if (e < 0 || (!shared && e >= p.experts)) continue;
-        const MoeMat m[1] = {moe_matrix(p.m[0], p.sh[0], shared, e, p.rows, p.cols)};
-        const float f = shared ? (coef ? coef[tok] : 1.0f) : scores[tok * p.top + j];
+    // the next item's loads ahead of an item's products
+    struct Item {
         OneStep<X_DT, SB_DT, 1> st;
-        st.load(m, p.x, (static_cast<size_t>(tok) * p.slots + j) * p.cols, row0 + c, p.cols, g0, kg);
-        float a[1] = {0.0f};
-        st.add(a, G - g0);
-        acc = fmaf(f, a[0], acc);
+        float f;
+        int g0;
+        bool has;
+    };
+    const int items = p.slots * steps;
+    auto fetch = [&](int it, Item& q) {
+        const int j = it / steps;
+        const bool shared = j >= p.top;
+        const int e = it >= items ? -1 : shared ? 0 : p.indices[tok * p.top + j];
+        q.g0 = kGroups * (it - j * steps);
+        q.has = e >= 0 && (shared || e < p.experts);
+        if (!q.has) return;
+        const MoeMat m[1] = {moe_matrix(p.m[0], p.sh[0], shared, e, p.rows, p.cols)};
+        q.f = shared ? (coef ? coef[tok] : 1.0f) : scores[tok * p.top + j];
+        q.st.load_w(m, row0 + c, p.cols, q.g0, kg);
+        q.st.load_x(p.x, (static_cast<size_t>(tok) * p.slots + j) * p.cols, p.cols, q.g0, lane);
+    };
+    Item q;
+    fetch(wave, q);
+    for (int it = wave; it < items; it += kOneWaves) {
+        Item next;
+        fetch(it + kOneWaves, next);
+        if (q.has) {
+            float a[1] = {0.0f};
+            q.st.add(a, G - q.g0, xs[wave], lane);
+            acc = fmaf(q.f, a[0], acc);
+        }
+        q = next;
     }
-    __shared__ float red[kOneWaves][16];
     if (lane < 16) red[wave][lane] = acc;
     __syncthreads();
     if (threadIdx.x < 16) {
-        const size_t o = static_cast<size_t>(tok) * p.rows + row0 + threadIdx.x;
-        float a = residual ? elem<Y_DT>::load(residual, o) : 0.0f;
+        float a = res;
 #pragma unroll
         for (int w = 0; w < kOneWaves; ++w) a += red[w][threadIdx.x];
         elem<Y_DT>::store(y, o, a);
