@@ -144,9 +144,9 @@ inline size_t moe_part_bytes(const qff_ctx_cfg& cfg) {
     return most > one ? most : one;
 }
 
-// Tiles of 32 pairs or more of any call: every expert's last one may be smaller.
+// Tiles of any call, of 8 pairs or more: every expert's last one may be smaller.
 inline size_t moe_tiles(const qff_ctx_cfg& cfg) {
-    return static_cast<size_t>(moe_tokens(cfg)) * (kMoeMaxTop + 1) / 32 + kMoeMaxExperts + 2;
+    return static_cast<size_t>(moe_tokens(cfg)) * (kMoeMaxTop + 1) / 8 + kMoeMaxExperts + 2;
 }
 
 struct WorkspaceLayout {

@@ -376,11 +376,10 @@ __global__ __launch_bounds__(64 * kOneWaves) void moe_down_one_kernel(MoeArgs p,
 
 // ---- several tokens of one expert ------------------------------------------------
 
-// Which pairs each expert has, and the tiles of up to `most` (a multiple of 32)
-// that they make: the pairs are counted, the counts summed up and the pairs written
+// Which pairs each expert has, and the tiles of up to `most` that they make: the pairs are counted, the counts summed up and the pairs written
 // expert by expert (in no fixed order within one: a pair's sums do not depend on
-// its place). An expert's tiles share its pairs evenly, in multiples of 32; the
-// shared expert, number `experts`, has every token. Up to kPlanAlone pairs one
+// its place). An expert's tiles share its pairs evenly, in multiples of `unit`
+// (8 to 32); the shared expert, number `experts`, has every token. Up to kPlanAlone pairs one
 // workgroup does it all (6 us at 4000 pairs, 69 at 65536); beyond, a workgroup for
 // each kPlanShare pairs counts its own, and each then sums up those before it.
 constexpr int kPlanThreads = 1024, kPlanShare = 1024, kPlanAlone = 4096;
@@ -398,18 +397,26 @@ __global__ __launch_bounds__(kPlanThreads) void moe_count_kernel(const int32_t* 
     if (t < experts) parts[static_cast<size_t>(blockIdx.x) * experts + t] = cnt[t];
 }
 
-__global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* __restrict__ indices, int experts, int top,
-                                                                int tokens, int shared, int most, const int* __restrict__ parts,
-                                                                int* __restrict__ count, int4* __restrict__ tiles,
-                                                                int* __restrict__ list) {
+struct PlanArgs {
+    const int32_t* indices;
+    int experts, top, tokens, shared, most, unit;
+    const int* parts;   // or null: one workgroup
+    int* count;
+    int4* tiles;
+    int* list;
+};
+__device__ __forceinline__ void moe_plan(const PlanArgs& q, int blocks) {
+    const int32_t* const indices = q.indices;
+    const int* const parts = q.parts;
+    const int experts = q.experts, most = q.most, unit = q.unit;
     __shared__ int cnt[kMoeMaxExperts], at[kMoeMaxExperts], wsum[2][kPlanThreads / 64];
-    const int t = threadIdx.x, n = tokens * top, share = parts ? kPlanShare : n, i0 = blockIdx.x * share, i1 = min(i0 + share, n);
+    const int t = threadIdx.x, n = q.tokens * q.top, share = parts ? kPlanShare : n, i0 = blockIdx.x * share, i1 = min(i0 + share, n);
     int mine = 0;   // pairs of expert t that other workgroups write ahead of this one's
     if (parts) {
         int all = 0;
         if (t < experts) {
 #pragma unroll 8
-            for (int b = 0; b < static_cast<int>(gridDim.x); ++b) {
+            for (int b = 0; b < blocks; ++b) {
                 const int c = parts[static_cast<size_t>(b) * experts + t];
                 all += c;
                 mine += b < static_cast<int>(blockIdx.x) ? c : 0;
@@ -425,7 +432,7 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* _
         }
     }
     __syncthreads();
-    const int own = t < experts ? cnt[t] : t == experts && shared ? tokens : 0;
+    const int own = t < experts ? cnt[t] : t == experts && q.shared ? q.tokens : 0;
     const int own_tiles = (own + most - 1) / most;
     const int incl = wave_inclusive_scan_int(t < experts ? own : 0), incl_tiles = wave_inclusive_scan_int(own_tiles);
     if ((t & 63) == 63) {
@@ -441,176 +448,23 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* _
     if (t < experts) at[t] = before + mine;
     if (blockIdx.x == 0) {
         if (t == experts) {
-            *count = tile + own_tiles;
+            *q.count = tile + own_tiles;
             before = 0;   // (its pairs are the tokens themselves)
         }
         if (own_tiles > 0) {
-            const int each = ((own + own_tiles - 1) / own_tiles + 31) / 32 * 32;
+            const int each = ((own + own_tiles - 1) / own_tiles + unit - 1) / unit * unit;
             // (rounded up, the last tiles may have fewer or none)
             for (int k = 0; k < own_tiles; ++k)
-                tiles[tile + k] = make_int4(t, before + k * each, min(each, max(own - k * each, 0)), 0);
+                q.tiles[tile + k] = make_int4(t, before + k * each, min(each, max(own - k * each, 0)), 0);
         }
     }
     __syncthreads();
     for (int i = i0 + t; i < i1; i += kPlanThreads) {
         const int e = indices[i];
-        if (e >= 0 && e < experts) list[atomicAdd(&at[e], 1)] = pair_code(i / top, i % top);
+        if (e >= 0 && e < experts) q.list[atomicAdd(&at[e], 1)] = pair_code(i / q.top, i % q.top);
     }
 }
-
-constexpr int kRowsWaves = 8;
-constexpr int kRowsTokens = 32;   // tokens of a call at most
-constexpr int kRowsScan = kRowsTokens * kMoeMaxTop;   // whose pairs each workgroup looks through by itself
-
-// 16 RT rows of one expert's matrices against its tokens, 16 at a time: WK waves
-// over K times RT row tiles. Outputs leave through `store(acc.., row, code)`.
-template <int X_DT, int SB_DT, int MATS, int WK>
-struct RowsKernel {
-    static constexpr int kRt = kRowsWaves / WK, kRows = 16 * kRt;
-    static constexpr int kRed = WK * kRt * MATS * 16 * 17;
-
-    template <class Store>
-    static __device__ __forceinline__ void run(const MoeArgs& p, float* lds, Store&& store) {
-        constexpr int T = XCols<X_DT>::kTerms;
-        const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 15, kg = lane >> 4;
-        const int wk = wave % WK, rt = wave / WK;
-        const int e = blockIdx.y;
-        const bool shared = e >= p.experts;
-        const int G = p.cols / 64, row0 = kRows * blockIdx.x;
-
-        __shared__ int list[kRowsScan], found;
-        int n;
-        if (shared) {
-            n = p.tokens;
-        } else {
-            if (t == 0) found = 0;
-            __syncthreads();
-            for (int i = t; i < p.tokens * p.top; i += 64 * kRowsWaves)
-                if (p.indices[i] == e) list[atomicAdd(&found, 1)] = pair_code(i / p.top, i % p.top);
-            __syncthreads();
-            n = found;
-        }
-        if (n == 0) return;
-
-        float* const scl = lds;                              // [MATS][G][kRows] 16 s
-        float* const bil = lds + MATS * G * kRows;           // [MATS][G][kRows] b - 16 s
-        float* const red = lds + 2 * MATS * G * kRows;       // [WK][kRt][MATS][16 tokens][17]
-        MoeMat m[MATS];
-#pragma unroll
-        for (int i = 0; i < MATS; ++i) {
-            m[i] = moe_matrix(p.m[i], p.sh[i], shared, e, p.rows, p.cols);
-            const size_t base = static_cast<size_t>(row0) * G;
-            for (int k = t; k < kRows * G; k += 64 * kRowsWaves) {
-                const int r = k / G, g = k - r * G;
-                const size_t at = min(base + k, static_cast<size_t>(p.rows) * G - 1);
-                const float s = 16.0f * elem<SB_DT>::load(m[i].s, at), b = elem<SB_DT>::load(m[i].b, at);
-                scl[(i * G + g) * kRows + r] = s;
-                bil[(i * G + g) * kRows + r] = b - s;
-            }
-        }
-        const int wrow = min(row0 + 16 * rt + c, p.rows - 1);
-        __syncthreads();
-
-        for (int t0 = 0; t0 < n; t0 += 16) {
-            const int place = min(t0 + c, n - 1);
-            const int code = shared ? pair_code(place, p.top) : list[place];
-            const size_t xrow = MATS == 2 ? static_cast<size_t>(code >> 5) * p.cols
-                                          : (static_cast<size_t>(code >> 5) * p.slots + (code & 31)) * p.cols;
-            f32x4_t acc[MATS];
-#pragma unroll
-            for (int i = 0; i < MATS; ++i) acc[i] = f32x4_t{};
-            for (int g0 = kGroups * wk; g0 < G; g0 += kGroups * WK) {
-                u32x4_t w[MATS][kGroups / 2];
-#pragma unroll
-                for (int i = 0; i < MATS; ++i)
-#pragma unroll
-                    for (int sp = 0; sp < kGroups / 2; ++sp)
-                        w[i][sp] = *reinterpret_cast<const u32x4_t*>(
-                            m[i].w + static_cast<size_t>(wrow) * (p.cols / 8) + 8 * min(g0 + 2 * sp + (kg >> 1), G - 1) +
-                            4 * (kg & 1));
-                XCols<X_DT> x[kGroups];
-#pragma unroll
-                for (int k = 0; k < kGroups; ++k)
-                    x[k].load(p.x, xrow + 64 * min(g0 + k, G - 1) + 32 * (kg & 1) + 16 * (kg >> 1));
-                const uint32_t one = q4_one();
-                const u32x4_t ones{one, one, one, one};
-                uint32_t words[MATS][kGroups / 2][4];
-#pragma unroll
-                for (int i = 0; i < MATS; ++i)
-#pragma unroll
-                    for (int sp = 0; sp < kGroups / 2; ++sp) span_words(w[i][sp], words[i][sp]);
-#pragma unroll
-                for (int k = 0; k < kGroups; ++k) {
-                    if (g0 + k >= G) break;
-                    f32x4_t P[MATS], X{};
-#pragma unroll
-                    for (int i = 0; i < MATS; ++i) P[i] = f32x4_t{};
-#pragma unroll
-                    for (int st = 0; st < 2; ++st) {
-                        u32x4_t tm[T];
-                        x[k].terms(st, tm);
-#pragma unroll
-                        for (int j = T - 1; j >= 0; --j) X = mfma_16x16x32_bf16(ones, tm[j], X);
-#pragma unroll
-                        for (int i = 0; i < MATS; ++i) {
-                            const u32x4_t q = q4_to_bf16(words[i][k / 2][2 * (k % 2) + st], one);
-#pragma unroll
-                            for (int j = T - 1; j >= 0; --j) P[i] = mfma_16x16x32_bf16(q, tm[j], P[i]);
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < MATS; ++i) {
-                        const int at = (i * G + g0 + k) * kRows + 16 * rt + 4 * kg;
-                        const f32x4_t s = *reinterpret_cast<const f32x4_t*>(scl + at);
-                        const f32x4_t b = *reinterpret_cast<const f32x4_t*>(bil + at);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) acc[i][r] = fmaf(s[r], P[i][r], fmaf(b[r], X[r], acc[i][r]));
-                    }
-                }
-            }
-            if (t0) __syncthreads();   // the tile before has been read
-#pragma unroll
-            for (int i = 0; i < MATS; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) red[(((wk * kRt + rt) * MATS + i) * 16 + c) * 17 + 4 * kg + r] = acc[i][r];
-            __syncthreads();
-            for (int k = t; k < 256 * kRt; k += 64 * kRowsWaves) {
-                const int r = k % 16, tok = k / 16 % 16, tile = k / 256, row = row0 + 16 * tile + r;
-                if (t0 + tok >= n || row >= p.rows) continue;
-                float v[MATS];
-#pragma unroll
-                for (int i = 0; i < MATS; ++i) {
-                    v[i] = 0.0f;
-#pragma unroll
-                    for (int q = 0; q < WK; ++q) v[i] += red[(((q * kRt + tile) * MATS + i) * 16 + tok) * 17 + r];
-                }
-                store(v, row, shared ? pair_code(t0 + tok, p.top) : list[t0 + tok]);
-            }
-        }
-    }
-};
-
-template <int X_DT, int SB_DT, int H_DT, int WK>
-__global__ __launch_bounds__(64 * kRowsWaves) void moe_gate_up_rows_kernel(MoeArgs p, void* __restrict__ h) {
-    extern __shared__ __attribute__((aligned(16))) float lds[];
-    RowsKernel<X_DT, SB_DT, 2, WK>::run(p, lds, [&](const float (&v)[2], int row, int code) {
-        const size_t o = (static_cast<size_t>(code >> 5) * p.slots + (code & 31)) * p.rows + row;
-        elem<H_DT>::store(h, o, silu(v[0]) * v[1]);
-    });
-}
-
-// The weighted row of each pair, for moe_combine_kernel.
-template <int X_DT, int SB_DT, int WK>
-__global__ __launch_bounds__(64 * kRowsWaves) void moe_down_rows_kernel(MoeArgs p, const float* __restrict__ scores,
-                                                                        const float* __restrict__ coef,
-                                                                        float* __restrict__ part) {
-    extern __shared__ __attribute__((aligned(16))) float lds[];
-    RowsKernel<X_DT, SB_DT, 1, WK>::run(p, lds, [&](const float (&v)[1], int row, int code) {
-        const int m = code >> 5, j = code & 31;
-        const float f = j < p.top ? scores[m * p.top + j] : coef ? coef[m] : 1.0f;
-        part[(static_cast<size_t>(m) * p.slots + j) * p.rows + row] = f * v[0];
-    });
-}
+__global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(PlanArgs q) { moe_plan(q, gridDim.x); }
 
 // y[m] = residual[m] + the rows of its pairs, in their order.
 template <int Y_DT>
@@ -636,8 +490,7 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const float* __restric
 
 // ---- many tokens ------------------------------------------------------------------
 //
-// From 33 tokens on: the plan's tiles against the matrices on 32x32x16 fp16
-// products. A weight is s q + b = s (q - 8) + (b + 8 s); its first part is exact
+// The plan's tiles against the matrices on 32x32x16 fp16 products. A weight is s q + b = s (q - 8) + (b + 8 s); its first part is exact
 // in fp16 where the scale has 8 significant bits (bf16): q - 8 is a power of two
 // or has three bits. The nibble becomes 16 + q (its bits are the top ones of the
 // mantissa), one packed FMA (16 + q) s - 24 s gives the product without a rounding,
@@ -660,11 +513,9 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const float* __restric
 constexpr int kX16Waves = 4;
 constexpr int kSumsPad = 16;
 template <int X_DT, int XT, bool COPY>
-__global__ __launch_bounds__(64 * kX16Waves) void moe_x16_kernel(const void* __restrict__ x, uint16_t* __restrict__ x16,
-                                                                 float2* __restrict__ fac, uint16_t* __restrict__ sums,
-                                                                 int cols, int rows) {
-    const int lane = threadIdx.x & 63, row = blockIdx.x * kX16Waves + (threadIdx.x >> 6), nb = cols / 8;
-    if (row >= rows) return;
+__device__ __forceinline__ void moe_x16(const void* __restrict__ x, uint16_t* __restrict__ x16, float2* __restrict__ fac,
+                                        uint16_t* __restrict__ sums, int cols, int row) {
+    const int lane = threadIdx.x & 63, nb = cols / 8;
     constexpr int kMax = 8;   // 8-column blocks of a lane: cols <= 4096
     float v[kMax][8], s[kMax];
     float mx = 0.0f, ms = 0.0f;
@@ -735,6 +586,23 @@ __global__ __launch_bounds__(64 * kX16Waves) void moe_x16_kernel(const void* __r
             if constexpr (XT == 2) *reinterpret_cast<u32x4_t*>(o + cols) = l;
         }
     }
+}
+template <int X_DT, int XT, bool COPY>
+__global__ __launch_bounds__(64 * kX16Waves) void moe_x16_kernel(const void* __restrict__ x, uint16_t* __restrict__ x16,
+                                                                 float2* __restrict__ fac, uint16_t* __restrict__ sums,
+                                                                 int cols, int rows) {
+    const int row = blockIdx.x * kX16Waves + (threadIdx.x >> 6);
+    if (row < rows) moe_x16<X_DT, XT, COPY>(x, x16, fac, sums, cols, row);
+}
+// The same and a plan of one workgroup in one launch (a launch less is 6 us of 60
+// at 32 tokens).
+template <int X_DT, int XT, bool COPY>
+__global__ __launch_bounds__(kPlanThreads) void moe_prepare_kernel(PlanArgs q, const void* __restrict__ x, uint16_t* __restrict__ x16,
+                                                                   float2* __restrict__ fac, uint16_t* __restrict__ sums,
+                                                                   int cols, int rows) {
+    if (blockIdx.x == 0) return moe_plan(q, 1);
+    const int row = (blockIdx.x - 1) * (kPlanThreads / 64) + (threadIdx.x >> 6);
+    if (row < rows) moe_x16<X_DT, XT, COPY>(x, x16, fac, sums, cols, row);
 }
 
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
@@ -841,9 +709,7 @@ __device__ __forceinline__ int tile_row(const MoeArgs& p, int row0) {
     return min(MATS == 2 ? row0 + 32 * (t >> 6) + (t & 31) : row0 + t, p.rows - 1);
 }
 template <int SB_DT>
-__device__ __forceinline__ void put_terms(uint16_t* to, int k, const u32x4_t& s8, const u32x4_t& b8) {
-    const int t = threadIdx.x;
-    u32x4_t bh, bl;
+__device__ __forceinline__ void const_terms(const u32x4_t& s8, const u32x4_t& b8, u32x4_t& bh, u32x4_t& bl) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         float v[2];
@@ -857,6 +723,12 @@ __device__ __forceinline__ void put_terms(uint16_t* to, int k, const u32x4_t& s8
         bh[j] = hi;
         bl[j] = lo;
     }
+}
+template <int SB_DT>
+__device__ __forceinline__ void put_terms(uint16_t* to, int k, const u32x4_t& s8, const u32x4_t& b8) {
+    const int t = threadIdx.x;
+    u32x4_t bh, bl;
+    const_terms<SB_DT>(s8, b8, bh, bl);
     uint16_t* o = to + k / 16 * 32 * kTileRows + 16 * t + 8 * ((k / 8 & 1) ^ (t >> 2 & 1));
     *reinterpret_cast<u32x4_t*>(o) = bh;
     *reinterpret_cast<u32x4_t*>(o + 16 * kTileRows) = bl;
@@ -1032,7 +904,7 @@ __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, co
                     for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
                         for (int mt = 0; mt < NMT; ++mt) {
-                            if (x == 1 && k == 1) continue;   // (2^-19 of the product's 2^-22 part)
+                            if (x == 1 && k == 1) continue;   // (the rest of a scale's eight bits by the rest of x: 2^-19 of the product)
                             acc[rt][mt] = mfma_32x32x16_f16(A[ks & 1][rt][k], B[ks & 1][mt][x], acc[rt][mt]);
                         }
             if (ks < 3) {
@@ -1237,6 +1109,207 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     tile_kernel<1, SB_DT, XT, WT, NATURAL, MMT>(p, a, DownOut<HALF>{p, scores, coef, part, exps});
 }
 
+// ---- few pairs an expert ---------------------------------------------------------
+//
+// Where experts have a handful of pairs each, the weights' bytes bound a call, and
+// the tiles above keep too few of them on their way. So the same operands in
+// workgroups of 128 weight rows (of gate and up 64 of each), four waves of two row
+// tiles, on 16x16x32 products; their 16 columns are 16 pairs, or 8 pairs by their
+// two terms. A stage is four groups, 128 bytes of each row of words and so whole
+// cache lines; three stages, 72 KB. Lane (c, kg) holds row c of a row tile and 32
+// consecutive columns kg of each 128, with their group's scale: k slots may stand
+// for any columns as long as both operands agree. The groups' constant parts are products whose
+// k slots are 32 groups, formed from the scales and biases that the lane loads and
+// leaves in LDS.
+constexpr int kSlimRows = 128, kSlimColumns = 16, kSlimStages = 3;
+constexpr int kSlimWords = kSlimRows * 128, kSlimStage = kSlimWords + kSlimColumns * 512;
+
+template <int MATS, int SB_DT, int XT, int WT, bool NATURAL, class Store>
+__device__ __forceinline__ void slim_kernel(const MoeArgs& p, const TileArgs& a, const Store& store) {
+    constexpr bool kExact = SB_DT == 1 || WT == 2;
+    constexpr int NS = kSlimStages, kOwn = kSlimRows / MATS, kPairs = kSlimColumns / XT;
+    __shared__ __attribute__((aligned(16))) char buf[NS * kSlimStage];
+    extern __shared__ __attribute__((aligned(16))) char sbl_bytes[];   // [groups in whole eights][128]
+    tile_sb<WT>* const sbl = reinterpret_cast<tile_sb<WT>*>(sbl_bytes);
+    const int blocks = (p.rows + kOwn - 1) / kOwn, item = blockIdx.x / blocks;
+    if (item >= *a.count) return;
+    const int4 tile = a.tiles[item];
+    if (tile.z == 0) return;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 15, kg = lane >> 4, G = p.cols / 64, steps = (G + 3) / 4;
+    const bool shared = tile.x >= p.experts;
+    const MoeMat m0 = moe_matrix(p.m[0], p.sh[0], shared, tile.x, p.rows, p.cols);
+    const MoeMat m1 = MATS == 2 ? moe_matrix(p.m[1], p.sh[1], shared, tile.x, p.rows, p.cols) : m0;
+    // the wave's rows: 16 of each of two matrices, or 32 (past the end: the last ones, whose results are left)
+    const int row0 = kOwn * (blockIdx.x % blocks), own = row0 + kOwn / 4 * wave, first = min(own, p.rows - kOwn / 4);
+    auto pair = [&](int col) {
+        const int k = min(col & (kPairs - 1), tile.z - 1);
+        return shared ? pair_code(tile.y + k, p.top) : a.list[tile.y + k];
+    };
+    auto x_row = [&](int code) { return static_cast<uint32_t>(MATS == 2 ? code >> 5 : (code >> 5) * p.slots + (code & 31)); };
+
+    // Copies of words: 8 rows each, lane l the piece of 16 bytes (l & 7) ^ row of row l >> 3; of x: two columns each, a
+    // column's 8-element blocks b at b ^ (column & 7). Past the last column, its last block again (the scales there are zeros).
+    const uint32_t lds = lds_addr(reinterpret_cast<const uint16_t*>(buf)), rbytes = p.cols / 2;
+    const uint32_t wrow = (first + (lane >> 3)) * rbytes, wpiece = 16 * ((lane & 7) ^ (lane >> 3));
+    uint32_t xrow[2], xblock[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int col = 4 * wave + 2 * i + (lane >> 5);
+        xrow[i] = (x_row(pair(col)) * XT + col / kPairs) * p.cols * 2;
+        xblock[i] = 16 * ((lane & 31) ^ (col & 7));
+    }
+    auto stage = [&](int to, int g) {
+        const uint32_t at = lds + to * kSlimStage, w = wrow + min(wpiece + 128 * g, rbytes - 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            dma16(reinterpret_cast<const char*>(MATS == 2 && i >= 2 ? m1.w : m0.w) + static_cast<size_t>(8 * (MATS == 2 ? i & 1 : i)) * rbytes,
+                  w, at + (4 * wave + i) * 1024);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            dma16(reinterpret_cast<const char*>(a.x16), xrow[i] + min(xblock[i] + 512u * g, 4 * rbytes - 16),
+                  at + kSlimWords + (2 * wave + i) * 1024);
+    };
+    uint32_t k16 = 0x4C004C00u;
+    asm("" : "+v"(k16));
+
+    f32x4_t acc[2] = {};
+    const int code = pair(c);
+    float2 fac = a.fac[x_row(code)];
+    fac.x *= store.weight(code);
+    {
+        const int gp = (G + kSumsPad - 1) / kSumsPad * kSumsPad;
+        const uint16_t* const S = a.sums + static_cast<size_t>(x_row(code)) * 2 * gp;
+        const bool vec = sb_vec(m0, G) && sb_vec(m1, G);
+        for (int k0 = 0; k0 < G; k0 += 32) {
+            const int k = k0 + 8 * kg;
+            u32x4_t xh{}, xl{}, s8[2], b8[2];
+            if (k < gp) {   // (16 pairs: both terms of their sums; 8: each column its own)
+                xh = *reinterpret_cast<const u32x4_t*>(S + k + c / kPairs * gp);
+                if constexpr (XT == 1) xl = *reinterpret_cast<const u32x4_t*>(S + gp + k);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const MoeMat& mm = MATS == 2 && j ? m1 : m0;
+                const size_t at = static_cast<size_t>(first + (MATS == 2 ? 0 : 16 * j) + c) * G;
+                s8[j] = load_u16x8(mm.s + at, k, G, vec);
+                b8[j] = load_u16x8(mm.b + at, k, G, vec);
+            }
+            if (k0 == 0) {
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < NS - 1; ++i)
+                    if (i < steps) stage(i, i);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                if (k < G) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        sbl[(k + i) * kSlimRows + 32 * wave + 16 * j + c] =
+                            k + i < G ? tile_scale<SB_DT, WT>(static_cast<uint16_t>(s8[j][i / 2] >> (16 * (i & 1)))) : 0;
+                }
+                u32x4_t bh, bl;
+                const_terms<SB_DT>(s8[j], b8[j], bh, bl);
+                acc[j] = mfma_16x16x32_f16(bl, xh, acc[j]);
+                if constexpr (XT == 1) acc[j] = mfma_16x16x32_f16(bh, xl, acc[j]);
+                acc[j] = mfma_16x16x32_f16(bh, xh, acc[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[j] *= fac.y;
+    }
+
+    constexpr int kPer = 6;
+    auto step = [&](auto st, int g) {
+        constexpr int s = decltype(st)::value;
+        __builtin_amdgcn_sched_barrier(0);
+        if (g + NS - 2 < steps) meet<(NS - 2) * kPer>();   // (the copies of the step behind may be under way)
+        else meet<0>();
+        if (g + NS - 1 < steps) stage((s + NS - 1) % NS, g + NS - 1);
+        __builtin_amdgcn_sched_barrier(0);
+        const char* const ws = buf + s * kSlimStage + (32 * wave + c) * 128;
+        const char* const xs = buf + s * kSlimStage + kSlimWords + c * 512;
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+            if (4 * g + 2 * d >= G) continue;
+            u32x4_t words[2], B[4];
+            f16x2_t sv[2][WT], cv[2][WT];
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) B[ks] = *reinterpret_cast<const u32x4_t*>(xs + 16 * ((16 * d + 4 * kg + ks) ^ (c & 7)));
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                words[j] = *reinterpret_cast<const u32x4_t*>(ws + 16 * j * 128 + 16 * ((4 * d + kg) ^ (c & 7)));
+                const uint32_t sc = sbl[(4 * g + 2 * d + (kg >> 1)) * kSlimRows + 32 * wave + 16 * j + c];
+#pragma unroll
+                for (int q = 0; q < WT; ++q) {
+                    const uint32_t one = sc >> (16 * q) & 0xffffu;
+                    sv[j][q] = __builtin_bit_cast(f16x2_t, one | one << 16);
+                    cv[j][q] = sv[j][q] * f16x2_t{static_cast<_Float16>(-24.0f), static_cast<_Float16>(-24.0f)};
+                }
+            }
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int q = WT - 1; q >= 0; --q)
+                        acc[j] = mfma_16x16x32_f16(q4_to_f16<kExact, NATURAL>(words[j][ks], sv[j][q], cv[j][q], k16), B[ks], acc[j]);
+        }
+    };
+    for (int g = 0; g < steps; g += NS) unroll<NS>([&](auto i) {
+        if (g + i.value < steps) step(i, g + i.value);
+    });
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (XT == 2) acc[j][i] += __shfl_xor(acc[j][i], 8);
+            acc[j][i] *= fac.x;
+        }
+    if (c < kPairs && c < tile.z && own < p.rows) store(acc, own + 4 * kg, code);
+}
+
+// A lane's rows 4 kg .. + 3 of its wave's two row tiles, for its pair.
+template <int H_DT>
+struct SlimUp {
+    const MoeArgs& p;
+    void* h;
+    __device__ __forceinline__ float weight(int) const { return 1.0f; }
+    __device__ __forceinline__ void operator()(const f32x4_t (&acc)[2], int row, int code) const {
+        f32x4_t v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = silu(acc[0][i]) * acc[1][i];
+        put4<H_DT>(static_cast<char*>(h) + (static_cast<size_t>(code >> 5) * p.slots + (code & 31)) * p.rows * (H_DT == 0 ? 4 : 2), row, v);
+    }
+};
+template <int SB_DT, int XT, int WT, int H_DT>
+__global__ __launch_bounds__(256) void moe_gate_up_slim_kernel(MoeArgs p, TileArgs a, void* __restrict__ h) {
+    slim_kernel<2, SB_DT, XT, WT, false>(p, a, SlimUp<H_DT>{p, h});
+}
+
+// The pairs' weighted rows, for moe_combine_kernel.
+struct SlimDown {
+    const MoeArgs& p;
+    const float* scores;
+    const float* coef;
+    float* part;
+    __device__ __forceinline__ float weight(int code) const {
+        const int m = code >> 5, s = code & 31;
+        return s < p.top ? scores[m * p.top + s] : coef ? coef[m] : 1.0f;
+    }
+    __device__ __forceinline__ void operator()(const f32x4_t (&acc)[2], int row, int code) const {
+        float* const to = part + (static_cast<size_t>(code >> 5) * p.slots + (code & 31)) * p.rows + row;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) *reinterpret_cast<f32x4_t*>(to + 16 * j) = acc[j];
+    }
+};
+template <int SB_DT, int XT, int WT, bool NATURAL>
+__global__ __launch_bounds__(256) void moe_down_slim_kernel(MoeArgs p, TileArgs a, const float* __restrict__ scores,
+                                                            const float* __restrict__ coef, float* __restrict__ part) {
+    slim_kernel<1, SB_DT, XT, WT, NATURAL>(p, a, SlimDown{p, scores, coef, part});
+}
+
 // y[m] = residual[m] + the rows of its pairs, in their order: a thread 8 columns.
 template <int Y_DT>
 __global__ __launch_bounds__(256) void moe_combine_half_kernel(const uint16_t* __restrict__ part, const float* __restrict__ exps,
@@ -1268,9 +1341,20 @@ MoeMat moe_mat(const qff_q4_matrices& q) {
     return MoeMat{q.w, static_cast<const uint16_t*>(q.scales), static_cast<const uint16_t*>(q.biases)};
 }
 
-// Pairs up to which each is a workgroup row of its own (their weights are read
-// for each pair).
-constexpr int kOnePairs = 36;
+// Pairs (with the shared expert's) up to which each takes its weights by itself, and
+// pairs an expert (for gate and up: by the terms of x) up to which the small tiles take them; up to
+// 32 tokens they always do, so the large ones have bf16 outputs of fewer terms alone.
+// Measured with 256 experts of 512 x 2048 and a shared one, 8 a token, us a call with what
+// stands ahead of and behind the products:
+//   gate and up, pairs   72   108   144       an expert   0.5    2    6    8 (fp32 x)    8   12   16 (bf16 x)
+//     by themselves    29.2  41.5  52.8
+//     small tiles      27.9    -   42.0                  49    79  100  118             91   99  118
+//     large tiles        -     -     -                   62    94  118  120            104  109  114
+//   down, pairs         144   216   288       an expert    1    2    4    6 (fp32 h)    2    4    6 (fp16 h, bf16 y)
+//     by themselves    34.2  47.8  61.5
+//     small tiles      39.9  45.8  50.7                  50.7 62.2 68   78              62   68   71
+//     large tiles        -     -     -                  53.6 65   68   73              64   65   70
+constexpr int kOneUp = 72, kOneDown = 200, kSlimUp = 14, kSlimDown = 2;
 
 template <int DT>
 using Dt = std::integral_constant<int, DT>;
@@ -1295,12 +1379,13 @@ void with_sb(qff_dtype d, F&& f) {
 
 size_t dtype_size(qff_dtype d) { return d == QFF_F32 ? 4 : 2; }
 
-// A call's rows in the tiles' operand form and the plan of its pairs.
 struct Terms {
     int x, w;   // fp16 terms of x and of a weight
 };
-Terms tile_terms(qff_dtype x, qff_dtype sb, qff_dtype out) {
-    return {x == QFF_F32 && out != QFF_BF16 ? 2 : 1, sb == QFF_F16 && out != QFF_BF16 ? 2 : 1};
+// (bf16 outputs of up to 32 tokens have all terms too)
+Terms tile_terms(qff_dtype x, qff_dtype sb, qff_dtype out, int tokens) {
+    const bool all = out != QFF_BF16 || tokens <= 32;
+    return {x == QFF_F32 && all ? 2 : 1, sb == QFF_F16 && all ? 2 : 1};
 }
 // Tokens of a tile, in units of 32: as many as an expert has on average, within
 // what fits the registers and LDS.
@@ -1309,35 +1394,41 @@ int tile_units(int pairs, int experts, int xt) {
     return xt == 1 && avg > 48 ? 4 : avg > 24 ? 2 : 1;
 }
 
-hipError_t moe_plan(qff_ctx* ctx, hipStream_t stream, const MoeArgs& p, bool shared, int units) {
+// What the tiles read: `rows` rows of p.x as fp16 terms, factors and sums (fp16 x
+// stays where it is), and the plan of up to `most` pairs a tile.
+TileArgs moe_prepare(qff_ctx* ctx, hipStream_t stream, const MoeArgs& p, bool shared, qff_dtype dtype, int xt, int rows, int most,
+                     int unit) {
     const int n = p.tokens * p.top, blocks = n > kPlanAlone ? (n + kPlanShare - 1) / kPlanShare : 1;
-    int* parts = blocks > 1 ? ctx->moe_parts : nullptr;
-    if (parts) {
-        ProfScope prof(ctx, stream, "moe_count");
-        moe_count_kernel<<<blocks, kPlanThreads, 0, stream>>>(p.indices, p.experts, n, parts);
-    }
-    ProfScope prof(ctx, stream, "moe_plan");
-    moe_plan_kernel<<<blocks, kPlanThreads, 0, stream>>>(p.indices, p.experts, p.top, p.tokens, shared, 32 * units, parts,
-                                                         ctx->moe_off, static_cast<int4*>(ctx->moe_tiles), ctx->moe_list);
-    return hipGetLastError();
-}
-
-// x as fp16 terms, factors and sums of `rows` rows; fp16 x stays where it is.
-void moe_x16(qff_ctx* ctx, hipStream_t stream, const void* x, qff_dtype dtype, int xt, int cols, int rows, TileArgs& a) {
-    ProfScope prof(ctx, stream, "moe_x16");
     float2* fac = reinterpret_cast<float2*>(ctx->moe_xs);
     uint16_t* sums = reinterpret_cast<uint16_t*>(fac + (rows + 1) / 2 * 2);   // (16-byte aligned)
-    const int grid = (rows + kX16Waves - 1) / kX16Waves;
-#define QFF_X16(X, XT, COPY) \
-    moe_x16_kernel<X, XT, COPY><<<grid, 64 * kX16Waves, 0, stream>>>(x, ctx->q4_x16, fac, sums, cols, rows)
-    if (dtype == QFF_F16) QFF_X16(2, 1, false);
-    else if (dtype == QFF_BF16) QFF_X16(1, 1, true);
-    else if (xt == 1) QFF_X16(0, 1, true);
-    else QFF_X16(0, 2, true);
-#undef QFF_X16
-    a.x16 = dtype == QFF_F16 ? static_cast<const uint16_t*>(x) : ctx->q4_x16;
-    a.fac = fac;
-    a.sums = sums;
+    const PlanArgs q{p.indices, p.experts, p.top, p.tokens, shared, most, unit, blocks > 1 ? ctx->moe_parts : nullptr,
+                     ctx->moe_off, static_cast<int4*>(ctx->moe_tiles), ctx->moe_list};
+    auto x16 = [&](auto X, auto XT, auto COPY) {
+        if (blocks == 1) {
+            ProfScope prof(ctx, stream, "moe_prepare");
+            constexpr int kRows = kPlanThreads / 64;
+            moe_prepare_kernel<X.value, XT.value, COPY.value><<<1 + (rows + kRows - 1) / kRows, kPlanThreads, 0, stream>>>(
+                q, p.x, ctx->q4_x16, fac, sums, p.cols, rows);
+        } else {
+            ProfScope prof(ctx, stream, "moe_x16");
+            moe_x16_kernel<X.value, XT.value, COPY.value><<<(rows + kX16Waves - 1) / kX16Waves, 64 * kX16Waves, 0, stream>>>(
+                p.x, ctx->q4_x16, fac, sums, p.cols, rows);
+        }
+    };
+    if (dtype == QFF_F16) x16(Dt<2>{}, Dt<1>{}, Dt<0>{});
+    else if (dtype == QFF_BF16) x16(Dt<1>{}, Dt<1>{}, Dt<1>{});
+    else if (xt == 1) x16(Dt<0>{}, Dt<1>{}, Dt<1>{});
+    else x16(Dt<0>{}, Dt<2>{}, Dt<1>{});
+    if (blocks > 1) {
+        {
+            ProfScope prof(ctx, stream, "moe_count");
+            moe_count_kernel<<<blocks, kPlanThreads, 0, stream>>>(p.indices, p.experts, n, ctx->moe_parts);
+        }
+        ProfScope prof(ctx, stream, "moe_plan");
+        moe_plan_kernel<<<blocks, kPlanThreads, 0, stream>>>(q);
+    }
+    return {ctx->moe_off, static_cast<const int4*>(ctx->moe_tiles), ctx->moe_list,
+            dtype == QFF_F16 ? static_cast<const uint16_t*>(p.x) : ctx->q4_x16, fac, sums};
 }
 
 // Tokens of a slice whose `rows` rows of x each fit the workspace.
@@ -1349,6 +1440,11 @@ int slice_tokens(const qff_ctx* ctx, int rows, int cols, int xt, bool copy, int 
     return static_cast<int>(std::min(most, (moe_part_bytes(ctx->cfg) / 16 - 8) / (rows * row)));
 }
 
+unsigned slim_grid(const MoeArgs& p, bool shared, int xt, int own_rows) {
+    const int most = kSlimColumns / xt, pairs = p.tokens * p.top;
+    const unsigned tiles = pairs / most + std::min(p.experts, pairs) + (shared ? (p.tokens + most - 1) / most : 0);
+    return tiles * ((p.rows + own_rows - 1) / own_rows);
+}
 unsigned tile_grid(const MoeArgs& p, bool shared, int units, int own_rows) {
     const int most = 32 * units, pairs = p.tokens * p.top;
     const int tiles = pairs / most + std::min(p.experts, pairs) + (shared ? (p.tokens + most - 1) / most : 0);
@@ -1384,7 +1480,7 @@ hipError_t launch_moe_gate_up(qff_ctx* ctx, hipStream_t stream, const qff_moe_we
     p.cols = w->hidden;
     p.tokens = tokens;
     const int G = p.cols / 64;
-    if (tokens * p.slots <= kOnePairs) {
+    if (tokens * p.slots <= kOneUp) {
         ProfScope prof(ctx, stream, "moe_gate_up_one");
         const dim3 grid(p.rows / 16, tokens * p.slots);
         with_io(x_dtype, [&](auto X) {
@@ -1396,38 +1492,36 @@ hipError_t launch_moe_gate_up(qff_ctx* ctx, hipStream_t stream, const qff_moe_we
         });
         return hipGetLastError();
     }
-    if (tokens <= kRowsTokens) {
-        ProfScope prof(ctx, stream, "moe_gate_up_rows");
-        auto launch = [&](auto X, auto S, auto H, auto K) {
-            using R = RowsKernel<X.value, S.value, 2, K.value>;
-            const dim3 grid((p.rows + R::kRows - 1) / R::kRows, p.experts + shared);
-            const size_t lds = (4 * static_cast<size_t>(G) * R::kRows + R::kRed) * sizeof(float);
-            moe_gate_up_rows_kernel<X.value, S.value, H.value, K.value><<<grid, 64 * kRowsWaves, lds, stream>>>(p, h);
-        };
-        with_io(x_dtype, [&](auto X) {
-            with_sb(w->sb_dtype, [&](auto S) {
-                with_dtype(h_dtype, [&](auto H) {
-                    if (G <= 8) launch(X, S, H, Dt<2>{});
-                    else launch(X, S, H, Dt<8>{});
-                });
-            });
-        });
-        return hipGetLastError();
-    }
-    const Terms tm = tile_terms(x_dtype, w->sb_dtype, h_dtype);
+    const Terms tm = tile_terms(x_dtype, w->sb_dtype, h_dtype, tokens);
     const int most = slice_tokens(ctx, 1, p.cols, tm.x, true, tokens);
     const size_t lds = static_cast<size_t>((G + 7) / 8 * 8) * kTileRows * 2 * tm.w;
     for (int t0 = 0; t0 < tokens; t0 += most) {
         p.tokens = std::min(most, tokens - t0);
         p.indices = indices + static_cast<size_t>(t0) * top;
-        TileArgs a{ctx->moe_off, static_cast<const int4*>(ctx->moe_tiles), ctx->moe_list, nullptr, nullptr, nullptr};
-        moe_x16(ctx, stream, static_cast<const char*>(x) + static_cast<size_t>(t0) * p.cols * dtype_size(x_dtype), x_dtype, tm.x,
-                p.cols, p.tokens, a);
-        const int units = tile_units(p.tokens * top, p.experts, tm.x);
-        if (const hipError_t e = moe_plan(ctx, stream, p, shared, units)) return e;
+        p.x = static_cast<const char*>(x) + static_cast<size_t>(t0) * p.cols * dtype_size(x_dtype);
+        const bool slim = tokens <= 32 || p.tokens * top * tm.x <= kSlimUp * p.experts;
+        const int units = tile_units(p.tokens * top, p.experts, tm.x), unit = slim ? kSlimColumns / tm.x : 32;
+        const TileArgs a = moe_prepare(ctx, stream, p, shared, x_dtype, tm.x, p.tokens, slim ? unit : 32 * units, unit);
+        void* to = static_cast<char*>(h) + static_cast<size_t>(t0) * p.slots * p.rows * dtype_size(h_dtype);
+        if (slim) {
+            ProfScope prof(ctx, stream, "moe_gate_up_slim");
+            const unsigned grid = slim_grid(p, shared, tm.x, kSlimRows / 2);
+            const size_t bytes = static_cast<size_t>((G + 7) / 8 * 8) * kSlimRows * 2 * tm.w;
+            with_sb(w->sb_dtype, [&](auto S) {
+                pick(tm.x, Ints<1, 2>{}, [&](auto XT) {
+                    auto go = [&](auto WT) {
+                        with_dtype(h_dtype, [&](auto H) {
+                            moe_gate_up_slim_kernel<S.value, XT.value, WT.value, H.value><<<grid, 256, bytes, stream>>>(p, a, to);
+                        });
+                    };
+                    if constexpr (S.value == 2) pick(tm.w, Ints<1, 2>{}, go);
+                    else go(Dt<1>{});
+                });
+            });
+            continue;
+        }
         ProfScope prof(ctx, stream, "moe_gate_up_tile");
         const unsigned grid = tile_grid(p, shared, units, kTileRows / 2);
-        void* to = static_cast<char*>(h) + static_cast<size_t>(t0) * p.slots * p.rows * dtype_size(h_dtype);
         auto launch = [&](auto S, auto XT, auto WT, auto H) {
             auto go = [&](auto U) {
                 moe_gate_up_tile_kernel<S.value, XT.value, WT.value, H.value, U.value><<<grid, 256, lds, stream>>>(p, a, to);
@@ -1460,7 +1554,7 @@ hipError_t launch_moe_down(qff_ctx* ctx, hipStream_t stream, const qff_moe_weigh
     p.rows = w->hidden;
     p.cols = w->inter;
     const int G = p.cols / 64;
-    if (tokens * p.slots <= kOnePairs) {
+    if (tokens * p.slots <= kOneDown) {
         p.x = h;
         p.indices = indices;
         p.tokens = tokens;
@@ -1476,12 +1570,12 @@ hipError_t launch_moe_down(qff_ctx* ctx, hipStream_t stream, const qff_moe_weigh
         });
         return hipGetLastError();
     }
-    const bool few = tokens <= kRowsTokens, half = !few && y_dtype == QFF_BF16;
-    const Terms tm = tile_terms(h_dtype, w->sb_dtype, y_dtype);
+    const Terms tm = tile_terms(h_dtype, w->sb_dtype, y_dtype, tokens);
+    const bool slim = tokens <= 32 || tokens * top <= kSlimDown * p.experts, half = !slim && y_dtype == QFF_BF16;
     // as many tokens at a time as the workspace has room for
     const size_t per = static_cast<size_t>(p.slots) * p.rows * (half ? 2 : 4);
     int most = static_cast<int>(std::min<size_t>({ctx->moe_part_bytes / per, static_cast<size_t>(tokens), 65535}));
-    if (!few) most = std::min(most, slice_tokens(ctx, p.slots, p.cols, tm.x, h_dtype != QFF_F16, tokens));
+    most = std::min(most, slice_tokens(ctx, p.slots, p.cols, tm.x, h_dtype != QFF_F16, tokens));
     for (int t0 = 0; t0 < tokens; t0 += most) {
         const int n = std::min(most, tokens - t0);
         p.tokens = n;
@@ -1492,26 +1586,25 @@ hipError_t launch_moe_down(qff_ctx* ctx, hipStream_t stream, const qff_moe_weigh
         const size_t yo = static_cast<size_t>(t0) * p.rows * dtype_size(y_dtype);
         const void* res = residual ? static_cast<const char*>(residual) + yo : nullptr;
         void* to = static_cast<char*>(y) + yo;
-        if (few) {
-            ProfScope prof(ctx, stream, "moe_down_rows");
-            auto launch = [&](auto X, auto S, auto K) {
-                using R = RowsKernel<X.value, S.value, 1, K.value>;
-                const dim3 grid((p.rows + R::kRows - 1) / R::kRows, p.experts + shared);
-                const size_t lds = (2 * static_cast<size_t>(G) * R::kRows + R::kRed) * sizeof(float);
-                moe_down_rows_kernel<X.value, S.value, K.value>
-                    <<<grid, 64 * kRowsWaves, lds, stream>>>(p, sc, cf, static_cast<float*>(ctx->moe_part));
+        const int units = tile_units(n * top, p.experts, tm.x), unit = slim ? kSlimColumns / tm.x : 32;
+        const TileArgs a = moe_prepare(ctx, stream, p, shared, h_dtype, tm.x, n * p.slots, slim ? unit : 32 * units, unit);
+        if (slim) {
+            ProfScope prof(ctx, stream, "moe_down_slim");
+            const unsigned grid = slim_grid(p, shared, tm.x, kSlimRows);
+            const size_t bytes = static_cast<size_t>((G + 7) / 8 * 8) * kSlimRows * 2 * tm.w;
+            auto launch = [&](auto S, auto XT, auto NAT) {
+                auto go = [&](auto WT) {
+                    moe_down_slim_kernel<S.value, XT.value, WT.value, NAT.value>
+                        <<<grid, 256, bytes, stream>>>(p, a, sc, cf, static_cast<float*>(ctx->moe_part));
+                };
+                if constexpr (S.value == 2) pick(tm.w, Ints<1, 2>{}, go);
+                else go(Dt<1>{});
             };
-            with_dtype(h_dtype, [&](auto X) {
-                with_sb(w->sb_dtype, [&](auto S) {
-                    if (G <= 8) launch(X, S, Dt<2>{});
-                    else launch(X, S, Dt<8>{});
-                });
+            with_sb(w->sb_dtype, [&](auto S) {
+                if (h_dtype == QFF_F16) launch(S, Dt<1>{}, Dt<1>{});
+                else pick(tm.x, Ints<1, 2>{}, [&](auto XT) { launch(S, XT, Dt<0>{}); });
             });
         } else {
-            TileArgs a{ctx->moe_off, static_cast<const int4*>(ctx->moe_tiles), ctx->moe_list, nullptr, nullptr, nullptr};
-            moe_x16(ctx, stream, p.x, h_dtype, tm.x, p.cols, n * p.slots, a);
-            const int units = tile_units(n * top, p.experts, tm.x);
-            if (const hipError_t e = moe_plan(ctx, stream, p, shared, units)) return e;
             ProfScope prof(ctx, stream, "moe_down_tile");
             const unsigned grid = tile_grid(p, shared, units, kTileRows);
             const size_t lds = static_cast<size_t>((G + 7) / 8 * 8) * kTileRows * 2 * tm.w;

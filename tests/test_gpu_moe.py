@@ -143,6 +143,22 @@ def test_down(hip, shape, h_dt, y_dt, sb, shared, kind, residual, coef):
     _check_down(_ctx(), w, h, _indices(rng, n, E, top, kind), DT[y_dt], residual, coef, rng)
 
 
+# few pairs an expert: odd numbers of groups, groups that 16-byte loads cannot take, more groups than one product's k slots
+@pytest.mark.parametrize("n,E,top,D,I", [(32, 96, 8, 192, 320), (64, 200, 4, 2112, 64), (48, 128, 9, 4096, 128), (150, 300, 2, 512, 576),
+                                         (32, 3, 3, 64, 64)])
+@pytest.mark.parametrize("x_dt,h_dt,sb,shared,kind", [("f32", "f32", "f16", True, "holes"), ("bf16", "f16", "bf16", False, "any"),
+                                                      ("f32", "bf16", "bf16", True, "one"), ("bf16", "bf16", "f16", True, "none")])
+def test_few_pairs_an_expert(hip, n, E, top, D, I, x_dt, h_dt, sb, shared, kind):
+    print(f"few {n} {E} {top} {D} {I} x={x_dt} h={h_dt} sb={sb} shared={shared} {kind}", flush=True)
+    rng = np.random.default_rng(n + E + D)
+    w = _weights(rng, E, D, I, sb, shared)
+    idx = _indices(rng, n, E, top, kind)
+    x = torch.from_numpy(rng.standard_normal((n, D))).to(DT[x_dt]).to(DEV)
+    _check_gate_up(_ctx(), w, x, idx, DT[h_dt], kind)
+    h = torch.from_numpy(rng.standard_normal((n, top + shared, I))).to(DT[h_dt]).to(DEV)
+    _check_down(_ctx(), w, h, idx, DT[x_dt], "own", True, rng)
+
+
 @pytest.mark.parametrize("n,y_dt", [(50, "f32"), (200, "bf16")])
 def test_down_in_slices(hip, n, y_dt):
     """A context whose workspace holds the rows of a few tokens only."""
