@@ -79,8 +79,8 @@ WorkspaceLayout workspace_layout(const qff_ctx_cfg& cfg) {
     L.moe_part = take(moe_part_bytes(cfg));
     L.moe_exps = take(moe_part_bytes(cfg) / 32);
     L.sm_range = take(B * kSampleChunks * sizeof(float2));
-    L.sm_mass = take(B * kSampleChunks * kSampleBins * sizeof(unsigned long long));
-    L.sm_count = take(B * kSampleChunks * kSampleBins * sizeof(uint32_t));
+    L.sm_mass = take(B * (kSampleChunks + 1) * kSampleBins * sizeof(unsigned long long));
+    L.sm_count = take(B * kSampleBins * sizeof(uint32_t));
     L.sm_cut = take(B * sizeof(SampleCut));
     L.sm_base = take(B * kSampleChunks * sizeof(unsigned long long));
     L.sm_listed = take(B * kSampleChunks * sizeof(int));

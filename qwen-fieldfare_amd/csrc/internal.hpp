@@ -27,7 +27,7 @@ struct qff_dn_bufs {
 };
 
 // Sampling: what its launches hand on, per row of up to kSampleChunks chunks.
-constexpr int kSampleChunks = 64, kSampleBins = 64, kSampleVocab = 262144;
+constexpr int kSampleChunks = 64, kSampleBins = 256, kSampleVocab = 262144;
 struct SampleCut {
     unsigned long long total, mass_before;   // weight of the row, and of the bins before lo
     int count_before;                        // tokens of those
@@ -36,8 +36,8 @@ struct SampleCut {
 };
 struct SampleWork {
     float2* range;                  // [max_batch][chunks] largest, least finite logit
-    unsigned long long* bin_mass;   // [max_batch][chunks][bins]
-    uint32_t* bin_count;            // same
+    unsigned long long* bin_mass;   // [max_batch][chunks + 1][bins], the last the row's
+    uint32_t* bin_count;            // [max_batch][bins]
     SampleCut* cut;                 // [max_batch]
     unsigned long long* base;       // [max_batch][chunks] weight kept of the bins before lo
     int* listed;                    // [max_batch][chunks] tokens listed of the others

@@ -12,15 +12,23 @@
 //
 // Four launches, a row's tokens cut into chunks, a workgroup each:
 //   max     each chunk's largest and least finite logit
-//   bins    each chunk's counts and weights in 64 bins of equal width in l
-//   gather  every chunk adds the bins up, finds the bins [lo, hi] that hold the
+//   bins    each chunk's weights, and the row's weights and counts, in 256 bins of
+//           equal width in l
+//   gather  every chunk finds the row's bins [lo, hi] that hold the
 //           borders of top-k and top-p, and lists its tokens in them in order;
 //           the tokens of the bins before lo are kept
-//   pick    one workgroup a row: the borders among the listed tokens by an
-//           8-bit radix selection over the bits of l (by count, then by weight),
-//           the chunk that u falls into and the token in it
+//   pick    one workgroup a row: the borders among the listed tokens, kept in LDS,
+//           by an 8-bit radix selection over the bits of l in which they differ (by
+//           count, then by weight), the chunk that u falls into, its 64 tokens and
+//           the token there
 // A row is read four times at most (three from the caches: 0.6 MB at 151936
 // logits); rows that need no border or no draw skip what they do not need.
+//
+// At 151936 fp32 logits (a read of all takes 0.1 us a row): one row 36 us, of
+// them max 4, bins 8, gather 7, pick 17; 32 rows with settings of their own
+// 7 + 18 + 18 + 23. What bounds it: the chain of dependent steps, for one row;
+// for 32 also the exponentials, one in 64 bits a token (an exact border needs a weight that
+// does not depend on who computes it), twice where min_p asks.
 #include <algorithm>
 
 #include "common.hpp"
@@ -32,8 +40,11 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kBins = 64, kCopies = 16;   // LDS copies of a chunk's bins: lanes of equal logits meet in fewer of them
+constexpr int kBins = kSampleBins, kCopies = 8;   // LDS copies of a chunk's bins: lanes of equal logits meet in fewer of them
 constexpr int kSampleThreads = 256, kPickThreads = 1024;
+static_assert(kBins == kSampleThreads, "a bin a thread");
+// Listed tokens that the last launch keeps in LDS; groups of 64 tokens of a chunk.
+constexpr int kPickCache = 15872, kGroups = kSampleVocab / 8 / 64;
 constexpr double kUnit = 17592186044416.0;   // 2^44
 
 struct SampleArgs {
@@ -71,20 +82,34 @@ __device__ __forceinline__ float logit(const SampleArgs& a, int b, int i) {
     return l != l ? -INFINITY : l;
 }
 
+// Tokens at, at + step, .. of a row, all requested at once; those from `end` on: -inf.
+constexpr int kBatch = 16;
+template <int DT>
+__device__ __forceinline__ void load_logits(const SampleArgs& a, int b, int at, int step, int end, float (&l)[kBatch]) {
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) l[q] = logit<DT>(a, b, min(at + q * step, end - 1));
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q)
+        if (at + q * step >= end) l[q] = -INFINITY;
+}
+
 // Monotone in l: larger logits have larger keys.
 __device__ __forceinline__ uint32_t key_of(float l) {
     const uint32_t u = __float_as_uint(l == 0.0f ? 0.0f : l);   // (-0 and 0 are equal)
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float logit_of(uint32_t key) {
+    return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
 
 // e^((l - best) / t) and its weight.
 struct Weigher {
-    double best, t, min_p;
+    double best, inv, min_p;
     float bestf;
-    __device__ __forceinline__ Weigher(const Row& r, float best_) : best(best_), t(r.t), min_p(r.min_p), bestf(best_) {}
+    __device__ __forceinline__ Weigher(const Row& r, float best_) : best(best_), inv(1.0 / r.t), min_p(r.min_p), bestf(best_) {}
     __device__ __forceinline__ double e(float l) const {
         if (l == bestf) return 1.0;
-        const double d = (static_cast<double>(l) - best) / t;
+        const double d = (static_cast<double>(l) - best) * inv;
         return d > -31.3 ? exp(d) : 0.0;   // (e^-31.3 rounds to no unit)
     }
     static __device__ __forceinline__ u64 units(double e) { return static_cast<u64>(rint(e * kUnit)); }
@@ -113,34 +138,48 @@ __device__ __forceinline__ float2 row_range(const SampleArgs& a, int b) {
     return make_float2(group_max<64>(m.x), -group_max<64>(-m.y));
 }
 
-__device__ __forceinline__ u64 shfl_u64(u64 v, int src) {
-    const uint32_t lo = __shfl(static_cast<int>(v), src), hi = __shfl(static_cast<int>(v >> 32), src);
+// The lane's value (the same lane for the whole wave).
+__device__ __forceinline__ u64 lane_u64(u64 v, int lane) {
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), lane);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), lane);
     return static_cast<u64>(hi) << 32 | lo;
 }
-__device__ __forceinline__ u64 wave_sum_u64(u64 v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v += shfl_u64(v, (threadIdx.x & 63) ^ d);
-    return v;
+template <int CTRL, int ROW_MASK = 0xf>
+__device__ __forceinline__ u64 dpp_u64(u64 v) {
+    const uint32_t lo = dpp_int<CTRL, ROW_MASK>(static_cast<int>(v)), hi = dpp_int<CTRL, ROW_MASK>(static_cast<int>(v >> 32));
+    return static_cast<u64>(hi) << 32 | lo;
 }
-// Sum over the lanes before and up to this one.
+// Sum over the lanes before and up to this one (as wave_inclusive_scan_int), and over all.
 __device__ __forceinline__ u64 wave_scan_u64(u64 v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const u64 o = shfl_u64(v, lane - d & 63);
-        if (lane >= d) v += o;
-    }
+    v += dpp_u64<0x111>(v);
+    v += dpp_u64<0x112>(v);
+    v += dpp_u64<0x114>(v);
+    v += dpp_u64<0x118>(v);
+    v += dpp_u64<0x142, 0xa>(v);
+    v += dpp_u64<0x143, 0xc>(v);
     return v;
 }
+__device__ __forceinline__ u64 wave_sum_u64(u64 v) { return lane_u64(wave_scan_u64(v), 63); }
+
+// Where chunk c's bins stand; kSampleChunks: the row's.
+__device__ __forceinline__ size_t bins_at(int b, int c) { return (static_cast<size_t>(b) * (kSampleChunks + 1) + c) * kBins; }
 
 template <int DT>
 __global__ __launch_bounds__(kSampleThreads) void sample_max_kernel(SampleArgs a) {
     const int b = blockIdx.y, i0 = blockIdx.x * a.per, i1 = min(i0 + a.per, a.vocab);
     float hi = -INFINITY, lo = INFINITY;
-    for (int i = i0 + threadIdx.x; i < i1; i += kSampleThreads) {
-        const float l = logit<DT>(a, b, i);
-        hi = fmaxf(hi, l);
-        if (l > -INFINITY) lo = fminf(lo, l);
+    if (blockIdx.x == 0) {   // (for the next launch's sums)
+        a.w.bin_mass[bins_at(b, kSampleChunks) + threadIdx.x] = 0;
+        a.w.bin_count[b * kBins + threadIdx.x] = 0;
+    }
+    for (int j = i0; j < i1; j += kBatch * kSampleThreads) {
+        float l[kBatch];
+        load_logits<DT>(a, b, j + threadIdx.x, kSampleThreads, i1, l);
+#pragma unroll
+        for (int q = 0; q < kBatch; ++q) {
+            hi = fmaxf(hi, l[q]);
+            if (l[q] > -INFINITY) lo = fminf(lo, l[q]);
+        }
     }
     __shared__ float2 part[kSampleThreads / 64];
     hi = group_max<64>(hi);
@@ -169,83 +208,102 @@ __global__ __launch_bounds__(kSampleThreads) void sample_bins_kernel(SampleArgs 
     __syncthreads();
     const Weigher weigh(r, range.x);
     const Binner bin(r, range.x, range.y);
-    for (int i = i0 + t; i < i1; i += kSampleThreads) {
-        const float l = logit<DT>(a, b, i);
-        const u64 m = weigh.mass(l);
-        if (m == 0) continue;
-        const int k = bin(l);
-        atomicAdd(&mass[k][t % kCopies], m);
-        atomicAdd(&count[k][t % kCopies], 1u);
+    for (int j = i0; j < i1; j += kBatch * kSampleThreads) {
+        float l[kBatch];
+        load_logits<DT>(a, b, j + t, kSampleThreads, i1, l);
+#pragma unroll
+        for (int q = 0; q < kBatch; ++q) {
+            const u64 m = weigh.mass(l[q]);
+            if (m == 0) continue;
+            const int k = bin(l[q]);
+            atomicAdd(&mass[k][t % kCopies], m);
+            atomicAdd(&count[k][t % kCopies], 1u);
+        }
     }
     __syncthreads();
-    if (t < kBins) {
-        u64 m = 0;
-        uint32_t n = 0;
-        for (int c = 0; c < kCopies; ++c) {
-            m += mass[t][(c + t) % kCopies];
-            n += count[t][(c + t) % kCopies];
-        }
-        const size_t o = (static_cast<size_t>(b) * kSampleChunks + blockIdx.x) * kBins + t;
-        a.w.bin_mass[o] = m;
-        a.w.bin_count[o] = n;
+    u64 m = 0;
+    uint32_t n = 0;
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) {
+        m += mass[t][(c + t) % kCopies];
+        n += count[t][(c + t) % kCopies];
+    }
+    a.w.bin_mass[bins_at(b, blockIdx.x) + t] = m;
+    if (n) {   // (whole numbers: any order)
+        atomicAdd(&a.w.bin_mass[bins_at(b, kSampleChunks) + t], m);
+        atomicAdd(&a.w.bin_count[b * kBins + t], n);
     }
 }
 
 // The bins that hold the borders, the same in every chunk's workgroup: bins
 // before lo are kept whole, those past hi not at all. lo > hi: there is no border.
-__device__ __forceinline__ SampleCut find_cut(const SampleArgs& a, const Row& r, int b, u64 (&ms)[kBins], uint32_t (&cs)[kBins]) {
-    const int t = threadIdx.x;
-    if (t < kBins) {
-        ms[t] = 0;
-        cs[t] = 0;
+// A bin a thread.
+struct CutWork {
+    u64 mass[kSampleThreads / 64];
+    uint32_t count[kSampleThreads / 64];
+    u64 least;
+    int by_count, last;
+    u64 mass_before;
+    int count_before;
+};
+__device__ __forceinline__ SampleCut find_cut(const SampleArgs& a, const Row& r, int b, CutWork& w) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const u64 mass = a.w.bin_mass[bins_at(b, kSampleChunks) + t];
+    const uint32_t count = a.w.bin_count[b * kBins + t];
+    u64 mass_to = wave_scan_u64(mass);
+    int count_to = wave_inclusive_scan_int(static_cast<int>(count));
+    if (lane == 63) {
+        w.mass[wave] = mass_to;
+        w.count[wave] = count_to;
     }
+    if (t == 0) w.last = 0;
     __syncthreads();
-    {
-        u64 m = 0;
-        uint32_t n = 0;
-        for (int c = t / kBins; c < a.chunks; c += kSampleThreads / kBins) {
-            const size_t o = (static_cast<size_t>(b) * kSampleChunks + c) * kBins + t % kBins;
-            m += a.w.bin_mass[o];
-            n += a.w.bin_count[o];
+    u64 total = 0;
+    int tokens = 0;
+#pragma unroll
+    for (int i = 0; i < kSampleThreads / 64; ++i) {
+        if (i < wave) {
+            mass_to += w.mass[i];
+            count_to += w.count[i];
         }
-        atomicAdd(&ms[t % kBins], m);
-        atomicAdd(&cs[t % kBins], n);
+        total += w.mass[i];
+        tokens += w.count[i];
     }
-    __syncthreads();
-    const int lane = t & 63;
-    const u64 mass = ms[lane], mass_to = wave_scan_u64(mass);
-    const uint32_t count = cs[lane];
-    const u64 count_to = wave_scan_u64(count);
-    const u64 total = shfl_u64(mass_to, 63), tokens = shfl_u64(count_to, 63);
+    const u64 mass_ahead = mass_to - mass;
+    const int count_ahead = count_to - static_cast<int>(count);
     SampleCut cut;
     cut.total = total;
-    cut.by_count = r.top_k > 0 && static_cast<u64>(r.top_k) < tokens;
+    cut.by_count = r.top_k > 0 && r.top_k < tokens;
     cut.by_mass = r.top_p < 1.0f;
     cut.lo = kBins;
     cut.hi = -1;
     u64 least = total;   // of what the top_k's tokens weigh
     if (cut.by_count) {
         // the first bin with which there are top_k
-        const uint64_t m = __ballot(count_to >= static_cast<u64>(r.top_k));
-        cut.lo = cut.hi = static_cast<int>(__builtin_ctzll(m));
-        least = shfl_u64(mass_to, cut.hi) - shfl_u64(mass, cut.hi);
+        if (count_ahead < r.top_k && count_to >= r.top_k) {
+            w.by_count = t;
+            w.least = mass_ahead;
+        }
+        __syncthreads();
+        cut.lo = cut.hi = w.by_count;
+        least = w.least;
     }
     if (cut.by_mass) {
         // the last bin before which less than top_p of it lies; where the
         // top_k's weight is not known yet, from the least that it can be
         const double aim = static_cast<double>(r.top_p) * static_cast<double>(least);
-        const uint64_t m = __ballot(count > 0 && static_cast<double>(mass_to - mass) < aim) | 1;
-        const int last = 63 - static_cast<int>(__builtin_clzll(m));
-        if (cut.by_count) {
-            cut.lo = min(cut.lo, last);
-        } else {
-            cut.lo = cut.hi = last;
-        }
+        if (count > 0 && static_cast<double>(mass_ahead) < aim) atomicMax(&w.last, t);
+        __syncthreads();
+        if (cut.by_count) cut.lo = min(cut.lo, w.last);
+        else cut.lo = cut.hi = w.last;
     }
-    const int at = min(cut.lo, kBins - 1);
-    const u64 mb = shfl_u64(mass_to - mass, at), cb = shfl_u64(count_to - count, at);
-    cut.mass_before = cut.lo < kBins ? mb : total;
-    cut.count_before = static_cast<int>(cut.lo < kBins ? cb : tokens);
+    if (t == min(cut.lo, kBins - 1)) {
+        w.mass_before = cut.lo < kBins ? mass_ahead : total;
+        w.count_before = cut.lo < kBins ? count_ahead : tokens;
+    }
+    __syncthreads();
+    cut.mass_before = w.mass_before;
+    cut.count_before = w.count_before;
     return cut;
 }
 
@@ -256,11 +314,10 @@ __global__ __launch_bounds__(kSampleThreads) void sample_gather_kernel(SampleArg
     const Row r = row_of(a, b);
     const float2 range = row_range(a, b);
     if (r.first || range.x == -INFINITY) return;
-    __shared__ u64 ms[kBins];
-    __shared__ uint32_t cs[kBins];
+    __shared__ CutWork cut_work;
     __shared__ int wcount[kSampleThreads / 64];
     __shared__ u64 wmass[kSampleThreads / 64];
-    const SampleCut cut = find_cut(a, r, b, ms, cs);
+    const SampleCut cut = find_cut(a, r, b, cut_work);
     if (blockIdx.x == 0 && t == 0) a.w.cut[b] = cut;
     const Weigher weigh(r, range.x);
     const Binner bin(r, range.x, range.y);
@@ -269,35 +326,45 @@ __global__ __launch_bounds__(kSampleThreads) void sample_gather_kernel(SampleArg
     int listed = 0;
     if (border || sift) {
         int32_t* const list = a.w.list + static_cast<size_t>(b) * a.vocab + i0;
-        for (int j = i0; j < i1; j += kSampleThreads) {
-            const int i = j + t;
-            const float l = i < i1 ? logit<DT>(a, b, i) : -INFINITY;
-            const int k = l > -INFINITY ? bin(l) : kBins;
-            bool mine = false;
-            if (k < cut.lo && k < kBins) {
-                if (sift) {
-                    const double e = weigh.e(l);
-                    if (weigh.passes(e)) base += Weigher::units(e);
+        // a wave's tokens of a batch follow one another
+        for (int j = i0; j < i1; j += kBatch * kSampleThreads) {
+            const int at0 = j + wave * kBatch * 64 + lane;
+            float l[kBatch];
+            load_logits<DT>(a, b, at0, 64, i1, l);
+            uint64_t m[kBatch];
+            int own = 0;
+#pragma unroll
+            for (int q = 0; q < kBatch; ++q) {
+                const int k = l[q] > -INFINITY ? bin(l[q]) : kBins;
+                bool mine = false;
+                if (k < cut.lo && k < kBins) {
+                    if (sift) {
+                        const double e = weigh.e(l[q]);
+                        if (weigh.passes(e)) base += Weigher::units(e);
+                    }
+                } else if (k <= cut.hi) {
+                    mine = weigh.mass(l[q]) > 0;
                 }
-            } else if (k <= cut.hi) {
-                mine = weigh.mass(l) > 0;
+                m[q] = __ballot(mine);
+                own += __popcll(m[q]);
             }
-            if (border) {
-                const uint64_t m = __ballot(mine);
-                if (lane == 0) wcount[wave] = __popcll(m);
-                __syncthreads();
-                int at = listed + __popcll(m & ((1ull << lane) - 1));
-                for (int w = 0; w < kSampleThreads / 64; ++w) {
-                    if (w < wave) at += wcount[w];
-                    listed += wcount[w];
-                }
-                if (mine) list[at] = i;
-                __syncthreads();
+            if (!border) continue;
+            if (lane == 0) wcount[wave] = own;
+            __syncthreads();
+            int at = listed;
+            for (int w = 0; w < kSampleThreads / 64; ++w) {
+                if (w < wave) at += wcount[w];
+                listed += wcount[w];
             }
+#pragma unroll
+            for (int q = 0; q < kBatch; ++q) {
+                if (m[q] >> lane & 1) list[at + __popcll(m[q] & ((1ull << lane) - 1))] = at0 + 64 * q;
+                at += __popcll(m[q]);
+            }
+            __syncthreads();
         }
     }
-    if (!sift && t < kBins && t < cut.lo)
-        base = a.w.bin_mass[(static_cast<size_t>(b) * kSampleChunks + blockIdx.x) * kBins + t];
+    if (!sift && t < cut.lo) base = a.w.bin_mass[bins_at(b, blockIdx.x) + t];
     base = wave_sum_u64(base);
     if (lane == 0) wmass[wave] = base;
     __syncthreads();
@@ -379,10 +446,34 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
         }
         return lo;
     };
-    auto token_at = [&](int k) {
-        const int c = chunk_of(k);
-        return lists[static_cast<size_t>(c) * a.per + (k - first[c])];
+    // a listed token: its key, then its index
+    auto read_entry = [&](int k) {
+        const int c = chunk_of(k), i = lists[static_cast<size_t>(c) * a.per + (k - first[c])];
+        return static_cast<u64>(key_of(logit<DT>(a, b, i))) << 32 | static_cast<uint32_t>(i);
     };
+    __shared__ u64 cache[kPickCache];
+    const bool cached = n <= kPickCache;
+    uint32_t differ = 0;   // the keys' bits that are not all alike
+    if (n > 0) {
+        const uint32_t any = read_entry(0) >> 32;
+#pragma unroll 4
+        for (int k = t; k < n; k += kPickThreads) {
+            const u64 e = read_entry(k);
+            if (cached) cache[k] = e;
+            differ |= static_cast<uint32_t>(e >> 32) ^ any;
+        }
+#pragma unroll
+        for (int d = 32; d; d >>= 1) differ |= __shfl_xor(static_cast<int>(differ), d);
+        if (t == 0) found = 0;
+        __syncthreads();
+        if (lane == 0 && differ) atomicOr(&found, static_cast<int>(differ));
+        __syncthreads();
+        differ = found;
+    }
+    auto entry = [&](int k) { return cached ? cache[k] : read_entry(k); };
+    // the selections' digits begin at the highest of these bits; those above it are the first token's
+    const int bits = 32 - (differ ? __builtin_clz(differ) : 32), top = bits > 8 ? bits : 8;
+    const uint32_t alike = n > 0 && top < 32 ? static_cast<uint32_t>(entry(0) >> 32) & (~0u << top) : 0u;
 
     // The border where `by_mass`: the last token before which (with `before` ahead of
     // the listed ones) less than `aim` lies; else: the aim-th token. Only keys
@@ -390,23 +481,24 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
     // kept and weighs: `before`, and what the listed tokens to the border weigh.
     auto select = [&](bool by_mass, double aim_mass, long long aim_count, u64 before, uint32_t least, long long least_ties,
                       Border& out) {
-        uint32_t prefix = 0;
+        uint32_t prefix = alike;
         u64 ahead = before;
         long long rank = aim_count;   // still to be taken
-        for (int sh = 24; sh >= 0; sh -= 8) {
+        for (int end = top; end > 0; end = max(end - 8, 0)) {   // bits [sh, end), eight or (the last) the rest
+            const int sh = max(end - 8, 0);
+            __syncthreads();   // (the scan before has been read)
             for (int i = t; i < 256; i += kPickThreads) {
                 sums[i] = 0;
                 counts[i] = 0;
             }
             __syncthreads();
-            const uint32_t mask = sh == 24 ? 0u : ~0u << (sh + 8);
+            const uint32_t mask = end < 32 ? ~0u << end : 0u;
             for (int k = t; k < n; k += kPickThreads) {
-                const float l = logit<DT>(a, b, token_at(k));
-                const uint32_t key = key_of(l);
+                const uint32_t key = entry(k) >> 32;
                 if ((key & mask) != prefix || key < least) continue;
-                const int d = key >> sh & 255;
+                const int d = key >> sh & ((1 << (end - sh)) - 1);
                 atomicAdd(&counts[d], 1u);
-                atomicAdd(&sums[d], weigh.mass(l));
+                atomicAdd(&sums[d], weigh.mass(logit_of(key)));
             }
             __syncthreads();
             if (wave == 0) {
@@ -421,7 +513,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
                     own += m[i];
                     ownc += c[i];
                 }
-                u64 am = ahead + wave_scan_u64(own) - own, ac = wave_scan_u64(ownc) - ownc;
+                u64 am = ahead + wave_scan_u64(own) - own, ac = wave_inclusive_scan_int(static_cast<int>(ownc)) - ownc;
                 int mine = -1;
                 u64 mine_ahead = 0, mine_count = 0, mine_mass = 0;
 #pragma unroll
@@ -449,7 +541,6 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
             prefix = pass.key;
             ahead = carry;
             if (!by_mass) rank = pass.ties;
-            __syncthreads();
         }
         // the tokens with this key weigh the same
         const long long same = found;
@@ -492,8 +583,8 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
         __syncthreads();
         for (int k0 = 0; k0 < n; k0 += kPickThreads) {
             const int k = k0 + t;
-            const int i = k < n ? token_at(k) : -1;
-            const bool tie = i >= 0 && key_of(logit<DT>(a, b, i)) == last.key;
+            const u64 e = k < n ? entry(k) : 0;
+            const bool tie = k < n && static_cast<uint32_t>(e >> 32) == last.key;
             const uint64_t m = __ballot(tie);
             if (lane == 0) wcount[wave] = __popcll(m);
             __syncthreads();
@@ -502,64 +593,65 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
                 if (w < wave) at += wcount[w];
                 seen += wcount[w];
             }
-            if (tie && at == last.ties - 1) found = i;
+            if (tie && at == last.ties - 1) found = static_cast<uint32_t>(e);
             __syncthreads();
             if (seen >= last.ties) break;
         }
         last_index = found;
     }
-    auto keeps = [&](float l, int i) {
-        const uint32_t key = key_of(l);
-        return key > last.key || (key == last.key && i <= last_index);
-    };
+    auto keeps = [&](uint32_t key, int i) { return key > last.key || (key == last.key && i <= last_index); };
     // each chunk's kept weight
-    for (int c = wave; c < a.chunks && border; c += kWaves) {
-        u64 m = 0;
-        for (int k = first[c] + lane; k < first[c + 1]; k += 64) {
-            const int i = lists[static_cast<size_t>(c) * a.per + (k - first[c])];
-            const float l = logit<DT>(a, b, i);
-            const double e = weigh.e(l);
-            if (keeps(l, i) && weigh.passes(e)) m += Weigher::units(e);
-        }
-        m = wave_sum_u64(m);
-        if (lane == 0) kept[c] += m;
+    for (int k = t; k < n; k += kPickThreads) {
+        const u64 at = entry(k);
+        const uint32_t key = at >> 32;
+        if (!keeps(key, static_cast<int>(static_cast<uint32_t>(at)))) continue;
+        const double e = weigh.e(logit_of(key));
+        if (weigh.passes(e)) atomicAdd(&kept[chunk_of(k)], Weigher::units(e));
     }
     __syncthreads();
     // the chunk that u falls into, the same in every wave
-    const u64 own = lane < a.chunks ? kept[lane] : 0, to = wave_scan_u64(own), total = shfl_u64(to, 63);
+    const u64 own = lane < a.chunks ? kept[lane] : 0, to = wave_scan_u64(own), total = lane_u64(to, 63);
     const double u = fmin(fmax(static_cast<double>(a.u[b]), 0.0), 1.0);
     u64 aim = static_cast<u64>(floor(u * static_cast<double>(total)));
     if (aim > total - 1) aim = total - 1;
     const int chunk = static_cast<int>(__builtin_ctzll(__ballot(to > aim)));
-    u64 before = shfl_u64(to - own, chunk);
-    // and the token there: a wave's 64 tokens after the other
-    __shared__ u64 wsum[kWaves];
-    const int i0 = chunk * a.per, i1 = min(i0 + a.per, a.vocab);
-    for (int j = i0; j < i1; j += kPickThreads) {
-        const int i = j + t;
-        u64 m = 0;
-        if (i < i1) {
-            const float l = logit<DT>(a, b, i);
-            if (l > -INFINITY && keeps(l, i)) {
-                const double e = weigh.e(l);
-                if (weigh.passes(e)) m = Weigher::units(e);
-            }
+    u64 before = lane_u64(to - own, chunk);
+    // the 64 tokens of it that hold this one, and the token there
+    __shared__ u64 groups[kGroups];
+    const int i0 = chunk * a.per, i1 = min(i0 + a.per, a.vocab), n64 = (i1 - i0 + 63) / 64;
+    auto mass_at = [&](int i, float l) -> u64 {
+        if (!(l > -INFINITY) || !keeps(key_of(l), i)) return 0;
+        const double e = weigh.e(l);
+        return weigh.passes(e) ? Weigher::units(e) : 0;
+    };
+    for (int g0 = wave; g0 < n64; g0 += 4 * kWaves) {
+        float l[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) l[q] = logit<DT>(a, b, min(i0 + 64 * (g0 + q * kWaves) + lane, i1 - 1));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int g = g0 + q * kWaves, i = i0 + 64 * g + lane;
+            const u64 m = wave_sum_u64(i < i1 ? mass_at(i, l[q]) : 0);
+            if (lane == 0 && g < n64) groups[g] = m;
         }
-        const u64 upto = wave_scan_u64(m);
-        if (lane == 63) wsum[wave] = upto;
-        __syncthreads();
-        u64 at = before + upto, all = 0;
-        for (int w = 0; w < kWaves; ++w) {
-            if (w < wave) at += wsum[w];
-            all += wsum[w];
-        }
-        if (m && at > aim && at - m <= aim) {
-            a.tokens[b] = i;
-            if (a.probs) a.probs[b] = static_cast<float>(static_cast<double>(m) / static_cast<double>(total));
-        }
-        before += all;
-        if (before > aim) break;
-        __syncthreads();
+    }
+    __syncthreads();
+    if (wave != 0) return;
+    const int each = (n64 + 63) / 64;
+    u64 sum = 0;
+    for (int k = 0; k < each; ++k)
+        if (each * lane + k < n64) sum += groups[each * lane + k];
+    u64 upto = before + wave_scan_u64(sum);
+    const int src = static_cast<int>(__builtin_ctzll(__ballot(upto > aim) | 1ull << 63));
+    before = lane_u64(upto - sum, src);
+    int g = each * src;
+    while (g + 1 < n64 && before + groups[g] <= aim) before += groups[g++];
+    const int i = i0 + 64 * g + lane;
+    const u64 m = i < i1 ? mass_at(i, logit<DT>(a, b, i)) : 0;
+    const u64 at = before + wave_scan_u64(m);
+    if (m && at > aim && at - m <= aim) {
+        a.tokens[b] = i;
+        if (a.probs) a.probs[b] = static_cast<float>(static_cast<double>(m) / static_cast<double>(total));
     }
 }
 
@@ -569,8 +661,8 @@ hipError_t launch_sample(qff_ctx* ctx, hipStream_t stream, const void* logits, q
                          const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                          int32_t* tokens, float* probs, int vocab, int batch) {
     SampleArgs a{logits, u, temperature, top_k, top_p, min_p, tokens, probs, vocab, 0, 0, ctx->sample};
-    // two workgroups a CU over all rows, 64 a row at most
-    const int chunks = std::min(std::max(2 * ctx->num_cu / batch, 8), kSampleChunks);
+    // four workgroups a CU over all rows, 64 a row at most (32 rows of 151936: 66 us, with two a CU 70)
+    const int chunks = std::min(std::max(4 * ctx->num_cu / batch, 8), kSampleChunks);
     a.per = (vocab + chunks - 1) / chunks;
     a.chunks = (vocab + a.per - 1) / a.per;
     const dim3 grid(a.chunks, batch);
