@@ -255,10 +255,18 @@ int qff_rms_norm(qff_ctx* ctx, qff_stream_t stream, const void* x, qff_dtype x_d
  *   indices [tokens, top] int32 device array, 1 <= top <= 16
  *   h       [tokens, top + shared, inter] of h_dtype (F32, BF16 or F16; what
  *           exceeds fp16 becomes infinite there)
- * x and h are 16-byte aligned. Nibbles, scales and biases enter the products
- * exactly, an fp32 x as three bf16 terms; from 33 tokens on, where h is BF16 or
- * F16, the products run on fp16 operands (qff_moe_down says how). tokens may be 0;
- * QFF_ERR_WORKSPACE above the larger of max_batch and max_prefill_tokens. */
+ * x and h are 16-byte aligned. tokens may be 0;
+ * QFF_ERR_WORKSPACE above the larger of max_batch and max_prefill_tokens.
+ *
+ * What both halves round, beside their outputs and the fp32 sums: up to 72 pairs
+ * (token, slot; down: 200) nothing. Above, products run on fp16 operands after
+ * power-of-two shifts: a weight is scale (q - 8), exact, and a part constant over
+ * its group of 64 columns, bias + 8 scale, which meets the group's sum of x; an
+ * fp32 input is two fp16 terms (2^-22 of its value, or 2^-37 of its row's
+ * largest), a BF16 one is exact beside the same 2^-37. With a BF16 output and 33 tokens or more fp32 inputs
+ * and F16 scales times q - 8 keep 11 bits, and what moe_down sums over the pairs 11 bits
+ * relative to the largest of each 64 outputs of a pair. Scales lie in 2^-22 .. 31 (smaller ones
+ * lose bits) and |bias + 8 scale| is at most 8. */
 int qff_moe_gate_up(qff_ctx* ctx, qff_stream_t stream, const qff_moe_weights* p, const void* x,
                     qff_dtype x_dtype, const int32_t* indices, int top, void* h, qff_dtype h_dtype,
                     int tokens);

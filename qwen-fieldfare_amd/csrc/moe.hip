@@ -4,7 +4,11 @@
 //   h[m, j] = silu(Wg x_m) * (Wu x_m),  W of expert indices[m, j]
 //   y[m]    = residual + sum_j score[m, j] Wd h[m, j]
 //
-// A weight is W = s q + b, q the nibble. The kernels below take the nibble as
+// Three forms, by how many pairs (token, slot) a call has and how many an expert
+// (the figures stand at kOneUp): each pair by itself, small tiles of an expert's pairs,
+// large tiles.
+//
+// A weight is W = s q + b, q the nibble. Pairs by themselves take the nibble as
 // the bf16 1 + q / 16 (its four bits are the top ones of the mantissa:
 // (q << 3) | 0x3F80, exact), so that per group of 64 columns, with
 // P = sum (1 + q / 16) x and X = sum x (a product with ones, from the same
@@ -376,11 +380,12 @@ __global__ __launch_bounds__(64 * kOneWaves) void moe_down_one_kernel(MoeArgs p,
 
 // ---- several tokens of one expert ------------------------------------------------
 
-// Which pairs each expert has, and the tiles of up to `most` that they make: the pairs are counted, the counts summed up and the pairs written
-// expert by expert (in no fixed order within one: a pair's sums do not depend on
-// its place). An expert's tiles share its pairs evenly, in multiples of `unit`
-// (8 to 32); the shared expert, number `experts`, has every token. Up to kPlanAlone pairs one
-// workgroup does it all (6 us at 4000 pairs, 69 at 65536); beyond, a workgroup for
+// Which pairs each expert has, and the tiles of up to `most` that they make: the
+// pairs are counted, the counts summed up and the pairs written expert by expert
+// (in no fixed order within one: a pair's sums do not depend on its place). An expert's tiles share its pairs evenly, in multiples of `unit`
+// (8 to 32); the shared expert, number `experts`, has every token. Up to kPlanAlone
+// pairs one workgroup does it all (6 us at 4000 pairs, 69 at 65536; by several 13);
+// beyond, a workgroup for
 // each kPlanShare pairs counts its own, and each then sums up those before it.
 constexpr int kPlanThreads = 1024, kPlanShare = 1024, kPlanAlone = 4096;
 static_assert(kMoeMaxExperts < kPlanThreads, "an expert a thread");
@@ -490,8 +495,8 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const float* __restric
 
 // ---- many tokens ------------------------------------------------------------------
 //
-// The plan's tiles against the matrices on 32x32x16 fp16 products. A weight is s q + b = s (q - 8) + (b + 8 s); its first part is exact
-// in fp16 where the scale has 8 significant bits (bf16): q - 8 is a power of two
+// The plan's tiles against the matrices on 32x32x16 fp16 products. A weight is
+// s q + b = s (q - 8) + (b + 8 s); its first part is exact in fp16 where the scale has 8 significant bits (bf16): q - 8 is a power of two
 // or has three bits. The nibble becomes 16 + q (its bits are the top ones of the
 // mantissa), one packed FMA (16 + q) s - 24 s gives the product without a rounding,
 // and the second part, constant over a group, meets the group's sums of x in a few
@@ -503,7 +508,7 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const float* __restric
 // bits (XT = 2); fp16 rows of h are taken as they lie. s 256 and x lie inside
 // fp16's normal range for scales of 2^-22 .. 31; b + 8 s may be up to 8 in magnitude.
 // So F32 and F16 outputs are sums of exact products (up to 2^-22 of x), and
-// bf16 ones carry 11 bits an operand.
+// bf16 ones carry 11 bits an operand (a bf16 result has 8).
 
 // Rows of x for the tiles: XT fp16 terms [row][XT][cols] (each 8 columns in the
 // order c0, c4, c1, c5, .., the nibbles' own) and the row's factor 2^(e - 8); and
@@ -891,7 +896,7 @@ __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, co
         };
         operands(0);
         // the next k step's reads, then its conversions between this one's products
-        constexpr int kProducts = 2 * NMT * (XT * WT == 4 ? 3 : XT * WT), kBetween = (2 * WT * 16 + kProducts - 1) / kProducts;
+        constexpr int kProducts = 2 * NMT * XT * WT, kBetween = (2 * WT * 16 + kProducts - 1) / kProducts;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
             __builtin_amdgcn_sched_barrier(0);
@@ -903,10 +908,8 @@ __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, co
 #pragma unroll
                     for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
-                        for (int mt = 0; mt < NMT; ++mt) {
-                            if (x == 1 && k == 1) continue;   // (the rest of a scale's eight bits by the rest of x: 2^-19 of the product)
+                        for (int mt = 0; mt < NMT; ++mt)
                             acc[rt][mt] = mfma_32x32x16_f16(A[ks & 1][rt][k], B[ks & 1][mt][x], acc[rt][mt]);
-                        }
             if (ks < 3) {
                 __builtin_amdgcn_sched_group_barrier(0x100, NMT * XT, 0);
                 unroll<kProducts>([&](auto) {

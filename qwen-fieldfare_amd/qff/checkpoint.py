@@ -20,6 +20,15 @@ fp32 (:558-572, 636-640). Here the same names map to device tensors:
     self_attn.{q,k}_norm.weight [256]                       -> fp32
   every layer: input_layernorm.weight [2048] (used as is, deltanet.metal
     :18-53), mlp.gate.* (Q8 router [256, 2048]).
+  expert block of a layer (expert_layer): post_attention_layernorm.weight
+    [2048], mlp.gate.*, mlp.switch_mlp.{gate,up,down}_proj.* (Q4, all experts
+    stacked), mlp.shared_expert.{gate,up,down}_proj.* (Q4) and
+    mlp.shared_expert_gate.* (Q8 [1, 2048]), the last four where there is a
+    shared expert
+  head: norm.weight [2048] and language_model.lm_head.* (Q4 [vocab, 2048]);
+    without one the embedding's rows, embed_tokens.*
+  (the names of the expert block and the head follow the format's naming of
+  this family; no file that the reference holds pins them)
 
 Quantized tensors stay in the checkpoint's bytes (uint32 words viewed as
 int32, bf16 scales/biases), so no repacking happens on load: the kernels
@@ -144,6 +153,30 @@ class Checkpoint:
         self._files.clear()
 
     # ---- per-layer views ---------------------------------------------------
+    def _maybe(self, stem: str, device):
+        return self.quant(stem, device) if stem + ".weight" in self.weight_map else None
+
+    def expert_layer(self, l: int, device="cuda") -> dict | None:
+        """Layer l's expert block, as AttentionStack takes it in the layer's "mlp";
+        None where the checkpoint has no experts for it."""
+        from .ops import ExpertWeights
+        p = self.prefix + f"layers.{l}."
+        if p + "mlp.switch_mlp.gate_proj.weight" not in self.weight_map:
+            return None
+        experts = [self.quant(p + f"mlp.switch_mlp.{n}_proj", device) for n in ("gate", "up", "down")]
+        shared = [self._maybe(p + f"mlp.shared_expert.{n}_proj", device) for n in ("gate", "up", "down")]
+        return {"norm_w": self.fp32(p + "post_attention_layernorm.weight", device),
+                "router": self.quant(p + "mlp.gate", device),
+                "gate": self._maybe(p + "mlp.shared_expert_gate", device),
+                "experts": ExpertWeights(*experts, *shared)}
+
+    def head(self, device="cuda") -> dict:
+        """The final norm and the product that gives the logits."""
+        stem = self.prefix.removesuffix("model.") + "lm_head"
+        if stem + ".weight" not in self.weight_map:
+            stem = self.prefix + "embed_tokens"
+        return {"norm_w": self.fp32(self.prefix + "norm.weight", device), "lm_head": self.quant(stem, device)}
+
     def layer_kind(self, l: int) -> str:
         return "gqa" if (self.prefix + f"layers.{l}.self_attn.q_proj.weight") in self.weight_map else "dn"
 

@@ -1,6 +1,6 @@
-"""The attention half of the decoder stack: the per-layer schedule of
+"""The decoder stack: the per-layer schedule of
 QwenQ4ActiveExpertStreamingRunner.forwardToken (Runner:924-1167) over the C
-ABI, with the MoE block replaced by identity.
+ABI. A layer whose dict has no "mlp" has identity in the expert block's place.
 
 Layer l is full attention when l % 4 == 3, Gated DeltaNet otherwise
 (Runner:554-556). Each layer reads the residual stream x [B, 2048] and adds
@@ -12,6 +12,11 @@ its attention output back into it (Runner:1034-1040, 1162-1166):
   full attn  input RMSNorm + q|gate, k, v projections (Runner:1043-1074)
              -> split / head norms / RoPE / KV append / attention / gate
                 (Runner:1076-1150) -> o_proj, added into x (Runner:1152-1166)
+  "mlp"      post-attention RMSNorm and the shared expert's coefficient ->
+             router -> the experts' gate and up -> down, weighted and added into x
+
+and from the last layer's x, final RMSNorm + head product -> the next tokens
+(next_tokens), for a stack that was given its head.
 
 The residual stream and every intermediate are fp32, as the reference keeps
 them (hiddenBuf0/1, qkvOutBuf, ... are float buffers, Runner:346-401); the KV
@@ -38,7 +43,9 @@ class AttentionStack:
     """Layers, their per-sequence state and the scratch tensors of one decode
     step for `batch` sequences. `layers[l]` is a dict with the keys of
     Checkpoint.deltanet_layer (DeltaNet) or Checkpoint.gqa_layer (full
-    attention); the kind follows l % 4 == 3 unless `kinds` says otherwise.
+    attention); the kind follows l % 4 == 3 unless `kinds` says otherwise. Its
+    "mlp" is what Checkpoint.expert_layer returns; `head` what Checkpoint.head
+    returns (None: the stack ends with x).
     States: DeltaNet conv [B, 8192, 4] / ssm [B, 32, 128, 128] fp32, full
     attention K / V caches [B, max_ctx, 2, 256] bf16; pass them in `states`
     or get zero states.
@@ -50,7 +57,7 @@ class AttentionStack:
     reserve() gives the new tokens their places."""
 
     def __init__(self, ctx: ops.Context, layers, batch: int, max_ctx: int, states=None, kinds=None,
-                 eps: float = 1e-6, device="cuda", pages=None):
+                 eps: float = 1e-6, device="cuda", pages=None, head=None):
         self.ctx = ctx
         self.layers = list(layers)
         self.B = batch
@@ -93,6 +100,49 @@ class AttentionStack:
         self.kn = torch.empty(batch, 512, **f32)
         self.vn = torch.empty(batch, 512, **f32)
         self.att = torch.empty(batch, 16, 256, **f32)
+        self._block = {}   # an expert block's tensors by what its shapes depend on: layers of one shape share them
+        for L in self.layers:
+            M = L.get("mlp")
+            if M is None:
+                continue
+            if M["experts"].hidden != HIDDEN or None in (M["experts"].matrices[0], M["experts"].matrices[2]):
+                raise ValueError(f"a layer's experts need gate, up and down of {HIDDEN} columns of x")
+            if M["router"][0].shape[0] != M["experts"].experts:
+                raise ValueError("a layer's router must have a row for each of its experts")
+            if M["gate"] is not None and M["experts"].matrices[3] is None:
+                raise ValueError("a shared expert's gate needs a shared expert")
+            if self._shape(M) not in self._block:
+                self._block[self._shape(M)] = self._block_tensors(M, batch, device)
+        self.head = head
+        if head is not None:
+            self.logits = torch.empty(batch, head["lm_head"][0].shape[0], **f32)
+            self.tokens = torch.empty(batch, dtype=torch.int32, device=device)
+            self.chances = torch.empty(batch, **f32)
+
+    @staticmethod
+    def _shape(M):
+        E = M["experts"]
+        return E.experts, E.inter, E.matrices[3] is not None
+
+    @staticmethod
+    def _block_tensors(M, n, device):
+        E = M["experts"]
+        f32 = dict(dtype=torch.float32, device=device)
+        return (torch.empty(n, HIDDEN, **f32), torch.empty(n, **f32), torch.empty(n, E.experts, **f32),
+                torch.empty(n, 8, dtype=torch.int32, device=device), torch.empty(n, 8, **f32),
+                torch.empty(n, 8 + (E.matrices[3] is not None), E.inter, **f32))
+
+    def _experts(self, M, x: torch.Tensor, tensors):
+        """A layer's expert block on the residual stream, in place."""
+        xn, coef, logits, indices, scores, h = tensors
+        if M["gate"] is not None:
+            ops.rms_norm(self.ctx, x, M["norm_w"], self.eps, gate=M["gate"], out=xn, coef=coef)
+        else:
+            ops.rms_norm(self.ctx, x, M["norm_w"], self.eps, out=xn)
+        ops.router_top8(self.ctx, *M["router"], xn, logits=logits, indices=indices, scores=scores)
+        ops.moe_gate_up(self.ctx, M["experts"], xn, indices, out=h)
+        ops.moe_down(self.ctx, M["experts"], h, indices, scores, coef=coef if M["gate"] is not None else None,
+                     residual=x, out=x)
 
     def layer_step(self, l: int, x: torch.Tensor, positions: torch.Tensor):
         """Layer l of one decode step: x [B, 2048] fp32, updated in place."""
@@ -116,6 +166,23 @@ class AttentionStack:
                 ops.gqa_decode_shared(ctx, L["params"], *new, S["k_pages"], S["v_pages"], P.table, positions,
                                       P.group, P.shared_len, out=self.att, eps=eps)
             ops.q4_matmul_parts(ctx, [L["out_proj"]], self.att.view(B, 4096), outs=(x,), residuals=(x,))
+        M = L.get("mlp")
+        if M is not None:
+            self._experts(M, x, self._block[self._shape(M)])
+
+    def next_tokens(self, x: torch.Tensor, u: torch.Tensor, temperature=None, top_k=None, top_p=None, min_p=None):
+        """The next tokens from the last layer's rows x [n, 2048] fp32, n <= batch (a
+        decode step's, or a prompt's last row), with the random numbers and
+        settings of ops.sample. Returns (tokens int32 [n], their chances f32 [n]),
+        views of the stack's own tensors that the next call writes again."""
+        if self.head is None:
+            raise ValueError("the stack was made without a head")
+        n = x.shape[0]
+        if x.dtype != torch.float32 or x.dim() != 2 or x.shape[1] != HIDDEN or not 1 <= n <= self.B:
+            raise ValueError(f"x must be float32 [1 .. {self.B}, {HIDDEN}]")
+        logits = self.logits[:n]
+        ops.q4_norm_matmul_parts(self.ctx, [self.head["lm_head"]], x, self.head["norm_w"], self.eps, outs=(logits,))
+        return ops.sample(self.ctx, logits, u, temperature, top_k, top_p, min_p, out=self.tokens[:n], prob=self.chances[:n])
 
     def decode_step(self, x: torch.Tensor, positions: torch.Tensor):
         """Every layer in order: x [B, 2048] fp32 (the residual stream, in
@@ -214,6 +281,7 @@ class AttentionStack:
         self._unpark(slot)
         self._copy_pages([s for s, _ in copies], [d for _, d in copies])
         P.sync()
+        blocks = {}
         for kind, L, S in zip(self.kinds, self.layers, self.states):
             y = ops.q4_norm_matmul_parts(ctx, L["in_proj"], x, L["in_norm_w"], eps)
             if kind == "dn":
@@ -228,6 +296,12 @@ class AttentionStack:
                                              y[2].view(T, 2, 256), S["k_pages"], S["v_pages"], P.table[slot],
                                              start_pos=start, out_dtype=torch.float32, eps=eps).view(T, 4096)
             ops.q4_matmul_parts(ctx, [L["out_proj"]], core, outs=(x,), residuals=(x,))
+            M = L.get("mlp")
+            if M is not None:
+                shape = self._shape(M)
+                if shape not in blocks:
+                    blocks[shape] = self._block_tensors(M, T, x.device)
+                self._experts(M, x, blocks[shape])
 
     def fork(self, src: int, dsts):
         """Slots `dsts` (empty) go on from where slot src stands: its pages are
@@ -270,6 +344,26 @@ def random_q4(rows: int, cols: int, gen: torch.Generator, device="cuda"):
     sc = (torch.rand(rows, cols // 64, device=device, generator=gen) * 0.015 + 0.005).half()
     bi = (torch.randn(rows, cols // 64, device=device, generator=gen) * 0.05).half()
     return w, sc, bi
+
+
+def random_q8(rows: int, cols: int, gen: torch.Generator, device="cuda"):
+    """An affine-Q8 weight of about the same spread, fp16 scales and biases."""
+    w = torch.randint(-2 ** 31, 2 ** 31 - 1, (rows, cols // 4), dtype=torch.int32, device=device, generator=gen)
+    sc = (torch.rand(rows, cols // 64, device=device, generator=gen) * 0.0009 + 0.0003).half()
+    return w, sc, (-127.5 * sc.float()).half()
+
+
+def random_mlp(experts: int, inter: int, gen: torch.Generator, device="cuda"):
+    """An expert block with a shared expert, random weights (see random_q4),
+    post-attention RMSNorm weights 1."""
+    def stacked(rows, cols):
+        w, sc, bi = random_q4(experts * rows, cols, gen, device)
+        return w.view(experts, rows, -1), sc.view(experts, rows, -1), bi.view(experts, rows, -1)
+    return {"norm_w": torch.ones(HIDDEN, device=device), "router": random_q8(experts, HIDDEN, gen, device),
+            "gate": random_q8(1, HIDDEN, gen, device),
+            "experts": ops.ExpertWeights(stacked(inter, HIDDEN), stacked(inter, HIDDEN), stacked(HIDDEN, inter),
+                                         random_q4(inter, HIDDEN, gen, device), random_q4(inter, HIDDEN, gen, device),
+                                         random_q4(HIDDEN, inter, gen, device))}
 
 
 def random_layers(n: int, gen: torch.Generator, dn_params: dict, gqa_params: dict, device="cuda"):
