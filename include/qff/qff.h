@@ -237,7 +237,7 @@ typedef struct qff_moe_weights {
  * Replaces qwen_rmsnorm_f32 (deltanet.metal:18-53) where the router and the
  * experts read the normalised rows. x [tokens, cols] of x_dtype, y of y_dtype,
  * norm_w [cols] of norm_dtype (each F32 or BF16), coef [tokens] fp32. y may be
- * x. cols is a multiple of 64, up to 8192; x, y, norm_w and gate->w are
+ * x where both have one type. cols is a multiple of 64, up to 8192; x, y, norm_w and gate->w are
  * 16-byte aligned. tokens may be 0. */
 int qff_rms_norm(qff_ctx* ctx, qff_stream_t stream, const void* x, qff_dtype x_dtype,
                  const void* norm_w, qff_dtype norm_dtype, float eps, const qff_q4_matrices* gate,

@@ -1121,9 +1121,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // two terms. A stage is four groups, 128 bytes of each row of words and so whole
 // cache lines; three stages, 72 KB. Lane (c, kg) holds row c of a row tile and 32
 // consecutive columns kg of each 128, with their group's scale: k slots may stand
-// for any columns as long as both operands agree. The groups' constant parts are products whose
-// k slots are 32 groups, formed from the scales and biases that the lane loads and
-// leaves in LDS.
+// for any columns as long as both operands agree. The groups' constant parts are
+// products whose k slots are 32 groups, formed from the scales and biases that the
+// lane loads and leaves in LDS.
+// At 32 tokens (256 experts of 512 x 2048 and a shared one, 8 a token, all fp32)
+// gate and up take 50 us, 200 MB read at 4.0 TB/s with the start and the last
+// round (two and a half) of workgroups, and down 36; by the large tiles 62 and 40,
+// with stages of one group and two waves of 64 rows 66 and 43. Words requested ahead
+// of what waits for the pairs, and workgroups that begin in different columns, gave
+// nothing (52, 51).
 constexpr int kSlimRows = 128, kSlimColumns = 16, kSlimStages = 3;
 constexpr int kSlimWords = kSlimRows * 128, kSlimStage = kSlimWords + kSlimColumns * 512;
 
@@ -1150,23 +1156,25 @@ __device__ __forceinline__ void slim_kernel(const MoeArgs& p, const TileArgs& a,
     };
     auto x_row = [&](int code) { return static_cast<uint32_t>(MATS == 2 ? code >> 5 : (code >> 5) * p.slots + (code & 31)); };
 
-    // Copies of words: 8 rows each, lane l the piece of 16 bytes (l & 7) ^ row of row l >> 3; of x: two columns each, a
-    // column's 8-element blocks b at b ^ (column & 7). Past the last column, its last block again (the scales there are zeros).
+    // Copies of words: 8 rows each, a row's 16-byte pieces p at p ^ (row / 2 % 8); of x: two columns each, a column's
+    // 8-element blocks b at b ^ column: 16 lanes' reads meet every bank once. Past the last column, its last block again (the
+    // scales there are zeros).
     const uint32_t lds = lds_addr(reinterpret_cast<const uint16_t*>(buf)), rbytes = p.cols / 2;
-    const uint32_t wrow = (first + (lane >> 3)) * rbytes, wpiece = 16 * ((lane & 7) ^ (lane >> 3));
+    const uint32_t wrow = (first + (lane >> 3)) * rbytes, wpiece = 16 * ((lane & 7) ^ (lane >> 4));   // (odd eights of rows: ^ 64)
     uint32_t xrow[2], xblock[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int col = 4 * wave + 2 * i + (lane >> 5);
         xrow[i] = (x_row(pair(col)) * XT + col / kPairs) * p.cols * 2;
-        xblock[i] = 16 * ((lane & 31) ^ (col & 7));
+        xblock[i] = 16 * ((lane & 31) ^ col);
     }
     auto stage = [&](int to, int g) {
-        const uint32_t at = lds + to * kSlimStage, w = wrow + min(wpiece + 128 * g, rbytes - 16);
+        const uint32_t at = lds + to * kSlimStage;
+        const uint32_t w[2] = {wrow + min(wpiece + 128 * g, rbytes - 16), wrow + min((wpiece ^ 64) + 128 * g, rbytes - 16)};
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             dma16(reinterpret_cast<const char*>(MATS == 2 && i >= 2 ? m1.w : m0.w) + static_cast<size_t>(8 * (MATS == 2 ? i & 1 : i)) * rbytes,
-                  w, at + (4 * wave + i) * 1024);
+                  w[i & 1], at + (4 * wave + i) * 1024);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
             dma16(reinterpret_cast<const char*>(a.x16), xrow[i] + min(xblock[i] + 512u * g, 4 * rbytes - 16),
@@ -1239,10 +1247,10 @@ __device__ __forceinline__ void slim_kernel(const MoeArgs& p, const TileArgs& a,
             u32x4_t words[2], B[4];
             f16x2_t sv[2][WT], cv[2][WT];
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) B[ks] = *reinterpret_cast<const u32x4_t*>(xs + 16 * ((16 * d + 4 * kg + ks) ^ (c & 7)));
+            for (int ks = 0; ks < 4; ++ks) B[ks] = *reinterpret_cast<const u32x4_t*>(xs + 16 * ((16 * d + 4 * kg + ks) ^ c));
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                words[j] = *reinterpret_cast<const u32x4_t*>(ws + 16 * j * 128 + 16 * ((4 * d + kg) ^ (c & 7)));
+                words[j] = *reinterpret_cast<const u32x4_t*>(ws + 16 * j * 128 + 16 * ((4 * d + kg) ^ (c >> 1)));
                 const uint32_t sc = sbl[(4 * g + 2 * d + (kg >> 1)) * kSlimRows + 32 * wave + 16 * j + c];
 #pragma unroll
                 for (int q = 0; q < WT; ++q) {

@@ -500,18 +500,23 @@ def pages_copy(ctx: Context, pools, src, dst) -> None:
 
 # ---- the expert block and the next token ---------------------------------------
 
+_WORDS, _SB = (torch.int32, torch.uint32), (torch.bfloat16, torch.float16)
+
+
 def _matrix(ctx: Context, name: str, q, bits: int, shape=None):
     """(w, scales, biases) of affine-quantized matrices on the context's device:
     their addresses, once shapes and types are what the library reads."""
     w, s, b = q
-    cols = w.shape[-1] * (32 // bits)
-    if w.dtype != _i32 and w.dtype != torch.uint32:
+    *rows, words = w.shape
+    cols = words * (32 // bits)
+    if w.dtype not in _WORDS:
         raise TypeError(f"{name}: the words must be int32")
-    if s.dtype != b.dtype or s.dtype not in (_bf16, _f16):
+    if s.dtype != b.dtype or s.dtype not in _SB:
         raise TypeError(f"{name}: scales and biases must both be bfloat16 or both float16")
-    if cols % 64 or s.shape != (*w.shape[:-1], cols // 64) or b.shape != s.shape:
+    groups = (*rows, cols // 64)
+    if cols % 64 or s.shape != groups or b.shape != groups:
         raise ValueError(f"{name}: scales and biases must be [.., cols / 64] of [.., {cols}]")
-    if shape is not None and (*w.shape[:-1], cols) != shape:
+    if shape is not None and (*rows, cols) != shape:
         raise ValueError(f"{name} must be {list(shape)}")
     return _ptr_on(ctx, name, w), _ptr_on(ctx, name + "'s scales", s), _ptr_on(ctx, name + "'s biases", b)
 

@@ -169,6 +169,19 @@ def test_down_in_slices(hip, n, y_dt):
     _check_down(_ctx(max_batch=n, max_prefill_tokens=1), w, h, _indices(rng, n, E, top, "holes"), DT[y_dt], "in place", True, rng)
 
 
+@pytest.mark.parametrize("x_dt", ["f32", "bf16"])
+def test_few_pairs_in_slices(hip, x_dt):
+    """The same with few pairs an expert, on the smallest workspace that takes them."""
+    rng = np.random.default_rng(6)
+    n, E, top, D, I = 50, 400, 16, 2048, 64
+    w = _weights(rng, E, D, I, "bf16", True)
+    idx = _indices(rng, n, E, top, "holes")
+    h = torch.from_numpy(rng.standard_normal((n, top + 1, I))).to(DEV, DT[x_dt])
+    ctx = _ctx(max_batch=n, max_prefill_tokens=1)
+    _check_down(ctx, w, h, idx, DT[x_dt], "in place", True, rng)
+    _check_gate_up(ctx, w, torch.from_numpy(rng.standard_normal((n, D))).to(DEV, DT[x_dt]), idx, DT[x_dt], "holes")
+
+
 def test_sizes_of_tokens(hip):
     """Every number of tokens about the borders between the forms."""
     import qff
