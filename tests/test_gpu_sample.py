@@ -75,6 +75,23 @@ def test_ties_and_borders(hip):
     _check(ctx, two, u, top_k=[150] * 8, top_p=[0.2, 0.5, 0.9, 0.95, 0.99, 0.999, 0.01, 0.7], temperature=[0.1, 5, 1, 100, 1e30, 1, 1e-30, 2])
 
 
+@pytest.mark.parametrize("vocab", [15872, 15873, 40000, 262144])
+def test_ties_of_a_whole_row(hip, vocab):
+    """More equal logits at a border than the last launch keeps in LDS, alone and beside larger and smaller ones."""
+    print("ties", vocab, flush=True)
+    ctx = _ctx()
+    rows = torch.zeros(6, vocab, device=DEV)
+    rows[1, ::3] = 0.25            # two values
+    rows[2, vocab // 2] = 3.0      # one ahead of the rest
+    rows[3, ::2] = -float("inf")
+    rows[4] = torch.arange(vocab, device=DEV) % 5 * 1e-3   # five values close together, all in the border's bin or not
+    rows[5, -1] = -20.0
+    u = [0.0, 0.3, 0.999, 0.5, 0.75, 1.0]
+    _check(ctx, rows, u, top_k=[1, vocab // 2, vocab - 1, 17, vocab // 3, vocab])
+    _check(ctx, rows, u, top_p=[0.5, 0.9, 0.1, 0.999, 0.3, 0.25])
+    _check(ctx, rows.bfloat16(), u, temperature=[0.7] * 6, top_k=[vocab // 2] * 6, top_p=[0.5] * 6, min_p=[0.0, 0.9, 0.0, 0.5, 0.99, 0.1])
+
+
 def test_greedy_and_odd_settings(hip):
     ctx = _ctx()
     inf, nan = float("inf"), float("nan")
