@@ -24,11 +24,14 @@
 // A row is read four times at most (three from the caches: 0.6 MB at 151936
 // logits); rows that need no border or no draw skip what they do not need.
 //
-// At 151936 fp32 logits (a read of all takes 0.1 us a row): one row 36 us, of
-// them max 4, bins 8, gather 7, pick 17; 32 rows with settings of their own
-// 7 + 18 + 18 + 23. What bounds it: the chain of dependent steps, for one row;
-// for 32 also the exponentials, one in 64 bits a token (an exact border needs a weight that
-// does not depend on who computes it), twice where min_p asks.
+// At 151936 fp32 logits (a read of all takes 0.1 us a row): one row 34 us, of
+// them max 4, bins 8, gather 6, pick 17; 32 rows with settings of their own
+// 7 + 16 + 17 + 23. What bounds it: the chain of dependent steps, for one row;
+// for 32 also the exponentials, one in 64 bits a token (an exact border needs a
+// weight that does not depend on who computes it), twice where min_p asks, and the
+// additions to bins in LDS. The row's bins are added up by atomics in the second launch (of
+// whole numbers, so in any order): by every chunk in the third, one row's gather
+// took 28 us and its bins 5.
 #include <algorithm>
 
 #include "common.hpp"
@@ -102,6 +105,20 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
+// e^d for d in (-32, 0]: d = k ln 2 + r, |r| <= ln 2 / 2, e^r by its Taylor series to
+// r^13 / 13! (what follows is 4e-18 of it). The library's, which serves other ranges
+// too, made 32 rows' bins 18 us instead of 16.
+__device__ __forceinline__ double exp_head(double d) {
+    const double k = rint(d * 1.4426950408889634);
+    const double r = fma(k, -2.3190468138462996e-17, fma(k, -0.6931471805599453, d));   // (ln 2 in two parts)
+    double p = 1.0 / 6227020800.0;
+    constexpr double kTerms[] = {1.0 / 479001600.0, 1.0 / 39916800.0, 1.0 / 3628800.0, 1.0 / 362880.0, 1.0 / 40320.0, 1.0 / 5040.0,
+                                 1.0 / 720.0, 1.0 / 120.0, 1.0 / 24.0, 1.0 / 6.0, 0.5, 1.0, 1.0};
+#pragma unroll
+    for (double c : kTerms) p = fma(p, r, c);
+    return ldexp(p, static_cast<int>(k));
+}
+
 // e^((l - best) / t) and its weight.
 struct Weigher {
     double best, inv, min_p;
@@ -110,9 +127,12 @@ struct Weigher {
     __device__ __forceinline__ double e(float l) const {
         if (l == bestf) return 1.0;
         const double d = (static_cast<double>(l) - best) * inv;
-        return d > -31.3 ? exp(d) : 0.0;   // (e^-31.3 rounds to no unit)
+        return d > -31.3 ? exp_head(d) : 0.0;   // (e^-31.3 rounds to no unit)
     }
-    static __device__ __forceinline__ u64 units(double e) { return static_cast<u64>(rint(e * kUnit)); }
+    // (e <= 1: added to 2^52, whose last bit is 1, it is rounded to the nearest unit and stands in the low bits)
+    static __device__ __forceinline__ u64 units(double e) {
+        return static_cast<u64>(__double_as_longlong(fma(e, kUnit, 4503599627370496.0))) & 0xfffffffffffffull;
+    }
     __device__ __forceinline__ u64 mass(float l) const { return units(e(l)); }
     __device__ __forceinline__ bool passes(double e) const { return !(min_p > 0.0) || e >= min_p; }
 };
@@ -196,6 +216,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_max_kernel(SampleArgs a
 template <int DT>
 __global__ __launch_bounds__(kSampleThreads) void sample_bins_kernel(SampleArgs a) {
     const int b = blockIdx.y, t = threadIdx.x, i0 = blockIdx.x * a.per, i1 = min(i0 + a.per, a.vocab);
+    float l[kBatch];   // (the first tokens are on their way beside what the row asks for)
+    load_logits<DT>(a, b, i0 + t, kSampleThreads, i1, l);
     const Row r = row_of(a, b);
     const float2 range = row_range(a, b);
     if (r.first || range.x == -INFINITY) return;
@@ -209,8 +231,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_bins_kernel(SampleArgs 
     const Weigher weigh(r, range.x);
     const Binner bin(r, range.x, range.y);
     for (int j = i0; j < i1; j += kBatch * kSampleThreads) {
-        float l[kBatch];
-        load_logits<DT>(a, b, j + t, kSampleThreads, i1, l);
+        if (j > i0) load_logits<DT>(a, b, j + t, kSampleThreads, i1, l);
 #pragma unroll
         for (int q = 0; q < kBatch; ++q) {
             const u64 m = weigh.mass(l[q]);
@@ -311,6 +332,8 @@ template <int DT>
 __global__ __launch_bounds__(kSampleThreads) void sample_gather_kernel(SampleArgs a) {
     const int b = blockIdx.y, t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int i0 = blockIdx.x * a.per, i1 = min(i0 + a.per, a.vocab);
+    float l[kBatch];
+    load_logits<DT>(a, b, i0 + wave * kBatch * 64 + lane, 64, i1, l);
     const Row r = row_of(a, b);
     const float2 range = row_range(a, b);
     if (r.first || range.x == -INFINITY) return;
@@ -329,8 +352,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_gather_kernel(SampleArg
         // a wave's tokens of a batch follow one another
         for (int j = i0; j < i1; j += kBatch * kSampleThreads) {
             const int at0 = j + wave * kBatch * 64 + lane;
-            float l[kBatch];
-            load_logits<DT>(a, b, at0, 64, i1, l);
+            if (j > i0) load_logits<DT>(a, b, at0, 64, i1, l);
             uint64_t m[kBatch];
             int own = 0;
 #pragma unroll
