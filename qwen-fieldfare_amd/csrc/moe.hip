@@ -77,68 +77,8 @@ __device__ __forceinline__ u32x4_t q4_to_bf16(uint32_t w, uint32_t one) {
     return r;
 }
 
-// 16 consecutive columns of x in a lane, and the bf16 operands of the two k
-// steps they make (columns 0-7 and 8-15), TERMS of them.
-template <int X_DT>
-struct XCols;
-template <>
-struct XCols<0> {
-    static constexpr int kTerms = 3;
-    f32x4_t v[4];
-    __device__ __forceinline__ void load(const void* x, size_t i) {
-        const f32x4_t* p = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(x) + i);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = p[k];
-    }
-    __device__ __forceinline__ void terms(int step, u32x4_t (&t)[3]) const {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float a = v[2 * step][j], b = v[2 * step + 1][j];
-            const uint32_t h = pack_bf16x2(a, b);
-            a -= __uint_as_float(h << 16);
-            b -= __uint_as_float(h & 0xffff0000u);
-            const uint32_t m = pack_bf16x2(a, b);
-            a -= __uint_as_float(m << 16);
-            b -= __uint_as_float(m & 0xffff0000u);
-            t[0][j] = h;
-            t[1][j] = m;
-            t[2][j] = pack_bf16x2(a, b);
-        }
-    }
-};
-template <>
-struct XCols<1> {
-    static constexpr int kTerms = 1;
-    u32x4_t v[2];
-    __device__ __forceinline__ void load(const void* x, size_t i) {
-        const u32x4_t* p = reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(x) + i);
-        v[0] = p[0];
-        v[1] = p[1];
-    }
-    // pairs (c0, c1), (c2, c3), (c4, c5), (c6, c7) -> (c0, c4), (c1, c5), (c2, c6), (c3, c7)
-    __device__ __forceinline__ u32x4_t paired(int step) const {
-        const u32x4_t u = v[step];
-        return u32x4_t{__builtin_amdgcn_perm(u[2], u[0], 0x05040100u), __builtin_amdgcn_perm(u[2], u[0], 0x07060302u),
-                       __builtin_amdgcn_perm(u[3], u[1], 0x05040100u), __builtin_amdgcn_perm(u[3], u[1], 0x07060302u)};
-    }
-    __device__ __forceinline__ void terms(int step, u32x4_t (&t)[1]) const { t[0] = paired(step); }
-};
-template <>
-struct XCols<2> : XCols<1> {
-    static constexpr int kTerms = 2;
-    __device__ __forceinline__ void terms(int step, u32x4_t (&t)[2]) const {
-        const u32x4_t u = paired(step);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float a = f16_to_f32(static_cast<uint16_t>(u[j])), b = f16_to_f32(static_cast<uint16_t>(u[j] >> 16));
-            const uint32_t h = pack_bf16x2(a, b);
-            a -= __uint_as_float(h << 16);
-            b -= __uint_as_float(h & 0xffff0000u);
-            t[0][j] = h;
-            t[1][j] = pack_bf16x2(a, b);
-        }
-    }
-};
+// bf16 terms of a value of x that hold all of it.
+constexpr int x_terms(int dtype) { return dtype == 0 ? 3 : dtype == 1 ? 1 : 2; }
 
 // The words of a 128-column span's two groups for this lane's quarter: w[2 gi
 // + step] feeds k step `step` of group gi.
@@ -150,7 +90,6 @@ __device__ __forceinline__ void span_words(const u32x4_t& u, uint32_t (&w)[4]) {
     w[2] = a[1];
     w[3] = b[1];
 }
-
 
 constexpr int kGroups = 4;   // groups of 64 columns that a wave requests at once: two 128-column spans
 
@@ -167,7 +106,7 @@ constexpr int kOneWaves = 8, kChunk = 64 * kGroups;
 // A lane's four columns of x, and their terms in the k order.
 template <int X_DT>
 struct XFour {
-    static constexpr int kTerms = XCols<X_DT>::kTerms;
+    static constexpr int kTerms = x_terms(X_DT);
     float v[4];
     __device__ __forceinline__ void load(const void* x, size_t i) {
         if constexpr (X_DT == 0) {
@@ -245,7 +184,7 @@ struct OneStep {
     }
     // xs: the wave's own [kTerms][kChunk]
     __device__ __forceinline__ void add(float (&acc)[MATS], int groups, uint16_t* xs, int lane) const {
-        constexpr int T = XCols<X_DT>::kTerms;
+        constexpr int T = x_terms(X_DT);
         const int kg = lane >> 4;
         const uint32_t one = q4_one();
         const u32x4_t ones{one, one, one, one};
@@ -290,7 +229,7 @@ struct OneStep {
 // Gate and up: one workgroup per (16 rows, pair), its waves over K.
 template <int X_DT, int SB_DT, int H_DT>
 __global__ __launch_bounds__(64 * kOneWaves) void moe_gate_up_one_kernel(MoeArgs p, void* __restrict__ h) {
-    __shared__ __attribute__((aligned(16))) uint16_t xs[kOneWaves][XCols<X_DT>::kTerms * kChunk];
+    __shared__ __attribute__((aligned(16))) uint16_t xs[kOneWaves][x_terms(X_DT) * kChunk];
     __shared__ float red[kOneWaves][2][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, kg = lane >> 4;
     const int tok = blockIdx.y / p.slots, j = blockIdx.y % p.slots, G = p.cols / 64, row0 = 16 * blockIdx.x;
@@ -329,7 +268,7 @@ template <int X_DT, int SB_DT, int Y_DT>
 __global__ __launch_bounds__(64 * kOneWaves) void moe_down_one_kernel(MoeArgs p, const float* __restrict__ scores,
                                                                       const float* __restrict__ coef, const void* residual,
                                                                       void* y) {
-    __shared__ __attribute__((aligned(16))) uint16_t xs[kOneWaves][XCols<X_DT>::kTerms * kChunk];
+    __shared__ __attribute__((aligned(16))) uint16_t xs[kOneWaves][x_terms(X_DT) * kChunk];
     __shared__ float red[kOneWaves][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, kg = lane >> 4;
     const int tok = blockIdx.y, row0 = 16 * blockIdx.x, G = p.cols / 64, steps = (G + kGroups - 1) / kGroups;
