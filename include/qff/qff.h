@@ -263,10 +263,11 @@ int qff_rms_norm(qff_ctx* ctx, qff_stream_t stream, const void* x, qff_dtype x_d
  * power-of-two shifts: a weight is scale (q - 8), exact, and a part constant over
  * its group of 64 columns, bias + 8 scale, which meets the group's sum of x; an
  * fp32 input is two fp16 terms (2^-22 of its value, or 2^-37 of its row's
- * largest), a BF16 one is exact beside the same 2^-37. With a BF16 output and 33 tokens or more fp32 inputs
- * and F16 scales times q - 8 keep 11 bits, and what moe_down sums over the pairs 11 bits
- * relative to the largest of each 64 outputs of a pair. Scales lie in 2^-22 .. 31 (smaller ones
- * lose bits) and |bias + 8 scale| is at most 8. */
+ * largest), a BF16 one is exact beside the same 2^-37. With a BF16 output and 33
+ * tokens or more, fp32 inputs and the products of F16 scales with q - 8 may keep 11
+ * bits, and so may what moe_down sums over the pairs, relative to the largest of
+ * each 64 outputs of a pair. There, scales lie in 2^-22 .. 31 in magnitude (smaller
+ * ones lose bits; 0 is exact) and |bias + 8 scale| is at most 8. */
 int qff_moe_gate_up(qff_ctx* ctx, qff_stream_t stream, const qff_moe_weights* p, const void* x,
                     qff_dtype x_dtype, const int32_t* indices, int top, void* h, qff_dtype h_dtype,
                     int tokens);
