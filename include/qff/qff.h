@@ -261,7 +261,8 @@ int qff_rms_norm(qff_ctx* ctx, qff_stream_t stream, const void* x, qff_dtype x_d
  * What both halves round, beside their outputs and the fp32 sums: up to 72 pairs
  * (token, slot; down: 200) nothing. Above, products run on fp16 operands after
  * power-of-two shifts: a weight is scale (q - 8), exact, and a part constant over
- * its group of 64 columns, bias + 8 scale, which meets the group's sum of x; an
+ * its group of 64 columns, bias + 8 scale (22 bits of it, or 2^-48), which meets the
+ * group's sum of x; an
  * fp32 input is two fp16 terms (2^-22 of its value, or 2^-37 of its row's
  * largest), a BF16 one is exact beside the same 2^-37. With a BF16 output and 33
  * tokens or more, fp32 inputs and the products of F16 scales with q - 8 may keep 11

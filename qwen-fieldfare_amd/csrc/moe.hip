@@ -497,7 +497,7 @@ __device__ __forceinline__ void moe_x16(const void* __restrict__ x, uint16_t* __
     // (exponents of at least -127 keep their powers finite for the smallest rows)
     const auto shift = [](float m) { return m > 0.0f ? max(__builtin_amdgcn_frexp_expf(m) - 14, -127) : 0; };
     const int e = COPY ? shift(group_max<64>(mx)) : 0, es = shift(group_max<64>(ms));
-    if (lane == 0) fac[row] = make_float2(ldexpf(1.0f, e - 8), ldexpf(1.0f, es - e - 5));
+    if (lane == 0) fac[row] = make_float2(ldexpf(1.0f, e - 8), ldexpf(1.0f, es - e - 4));
     const float p = ldexpf(1.0f, -e), ps = ldexpf(1.0f, -es);
     const int G = cols / 64, gp = (G + kSumsPad - 1) / kSumsPad * kSumsPad;
     uint16_t* const so = sums + static_cast<size_t>(row) * 2 * gp;
@@ -643,8 +643,10 @@ __device__ __forceinline__ constexpr int tile_terms_at(int xt, int mmt, int grou
     return groups <= 16 ? (tile_stages(xt, mmt) - 1) * tile_stage_bytes(xt, mmt) : 0;
 }
 
-// The constant parts' terms of groups k0 .. k0 + 31: (b + 8 s) 2^13 in two fp16
-// terms. Thread t forms row t's (of two matrices 32 rows of the first, 32 of the
+// The constant parts' terms of groups k0 .. k0 + 31: (b + 8 s) 2^12 as an fp16 term and
+// 2^11 times its rest as another (which meets the sums 2^-11 times), so that 8 stays inside
+// fp16 (8 2^13 does not) and 22 bits are there down to 2^-26, an absolute 2^-48 below.
+// Thread t forms row t's (of two matrices 32 rows of the first, 32 of the
 // second, ..): [16 groups][term][row][16], a row's halves swapped in every other four
 // rows. Groups past the last (which meet sums of zero) take its.
 template <int MATS>
@@ -660,13 +662,20 @@ __device__ __forceinline__ void const_terms(const u32x4_t& s8, const u32x4_t& b8
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const uint16_t sq = static_cast<uint16_t>(s8[j] >> (16 * i)), bq = static_cast<uint16_t>(b8[j] >> (16 * i));
-            v[i] = 8192.0f * fmaf(8.0f, elem<SB_DT>::load(&sq, 0), elem<SB_DT>::load(&bq, 0));
+            v[i] = 4096.0f * fmaf(8.0f, elem<SB_DT>::load(&sq, 0), elem<SB_DT>::load(&bq, 0));
         }
-        uint32_t hi, lo;
-        split_f16x2(v[0], v[1], hi, lo);
-        bh[j] = hi;
-        bl[j] = lo;
+        const f16x2_t hi = {static_cast<_Float16>(v[0]), static_cast<_Float16>(v[1])};
+        bh[j] = __builtin_bit_cast(uint32_t, hi);
+        bl[j] = pack_f16x2(2048.0f * (v[0] - static_cast<float>(hi[0])), 2048.0f * (v[1] - static_cast<float>(hi[1])));
     }
+}
+// Eight sums for the products with bl.
+__device__ __forceinline__ u32x4_t rest_sums(const u32x4_t& x) {
+    constexpr _Float16 k = static_cast<_Float16>(1.0f / 2048.0f);
+    u32x4_t r;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, static_cast<uint32_t>(x[j])) * f16x2_t{k, k});
+    return r;
 }
 template <int SB_DT>
 __device__ __forceinline__ void put_terms(uint16_t* to, int k, const u32x4_t& s8, const u32x4_t& b8) {
@@ -751,7 +760,7 @@ __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, co
         }
         const uint16_t* const terms = Xl + tile_terms_at(XT, MMT, G) / 2;
         for (int k0 = 0; k0 < G; k0 += 16) {
-            u32x4_t xh[NMT], xl[NMT];
+            u32x4_t xh[NMT], xl[NMT], xr[NMT];
 #pragma unroll
             for (int mt = 0; mt < NMT; ++mt) {
                 xh[mt] = *reinterpret_cast<const u32x4_t*>(S[mt] + k0);
@@ -769,13 +778,15 @@ __device__ __forceinline__ void tile_run(const MoeArgs& p, const TileArgs& a, co
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
+            for (int mt = 0; mt < NMT; ++mt) xr[mt] = rest_sums(xh[mt]);
+#pragma unroll
             for (int rt = 0; rt < 2; ++rt) {
                 const int q = 64 * wave + 32 * rt + r;
                 const uint16_t* o = terms + k0 % 32 * 2 * kTileRows + 16 * q + 8 * (h ^ (q >> 2 & 1));
                 const u32x4_t bh = *reinterpret_cast<const u32x4_t*>(o), bl = *reinterpret_cast<const u32x4_t*>(o + 16 * kTileRows);
 #pragma unroll
                 for (int mt = 0; mt < NMT; ++mt) {
-                    acc[rt][mt] = mfma_32x32x16_f16(bl, xh[mt], acc[rt][mt]);
+                    acc[rt][mt] = mfma_32x32x16_f16(bl, xr[mt], acc[rt][mt]);
                     acc[rt][mt] = mfma_32x32x16_f16(bh, xl[mt], acc[rt][mt]);
                     acc[rt][mt] = mfma_32x32x16_f16(bh, xh[mt], acc[rt][mt]);
                 }
@@ -1151,6 +1162,7 @@ __device__ __forceinline__ void slim_kernel(const MoeArgs& p, const TileArgs& a,
                     if (i < steps) stage(i, i);
                 __builtin_amdgcn_sched_barrier(0);
             }
+            const u32x4_t xr = rest_sums(xh);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 if (k < G) {
@@ -1161,7 +1173,7 @@ __device__ __forceinline__ void slim_kernel(const MoeArgs& p, const TileArgs& a,
                 }
                 u32x4_t bh, bl;
                 const_terms<SB_DT>(s8[j], b8[j], bh, bl);
-                acc[j] = mfma_16x16x32_f16(bl, xh, acc[j]);
+                acc[j] = mfma_16x16x32_f16(bl, xr, acc[j]);
                 if constexpr (XT == 1) acc[j] = mfma_16x16x32_f16(bh, xl, acc[j]);
                 acc[j] = mfma_16x16x32_f16(bh, xh, acc[j]);
             }
