@@ -444,13 +444,15 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const float* __restric
 // it; for bf16 outputs (q - 8) s is rounded to fp16 (WT = 1).
 // x enters as fp16 after a power-of-two shift that puts its row's largest
 // magnitude into [2^13, 2^14), for fp32 x and F32 or F16 outputs as two terms of 11
-// bits (XT = 2); fp16 rows of h are taken as they lie. s 256 and x lie inside
-// fp16's normal range for scales of 2^-22 .. 31; b + 8 s may be up to 8 in magnitude.
+// bits (XT = 2); fp16 rows of h are taken as they lie. The scale enters as 64 s: at 31 the
+// FMA's 24 (64 s) is 47616, inside fp16 (256 s left it from 10.7 on), and at 2^-22 the last
+// of eight bits is one of fp16's smallest numbers, 2^-23, which the FMA and the matrix
+// cores take as they are; b + 8 s may be up to 8 in magnitude.
 // So F32 and F16 outputs are sums of exact products (up to 2^-22 of x), and
 // bf16 ones carry 11 bits an operand (a bf16 result has 8).
 
 // Rows of x for the tiles: XT fp16 terms [row][XT][cols] (each 8 columns in the
-// order c0, c4, c1, c5, .., the nibbles' own) and the row's factor 2^(e - 8); and
+// order c0, c4, c1, c5, .., the nibbles' own) and the row's factor 2^(e - 6); and
 // the sums of its groups as two fp16 terms [row][2][gp] (gp: groups rounded up to
 // 16, the rest zeros), shifted as x is, with the factor that takes them back. One
 // wave a row. COPY false (fp16 rows, used where they lie): the sums alone.
@@ -497,7 +499,7 @@ __device__ __forceinline__ void moe_x16(const void* __restrict__ x, uint16_t* __
     // (exponents of at least -127 keep their powers finite for the smallest rows)
     const auto shift = [](float m) { return m > 0.0f ? max(__builtin_amdgcn_frexp_expf(m) - 14, -127) : 0; };
     const int e = COPY ? shift(group_max<64>(mx)) : 0, es = shift(group_max<64>(ms));
-    if (lane == 0) fac[row] = make_float2(ldexpf(1.0f, e - 8), ldexpf(1.0f, es - e - 4));
+    if (lane == 0) fac[row] = make_float2(ldexpf(1.0f, e - 6), ldexpf(1.0f, es - e - 6));
     const float p = ldexpf(1.0f, -e), ps = ldexpf(1.0f, -es);
     const int G = cols / 64, gp = (G + kSumsPad - 1) / kSumsPad * kSumsPad;
     uint16_t* const so = sums + static_cast<size_t>(row) * 2 * gp;
@@ -551,13 +553,13 @@ __global__ __launch_bounds__(kPlanThreads) void moe_prepare_kernel(PlanArgs q, c
 
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 
-// A group's scale for one row of the tile: s 256 (its first eight bits for WT = 2)
+// A group's scale for one row of the tile: 64 s (its first eight bits for WT = 2)
 // and the rest of it.
 template <int WT>
 using tile_sb = std::conditional_t<WT == 1, uint16_t, uint32_t>;
 template <int SB_DT, int WT>
 __device__ __forceinline__ tile_sb<WT> tile_scale(uint16_t s) {
-    const float v = 256.0f * elem<SB_DT>::load(&s, 0);
+    const float v = 64.0f * elem<SB_DT>::load(&s, 0);
     if constexpr (WT == 1) {
         return f32_to_f16(v);
     } else {
@@ -566,7 +568,7 @@ __device__ __forceinline__ tile_sb<WT> tile_scale(uint16_t s) {
     }
 }
 
-// Nibble word -> fp16 pairs 256 s (q - 8): the pairs (q_j, q_j+4), or with NATURAL
+// Nibble word -> fp16 pairs 64 s (q - 8): the pairs (q_j, q_j+4), or with NATURAL
 // (q_2j, q_2j+1) from the even and the odd nibbles' bytes.
 template <bool EXACT, bool NATURAL>
 __device__ __forceinline__ u32x4_t q4_to_f16(uint32_t w, f16x2_t s, f16x2_t c, uint32_t k16) {

@@ -41,7 +41,7 @@ def _extreme(rng, shape, cols, sb, end):
         w.fill_(-2004318072)
         s, c = np.zeros(g), _bits(rng, g, 2.0 ** -34, 2.0 ** -30, 8)
     else:
-        s = _bits(rng, g, 2.0 ** -22, 2.0 ** -20, 3)
+        s = _bits(rng, g, 2.0 ** -22, 2.0 ** -20, 8 if sb == "bf16" else 3)   # (fp16 ends at 2^-24)
         c = _bits(rng, g, 2.0 ** -22, 2.0 ** -19, 4)
     s = torch.from_numpy(s).to(DT[sb])
     b = (torch.from_numpy(c) - 8 * s.double()).to(DT[sb])
@@ -93,7 +93,7 @@ def _terms(form, dtype, sb, out):
 
 
 @pytest.mark.parametrize("form", FORMS)
-@pytest.mark.parametrize("end", ["parts", "small parts"])
+@pytest.mark.parametrize("end", ["parts", "small parts", "large", "small"])
 @pytest.mark.parametrize("x_dt,h_dt,sb", [("f32", "f32", "bf16"), ("f32", "f16", "f16"), ("bf16", "f32", "f16"), ("f32", "bf16", "bf16"),
                                           ("bf16", "bf16", "f16")])
 def test_gate_up_at_the_ends(hip, form, end, x_dt, h_dt, sb):
@@ -119,7 +119,7 @@ def test_gate_up_at_the_ends(hip, form, end, x_dt, h_dt, sb):
 
 
 @pytest.mark.parametrize("form", DOWN_FORMS)
-@pytest.mark.parametrize("end", ["parts", "small parts"])
+@pytest.mark.parametrize("end", ["parts", "small parts", "large", "small"])
 @pytest.mark.parametrize("h_dt,y_dt,sb", [("f32", "f32", "f16"), ("f16", "f32", "bf16"), ("bf16", "f32", "f16"), ("f32", "bf16", "bf16"),
                                           ("f16", "bf16", "f16")])
 def test_down_at_the_ends(hip, form, end, h_dt, y_dt, sb):
