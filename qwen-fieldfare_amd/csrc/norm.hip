@@ -37,9 +37,10 @@ __device__ __forceinline__ void load8(const void* p, size_t i, float (&v)[8]) {
     }
 }
 
+// (x may be y: neither is declared to overlap nothing)
 template <int X_DT, int Y_DT, int W_DT, int NB>
-__global__ __launch_bounds__(kNormThreads) void rms_norm_kernel(const void* __restrict__ x, const void* __restrict__ w,
-                                                                float eps, const uint32_t* __restrict__ gw,
+__global__ __launch_bounds__(kNormThreads) void rms_norm_kernel(const void* x, const void* __restrict__ w, float eps,
+                                                                const uint32_t* __restrict__ gw,
                                                                 const uint16_t* __restrict__ gs,
                                                                 const uint16_t* __restrict__ gb, int g_bf16,
                                                                 void* y, float* __restrict__ coef, int cols) {
