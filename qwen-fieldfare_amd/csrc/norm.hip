@@ -101,12 +101,20 @@ __global__ __launch_bounds__(kNormThreads) void rms_norm_kernel(const void* x, c
 template <int X_DT, int Y_DT, int W_DT>
 static void rms_norm_launch(hipStream_t stream, const void* x, const void* w, float eps, const uint32_t* gw,
                             const uint16_t* gs, const uint16_t* gb, int g_bf16, void* y, float* coef, int cols, int tokens) {
-#define QFF_NORM(NB) \
-    rms_norm_kernel<X_DT, Y_DT, W_DT, NB><<<tokens, kNormThreads, 0, stream>>>(x, w, eps, gw, gs, gb, g_bf16, y, coef, cols)
-    if (cols <= 8 * kNormThreads) QFF_NORM(1);
-    else if (cols <= 16 * kNormThreads) QFF_NORM(2);
-    else QFF_NORM(4);
+    constexpr int kMost = static_cast<int>(((1ll << 32) - 1) / kNormThreads);   // a grid has fewer than 2^32 work-items
+    for (int t0 = 0; t0 < tokens; t0 += kMost) {
+        const int n = tokens - t0 < kMost ? tokens - t0 : kMost;
+        const size_t at = static_cast<size_t>(t0) * cols;
+        const void* const from = static_cast<const char*>(x) + at * (X_DT == 0 ? 4 : 2);
+        void* const to = static_cast<char*>(y) + at * (Y_DT == 0 ? 4 : 2);
+        float* const c = gw ? coef + t0 : nullptr;
+#define QFF_NORM(NB) rms_norm_kernel<X_DT, Y_DT, W_DT, NB><<<n, kNormThreads, 0, stream>>>(from, w, eps, gw, gs, gb, g_bf16, to, c, cols)
+        if (cols <= 8 * kNormThreads) QFF_NORM(1);
+        else if (cols <= 16 * kNormThreads) QFF_NORM(2);
+        else QFF_NORM(4);
 #undef QFF_NORM
+        if (tokens - t0 <= kMost) break;   // (t0 stays within an int)
+    }
 }
 
 hipError_t launch_rms_norm(qff_ctx* ctx, hipStream_t stream, const void* x, qff_dtype x_dtype, const void* norm_w,

@@ -115,3 +115,19 @@ def test_rows_of_any_size(hip, n, E, top, x_dt):
         ref, err = R.gate_up(w["gate"], w["up"], None, None, x64, idx, x_err)
     # (what lies below 2^-120, where fp32's smallest numbers end, is held to 2^-149)
     assert (np.abs(got - ref) <= err * (1 + R.U32) + R.U32 * np.abs(ref) + 2.0 ** -148).all()
+
+
+def test_rms_norm_of_more_rows_than_a_grid(hip):
+    """2^24 + 5 rows: a launch holds 2^24 - 1 (2^32 work-items, 256 a row). Rows on both sides of the border equal those
+    of a call of their own."""
+    import qff
+    n, cols, ctx = 2 ** 24 + 5, 64, _ctx()
+    x = torch.randn(2 ** 16, cols, device=DEV).bfloat16().repeat(n // 2 ** 16 + 1, 1)[:n]
+    w = 1 + 0.1 * torch.randn(cols, device=DEV)
+    gate = _to(R.quantized(np.random.default_rng(0), (1,), cols, 8, torch.bfloat16))
+    y, coef = torch.full_like(x, 7.0), torch.full((n,), 7.0, device=DEV)
+    qff.rms_norm(ctx, x, w, gate=gate, out=y, coef=coef)
+    for a, b in ((0, 64), (2 ** 24 - 40, n)):
+        ref = qff.rms_norm(ctx, x[a:b], w, gate=gate)
+        assert torch.equal(y[a:b], ref[0]) and torch.equal(coef[a:b], ref[1])
+    assert torch.equal(y[:2 ** 16], y[2 ** 23:2 ** 23 + 2 ** 16])
