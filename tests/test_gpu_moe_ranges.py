@@ -1,5 +1,4 @@
-"""The expert block at the ends of what its weights and inputs may hold, and in the forms and sizes beside those of
-tests/test_gpu_moe.py. Rows of x (or h) with one column that is not 0 make every output a single weight times x: a few
+"""The expert block at the ends of what its weights may hold, and between them, in every form. Rows of x (or h) with one column that is not 0 make every output a single weight times x: a few
 roundings, so that a bound is sharp enough to show a part that a kernel lost."""
 import numpy as np
 import pytest
@@ -32,6 +31,8 @@ def _extreme(rng, shape, cols, sb, end):
     if end == "large":
         s = rng.choice([31.0, 30.875, 24.0, 16.125, 10.75, 10.5], g) * rng.choice([-1.0, 1.0], g)
         c = rng.choice([0.0, 1.0, -3.0, 7.0, 8.0, -8.0], g)
+    elif end == "usual":   # neither end, scales of all the bits that their type has
+        s, c = (_bits(rng, g, lo, hi, 8 if sb == "bf16" else 11) for lo, hi in ((2.0 ** -8, 2.0 ** -6), (2.0 ** -6, 2.0 ** -3)))
     elif end == "parts":   # the constant parts alone: every nibble 8
         w.fill_(-2004318072)
         s = rng.choice([0.0, 1.0, 2.0 ** -10, 2.0 ** -20], g)
@@ -93,7 +94,7 @@ def _terms(form, dtype, sb, out):
 
 
 @pytest.mark.parametrize("form", FORMS)
-@pytest.mark.parametrize("end", ["parts", "small parts", "large", "small"])
+@pytest.mark.parametrize("end", ["parts", "small parts", "large", "small", "usual"])
 @pytest.mark.parametrize("x_dt,h_dt,sb", [("f32", "f32", "bf16"), ("f32", "f16", "f16"), ("bf16", "f32", "f16"), ("f32", "bf16", "bf16"),
                                           ("bf16", "bf16", "f16")])
 def test_gate_up_at_the_ends(hip, form, end, x_dt, h_dt, sb):
@@ -103,7 +104,7 @@ def test_gate_up_at_the_ends(hip, form, end, x_dt, h_dt, sb):
     D, I = 192, 128
     rng = np.random.default_rng(len(form) + 10 * len(end))
     gate, up = (_extreme(rng, (E, I), D, sb, end) for _ in range(2))
-    x = _one_column(rng, (n,), D, {"large": 2.0 ** -6, "small": 2.0 ** 20, "parts": 0.5, "small parts": 2.0 ** 20}[end]).to(DT[x_dt])
+    x = _one_column(rng, (n,), D, {"large": 2.0 ** -6, "small": 2.0 ** 20, "parts": 0.5, "small parts": 2.0 ** 20, "usual": 32.0}[end]).to(DT[x_dt])
     idx = _indices(rng, n, E, top, "any")
     got = _np64(qff.moe_gate_up(_ctx(), qff.ExpertWeights(_to(gate), _to(up)), x.to(DEV), torch.from_numpy(idx).to(DEV), out_dtype=DT[h_dt]))
     x64, terms = x.double().numpy(), _terms(form, x_dt, sb, h_dt)
@@ -119,7 +120,7 @@ def test_gate_up_at_the_ends(hip, form, end, x_dt, h_dt, sb):
 
 
 @pytest.mark.parametrize("form", DOWN_FORMS)
-@pytest.mark.parametrize("end", ["parts", "small parts", "large", "small"])
+@pytest.mark.parametrize("end", ["parts", "small parts", "large", "small", "usual"])
 @pytest.mark.parametrize("h_dt,y_dt,sb", [("f32", "f32", "f16"), ("f16", "f32", "bf16"), ("bf16", "f32", "f16"), ("f32", "bf16", "bf16"),
                                           ("f16", "bf16", "f16")])
 def test_down_at_the_ends(hip, form, end, h_dt, y_dt, sb):
