@@ -500,6 +500,7 @@ def pages_copy(ctx: Context, pools, src, dst) -> None:
 
 # ---- the expert block and the next token ---------------------------------------
 
+_data_ptr = torch.Tensor.data_ptr
 _WORDS, _SB = (torch.int32, torch.uint32), (torch.bfloat16, torch.float16)
 
 
@@ -526,7 +527,8 @@ class ExpertWeights:
     matrices: gate, up [experts, inter, hidden], down [experts, hidden, inter] and
     the shared expert's [inter, hidden], [hidden, inter] (None: there is none).
     moe_gate_up needs gate and up, moe_down needs down; what only the other needs
-    may be None. The tensors are kept and stay where they are."""
+    may be None. The tensors are kept; a call whose matrices no longer lie where they
+    lay (set_, resize_, .data) checks all of them again and reads the new ones."""
 
     def __init__(self, gate=None, up=None, down=None, shared_gate=None, shared_up=None, shared_down=None):
         self.matrices = (gate, up, down, shared_gate, shared_up, shared_down)
@@ -545,11 +547,18 @@ class ExpertWeights:
         self.experts = w.shape[0]
         self.inter, self.hidden = (rows, cols) if gate is not None else (cols, rows)
         self.dtype = next(q[1].dtype for q in self.matrices if q is not None)
-        self._packed = None   # (context's device, parameter block): made by the first call, checked there
+        # the tensors that gate_up and down read
+        self._read = tuple(tuple(t for i in at for t in self.matrices[i] or ()) for at in ((0, 1, 3, 4), (2, 5)))
+        # (context's device, both halves' addresses, parameter block, aliases): made by the first call, checked there. The
+        # aliases keep the memory that was checked, so that nothing else can come to lie at its addresses.
+        self._packed = None
 
-    def _block(self, ctx: Context) -> bytes:
-        if self._packed is not None and self._packed[0] == ctx.device:
-            return self._packed[1]
+    def _block(self, ctx: Context, half: int) -> bytes:
+        """The parameter block for moe_gate_up (half 0) or moe_down (1)."""
+        P = self._packed
+        if P is not None and P[0] == ctx.device and P[1][half] == tuple(map(_data_ptr, self._read[half])):
+            return P[2]
+        self._packed = None
         up, down = (self.inter, self.hidden), (self.hidden, self.inter)
         flat = []
         for name, q, shape in zip(("gate", "up", "down", "shared_gate", "shared_up", "shared_down"), self.matrices,
@@ -558,14 +567,17 @@ class ExpertWeights:
                 raise TypeError("all scales and biases must have one type")
             flat += _matrix(ctx, name, q, 4, shape) if q is not None else (0, 0, 0)
         block = _P_MOE.pack(*flat, _DT[self.dtype], self.experts, self.hidden, self.inter)
-        self._packed = (ctx.device, block)
+        self._packed = (ctx.device, tuple(tuple(map(_data_ptr, r)) for r in self._read), block,
+                        [t.detach() for r in self._read for t in r])
         return block
 
 
-def _indices(ctx: Context, indices, tokens: int) -> int:
-    if indices.dim() != 2 or indices.shape[0] != tokens:
+def _indices(ctx: Context, indices, tokens: int):
+    """Their address and shape."""
+    shape = indices.shape
+    if len(shape) != 2 or shape[0] != tokens:
         raise ValueError(f"indices must be [{tokens}, top]")
-    return _ptr_on(ctx, "indices", indices, _i32)
+    return _ptr_on(ctx, "indices", indices, _i32), shape
 
 
 def rms_norm(ctx: Context, x: torch.Tensor, norm_w: torch.Tensor, eps: float = 1e-6, gate=None, out=None, out_dtype=None,
@@ -602,18 +614,19 @@ def moe_gate_up(ctx: Context, experts: ExpertWeights, x: torch.Tensor, indices: 
     (f32 or bf16), indices int32 [tokens, top] -> silu(x Wg^T) * (x Wu^T) [tokens,
     top (+ 1, the shared expert), inter] (f32, bf16 or f16). An index that is no
     expert's leaves its row as it was (a new tensor's: undefined)."""
-    n = x.shape[0]
     if experts.matrices[0] is None:
         raise ValueError("the weights have no gate and up matrices")
-    if x.dim() != 2 or x.shape[1] != experts.hidden:
+    shape = x.shape
+    if len(shape) != 2 or shape[1] != experts.hidden:
         raise ValueError(f"x must be [tokens, {experts.hidden}]")
-    block, ip = experts._block(ctx), _indices(ctx, indices, n)
-    shape = (n, indices.shape[1] + (experts.matrices[3] is not None), experts.inter)
+    n, block = shape[0], experts._block(ctx, 0)
+    ip, (_, top) = _indices(ctx, indices, n)
+    shape = (n, top + (experts.matrices[3] is not None), experts.inter)
     if out is None:
         out = torch.empty(shape, dtype=out_dtype, device=x.device)
     elif out.shape != shape:
         raise ValueError(f"out must be {list(shape)}")
-    st = _hot().qff_moe_gate_up(ctx.handle, _stream_of(ctx), block, _ptr_on(ctx, "x", x), _code(x), ip, indices.shape[1],
+    st = _hot().qff_moe_gate_up(ctx.handle, _stream_of(ctx), block, _ptr_on(ctx, "x", x), _code(x), ip, top,
                                 _ptr_on(ctx, "out", out), _code(out), n)
     if st:
         raise QffError("qff_moe_gate_up", st)
@@ -626,29 +639,32 @@ def moe_down(ctx: Context, experts: ExpertWeights, h: torch.Tensor, indices: tor
     f16), weighted with scores f32 [tokens, top] (the shared expert's row with coef f32
     [tokens], or 1) and summed on top of residual [tokens, hidden] (out's type; may be
     out) -> [tokens, hidden] (f32 or bf16)."""
-    n = h.shape[0]
     if experts.matrices[2] is None:
         raise ValueError("the weights have no down matrices")
-    block, ip = experts._block(ctx), _indices(ctx, indices, n)
-    if h.shape != (n, indices.shape[1] + (experts.matrices[5] is not None), experts.inter):
-        raise ValueError(f"h must be [{n}, {indices.shape[1] + (experts.matrices[5] is not None)}, {experts.inter}]")
-    if scores.shape != indices.shape:
-        raise ValueError(f"scores must be {list(indices.shape)}")
+    shape = h.shape
+    n, block = shape[0], experts._block(ctx, 1)
+    ip, (_, top) = _indices(ctx, indices, n)
+    slots = top + (experts.matrices[5] is not None)
+    if shape != (n, slots, experts.inter):
+        raise ValueError(f"h must be [{n}, {slots}, {experts.inter}]")
+    if scores.shape != (n, top):
+        raise ValueError(f"scores must be {[n, top]}")
+    shape = (n, experts.hidden)
     if out is None:
-        out = torch.empty(n, experts.hidden, dtype=out_dtype, device=h.device)
-    elif out.shape != (n, experts.hidden):
-        raise ValueError(f"out must be [{n}, {experts.hidden}]")
+        out = torch.empty(shape, dtype=out_dtype, device=h.device)
+    elif out.shape != shape:
+        raise ValueError(f"out must be {list(shape)}")
     cp = rp = 0
     if coef is not None:
         if coef.numel() != n:
             raise ValueError(f"coef must be [{n}]")
         cp = _ptr_on(ctx, "coef", coef, _f32)
     if residual is not None:
-        if residual.shape != out.shape or residual.dtype != out.dtype:
+        if residual.dtype != out.dtype or residual.shape != shape:
             raise ValueError("a residual must match its output's dtype and shape")
         rp = _ptr_on(ctx, "residual", residual)
     st = _hot().qff_moe_down(ctx.handle, _stream_of(ctx), block, _ptr_on(ctx, "h", h), _code(h), ip,
-                             _ptr_on(ctx, "scores", scores, _f32), indices.shape[1], cp, rp, _ptr_on(ctx, "out", out),
+                             _ptr_on(ctx, "scores", scores, _f32), top, cp, rp, _ptr_on(ctx, "out", out),
                              _code(out), n)
     if st:
         raise QffError("qff_moe_down", st)
