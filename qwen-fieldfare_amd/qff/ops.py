@@ -504,9 +504,8 @@ _data_ptr = torch.Tensor.data_ptr
 _WORDS, _SB = (torch.int32, torch.uint32), (torch.bfloat16, torch.float16)
 
 
-def _matrix(ctx: Context, name: str, q, bits: int, shape=None):
-    """(w, scales, biases) of affine-quantized matrices on the context's device:
-    their addresses, once shapes and types are what the library reads."""
+def _check_matrix(name: str, q, bits: int, shape=None):
+    """Whether (w, scales, biases) of affine-quantized matrices have shapes and types that the library reads."""
     w, s, b = q
     *rows, words = w.shape
     cols = words * (32 // bits)
@@ -519,6 +518,12 @@ def _matrix(ctx: Context, name: str, q, bits: int, shape=None):
         raise ValueError(f"{name}: scales and biases must be [.., cols / 64] of [.., {cols}]")
     if shape is not None and (*rows, cols) != shape:
         raise ValueError(f"{name} must be {list(shape)}")
+
+
+def _matrix(ctx: Context, name: str, q, bits: int, shape=None):
+    """Their addresses on the context's device, once they are."""
+    _check_matrix(name, q, bits, shape)
+    w, s, b = q
     return _ptr_on(ctx, name, w), _ptr_on(ctx, name + "'s scales", s), _ptr_on(ctx, name + "'s biases", b)
 
 
@@ -553,19 +558,28 @@ class ExpertWeights:
         # aliases keep the memory that was checked, so that nothing else can come to lie at its addresses.
         self._packed = None
 
+    _NAMES = ("gate", "up", "down", "shared_gate", "shared_up", "shared_down")
+
+    def check(self):
+        """Raises where the matrices' shapes or types do not go together (as the first call does)."""
+        up, down = (self.inter, self.hidden), (self.hidden, self.inter)
+        for name, q, shape in zip(self._NAMES, self.matrices, [(self.experts, *s) for s in (up, up, down)] + [up, up, down]):
+            if q is None:
+                continue
+            if q[1].dtype != self.dtype:
+                raise TypeError("all scales and biases must have one type")
+            _check_matrix(name, q, 4, shape)
+
     def _block(self, ctx: Context, half: int) -> bytes:
         """The parameter block for moe_gate_up (half 0) or moe_down (1)."""
         P = self._packed
         if P is not None and P[0] == ctx.device and P[1][half] == tuple(map(_data_ptr, self._read[half])):
             return P[2]
         self._packed = None
-        up, down = (self.inter, self.hidden), (self.hidden, self.inter)
+        self.check()
         flat = []
-        for name, q, shape in zip(("gate", "up", "down", "shared_gate", "shared_up", "shared_down"), self.matrices,
-                                  [(self.experts, *s) for s in (up, up, down)] + [up, up, down]):
-            if q is not None and q[1].dtype != self.dtype:
-                raise TypeError("all scales and biases must have one type")
-            flat += _matrix(ctx, name, q, 4, shape) if q is not None else (0, 0, 0)
+        for name, q in zip(self._NAMES, self.matrices):
+            flat += _matrix(ctx, name, q, 4) if q is not None else (0, 0, 0)
         block = _P_MOE.pack(*flat, _DT[self.dtype], self.experts, self.hidden, self.inter)
         self._packed = (ctx.device, tuple(tuple(map(_data_ptr, r)) for r in self._read), block,
                         [t.detach() for r in self._read for t in r])

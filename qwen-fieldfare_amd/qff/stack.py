@@ -33,6 +33,8 @@ from . import ops
 from .pages import OutOfPages
 
 HIDDEN = 2048
+MOST_VOCAB, MOST_INTER = 262144, 4096   # of the sampling and the expert block
+ROUTER_EXPERTS = range(8, 257)
 
 
 def is_full_attention(l: int) -> bool:
@@ -105,19 +107,67 @@ class AttentionStack:
             M = L.get("mlp")
             if M is None:
                 continue
-            if M["experts"].hidden != HIDDEN or None in (M["experts"].matrices[0], M["experts"].matrices[2]):
-                raise ValueError(f"a layer's experts need gate, up and down of {HIDDEN} columns of x")
-            if M["router"][0].shape[0] != M["experts"].experts:
-                raise ValueError("a layer's router must have a row for each of its experts")
-            if M["gate"] is not None and M["experts"].matrices[3] is None:
-                raise ValueError("a shared expert's gate needs a shared expert")
+            self._check_block(M)
             if self._shape(M) not in self._block:
                 self._block[self._shape(M)] = self._block_tensors(M, batch, device)
+        self._placed = not self._block   # whether _ready has seen the blocks' tensors
         self.head = head
+        if (head is not None or self._block) and batch > ctx.cfg.max_batch:
+            raise ValueError(f"a batch of {batch} exceeds the context's max_batch of {ctx.cfg.max_batch}")
         if head is not None:
+            self._check_norm("the head's", head["norm_w"])
+            vocab = head["lm_head"][0].shape[0]
+            ops._check_matrix("lm_head", head["lm_head"], 4, (vocab, HIDDEN))
+            if not 1 <= vocab <= MOST_VOCAB:
+                raise ValueError(f"lm_head must have 1 .. {MOST_VOCAB} rows")
             self.logits = torch.empty(batch, head["lm_head"][0].shape[0], **f32)
             self.tokens = torch.empty(batch, dtype=torch.int32, device=device)
             self.chances = torch.empty(batch, **f32)
+
+    @staticmethod
+    def _check_norm(whose, w):
+        if w.numel() != HIDDEN or w.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"{whose} norm_w must be float32 or bfloat16 [{HIDDEN}]")
+
+    def _check_block(self, M):
+        """What the calls of an expert block would refuse, whatever the device (here, and not by one of them with the
+        layer's recurrent state or its cache advanced before it)."""
+        E = M["experts"]
+        if E.hidden != HIDDEN or None in (E.matrices[0], E.matrices[2]):
+            raise ValueError(f"a layer's experts need gate, up and down of {HIDDEN} columns of x")
+        if M["router"][0].shape[0] != E.experts:
+            raise ValueError("a layer's router must have a row for each of its experts")
+        if E.experts not in ROUTER_EXPERTS or E.inter > MOST_INTER:
+            raise ValueError(f"a layer takes {ROUTER_EXPERTS.start} .. {ROUTER_EXPERTS.stop - 1} experts of up to {MOST_INTER} rows")
+        if M["gate"] is not None and E.matrices[3] is None:
+            raise ValueError("a shared expert's gate needs a shared expert")
+        self._check_norm("a layer's", M["norm_w"])
+        ops._check_matrix("router", M["router"], 8, (E.experts, HIDDEN))
+        if M["gate"] is not None:
+            ops._check_matrix("gate", M["gate"], 8, (1, HIDDEN))
+        E.check()
+
+    def _ready(self):
+        """The rest of it, once, ahead of the first step or slice: where the blocks' tensors lie, by calls of no tokens."""
+        if self._placed:
+            return
+        ctx = self.ctx
+        for L in self.layers:
+            M = L.get("mlp")
+            if M is None:
+                continue
+            x, idx, sc = self._none(M["norm_w"].device)
+            ops.rms_norm(ctx, x, M["norm_w"], self.eps, gate=M["gate"])
+            ops._matrix(ctx, "router", M["router"], 8)
+            h = ops.moe_gate_up(ctx, M["experts"], x, idx)
+            ops.moe_down(ctx, M["experts"], h, idx, sc)
+        self._placed = True
+
+    @staticmethod
+    def _none(device):
+        """x, indices and scores of no tokens."""
+        return (torch.empty(0, HIDDEN, device=device), torch.empty(0, 8, dtype=torch.int32, device=device),
+                torch.empty(0, 8, device=device))
 
     @staticmethod
     def _shape(M):
@@ -195,6 +245,7 @@ class AttentionStack:
             raise TypeError(f"positions must be int32 [{self.B}]")
         if positions.device != x.device or not positions.is_contiguous():
             raise ValueError("positions must be contiguous, on x's device")
+        self._ready()
         for l in range(len(self.layers)):
             self.layer_step(l, x, positions)
 
@@ -235,6 +286,7 @@ class AttentionStack:
         pages, copies = self._paged(), []
         if len(positions) != self.B:
             raise ValueError(f"positions must have {self.B} entries")
+        self._ready()
         held = list(pages.lengths)
         for b, p in enumerate(positions):
             if p > held[b] or 0 <= p < held[b] and "dn" in self.kinds:
@@ -277,6 +329,7 @@ class AttentionStack:
                              f"position {ctx.cfg.max_ctx}")
         if start != P.lengths[slot] and "dn" in self.kinds:
             raise ValueError(f"slot {slot} holds {P.lengths[slot]} positions: a slice follows them, or begins in a released slot")
+        self._ready()
         copies = P.reserve(slot, start, start + T)
         self._unpark(slot)
         self._copy_pages([s for s, _ in copies], [d for _, d in copies])
