@@ -910,23 +910,26 @@ __device__ __forceinline__ void tile_begin(const MoeArgs& p, const TileArgs& a, 
         if (k < 4) put_terms<SB_DT>(terms, 8 * k, s8, b8);
     };
     const int eights = (G + 7) / 8;
-    if (vec && G == 8) {
-        const u32x4_t s8 = *reinterpret_cast<const u32x4_t*>(mm.s + base), b8 = *reinterpret_cast<const u32x4_t*>(mm.b + base);
-        put(0, s8, b8);
-        put_terms<SB_DT>(terms, 8, s8, b8);
-    } else if (vec && G == 32) {
-        u32x4_t s8[4], b8[4];
+    if (vec) {
+        // 32 groups in one round of loads (one for each eight: 4096 columns of 8192 tokens 731 us instead of 719)
+        for (int k0 = 0; k0 < eights; k0 += 4) {
+            u32x4_t s8[4], b8[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            s8[k] = *reinterpret_cast<const u32x4_t*>(mm.s + base + 8 * k);
-            b8[k] = *reinterpret_cast<const u32x4_t*>(mm.b + base + 8 * k);
+            for (int k = 0; k < 4; ++k) {
+                if (k0 + k >= eights) break;
+                s8[k] = *reinterpret_cast<const u32x4_t*>(mm.s + base + 8 * (k0 + k));
+                b8[k] = *reinterpret_cast<const u32x4_t*>(mm.b + base + 8 * (k0 + k));
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (k0 + k >= eights) break;
+                put(k0 + k, s8[k], b8[k]);
+            }
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) put(k, s8[k], b8[k]);
     } else {
-        for (int k = 0; k < eights; ++k) put(k, load_u16x8(mm.s + base, 8 * k, G, vec), load_u16x8(mm.b + base, 8 * k, G, vec));
-        if (eights < 4 && (eights & 1)) put_terms<SB_DT>(terms, 8 * eights, u32x4_t{}, u32x4_t{});   // (the half that meets sums of zero)
+        for (int k = 0; k < eights; ++k) put(k, load_u16x8(mm.s + base, 8 * k, G, false), load_u16x8(mm.b + base, 8 * k, G, false));
     }
+    if (eights < 4 && (eights & 1)) put_terms<SB_DT>(terms, 8 * eights, u32x4_t{}, u32x4_t{});   // (the half that meets sums of zero)
     __syncthreads();
     body(tile, m0, m1, row0);
 }
