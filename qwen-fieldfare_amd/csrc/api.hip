@@ -61,6 +61,9 @@ WorkspaceLayout workspace_layout(const qff_ctx_cfg& cfg) {
     L.pf_md = take(PS * 32 * sizeof(float));
     L.sched = take(2 * kSchedSlots * sizeof(unsigned));
     L.dn_arrive = take(B * 16 * sizeof(unsigned));
+    // From here on three kinds of calls have their own scratch, dead when the call's kernels are done, in the same bytes:
+    // the chunked DeltaNet prefill, the expert block, sampling.
+    const size_t shared = off;
     // DeltaNet prefill chunk records (deltanet_chunked.hip): per chunk and key
     // head the K image and Q blocks (hi, lo), per chunk and value head the T
     // and P blocks (hi, lo), gate factors and beta V
@@ -71,6 +74,8 @@ WorkspaceLayout workspace_layout(const qff_ctx_cfg& cfg) {
     L.pop = take(NC * 32 * 2 * 6 * 512 * sizeof(uint16_t));
     L.gates = take(NC * 32 * 4 * 64 * sizeof(float));
     L.bv = take(NC * 32 * 64 * 128 * sizeof(float));
+    size_t end = off;
+    off = shared;
     L.moe_off = take(sizeof(int));
     L.moe_tiles = take(moe_tiles(cfg) * 16);
     L.moe_list = take(static_cast<size_t>(moe_tokens(cfg)) * kMoeMaxTop * sizeof(int));
@@ -78,6 +83,8 @@ WorkspaceLayout workspace_layout(const qff_ctx_cfg& cfg) {
     L.moe_xs = take(moe_part_bytes(cfg) / 16);
     L.moe_part = take(moe_part_bytes(cfg));
     L.moe_exps = take(moe_part_bytes(cfg) / 32);
+    end = std::max(end, off);
+    off = shared;
     L.sm_range = take(B * kSampleChunks * sizeof(float2));
     L.sm_mass = take(B * (kSampleChunks + 1) * kSampleBins * sizeof(unsigned long long));
     L.sm_count = take(B * kSampleBins * sizeof(uint32_t));
@@ -85,7 +92,7 @@ WorkspaceLayout workspace_layout(const qff_ctx_cfg& cfg) {
     L.sm_base = take(B * kSampleChunks * sizeof(unsigned long long));
     L.sm_listed = take(B * kSampleChunks * sizeof(int));
     L.sm_list = take(B * kSampleVocab * sizeof(int32_t));
-    L.total = off;
+    L.total = std::max(end, off);
     return L;
 }
 
