@@ -258,7 +258,7 @@ int qff_rms_norm(qff_ctx* ctx, qff_stream_t stream, const void* x, qff_dtype x_d
  * x and h are 16-byte aligned. tokens may be 0;
  * QFF_ERR_WORKSPACE above the larger of max_batch and max_prefill_tokens.
  *
- * What both halves round, beside their outputs and the fp32 sums: up to 72 pairs
+ * What both halves round, beside their outputs and the fp32 sums: up to 60 pairs
  * (token, slot; down: 200) nothing. Above, products run on fp16 operands after
  * power-of-two shifts: a weight is scale (q - 8), exact, and a part constant over
  * its group of 64 columns, bias + 8 scale (22 bits of it, or 2^-48), which meets the

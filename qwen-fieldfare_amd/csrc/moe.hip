@@ -1312,16 +1312,17 @@ MoeMat moe_mat(const qff_q4_matrices& q) {
 // pairs an expert (for gate and up: by the terms of x) up to which the small tiles take them; up to
 // 32 tokens they always do, so the large ones have bf16 outputs of fewer terms alone.
 // Measured with 256 experts of 512 x 2048 and a shared one, 8 a token, us a call with what
-// stands ahead of and behind the products:
-//   gate and up, pairs   72   108   144       an expert   0.5    2    6    8 (fp32 x)    8   12   16 (bf16 x)
-//     by themselves    29.2  41.5  52.8
-//     small tiles      27.9    -   42.0                  49    79  100  118             91   99  118
-//     large tiles        -     -     -                   62    94  118  120            104  109  114
-//   down, pairs         144   216   288       an expert    1    2    4    6 (fp32 h)    2    4    6 (fp16 h, bf16 y)
-//     by themselves    34.2  47.8  61.5
-//     small tiles      39.9  45.8  50.7                  50.7 62.2 68   78              62   68   71
-//     large tiles        -     -     -                  53.6 65   68   73              64   65   70
-constexpr int kOneUp = 72, kOneDown = 200, kSlimUp = 14, kSlimDown = 2;
+// stands ahead of and behind the products, other weights each time (two runs differ by up to
+// 0.5, the single pairs of down by 3):
+//   gate and up, pairs   36    54    63    72    81    90   an expert   6    7    8    9 (fp32 x)   14   15   16 (bf16 x)
+//     by themselves    16.5  21.3  23.7  25.8  29.5  32.0
+//     small tiles      18.6  22.9  23.1  23.1  30.0  29.9              86   95  101  108             91   96  101
+//     large tiles                                                     109  110  111  112            100  100  101
+//   down, pairs         126   144   162   180   198   216   an expert  1.5   2   2.5   3    4 (fp32 h)   1.5   2    3    4 (fp16 h, bf16 y)
+//     by themselves    29.1  31.4  34.2  40.6  41.3  43.4
+//     small tiles      31.7  34.4  36.5  39.5  39.5  39.1             52.5 55.8 59.8 61.9 64.2          51.4 55.6 60.3 62.6
+//     large tiles                                                     53.8 54.5 60.1 60.5 61.3          54.0 55.3 61.0 61.7
+constexpr int kOneUp = 60, kOneDown = 200, kSlimUp = 16, kSlimDown = 2;
 
 template <int DT>
 using Dt = std::integral_constant<int, DT>;
