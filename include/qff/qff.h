@@ -262,13 +262,14 @@ int qff_rms_norm(qff_ctx* ctx, qff_stream_t stream, const void* x, qff_dtype x_d
  * (token, slot; down: 200) nothing. Above, products run on fp16 operands after
  * power-of-two shifts: a weight is scale (q - 8), exact, and a part constant over
  * its group of 64 columns, bias + 8 scale (22 bits of it, or 2^-48), which meets the
- * group's sum of x; an
- * fp32 input is two fp16 terms (2^-22 of its value, or 2^-37 of its row's
- * largest), a BF16 one is exact beside the same 2^-37. With a BF16 output and 33
- * tokens or more, fp32 inputs and the products of F16 scales with q - 8 may keep 11
- * bits, and so may what moe_down sums over the pairs, relative to the largest of
- * each 64 outputs of a pair. There, scales lie in 2^-22 .. 31 in magnitude (smaller
- * ones lose bits; 0 is exact) and |bias + 8 scale| is at most 8. */
+ * group's sum of x; an fp32 input is two fp16 terms (2^-22 of its value, or 2^-37 of
+ * its row's largest), a BF16 one is exact beside the same 2^-37. With a BF16 output and
+ * 33 tokens or more, fp32 inputs and the products of F16 scales with q - 8 may keep 11
+ * bits, and so may the pairs' rows that moe_down sums (11 bits of each value, or 2^-39
+ * of the largest of the 64 beside it). There, scales lie in 2^-22 .. 31 in magnitude
+ * (smaller ones lose bits; 0 is exact) and |bias + 8 scale| is at most 8. A row's
+ * largest |x| lies in 2^-100 .. 2^110 or is 0 (smaller ones lose bits, sums of larger
+ * ones may leave fp32). */
 int qff_moe_gate_up(qff_ctx* ctx, qff_stream_t stream, const qff_moe_weights* p, const void* x,
                     qff_dtype x_dtype, const int32_t* indices, int top, void* h, qff_dtype h_dtype,
                     int tokens);
@@ -276,7 +277,9 @@ int qff_moe_gate_up(qff_ctx* ctx, qff_stream_t stream, const qff_moe_weights* p,
 /* The second half:
  *   y[m] = residual[m] + sum_{j < top} scores[m, j] h[m, j] Wd^T
  *          (+ coef[m] h[m, top] Wsd^T with a shared expert, p->shared_down),
- * summed in fp32 in the order of j. Replaces the down-accumulate and combine
+ * summed in fp32: in the order of j, or (up to 200 pairs) in an order over the slots and
+ * their columns that depends on top, the shared expert and inter alone, so that a
+ * call's bits never change from one to the next. Replaces the down-accumulate and combine
  * kernels of deltanet.metal:904-1114, 1212-1832, 1985-2227. Pairs whose index lies
  * outside 0 .. experts - 1 add nothing, whatever h holds there.
  *   h        [tokens, top + shared, inter] of h_dtype (F32, BF16 or F16), finite

@@ -449,7 +449,7 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const float* __restric
 // of eight bits is one of fp16's smallest numbers, 2^-23, which the FMA and the matrix
 // cores take as they are; b + 8 s may be up to 8 in magnitude.
 // So F32 and F16 outputs are sums of exact products (up to 2^-22 of x), and
-// bf16 ones carry 11 bits an operand (a bf16 result has 8).
+// bf16 ones carry 11 bits an operand (a bf16 result has 8) from 33 tokens on.
 
 // Rows of x for the tiles: XT fp16 terms [row][XT][cols] (each 8 columns in the
 // order c0, c4, c1, c5, .., the nibbles' own) and the row's factor 2^(e - 6); and
@@ -1016,8 +1016,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     tile_kernel<2, SB_DT, XT, WT, false, MMT>(p, a, GateUpOut<H_DT>{p, h});
 }
 
-// The pairs' weighted rows: fp32, or (HALF) fp16 relative to the power of two above
-// the largest of each 64, which stands in `exps` [pair][rows / 64].
+// The pairs' weighted rows: fp32, or (HALF, for bf16 y) fp16 after a power-of-two shift that
+// puts the largest of each 64 into [2^14, 2^15), which stands in `exps` [pair][rows / 64]. fp16
+// has 28 powers of two below that with all of its 11 bits, so a value keeps 11 bits of its
+// own beside a much larger one; y has 8. It halves the rows' bytes (302 MB instead of 604 each way
+// for 8192 tokens of nine pairs). Against 64 bits y is off as the plain form is (1.7e-3, its
+// own rounding); from that form it differs by 5.8e-4, where the two round to different neighbours.
 template <bool HALF>
 struct DownOut {
     static constexpr int kBytes = HALF ? 128 : 256;
