@@ -533,7 +533,8 @@ class ExpertWeights:
     the shared expert's [inter, hidden], [hidden, inter] (None: there is none).
     moe_gate_up needs gate and up, moe_down needs down; what only the other needs
     may be None. The tensors are kept; a call whose matrices no longer lie where they
-    lay (set_, resize_, .data) checks all of them again and reads the new ones."""
+    lay (set_, resize_, .data) checks all of them again and reads the new ones (the
+    memory of the former is held until then)."""
 
     def __init__(self, gate=None, up=None, down=None, shared_gate=None, shared_up=None, shared_down=None):
         self.matrices = (gate, up, down, shared_gate, shared_up, shared_down)
