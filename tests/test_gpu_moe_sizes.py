@@ -131,3 +131,39 @@ def test_rms_norm_of_more_rows_than_a_grid(hip):
         ref = qff.rms_norm(ctx, x[a:b], w, gate=gate)
         assert torch.equal(y[a:b], ref[0]) and torch.equal(coef[a:b], ref[1])
     assert torch.equal(y[:2 ** 16], y[2 ** 23:2 ** 23 + 2 ** 16])
+
+
+def test_most_experts_and_slots(hip):
+    """512 experts, 16 a token and a shared one, in small and large tiles."""
+    rng = np.random.default_rng(12)
+    E, top, D, I = 512, 16, 128, 64
+    w = _weights(rng, E, D, I, "f16", True)
+    ctx = _ctx()
+    for n, dt in ((40, "f32"), (300, "f32"), (600, "bf16")):
+        print("512 experts", n, flush=True)
+        idx = _indices(rng, n, E, top, "holes")
+        x = torch.from_numpy(rng.standard_normal((n, D))).to(DEV, DT[dt])
+        _check_gate_up(ctx, w, x, idx, DT[dt], "holes")
+        h = torch.from_numpy(rng.standard_normal((n, top + 1, I))).to(DEV, DT[dt])
+        _check_down(ctx, w, h, idx, DT[dt], "in place", True, rng)
+
+
+def test_more_tokens_than_a_grid_has_rows(hip):
+    """66000 tokens: slices of at most 65535. The last slice's tokens against a call of their own, the others by parts."""
+    import qff
+    rng = np.random.default_rng(13)
+    n, E, top, D, I = 66000, 4, 2, 64, 64
+    w = _handle(_weights(rng, E, D, I, "bf16", True))
+    ctx = _ctx(max_batch=1, max_prefill_tokens=n)
+    x = torch.randn(n, D, device=DEV)
+    idx = torch.randint(-1, E + 1, (n, top), dtype=torch.int32, device=DEV)
+    sc = torch.rand(n, top, device=DEV)
+    h = qff.moe_gate_up(ctx, w, x, idx, out=torch.zeros(n, top + 1, I, device=DEV))
+    y = qff.moe_down(ctx, w, h, idx, sc, residual=x)
+    torch.cuda.synchronize()
+    for a, b in ((0, 1000), (65000, n), (65535, n)):
+        g = qff.moe_gate_up(ctx, w, x[a:b], idx[a:b].contiguous(), out=torch.zeros(b - a, top + 1, I, device=DEV))
+        z = qff.moe_down(ctx, w, h[a:b], idx[a:b].contiguous(), sc[a:b].contiguous(), residual=x[a:b])
+        # (the same exact products; a call's form decides their order: 20 roundings of sums a few times the results)
+        assert (g - h[a:b]).norm() <= 1e-6 * g.norm() and (z - y[a:b]).norm() <= 1e-6 * z.norm()
+    ctx.close()
