@@ -310,7 +310,7 @@ int qff_moe_down(qff_ctx* ctx, qff_stream_t stream, const qff_moe_weights* p, co
  * arrays temperature, top_k, top_p and min_p may each be NULL: 1, off, off, off.
  * probs may be NULL. Counterpart of QwenLogitSelector (Runtime/Generation/
  * QwenGenerationSupport.swift:228-362), which runs on the host.
- * 1 <= vocab <= 262144. batch may be 0; QFF_ERR_WORKSPACE above max_batch. */
+ * 1 <= vocab <= 262144, batch <= 65535. batch may be 0; QFF_ERR_WORKSPACE above max_batch. */
 int qff_sample(qff_ctx* ctx, qff_stream_t stream, const void* logits, qff_dtype dtype, const float* u,
                const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                int32_t* tokens, float* probs, int vocab, int batch);

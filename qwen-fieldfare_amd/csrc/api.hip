@@ -651,7 +651,7 @@ int qff_sample(qff_ctx* ctx, qff_stream_t stream, const void* logits, qff_dtype 
                float* probs, int vocab, int batch) {
     if (!ctx || !dtype_ok(dtype) || batch < 0 || vocab <= 0) return QFF_ERR_INVALID_ARG;
     if (batch > 0 && (!logits || !u || !tokens)) return QFF_ERR_INVALID_ARG;
-    if (vocab > kSampleVocab) return QFF_ERR_UNSUPPORTED;
+    if (vocab > kSampleVocab || batch > 65535) return QFF_ERR_UNSUPPORTED;   // (a grid's second dimension)
     if (batch > ctx->cfg.max_batch) return QFF_ERR_WORKSPACE;
     if (batch == 0) return QFF_OK;
     const OnDevice on(ctx->device);

@@ -1,5 +1,8 @@
-"""What a context's workspace holds, from its size alone."""
+"""What a context's workspace holds, from its size alone, and what a large one does not allow."""
 import ctypes
+import subprocess
+
+from test_paged_host import _program
 
 
 def _size(*cfg):
@@ -26,3 +29,11 @@ def test_many_sequences_cost_what_sampling_lists():
     of the attention's partials 2 MB)."""
     per = (_size(2064, 64, 1) - _size(2063, 64, 1)) - 2 * 128 * 8 * (2 + 256) * 4
     assert 0 <= per - (262144 * 4 + 65 * 256 * 8) < 1 << 16
+
+
+def test_batches_that_sampling_refuses(tmp_path):
+    """A context whose max_batch is more than a grid's second dimension holds."""
+    import qff
+    qff.lib()
+    r = subprocess.run([_program(tmp_path, "sample_batch")], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout
